@@ -498,6 +498,148 @@ typedef struct tc_decode_init_args {
  * history rows stay with the caller). */
 int tc_decode_init(const tc_decode_init_args* a, void* stream);
 
+/* ------------------------------------------------------------------------ */
+/* full attention: rotary positions, packed causal attention, 8-bit cache    */
+/* (no reference counterpart: the layers a hybrid stack keeps at full        */
+/* attention next to its telescoping ones)                                   */
+/* ------------------------------------------------------------------------ */
+
+typedef struct tc_rotary_args {
+  int32_t B, N, Hq, Hk, D;
+  int32_t R;                 /* even: the first R dims of a head rotate      */
+  int32_t dtype;
+  int32_t interleaved;       /* pairs (2i, 2i + 1); 0: (i, i + R / 2)        */
+  int32_t inverse;           /* rotate by the negative angle (the VJP)       */
+  int32_t n_pos;
+  const void* q;             /* [B, N, Hq, D] through strides, head dim dense */
+  int64_t q_stride_b, q_stride_n, q_stride_h;
+  const void* k;             /* [B, N, Hk, D] (Hk 0: q alone)                */
+  int64_t k_stride_b, k_stride_n, k_stride_h;
+  void* q_out;               /* [B, N, Hq, D] dense                          */
+  void* k_out;
+  const float* cos_t;        /* [n_pos, R / 2]                               */
+  const float* sin_t;
+  const int32_t* positions;  /* [B, N] (row stride pos_stride_b) or NULL: n  */
+  int64_t pos_stride_b;
+} tc_rotary_args;
+
+/* Rotary positions of q and k in one launch: (x1, x2) -> (x1 c - x2 s,
+ * x2 c + x1 s) in fp32, each operation rounded, the result rounded once to
+ * the element type.  A position outside [0, n_pos) makes its rows' rotated
+ * dims NaN. */
+int tc_rotary(const tc_rotary_args* a, void* stream);
+
+/* First token and end of the run of equal ids that each token of seq_idx
+ * [B, N] lies in (int32 [B, N] each, token indices of its row).  Tokens with a
+ * negative id belong to no run: start = n + 1, end = n. */
+int tc_segment_bounds(int32_t B, int32_t N, const int32_t* seq_idx, int32_t* starts, int32_t* ends, void* stream);
+
+#define TC_KV_INT8 0  /* code = round(x 127 / amax) + 128 in a byte          */
+#define TC_KV_FP8 1   /* code = e4m3 float of x 448 / amax                   */
+
+typedef struct tc_kv_cache {
+  int32_t rows, Hkv, Dk, Dv;
+  int32_t capacity;          /* slots per row                                */
+  int32_t store;             /* TC_KV_*                                      */
+  uint8_t* k;                /* [rows, Hkv, capacity, Dk] codes              */
+  uint8_t* v;                /* [rows, Hkv, capacity, Dv]                    */
+  float* k_scale;            /* [rows, Hkv, capacity]                        */
+  float* v_scale;
+  int32_t* lengths;          /* [rows] tokens held                           */
+} tc_kv_cache;
+
+typedef struct tc_kv_write_args {
+  int32_t B, N, dtype;
+  int32_t fresh;             /* slots from 0 on; 0: behind the row's length  */
+  const void* k;             /* [B, N, Hkv, Dk] through strides              */
+  int64_t k_stride_b, k_stride_n, k_stride_h;
+  const void* v;             /* [B, N, Hkv, Dv]                              */
+  int64_t v_stride_b, v_stride_n, v_stride_h;
+  const int32_t* seq_idx;    /* [B, N] cache row of each token (negative:
+                                none; one run per row), or NULL: row b       */
+  const int32_t* starts;     /* tc_segment_bounds' starts of seq_idx         */
+  int32_t* dev_status;       /* TC_DEV_BAD_INDEX: a token had no row or slot
+                                and was dropped                              */
+} tc_kv_write_args;
+
+/* Quantise keys and values into the cache and move the rows' lengths on. */
+int tc_kv_write(const tc_kv_cache* c, const tc_kv_write_args* a, void* stream);
+
+/* The values that the first `length` slots of every row stand for, as
+ * [rows, length, Hkv, D] of dtype; zeros past a row's length. */
+int tc_kv_read(const tc_kv_cache* c, int32_t length, int32_t dtype, void* k_out, void* v_out, void* stream);
+
+typedef struct tc_kv_attend_args {
+  int32_t B, Hq;             /* rows 0 .. B - 1 of the cache                 */
+  int32_t max_tokens;        /* most tokens that a row attends (a plan, not a
+                                limit: longer rows come out right, slower)   */
+  int32_t dtype;             /* q, k_t, v_t, out                             */
+  const void* q;             /* [B, Hq, Dk] through strides                  */
+  int64_t q_stride_b, q_stride_h;
+  const void* k_t;           /* step: the new token's key [B, Hkv, Dk], written
+                                to slot lengths[b] and attended; NULL: attend
+                                the slots below lengths[b] only              */
+  int64_t k_stride_b, k_stride_h;
+  const void* v_t;
+  int64_t v_stride_b, v_stride_h;
+  const float* rope_cos;     /* step: rotate q and k_t to position lengths[b] */
+  const float* rope_sin;     /* [n_pos, R / 2], or NULL with R = 0           */
+  int32_t R, interleaved, n_pos;
+  int32_t has_softcap;
+  float softcap, scale;
+  int32_t advance;           /* step: lengths[b] += 1                        */
+  void* out;                 /* [B, Hq, Dv]                                  */
+  float* lse;                /* [B, Hq] natural log; -inf for an empty row
+                                (whose out is zero)                          */
+  void* k_new;               /* step: the key and value as stored [B, Hkv, D] */
+  void* v_new;               /* of new_dtype, or NULL                        */
+  int32_t new_dtype;
+  float* scratch;            /* tc_kv_attend_scratch_floats floats           */
+  int64_t scratch_floats;
+  int32_t* counters;         /* B (Hkv ceil(Hq / Hkv / 8) + 1) int32, zeros
+                                before the first call; every call leaves zeros */
+  int64_t num_counters;
+  int32_t* dev_status;
+} tc_kv_attend_args;
+
+int64_t tc_kv_attend_scratch_floats(const tc_kv_cache* c, int32_t B, int32_t Hq, int32_t max_tokens);
+int tc_kv_attend(const tc_kv_cache* c, const tc_kv_attend_args* a, void* stream);
+
+typedef struct tc_causal_args {
+  int32_t B, N, Hq, Hkv, Dk, Dv, dtype;
+  int32_t has_softcap;
+  float softcap, scale;
+  const void* q;             /* [B, N, Hq, Dk] through strides, head dim dense */
+  int64_t q_stride_b, q_stride_n, q_stride_h;
+  const void* k;             /* [B, N, Hkv, Dk]                              */
+  int64_t k_stride_b, k_stride_n, k_stride_h;
+  const void* v;             /* [B, N, Hkv, Dv]                              */
+  int64_t v_stride_b, v_stride_n, v_stride_h;
+  const int32_t* starts;     /* tc_segment_bounds of the example ids, or NULL */
+  const int32_t* ends;       /* (both): one example per row                  */
+  void* out;                 /* [B, N, Hq, Dv] dense                         */
+  float* lse;                /* [B, N, Hq] natural log; -inf, out 0 for a
+                                token of no example                          */
+  /* backward only */
+  const void* o;             /* forward out, dense                           */
+  const void* dout;          /* [B, N, Hq, Dv] dense                         */
+  const float* dlse;         /* [B, N, Hq] or NULL                           */
+  float* delta;              /* scratch [B, N, Hq]                           */
+  void* dq;                  /* [B, N, Hq, Dk] dense                         */
+  void* dk;                  /* [B, N, Hkv, Dk]                              */
+  void* dv;                  /* [B, N, Hkv, Dv]                              */
+  int32_t* dev_status;
+  int32_t impl;              /* 0 auto, 1 SIMT, 2 tensor core                */
+} tc_causal_args;
+
+/* Causal attention with grouped heads over packed examples: token n of a row
+ * attends tokens [starts[n], n] of the row.  logit = c tanh(x / c),
+ * x = scale q.k (x without softcap).  bf16 / f16 with Dk = Dv = 64 or 128 and
+ * 16-byte aligned strides run on the tensor cores. */
+int tc_causal_fwd(const tc_causal_args* a, void* stream);
+/* Its gradients, the lse's among the incoming ones; deterministic. */
+int tc_causal_bwd(const tc_causal_args* a, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

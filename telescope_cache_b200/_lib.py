@@ -98,6 +98,40 @@ class DecodeInitArgs(ctypes.Structure):
     ]
 
 
+def _fields(spec):
+    """ctypes fields from 'type name name; ...' (i int32, l int64, f float, p pointer)."""
+    kinds = {"i": _c_i32, "l": _c_i64, "f": _c_f32, "p": _c_vp}
+    return [(n, kinds[g.split()[0]]) for g in spec.split(";") for n in g.split()[1:]]
+
+
+class RotaryArgs(ctypes.Structure):
+    _fields_ = _fields("i B N Hq Hk D R dtype interleaved inverse n_pos; p q; l q_stride_b q_stride_n q_stride_h;"
+                       "p k; l k_stride_b k_stride_n k_stride_h; p q_out k_out cos_t sin_t positions;"
+                       "l pos_stride_b")
+
+
+class KVCacheArgs(ctypes.Structure):
+    _fields_ = _fields("i rows Hkv Dk Dv capacity store; p k v k_scale v_scale lengths")
+
+
+class KVWriteArgs(ctypes.Structure):
+    _fields_ = _fields("i B N dtype fresh; p k; l k_stride_b k_stride_n k_stride_h; p v;"
+                       "l v_stride_b v_stride_n v_stride_h; p seq_idx starts dev_status")
+
+
+class KVAttendArgs(ctypes.Structure):
+    _fields_ = _fields("i B Hq max_tokens dtype; p q; l q_stride_b q_stride_h; p k_t; l k_stride_b k_stride_h; p v_t;"
+                       "l v_stride_b v_stride_h; p rope_cos rope_sin; i R interleaved n_pos has_softcap;"
+                       "f softcap scale; i advance; p out lse k_new v_new; i new_dtype; p scratch; l scratch_floats;"
+                       "p counters; l num_counters; p dev_status")
+
+
+class CausalArgs(ctypes.Structure):
+    _fields_ = _fields("i B N Hq Hkv Dk Dv dtype has_softcap; f softcap scale; p q; l q_stride_b q_stride_n q_stride_h;"
+                       "p k; l k_stride_b k_stride_n k_stride_h; p v; l v_stride_b v_stride_n v_stride_h;"
+                       "p starts ends out lse o dout dlse delta dq dk dv dev_status; i impl")
+
+
 # (name, argtypes) of every exported symbol; the CPU test checks that each one
 # exists and that this list matches include/telescope_cache.h.
 SIGNATURES = {
@@ -141,6 +175,14 @@ SIGNATURES = {
     "tc_gate_apply": [_c_i64, _c_i32, _c_vp, _c_i32, _c_vp, _c_i32, _c_vp, _c_vp],
     "tc_decode_step": [ctypes.POINTER(DecodeArgs), _c_vp],
     "tc_decode_init": [ctypes.POINTER(DecodeInitArgs), _c_vp],
+    "tc_rotary": [ctypes.POINTER(RotaryArgs), _c_vp],
+    "tc_segment_bounds": [_c_i32, _c_i32, _c_vp, _c_vp, _c_vp, _c_vp],
+    "tc_kv_write": [ctypes.POINTER(KVCacheArgs), ctypes.POINTER(KVWriteArgs), _c_vp],
+    "tc_kv_read": [ctypes.POINTER(KVCacheArgs), _c_i32, _c_i32, _c_vp, _c_vp, _c_vp],
+    "tc_kv_attend_scratch_floats": [ctypes.POINTER(KVCacheArgs), _c_i32, _c_i32, _c_i32],
+    "tc_kv_attend": [ctypes.POINTER(KVCacheArgs), ctypes.POINTER(KVAttendArgs), _c_vp],
+    "tc_causal_fwd": [ctypes.POINTER(CausalArgs), _c_vp],
+    "tc_causal_bwd": [ctypes.POINTER(CausalArgs), _c_vp],
 }
 
 _LIB = None
@@ -164,6 +206,7 @@ def lib():
         handle.tc_tree_bwd_scratch_bytes.restype = ctypes.c_int64
         handle.tc_linear_wgrad_scratch_floats.restype = ctypes.c_int64
         handle.tc_linear_scratch_floats.restype = ctypes.c_int64
+        handle.tc_kv_attend_scratch_floats.restype = ctypes.c_int64
         _LIB = handle
     return _LIB
 

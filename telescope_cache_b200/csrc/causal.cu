@@ -1,0 +1,498 @@
+// Packed causal attention: the C entries, the example bounds, Delta, and the
+// CUDA-core kernels (fp32, and the head dims that the tensor-core kernels of
+// causal_fwd.cu and causal_bwd.cu do not cover).
+//
+//   X_ij = scale q_i . k_j,  S = c tanh(X / c) (or X),  i sees starts[i] <= j <= i
+//   P = exp(S - lse),  out = P V
+//   dS = P (dO V^T - Delta),  Delta = rowsum(dO * out) - dlse,  dX = dS (1 - tanh^2)
+//   dQ = scale dX K,  dK = scale dX^T Q,  dV = P^T dO
+#include "causal.cuh"
+
+using namespace tc;
+
+namespace {
+
+// ---------------------------------------------------------------------------
+// example bounds
+// ---------------------------------------------------------------------------
+// One CTA per row; a thread owns consecutive tokens, so the largest run start
+// behind it and the smallest ahead of it come from one scan over the threads.
+// Bound by its two passes' latency (a few us at 16384 tokens, against the
+// attention that it precedes).
+constexpr int kBoundThreads = 1024;
+__global__ void __launch_bounds__(kBoundThreads) bounds_kernel(int N, const int32_t* seq, int32_t* starts, int32_t* ends) {
+  __shared__ int last_w[32], first_w[32];
+  const int64_t row = (int64_t)blockIdx.x * N;
+  const int32_t* id = seq + row;
+  const int per = (N + kBoundThreads - 1) / kBoundThreads;
+  const int n0 = min(N, (int)threadIdx.x * per), n1 = min(N, n0 + per);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int first = N, last = -1;  // run starts among this thread's tokens
+  int prev = n0 > 0 && n0 < N ? id[n0 - 1] : 0;
+  for (int n = n0; n < n1; ++n) {
+    const int cur = id[n];
+    if (n == 0 || cur != prev) {
+      if (first == N) first = n;
+      last = n;
+    }
+    prev = cur;
+  }
+  // exclusive scans: the largest start before this thread, the smallest after it
+  int before = last, after = first;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int x = __shfl_up_sync(0xffffffffu, before, o), y = __shfl_down_sync(0xffffffffu, after, o);
+    if (lane >= o) before = max(before, x);
+    if (lane + o < 32) after = min(after, y);
+  }
+  if (lane == 31) last_w[warp] = before;
+  if (lane == 0) first_w[warp] = after;
+  before = __shfl_up_sync(0xffffffffu, before, 1);
+  after = __shfl_down_sync(0xffffffffu, after, 1);
+  if (lane == 0) before = -1;
+  if (lane == 31) after = N;
+  __syncthreads();
+  for (int w = 0; w < warp; ++w) before = max(before, last_w[w]);
+  for (int w = warp + 1; w < 32; ++w) after = min(after, first_w[w]);
+  int start = before;
+  prev = n0 > 0 && n0 < N ? id[n0 - 1] : 0;
+  for (int n = n0; n < n1; ++n) {
+    const int cur = id[n];
+    if (n == 0 || cur != prev) start = n;
+    prev = cur;
+    starts[row + n] = cur < 0 ? n + 1 : start;
+  }
+  int end = after;
+  for (int n = n1 - 1; n >= n0; --n) {
+    const int cur = id[n];
+    ends[row + n] = cur < 0 ? n : end;
+    if (n == 0 || id[n - 1] != cur) end = n;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Delta = rowsum(dO * out) - dlse
+// ---------------------------------------------------------------------------
+template <typename T>
+__global__ void __launch_bounds__(256) delta_rows(CausalParams p, int64_t rows) {
+  const int64_t r = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
+  const int lane = threadIdx.x & 31;
+  if (r >= rows) return;
+  const T* o = static_cast<const T*>(p.o) + r * p.Dv;
+  const T* g = static_cast<const T*>(p.dout) + r * p.Dv;
+  float s = 0.f;
+  for (int d = lane; d < p.Dv; d += 32) s += to_f(o[d]) * to_f(g[d]);
+#pragma unroll
+  for (int x = 16; x; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
+  if (lane == 0) p.delta[r] = s - (p.dlse ? p.dlse[r] : 0.f);
+}
+
+// ---------------------------------------------------------------------------
+// CUDA-core tiles: 256 threads as 16 x 16; thread (ty, tx) owns rows ty + 16 i
+// and columns tx + 16 j of a TM x TM score tile, and output rows ty + 16 i with
+// the four-wide columns 4 tx + 64 j of a DM-wide row.  Shared rows are DM + 4
+// floats, so that 16 lanes reading float4s of 16 rows meet no bank twice.
+// fp32 throughout with the accurate expf / tanhf; bound by FMA issue and shared
+// memory reads (8 float4 loads for 64 multiply-adds of a thread's 4 x 4 scores).
+// ---------------------------------------------------------------------------
+constexpr int NT = 256;
+
+template <int TM, int DM> struct Tile {
+  static constexpr int RS = DM + 4;     // operand row stride
+  static constexpr int PS = TM + 4;     // score row stride
+  static constexpr int R = TM / 16;     // rows (and score columns) per thread
+  static constexpr int C = DM / 64;     // float4 output columns per thread
+};
+
+// rows [r0, r0 + TM) of head h of x, zeros outside [0, N) x [0, D)
+template <typename T, int TM, int DM>
+__device__ __forceinline__ void load_tile(float* s, const void* x, int64_t base, int64_t sn, int r0, int N, int D) {
+  const T* src = static_cast<const T*>(x) + base;
+  for (int i = threadIdx.x; i < TM * DM; i += NT) {
+    const int r = i / DM, d = i - r * DM;
+    s[r * Tile<TM, DM>::RS + d] = (r0 + r < N && d < D) ? to_f(src[(int64_t)(r0 + r) * sn + d]) : 0.f;
+  }
+}
+
+// acc[i][j] = a row (ty + 16 i) . b row (tx + 16 j)
+template <int TM, int DM>
+__device__ __forceinline__ void dot_tile(const float* a, const float* b, int D, float (*acc)[Tile<TM, DM>::R]) {
+  using Z = Tile<TM, DM>;
+  const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
+#pragma unroll
+  for (int i = 0; i < Z::R; ++i)
+#pragma unroll
+    for (int j = 0; j < Z::R; ++j) acc[i][j] = 0.f;
+  for (int d = 0; d < D; d += 4) {
+    float4 x[Z::R], y[Z::R];
+#pragma unroll
+    for (int i = 0; i < Z::R; ++i) {
+      x[i] = *reinterpret_cast<const float4*>(a + (ty + 16 * i) * Z::RS + d);
+      y[i] = *reinterpret_cast<const float4*>(b + (tx + 16 * i) * Z::RS + d);
+    }
+#pragma unroll
+    for (int i = 0; i < Z::R; ++i)
+#pragma unroll
+      for (int j = 0; j < Z::R; ++j)
+        acc[i][j] += x[i].x * y[j].x + x[i].y * y[j].y + x[i].z * y[j].z + x[i].w * y[j].w;
+  }
+}
+
+// acc[i][j] += sum_c w[ty + 16 i][c] m[c][4 tx + 64 j ..]
+template <int TM, int DM>
+__device__ __forceinline__ void mul_tile(const float* w, const float* m, float4 (*acc)[Tile<TM, DM>::C]) {
+  using Z = Tile<TM, DM>;
+  const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
+  for (int c = 0; c < TM; c += 4) {
+    float4 x[Z::R];
+#pragma unroll
+    for (int i = 0; i < Z::R; ++i) x[i] = *reinterpret_cast<const float4*>(w + (ty + 16 * i) * Z::PS + c);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+#pragma unroll
+      for (int j = 0; j < Z::C; ++j) {
+        const float4 y = *reinterpret_cast<const float4*>(m + (c + k) * Z::RS + 4 * tx + 64 * j);
+#pragma unroll
+        for (int i = 0; i < Z::R; ++i) {
+          const float f = k == 0 ? x[i].x : k == 1 ? x[i].y : k == 2 ? x[i].z : x[i].w;
+          acc[i][j].x += f * y.x;
+          acc[i][j].y += f * y.y;
+          acc[i][j].z += f * y.z;
+          acc[i][j].w += f * y.w;
+        }
+      }
+    }
+  }
+}
+
+template <typename T, int TM, int DM>
+__device__ __forceinline__ void store_rows(T* out, int64_t row_stride, int r0, int N, int D, float mul,
+                                           float4 (*acc)[Tile<TM, DM>::C]) {
+  using Z = Tile<TM, DM>;
+  const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
+#pragma unroll
+  for (int i = 0; i < Z::R; ++i) {
+    const int r = r0 + ty + 16 * i;
+    if (r >= N) continue;
+#pragma unroll
+    for (int j = 0; j < Z::C; ++j) {
+      const float v[4] = {acc[i][j].x, acc[i][j].y, acc[i][j].z, acc[i][j].w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int d = 4 * tx + 64 * j + k;
+        if (d < D) out[(int64_t)r * row_stride + d] = from_f<T>(v[k] * mul);
+      }
+    }
+  }
+}
+
+template <typename T, int TM, int DM>
+__global__ void __launch_bounds__(NT) fwd_cores(CausalParams p) {
+  using Z = Tile<TM, DM>;
+  extern __shared__ __align__(16) float sm[];
+  float* q_s = sm;                   // [TM][RS]
+  float* kv_s = q_s + TM * Z::RS;    // keys, then values
+  float* p_s = kv_s + TM * Z::RS;    // [TM][PS]
+  const int q0 = (gridDim.x - 1 - blockIdx.x) * TM, hq = blockIdx.y, b = blockIdx.z, hkv = hq / p.E;
+  const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
+  load_tile<T, TM, DM>(q_s, p.q, b * p.q_sb + hq * p.q_sh, p.q_sn, q0, p.N, p.Dk);
+  int lo[Z::R];
+  float m[Z::R], l[Z::R];
+  float4 o[Z::R][Z::C];
+#pragma unroll
+  for (int i = 0; i < Z::R; ++i) {
+    const int q = q0 + ty + 16 * i;
+    lo[i] = q < p.N ? first_key(p, b, q) : p.N;
+    m[i] = -INFINITY;
+    l[i] = 0.f;
+#pragma unroll
+    for (int j = 0; j < Z::C; ++j) o[i][j] = make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+  const int end = min(q0 + TM, p.N);
+  for (int k0 = first_key(p, b, q0) / TM * TM; k0 < end; k0 += TM) {
+    __syncthreads();
+    load_tile<T, TM, DM>(kv_s, p.k, b * p.k_sb + hkv * p.k_sh, p.k_sn, k0, p.N, p.Dk);
+    __syncthreads();
+    float s[Z::R][Z::R];
+    dot_tile<TM, DM>(q_s, kv_s, p.Dk, s);
+#pragma unroll
+    for (int i = 0; i < Z::R; ++i) {
+      const int q = q0 + ty + 16 * i;
+      float mx = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < Z::R; ++j) {
+        const int k = k0 + tx + 16 * j;
+        float x = s[i][j] * p.scale;
+        if (p.has_cap) x = p.cap * tanhf(x / p.cap);
+        s[i][j] = k >= lo[i] && k <= q ? x : -INFINITY;
+        mx = fmaxf(mx, s[i][j]);
+      }
+#pragma unroll
+      for (int x = 8; x; x >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
+      const float mn = fmaxf(m[i], mx), me = mn == -INFINITY ? 0.f : mn;
+      const float c = expf(m[i] - me);
+      float sum = 0.f;
+#pragma unroll
+      for (int j = 0; j < Z::R; ++j) {
+        // a NaN score (a NaN in a visible key) stays one; a masked one is 0
+        const float e = expf(s[i][j] - me);
+        sum += e;
+        p_s[(ty + 16 * i) * Z::PS + tx + 16 * j] = e;
+      }
+#pragma unroll
+      for (int x = 8; x; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+      l[i] = l[i] * c + sum;
+      m[i] = mn;
+#pragma unroll
+      for (int j = 0; j < Z::C; ++j) o[i][j].x *= c, o[i][j].y *= c, o[i][j].z *= c, o[i][j].w *= c;
+    }
+    __syncthreads();
+    load_tile<T, TM, DM>(kv_s, p.v, b * p.v_sb + hkv * p.v_sh, p.v_sn, k0, p.N, p.Dv);
+    __syncthreads();
+    mul_tile<TM, DM>(p_s, kv_s, o);
+  }
+#pragma unroll
+  for (int i = 0; i < Z::R; ++i) {
+    const float inv = l[i] != 0.f ? 1.f / l[i] : 0.f;
+#pragma unroll
+    for (int j = 0; j < Z::C; ++j) o[i][j].x *= inv, o[i][j].y *= inv, o[i][j].z *= inv, o[i][j].w *= inv;
+    const int q = q0 + ty + 16 * i;
+    if (tx == 0 && q < p.N)
+      p.lse[((int64_t)b * p.N + q) * p.Hq + hq] = l[i] != 0.f ? m[i] + logf(l[i]) : -INFINITY;
+  }
+  store_rows<T, TM, DM>(static_cast<T*>(p.out) + ((int64_t)b * p.N * p.Hq + hq) * p.Dv, (int64_t)p.Hq * p.Dv, q0, p.N,
+                        p.Dv, 1.f, o);
+}
+
+// P and dX of a score tile whose rows are queries (ROWS_Q) or keys.
+struct RowStat {
+  float lse, delta;
+  int lo, q;  // query q sees keys lo .. q
+};
+__device__ __forceinline__ RowStat row_stat(const CausalParams& p, int b, int hq, int q) {
+  RowStat r{0.f, 0.f, 1, 0};  // sees nothing
+  if (q < p.N) {
+    const int64_t i = ((int64_t)b * p.N + q) * p.Hq + hq;
+    r.lse = p.lse[i];
+    r.delta = p.delta[i];
+    r.lo = first_key(p, b, q);
+    r.q = q;
+  }
+  return r;
+}
+__device__ __forceinline__ void grad_of(const CausalParams& p, const RowStat& r, int k, float s, float dp, float* pr,
+                                        float* dx) {
+  float x = s * p.scale, g = 1.f;
+  if (p.has_cap) {
+    const float t = tanhf(x / p.cap);
+    x = p.cap * t;
+    g = 1.f - t * t;
+  }
+  const bool see = k >= r.lo && k <= r.q;
+  *pr = see ? expf(x - r.lse) : 0.f;
+  *dx = see ? *pr * (dp - r.delta) * g : 0.f;
+}
+
+template <typename T, int TM, int DM>
+__global__ void __launch_bounds__(NT) dq_cores(CausalParams p) {
+  using Z = Tile<TM, DM>;
+  extern __shared__ __align__(16) float sm[];
+  float* q_s = sm;
+  float* g_s = q_s + TM * Z::RS;
+  float* k_s = g_s + TM * Z::RS;
+  float* v_s = k_s + TM * Z::RS;
+  float* x_s = v_s + TM * Z::RS;
+  const int q0 = (gridDim.x - 1 - blockIdx.x) * TM, hq = blockIdx.y, b = blockIdx.z, hkv = hq / p.E;
+  const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
+  load_tile<T, TM, DM>(q_s, p.q, b * p.q_sb + hq * p.q_sh, p.q_sn, q0, p.N, p.Dk);
+  load_tile<T, TM, DM>(g_s, p.dout, ((int64_t)b * p.N * p.Hq + hq) * p.Dv, (int64_t)p.Hq * p.Dv, q0, p.N, p.Dv);
+  RowStat st[Z::R];
+  float4 acc[Z::R][Z::C];
+#pragma unroll
+  for (int i = 0; i < Z::R; ++i) {
+    st[i] = row_stat(p, b, hq, q0 + ty + 16 * i);
+#pragma unroll
+    for (int j = 0; j < Z::C; ++j) acc[i][j] = make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+  const int end = min(q0 + TM, p.N);
+  for (int k0 = first_key(p, b, q0) / TM * TM; k0 < end; k0 += TM) {
+    __syncthreads();
+    load_tile<T, TM, DM>(k_s, p.k, b * p.k_sb + hkv * p.k_sh, p.k_sn, k0, p.N, p.Dk);
+    load_tile<T, TM, DM>(v_s, p.v, b * p.v_sb + hkv * p.v_sh, p.v_sn, k0, p.N, p.Dv);
+    __syncthreads();
+    float s[Z::R][Z::R], d[Z::R][Z::R];
+    dot_tile<TM, DM>(q_s, k_s, p.Dk, s);
+    dot_tile<TM, DM>(g_s, v_s, p.Dv, d);
+#pragma unroll
+    for (int i = 0; i < Z::R; ++i)
+#pragma unroll
+      for (int j = 0; j < Z::R; ++j) {
+        float pr, dx;
+        grad_of(p, st[i], k0 + tx + 16 * j, s[i][j], d[i][j], &pr, &dx);
+        x_s[(ty + 16 * i) * Z::PS + tx + 16 * j] = dx;
+      }
+    __syncthreads();
+    mul_tile<TM, DM>(x_s, k_s, acc);
+  }
+  store_rows<T, TM, DM>(static_cast<T*>(p.dq) + ((int64_t)b * p.N * p.Hq + hq) * p.Dk, (int64_t)p.Hq * p.Dk, q0, p.N,
+                        p.Dk, p.scale, acc);
+}
+
+// dK, dV of TM keys of one key head: the queries that see them, head by head of
+// the group, in order (no atomics: the sum's order is fixed).
+template <typename T, int TM, int DM>
+__global__ void __launch_bounds__(NT) dkv_cores(CausalParams p) {
+  using Z = Tile<TM, DM>;
+  extern __shared__ __align__(16) float sm[];
+  float* k_s = sm;
+  float* v_s = k_s + TM * Z::RS;
+  float* q_s = v_s + TM * Z::RS;
+  float* g_s = q_s + TM * Z::RS;
+  float* p_s = g_s + TM * Z::RS;
+  float* x_s = p_s + TM * Z::PS;
+  __shared__ RowStat st_s[TM];
+  const int k0 = blockIdx.x * TM, hkv = blockIdx.y, b = blockIdx.z;
+  const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
+  load_tile<T, TM, DM>(k_s, p.k, b * p.k_sb + hkv * p.k_sh, p.k_sn, k0, p.N, p.Dk);
+  load_tile<T, TM, DM>(v_s, p.v, b * p.v_sb + hkv * p.v_sh, p.v_sn, k0, p.N, p.Dv);
+  float4 dk[Z::R][Z::C], dv[Z::R][Z::C];
+#pragma unroll
+  for (int i = 0; i < Z::R; ++i)
+#pragma unroll
+    for (int j = 0; j < Z::C; ++j) dk[i][j] = dv[i][j] = make_float4(0.f, 0.f, 0.f, 0.f);
+  const int end = query_end(p, b, min(k0 + TM, p.N) - 1);
+  for (int e = 0; e < p.E; ++e) {
+    const int hq = hkv * p.E + e;
+    for (int q0 = k0; q0 < end; q0 += TM) {
+      __syncthreads();
+      load_tile<T, TM, DM>(q_s, p.q, b * p.q_sb + hq * p.q_sh, p.q_sn, q0, p.N, p.Dk);
+      load_tile<T, TM, DM>(g_s, p.dout, ((int64_t)b * p.N * p.Hq + hq) * p.Dv, (int64_t)p.Hq * p.Dv, q0, p.N, p.Dv);
+      if (threadIdx.x < TM) st_s[threadIdx.x] = row_stat(p, b, hq, q0 + threadIdx.x);
+      __syncthreads();
+      float s[Z::R][Z::R], d[Z::R][Z::R];
+      dot_tile<TM, DM>(k_s, q_s, p.Dk, s);
+      dot_tile<TM, DM>(v_s, g_s, p.Dv, d);
+#pragma unroll
+      for (int i = 0; i < Z::R; ++i)
+#pragma unroll
+        for (int j = 0; j < Z::R; ++j) {
+          float pr, dx;
+          grad_of(p, st_s[tx + 16 * j], k0 + ty + 16 * i, s[i][j], d[i][j], &pr, &dx);
+          p_s[(ty + 16 * i) * Z::PS + tx + 16 * j] = pr;
+          x_s[(ty + 16 * i) * Z::PS + tx + 16 * j] = dx;
+        }
+      __syncthreads();
+      mul_tile<TM, DM>(p_s, g_s, dv);
+      mul_tile<TM, DM>(x_s, q_s, dk);
+    }
+  }
+  store_rows<T, TM, DM>(static_cast<T*>(p.dk) + ((int64_t)b * p.N * p.Hkv + hkv) * p.Dk, (int64_t)p.Hkv * p.Dk, k0, p.N,
+                        p.Dk, p.scale, dk);
+  store_rows<T, TM, DM>(static_cast<T*>(p.dv) + ((int64_t)b * p.N * p.Hkv + hkv) * p.Dv, (int64_t)p.Hkv * p.Dv, k0, p.N,
+                        p.Dv, 1.f, dv);
+}
+
+template <typename K>
+int launch_cores(K kernel, dim3 grid, size_t smem, const CausalParams& p, cudaStream_t st) {
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
+    return TC_ERR_CUDA;
+  kernel<<<grid, NT, smem, st>>>(p);
+  return launch_status();
+}
+
+template <typename T, int TM, int DM>
+int fwd_cores_launch(const CausalParams& p, cudaStream_t st) {
+  using Z = Tile<TM, DM>;
+  const size_t smem = sizeof(float) * (2 * TM * Z::RS + TM * Z::PS);
+  return launch_cores(fwd_cores<T, TM, DM>, dim3((p.N + TM - 1) / TM, p.Hq, p.B), smem, p, st);
+}
+template <typename T, int TM, int DM>
+int bwd_cores_launch(const CausalParams& p, cudaStream_t st) {
+  using Z = Tile<TM, DM>;
+  const size_t sa = sizeof(float) * (4 * TM * Z::RS + TM * Z::PS), sb = sa + sizeof(float) * TM * Z::PS;
+  if (int rc = launch_cores(dq_cores<T, TM, DM>, dim3((p.N + TM - 1) / TM, p.Hq, p.B), sa, p, st)) return rc;
+  return launch_cores(dkv_cores<T, TM, DM>, dim3((p.N + TM - 1) / TM, p.Hkv, p.B), sb, p, st);
+}
+
+// 64 x 64 tiles while the operands of a head dim fit the shared memory.
+template <typename T>
+int fwd_cores_any(const CausalParams& p, cudaStream_t st) {
+  const int D = imax(p.Dk, p.Dv);
+  if (D <= 64) return fwd_cores_launch<T, 64, 64>(p, st);
+  if (D <= 128) return fwd_cores_launch<T, 64, 128>(p, st);
+  return fwd_cores_launch<T, 32, 256>(p, st);
+}
+template <typename T>
+int bwd_cores_any(const CausalParams& p, cudaStream_t st) {
+  const int D = imax(p.Dk, p.Dv);
+  if (D <= 64) return bwd_cores_launch<T, 64, 64>(p, st);
+  if (D <= 128) return bwd_cores_launch<T, 64, 128>(p, st);
+  return bwd_cores_launch<T, 32, 256>(p, st);
+}
+
+int make_params(const tc_causal_args* a, CausalParams* p) {
+  if (!a || a->B < 0 || a->N < 0 || a->Hq <= 0 || a->Hkv <= 0 || a->Hq % a->Hkv || a->Dk <= 0 || a->Dv <= 0)
+    return TC_ERR_ARG;
+  if ((a->starts == nullptr) != (a->ends == nullptr)) return TC_ERR_ARG;
+  if (a->dtype != TC_F32 && a->dtype != TC_BF16 && a->dtype != TC_F16) return TC_ERR_ARG;
+  if (a->impl < 0 || a->impl > 2 || (a->has_softcap && !(a->softcap > 0.f))) return TC_ERR_ARG;
+  if (a->B > 65535 || a->Hq > 65535) return TC_ERR_UNSUPPORTED;
+  p->B = a->B, p->N = a->N, p->Hq = a->Hq, p->Hkv = a->Hkv, p->E = a->Hq / a->Hkv, p->Dk = a->Dk, p->Dv = a->Dv;
+  p->scale = a->scale, p->cap = a->has_softcap ? a->softcap : 1.f, p->has_cap = a->has_softcap != 0;
+  p->q = a->q, p->k = a->k, p->v = a->v;
+  p->q_sb = a->q_stride_b, p->q_sn = a->q_stride_n, p->q_sh = a->q_stride_h;
+  p->k_sb = a->k_stride_b, p->k_sn = a->k_stride_n, p->k_sh = a->k_stride_h;
+  p->v_sb = a->v_stride_b, p->v_sn = a->v_stride_n, p->v_sh = a->v_stride_h;
+  p->starts = a->starts, p->ends = a->ends;
+  p->out = a->out, p->lse = a->lse;
+  p->o = a->o, p->dout = a->dout, p->dlse = a->dlse, p->delta = a->delta;
+  p->dq = a->dq, p->dk = a->dk, p->dv = a->dv;
+  p->status = a->dev_status;
+  return TC_OK;
+}
+
+}  // namespace
+
+namespace tc {
+int causal_delta(const CausalParams& p, int dtype, cudaStream_t st) {
+  const int64_t rows = (int64_t)p.B * p.N * p.Hq, grid = (rows + 7) / 8;
+  if (grid > INT32_MAX) return TC_ERR_UNSUPPORTED;
+  TC_DISPATCH(dtype, T, delta_rows<T><<<(unsigned)grid, 256, 0, st>>>(p, rows));
+  return launch_status();
+}
+}  // namespace tc
+
+extern "C" int tc_segment_bounds(int32_t B, int32_t N, const int32_t* seq_idx, int32_t* starts, int32_t* ends,
+                                 void* stream) {
+  if (B < 0 || N < 0) return TC_ERR_ARG;
+  if ((int64_t)B * N == 0) return TC_OK;
+  if (!seq_idx || !starts || !ends) return TC_ERR_ARG;
+  bounds_kernel<<<B, kBoundThreads, 0, (cudaStream_t)stream>>>(N, seq_idx, starts, ends);
+  return launch_status();
+}
+
+extern "C" int tc_causal_fwd(const tc_causal_args* a, void* stream) {
+  CausalParams p;
+  if (int rc = make_params(a, &p)) return rc;
+  if ((int64_t)a->B * a->N == 0) return TC_OK;
+  if (!a->q || !a->k || !a->v || !a->out || !a->lse) return TC_ERR_ARG;
+  cudaStream_t st = (cudaStream_t)stream;
+  const bool tensor = a->impl != 1 && causal_tc_supported(p, a->dtype);
+  if (tensor) return causal_fwd_tc(p, a->dtype, st);
+  if (a->impl == 2 || p.Dk > 256 || p.Dv > 256) return TC_ERR_UNSUPPORTED;
+  TC_DISPATCH(a->dtype, T, return fwd_cores_any<T>(p, st));
+}
+
+extern "C" int tc_causal_bwd(const tc_causal_args* a, void* stream) {
+  CausalParams p;
+  if (int rc = make_params(a, &p)) return rc;
+  if ((int64_t)a->B * a->N == 0) return TC_OK;
+  if (!a->q || !a->k || !a->v || !a->o || !a->dout || !a->lse || !a->delta || !a->dq || !a->dk || !a->dv)
+    return TC_ERR_ARG;
+  cudaStream_t st = (cudaStream_t)stream;
+  const bool tensor = a->impl != 1 && causal_bwd_tc_supported(p, a->dtype);
+  if (!tensor && (a->impl == 2 || p.Dk > 256 || p.Dv > 256)) return TC_ERR_UNSUPPORTED;
+  if (int rc = causal_delta(p, a->dtype, st)) return rc;
+  if (tensor) return causal_bwd_tc(p, a->dtype, st);
+  TC_DISPATCH(a->dtype, T, return bwd_cores_any<T>(p, st));
+}

@@ -1,0 +1,999 @@
+// 8-bit key / value cache: quantising rows as they are written, reading them
+// back, and single-token attention over the codes (sm_100a).
+//
+// A row (one token's key or value of one head) is kept as D codes and one fp32
+// scale:  scale = amax / top,  code = round(x (top / amax)),  with top 127 and
+// the code + 128 in a byte (TC_KV_INT8), or top 448 and an e4m3 float
+// (TC_KV_FP8).  Quotients and products are the rounded IEEE ones, so the codes
+// of a value do not depend on which kernel wrote it.  Rows with amax < 1e-30
+// are zeros; a row with a NaN or an infinity reads back as NaN.
+//
+// Layout [rows, Hkv, capacity, D]: a head's tokens are consecutive, so a split
+// of a sequence streams one contiguous range of codes.
+#include <cuda_fp8.h>
+#include <float.h>
+
+#include <type_traits>
+
+#include "common.cuh"
+#include "rotary.cuh"
+
+using namespace tc;
+
+namespace {
+
+constexpr float kTiny = 1e-30f;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+
+template <int STORE> struct Codec;
+template <> struct Codec<TC_KV_INT8> {
+  static constexpr float kTop = 127.f;
+  static __device__ __forceinline__ uint32_t code(float y) {
+    return (uint32_t)(min(max(__float2int_rn(y), -127), 127) + 128);
+  }
+  static __device__ __forceinline__ float value(uint32_t c) { return (float)((int)c - 128); }
+  // bytes 0, 1 (hi: 2, 3) of x as two f16 values: 0x6400 | u is 1024 + u exactly
+  template <bool HI> static __device__ __forceinline__ uint32_t pair(uint32_t x) {
+    const uint32_t r = __byte_perm(x, 0x64646464u, HI ? 0x4342 : 0x4140);
+    const __half2 v = __hsub2(*reinterpret_cast<const __half2*>(&r), __half2half2(__ushort_as_half(0x6480)));
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
+};
+template <> struct Codec<TC_KV_FP8> {
+  static constexpr float kTop = 448.f;
+  static __device__ __forceinline__ uint32_t code(float y) {
+    return __nv_cvt_float_to_fp8(y, __NV_SATFINITE, __NV_E4M3);
+  }
+  static __device__ __forceinline__ float value(uint32_t c) {
+    return __half2float(__half(__nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)c, __NV_E4M3)));
+  }
+  template <bool HI> static __device__ __forceinline__ uint32_t pair(uint32_t x) {
+    const __half2_raw v = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(HI ? x >> 16 : x & 0xffffu), __NV_E4M3);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
+};
+
+// scale and top / amax of a row from its amax (NaN and infinity kept).
+template <int STORE>
+__device__ __forceinline__ void row_scale(float amax, float* scale, float* inv) {
+  const bool tiny = amax < kTiny;
+  *scale = tiny ? 0.f : __fdiv_rn(amax, Codec<STORE>::kTop);
+  *inv = tiny ? 0.f : __fdiv_rn(Codec<STORE>::kTop, amax);
+}
+
+// |x| as bits: ordered as the floats are, with every NaN above infinity.
+__device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+
+// The value of a code: infinite or NaN only where the scale is (127 times a
+// scale that was rounded up may pass the largest float).
+template <int STORE>
+__device__ __forceinline__ float dequant(uint32_t c, float scale) {
+  const float v = Codec<STORE>::value(c) * scale;
+  return scale <= FLT_MAX ? fminf(fmaxf(v, -FLT_MAX), FLT_MAX) : v;
+}
+
+// ---------------------------------------------------------------------------
+// write
+// ---------------------------------------------------------------------------
+struct WriteParams {
+  int B, N, H, D, rows, fresh;
+  int64_t cap;
+  const void* src[2];  // k, v
+  int64_t sb[2], sn[2], sh[2];
+  uint8_t* codes[2];
+  float* scales[2];
+  int dim[2];
+  int32_t* lengths;
+  const int32_t* seq;     // [B, N] or null: token (b, n) belongs to cache row b
+  const int32_t* starts;  // [B, N] first token of each run of equal ids (with seq)
+  int32_t* status;
+};
+
+// Cache row and slot of token (b, n); row -1 where it is not written.
+__device__ __forceinline__ void place(const WriteParams& p, int b, int n, int* row, int64_t* slot) {
+  int r = b, first = 0;
+  if (p.seq) {
+    r = p.seq[(int64_t)b * p.N + n];
+    first = p.starts[(int64_t)b * p.N + n];
+  }
+  *row = -1;
+  if (r < 0) return;
+  if (r >= p.rows) {
+    if (p.status) atomicOr(p.status, TC_DEV_BAD_INDEX);
+    return;
+  }
+  const int64_t s = (int64_t)(p.fresh ? 0 : p.lengths[r]) + (n - first);
+  if (s < 0 || s >= p.cap) {
+    if (p.status) atomicOr(p.status, TC_DEV_BAD_INDEX);
+    return;
+  }
+  *row = r;
+  *slot = s;
+}
+
+// A row's new length is set where its run ends; with fresh nothing else reads
+// the lengths, so the write kernel does it, otherwise a kernel behind it.
+__device__ __forceinline__ void advance_row(const WriteParams& p, int b, int n) {
+  int r = b, first = 0;
+  if (p.seq) {
+    const int64_t i = (int64_t)b * p.N + n;
+    r = p.seq[i];
+    if (r < 0 || r >= p.rows || (n + 1 < p.N && p.seq[i + 1] == r)) return;
+    first = p.starts[i];
+  } else if (n + 1 < p.N) {
+    return;
+  }
+  const int64_t len = (int64_t)(p.fresh ? 0 : p.lengths[r]) + (n + 1 - first);
+  p.lengths[r] = (int32_t)(len < p.cap ? len : p.cap);
+}
+
+__global__ void __launch_bounds__(256) advance_kernel(WriteParams p) {
+  const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+  if (i < (int64_t)p.B * p.N) advance_row(p, (int)(i / p.N), (int)(i % p.N));
+}
+
+// LANES lanes per row, 16 bytes each; blockIdx.y: 0 keys, 1 values.  Bound by
+// HBM: the row is read once, its maximum goes round the lanes by shuffles, and
+// the codes leave as 8-byte (fp32: 4-byte) pieces of whole 32-byte sectors.
+// kTok consecutive tokens of one head per lane group keep as many loads in
+// flight.
+constexpr int kTok = 4;
+template <typename T, int STORE, int LANES>
+__global__ void __launch_bounds__(256) write_vec(WriteParams p) {
+  constexpr int VE = 16 / sizeof(T);
+  const int which = blockIdx.y;
+  const int lane = threadIdx.x % LANES;
+  const int64_t group = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) / LANES;
+  const int tiles = (p.N + kTok - 1) / kTok;
+  const int h = (int)(group % p.H);
+  const int64_t bt = group / p.H;
+  if (bt >= (int64_t)p.B * tiles) return;  // whole lane groups leave; the shuffles below name their own lanes
+  const int b = (int)(bt / tiles), n0 = (int)(bt % tiles) * kTok;
+  const uint32_t mask = LANES == 32 ? 0xffffffffu : ((1u << LANES) - 1u) << ((threadIdx.x & 31) / LANES * LANES);
+  const T* src = static_cast<const T*>(p.src[which]) + b * p.sb[which] + h * p.sh[which] + lane * VE;
+  uint4 raw[kTok];
+#pragma unroll
+  for (int j = 0; j < kTok; ++j)
+    if (n0 + j < p.N) raw[j] = *reinterpret_cast<const uint4*>(src + (int64_t)(n0 + j) * p.sn[which]);
+#pragma unroll
+  for (int j = 0; j < kTok; ++j) {
+    const int n = n0 + j;
+    if (n >= p.N) break;
+    int row;
+    int64_t slot = 0;
+    place(p, b, n, &row, &slot);
+    if (p.fresh && which == 0 && h == 0 && lane == 0) advance_row(p, b, n);
+    if (row < 0) continue;
+    const T* e = reinterpret_cast<const T*>(&raw[j]);
+    float x[VE];
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < VE; ++i) {
+      x[i] = to_f(e[i]);
+      m = max(m, abs_bits(x[i]));
+    }
+#pragma unroll
+    for (int o = LANES / 2; o; o >>= 1) m = max(m, __shfl_xor_sync(mask, m, o));
+    float scale, inv;
+    row_scale<STORE>(__uint_as_float(m), &scale, &inv);
+    uint32_t w[VE / 4];
+#pragma unroll
+    for (int i = 0; i < VE / 4; ++i) {
+      w[i] = 0;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) w[i] |= Codec<STORE>::code(__fmul_rn(x[4 * i + k], inv)) << (8 * k);
+    }
+    const int64_t at = ((int64_t)row * p.H + h) * p.cap + slot;
+    uint8_t* dst = p.codes[which] + at * p.dim[which] + lane * VE;
+    if constexpr (VE == 8) *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);
+    else *reinterpret_cast<uint32_t*>(dst) = w[0];
+    if (lane == 0) p.scales[which][at] = scale;
+  }
+}
+
+// Any head dim and strides: a warp per row, two passes over it.
+template <typename T, int STORE>
+__global__ void __launch_bounds__(256) write_any(WriteParams p) {
+  const int which = blockIdx.y, lane = threadIdx.x & 31;
+  const int64_t i = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
+  const int h = (int)(i % p.H);
+  const int64_t tok = i / p.H;
+  if (tok >= (int64_t)p.B * p.N) return;
+  const int b = (int)(tok / p.N), n = (int)(tok % p.N);
+  int row;
+  int64_t slot = 0;
+  place(p, b, n, &row, &slot);
+  if (p.fresh && which == 0 && h == 0 && lane == 0) advance_row(p, b, n);
+  if (row < 0) return;
+  const T* src = static_cast<const T*>(p.src[which]) + b * p.sb[which] + (int64_t)n * p.sn[which] + h * p.sh[which];
+  const int D = p.dim[which];
+  uint32_t m = 0;
+  for (int d = lane; d < D; d += 32) m = max(m, abs_bits(to_f(src[d])));
+#pragma unroll
+  for (int o = 16; o; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+  float scale, inv;
+  row_scale<STORE>(__uint_as_float(m), &scale, &inv);
+  const int64_t at = ((int64_t)row * p.H + h) * p.cap + slot;
+  for (int d = lane; d < D; d += 32) p.codes[which][at * D + d] = (uint8_t)Codec<STORE>::code(__fmul_rn(to_f(src[d]), inv));
+  if (lane == 0) p.scales[which][at] = scale;
+}
+
+template <typename T, int STORE>
+int launch_write(const WriteParams& p, cudaStream_t st) {
+  constexpr int VE = 16 / sizeof(T);
+  bool vec = p.dim[0] == p.dim[1];
+  for (int w = 0; w < 2; ++w) {
+    vec = vec && (uintptr_t)p.src[w] % 16 == 0 && p.sb[w] % VE == 0 && p.sn[w] % VE == 0 && p.sh[w] % VE == 0 &&
+          (uintptr_t)p.codes[w] % 8 == 0;
+  }
+  const int lanes = p.dim[0] / VE;
+  vec = vec && p.dim[0] % VE == 0 && (lanes == 8 || lanes == 16 || lanes == 32);
+  const int64_t units = vec ? (int64_t)p.B * ((p.N + kTok - 1) / kTok) * p.H * lanes : (int64_t)p.B * p.N * p.H * 32;
+  const int64_t grid = (units + 255) / 256;
+  if (grid > INT32_MAX) return TC_ERR_UNSUPPORTED;
+  const dim3 g((unsigned)grid, 2);
+  if (!vec) write_any<T, STORE><<<g, 256, 0, st>>>(p);
+  else if (lanes == 8) write_vec<T, STORE, 8><<<g, 256, 0, st>>>(p);
+  else if (lanes == 16) write_vec<T, STORE, 16><<<g, 256, 0, st>>>(p);
+  else write_vec<T, STORE, 32><<<g, 256, 0, st>>>(p);
+  if (int rc = launch_status()) return rc;
+  if (!p.fresh) {
+    advance_kernel<<<(unsigned)(((int64_t)p.B * p.N + 255) / 256), 256, 0, st>>>(p);
+    return launch_status();
+  }
+  return TC_OK;
+}
+
+// ---------------------------------------------------------------------------
+// read back
+// ---------------------------------------------------------------------------
+struct ReadParams {
+  int rows, H, L;
+  int64_t cap;
+  const uint8_t* codes[2];
+  const float* scales[2];
+  int dim[2];
+  const int32_t* lengths;
+  void* out[2];  // [rows, L, H, D]
+};
+
+// A thread per V codes of one row (V = 16 / element size, or 1), heads fastest
+// in the output; slots past a row's length are zeros and read nothing.
+template <typename T, int STORE, int V>
+__global__ void __launch_bounds__(256) read_kernel(ReadParams p) {
+  const int which = blockIdx.y, D = p.dim[which], per = D / V;
+  const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+  if (i >= (int64_t)p.rows * p.L * p.H * per) return;
+  const int d = (int)(i % per) * V;
+  const int64_t rh = i / per;
+  const int h = (int)(rh % p.H);
+  const int64_t bt = rh / p.H;
+  const int n = (int)(bt % p.L), b = (int)(bt / p.L);
+  T* out = static_cast<T*>(p.out[which]) + rh * D + d;
+  float v[V];
+  if (n < p.lengths[b] && n < p.cap) {
+    const int64_t at = ((int64_t)b * p.H + h) * p.cap + n;
+    const float s = p.scales[which][at];
+    const uint8_t* c = p.codes[which] + at * D + d;
+    if constexpr (V == 8) {
+      const uint2 w = *reinterpret_cast<const uint2*>(c);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = dequant<STORE>(((k < 4 ? w.x : w.y) >> (8 * (k & 3))) & 255u, s);
+    } else if constexpr (V == 4) {
+      const uint32_t w = *reinterpret_cast<const uint32_t*>(c);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) v[k] = dequant<STORE>((w >> (8 * k)) & 255u, s);
+    } else {
+      v[0] = dequant<STORE>(c[0], s);
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < V; ++k) v[k] = 0.f;
+  }
+  if constexpr (V == 1) {
+    out[0] = from_f<T>(v[0]);
+  } else {
+    uint4 w;
+    T* e = reinterpret_cast<T*>(&w);
+#pragma unroll
+    for (int k = 0; k < V; ++k) e[k] = from_f<T>(v[k]);
+    *reinterpret_cast<uint4*>(out) = w;
+  }
+}
+
+template <typename T, int STORE>
+int launch_read(const ReadParams& p, cudaStream_t st) {
+  constexpr int V = 16 / sizeof(T);
+  bool vec = true;
+  for (int w = 0; w < 2; ++w)
+    vec = vec && p.dim[w] % V == 0 && (uintptr_t)p.codes[w] % V == 0 && (uintptr_t)p.out[w] % 16 == 0;
+  const int D = p.dim[0] > p.dim[1] ? p.dim[0] : p.dim[1];
+  const int64_t units = (int64_t)p.rows * p.L * p.H * (vec ? D / V : D);
+  const int64_t grid = (units + 255) / 256;
+  if (grid > INT32_MAX) return TC_ERR_UNSUPPORTED;
+  if (vec) read_kernel<T, STORE, V><<<dim3((unsigned)grid, 2), 256, 0, st>>>(p);
+  else read_kernel<T, STORE, 1><<<dim3((unsigned)grid, 2), 256, 0, st>>>(p);
+  return launch_status();
+}
+
+// ---------------------------------------------------------------------------
+// single-token attention over the codes
+// ---------------------------------------------------------------------------
+struct AttendParams {
+  int B, Hq, Hkv, E, groups;   // groups: eights of query heads per key head
+  int Dk, Dv;
+  int64_t cap;
+  uint8_t* k;
+  uint8_t* v;
+  float* ks;
+  float* vs;
+  int32_t* lengths;
+  const void* q;
+  int64_t q_sb, q_sh;
+  const void* k_t;             // step: the new token's key and value
+  const void* v_t;
+  int64_t k_sb, k_sh, v_sb, v_sh;
+  const float* cos_t;          // step: [n_pos, R / 2] or null
+  const float* sin_t;
+  int R, interleaved, n_pos;
+  float qscale, softcap;       // logit = qscale q.k (1 / sqrt(Dk) unless given)
+  int has_cap, advance;
+  void* out;                   // [B, Hq, Dv]
+  float* lse;                  // [B, Hq]
+  void* k_new;                 // step: the values as stored, [B, Hkv, D], or null
+  void* v_new;
+  int new_dtype;
+  int chunk, splits;           // tokens per CTA, CTAs per (sequence, head group)
+  float* part;                 // [B * Hkv * groups * splits][8][Dv + 2]
+  int32_t* done;               // [B * Hkv * groups + B] arrival counts, zero between calls
+  int32_t* status;
+};
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ void mma16816(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t pack_h2(float a, float b) {
+  const __half2 v = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ float2 unpack_h2(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
+
+__device__ __forceinline__ float warp_max(float x) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
+  return x;
+}
+__device__ __forceinline__ float warp_sum(float x) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+  return x;
+}
+
+// Dims of pair u of a D-dim head whose first R dims rotate: the rotary pair for
+// u < R / 2, else two neighbours behind them (an odd last dim pairs with itself).
+__device__ __forceinline__ void pair_dims(int u, int R, int interleaved, int D, int* i1, int* i2) {
+  const int half = R / 2;
+  if (u < half) {
+    *i1 = interleaved ? 2 * u : u;
+    *i2 = interleaved ? 2 * u + 1 : u + half;
+  } else {
+    *i1 = R + 2 * (u - half);
+    *i2 = *i1 + 1 < D ? *i1 + 1 : *i1;
+  }
+}
+
+// Pair u of a head's row x, rotated to position pos where the step has tables.
+template <typename T>
+__device__ __forceinline__ void load_pair(const AttendParams& p, const T* x, int u, int D, int R, int pos, int* i1,
+                                          int* i2, float* y1, float* y2) {
+  pair_dims(u, R, p.interleaved, D, i1, i2);
+  const float x1 = to_f(x[*i1]), x2 = to_f(x[*i2]);
+  *y1 = x1;
+  *y2 = x2;
+  if (u < R / 2) {
+    float c = NAN, s = NAN;
+    if (pos < p.n_pos) {
+      c = p.cos_t[(int64_t)pos * (R / 2) + u];
+      s = p.sin_t[(int64_t)pos * (R / 2) + u];
+    }
+    rotate_pair(x1, x2, c, s, y1, y2);
+  }
+}
+
+// One warp quantises the new token's row into slot `pos` of its head.
+template <typename T, int STORE>
+__device__ void write_token(const AttendParams& p, const T* x, int D, int R, int pos, int64_t head, uint8_t* codes,
+                            float* scales, void* stored) {
+  const int lane = threadIdx.x & 31, pairs = (D + 1) / 2;
+  uint32_t m = 0;
+  for (int u = lane; u < pairs; u += 32) {
+    int i1, i2;
+    float y1, y2;
+    load_pair(p, x, u, D, R, pos, &i1, &i2, &y1, &y2);
+    m = max(m, max(abs_bits(y1), abs_bits(y2)));
+  }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+  float scale, inv;
+  row_scale<STORE>(__uint_as_float(m), &scale, &inv);
+  const int64_t at = head * p.cap + pos;
+  for (int u = lane; u < pairs; u += 32) {
+    int i1, i2;
+    float y1, y2;
+    load_pair(p, x, u, D, R, pos, &i1, &i2, &y1, &y2);
+    const uint32_t c1 = Codec<STORE>::code(__fmul_rn(y1, inv)), c2 = Codec<STORE>::code(__fmul_rn(y2, inv));
+    codes[at * D + i1] = (uint8_t)c1;
+    codes[at * D + i2] = (uint8_t)c2;
+    if (stored) {
+      store_any(stored, head * D + i1, p.new_dtype, dequant<STORE>(c1, scale));
+      store_any(stored, head * D + i2, p.new_dtype, dequant<STORE>(c2, scale));
+    }
+  }
+  if (lane == 0) scales[at] = scale;
+}
+
+// Joins the partial (m, l, O) of `active` splits of nE heads and writes out, lse.
+template <typename TQ>
+__device__ void join_splits(const AttendParams& p, int b, int hkv, int e0, int nE, int64_t slot0, int active) {
+  const int D = p.Dv, stride = D + 2;
+  for (int i = threadIdx.x; i < nE * D; i += blockDim.x) {
+    const int e = i / D, d = i - e * D;
+    const float* base = p.part + (slot0 * 8 + e) * stride;
+    float M = -INFINITY;
+    for (int s = 0; s < active; ++s) M = fmaxf(M, __ldcg(base + (int64_t)s * 8 * stride));
+    float l = 0.f, o = 0.f;
+    if (M > -INFINITY) {
+#pragma unroll 4
+      for (int s = 0; s < active; ++s) {
+        const float* q = base + (int64_t)s * 8 * stride;
+        const float w = ex2(__ldcg(q) - M);
+        l += w * __ldcg(q + 1);
+        o += w * __ldcg(q + 2 + d);
+      }
+    }
+    const int64_t head = (int64_t)b * p.Hq + hkv * p.E + e0 + e;
+    static_cast<TQ*>(p.out)[head * D + d] = from_f<TQ>(l != 0.f ? o / l : 0.f);
+    if (d == 0) p.lse[head] = l != 0.f ? (M + log2f(l)) * kLn2 : -INFINITY;
+  }
+}
+
+// Every CTA's last act, behind its global writes: the last split of a (sequence,
+// head group) to arrive joins the partials, and the last head group of a
+// sequence moves its length on.  With `advance` the splits without tokens of
+// their own arrive too: each CTA must have read the old length before it moves.
+// The counts return to zero.
+template <typename TQ>
+__device__ void close_split(const AttendParams& p, int b, int hg, int e0, int nE, int64_t slot0, int active, int pos,
+                            int* flag) {
+  const int total = p.advance ? p.splits : active, per = p.Hkv * p.groups;
+  if (total > 1) {
+    __threadfence();
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      int32_t* d = p.done + (int64_t)b * per + hg;
+      const bool last = atomicAdd(d, 1) == total - 1;
+      if (last) *d = 0;
+      *flag = last;
+    }
+    __syncthreads();
+    if (!*flag) return;
+    __threadfence();
+    if (active > 1) join_splits<TQ>(p, b, hg / p.groups, e0, nE, slot0, active);
+  }
+  if (p.advance && threadIdx.x == 0) {
+    int32_t* d = p.done + (int64_t)p.B * per + b;
+    if (atomicAdd(d, 1) == per - 1) {
+      *d = 0;
+      p.lengths[b] = (int32_t)min((int64_t)pos + 1, p.cap);
+    }
+  }
+}
+
+// Tensor-core path, Dk = Dv = D (64 or 128).  CTA = one chunk of one sequence
+// and up to eight query heads of one key head; four warps, sixteen tokens a
+// warp and step, m16n8k16 f16 products with fp32 accumulators:
+//   S[head, token] = q K^T:  A = q, rows 0-7 the f16 roundings of the heads'
+//     q and rows 8-15 what the roundings left over, so S = row h + row h + 8
+//     has q to 22 bits; B = codes, exact in f16.
+//   O[head, dim] += P V:     A = P, split in two the same way, with the value
+//     rows' scales folded into it (relative to their largest so far, times 2^14:
+//     the f16 leftovers of a weight 2^-k keep 22 - max(0, k - 17) bits).
+// A dot product does not care about the order of its terms, so a lane loads 16
+// consecutive codes of a token (64 or 128 bytes of a row per four lanes) and
+// the A operand follows that order; likewise output dims follow the value
+// loads.  P leaves S's accumulator layout as the A operand without a shuffle.
+// Codes go from global memory straight to registers, one step ahead.
+constexpr int kAtThreads = 128;
+constexpr float kUp = 16384.f;
+template <typename TQ, int STORE, int D, bool CAP, bool STEP>
+__global__ void __launch_bounds__(kAtThreads, 3) attend_mma(AttendParams p) {
+  constexpr int KS = D / 16;        // k steps of S
+  constexpr int NC = D / 64;        // 16-byte key chunks per lane and token
+  constexpr int ND = D / 8;         // n tiles of O
+  constexpr int VB = D / 8;         // value codes per lane and token
+  constexpr int QS = D + 8;         // q row stride in shared memory (halves)
+  constexpr int OS = D + D / 32 * 4;  // O row stride (floats)
+  __shared__ __align__(16) union {
+    __half q[16 * QS];
+    float o[4 * 8 * OS];
+  } sm;
+  __shared__ float qf_s[8], m_s[4][8], l_s[4][8];
+  __shared__ int flag;
+
+  const int split = blockIdx.x;
+  const int hg = blockIdx.y, b = blockIdx.z;
+  const int hkv = hg / p.groups, e0 = (hg - hkv * p.groups) * 8;
+  const int nE = min(8, p.E - e0);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int pos = p.lengths[b];
+  const int ntok = (int)min((int64_t)(STEP ? pos + 1 : pos), p.cap);
+  const int active = max(1, min(p.splits, (ntok + p.chunk - 1) / p.chunk));
+  const int64_t slot0 = ((int64_t)b * p.Hkv * p.groups + hg) * p.splits;
+  if (split >= active) {
+    if (p.advance) close_split<TQ>(p, b, hg, e0, nE, slot0, active, pos, &flag);
+    return;
+  }
+  const int c0 = split * p.chunk, c1 = split == active - 1 ? ntok : c0 + p.chunk;
+  const int64_t head = (int64_t)b * p.Hkv + hkv;
+
+  // q: rotate, bring each head's largest element to [2^13, 2^14), split in two
+  for (int e = warp; e < 8; e += 4) {
+    const TQ* x = static_cast<const TQ*>(p.q) + b * p.q_sb + (int64_t)(hkv * p.E + e0 + e) * p.q_sh;
+    float y1[D / 64], y2[D / 64];
+    int i1[D / 64], i2[D / 64];
+    uint32_t m = 0;
+#pragma unroll
+    for (int j = 0; j < D / 64; ++j) {
+      const int u = lane + 32 * j;
+      y1[j] = y2[j] = 0.f;
+      if (e < nE) load_pair(p, x, u, D, STEP ? p.R : 0, pos, &i1[j], &i2[j], &y1[j], &y2[j]);
+      else pair_dims(u, STEP ? p.R : 0, p.interleaved, D, &i1[j], &i2[j]);
+      m = max(m, max(abs_bits(y1[j]), abs_bits(y2[j])));
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+    const int ex = min(max((int)(m >> 23) - 127, -100), 126);
+    const float up = m ? __int_as_float((127 + 13 - ex) << 23) : 1.f;
+    const float down = m ? __int_as_float((127 - 13 + ex) << 23) : 1.f;
+#pragma unroll
+    for (int j = 0; j < D / 64; ++j) {
+      const float a = y1[j] * up, c = y2[j] * up;
+      const __half ah = __float2half_rn(a), ch = __float2half_rn(c);
+      sm.q[e * QS + i1[j]] = ah;
+      sm.q[e * QS + i2[j]] = ch;
+      sm.q[(e + 8) * QS + i1[j]] = __float2half_rn(a - __half2float(ah));
+      sm.q[(e + 8) * QS + i2[j]] = __float2half_rn(c - __half2float(ch));
+    }
+    if (lane == 0) qf_s[e] = down * p.qscale * (CAP ? 1.f / p.softcap : kLog2e);
+  }
+  if constexpr (STEP) {
+    // the CTA whose chunk holds the new slot writes it before it reads its chunk
+    // (head groups of one key head write the same bytes)
+    if (split == active - 1 && pos < p.cap) {
+      if (warp == 2)
+        write_token<TQ, STORE>(p, static_cast<const TQ*>(p.k_t) + b * p.k_sb + hkv * p.k_sh, D, p.R, pos, head, p.k, p.ks,
+                               p.k_new);
+      if (warp == 3)
+        write_token<TQ, STORE>(p, static_cast<const TQ*>(p.v_t) + b * p.v_sb + hkv * p.v_sh, D, 0, pos, head, p.v, p.vs,
+                               p.v_new);
+    } else if (split == active - 1 && threadIdx.x == 0 && p.status) {
+      atomicOr(p.status, TC_DEV_BAD_INDEX);
+    }
+  }
+  __syncthreads();
+
+  // A operand of S: k step 4 c + w covers, for lane t, the codes of word w of
+  // its 16-byte chunk c, dims 64 c + 16 t + 4 w + {0, 1 | 2, 3}
+  uint32_t qa[KS][4];
+#pragma unroll
+  for (int s = 0; s < KS; ++s) {
+    const int d = 64 * (s / 4) + 16 * t + 4 * (s % 4);
+    const uint2 hi = *reinterpret_cast<const uint2*>(sm.q + g * QS + d);
+    const uint2 lo = *reinterpret_cast<const uint2*>(sm.q + (g + 8) * QS + d);
+    qa[s][0] = hi.x, qa[s][1] = lo.x, qa[s][2] = hi.y, qa[s][3] = lo.y;
+  }
+  const float qf = qf_s[g];
+  const float kc = p.softcap * kLog2e;
+  __syncthreads();  // sm.o takes q's place below
+
+  const uint8_t* kb = p.k + head * p.cap * D + 16 * t;
+  const uint8_t* vb = p.v + head * p.cap * D + VB * g;
+  const float* ksb = p.ks + head * p.cap;
+  const float* vsb = p.vs + head * p.cap;
+
+  uint4 kw[2][NC];
+  uint32_t vw[4][VB / 4];
+  float ksv[4], vsv[4];
+  auto load = [&](int base) {
+#pragma unroll
+    for (int nt = 0; nt < 2; ++nt) {
+      const int tok = base + 8 * nt + g;
+#pragma unroll
+      for (int c = 0; c < NC; ++c)
+        kw[nt][c] = tok < c1 ? *reinterpret_cast<const uint4*>(kb + (int64_t)tok * D + 64 * c) : make_uint4(0, 0, 0, 0);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int tok = base + (i & 1) + 2 * t + 8 * (i >> 1);
+      const bool ok = tok < c1;
+      if constexpr (VB == 16) {
+        const uint4 w = ok ? *reinterpret_cast<const uint4*>(vb + (int64_t)tok * D) : make_uint4(0, 0, 0, 0);
+        vw[i][0] = w.x, vw[i][1] = w.y, vw[i][2] = w.z, vw[i][3] = w.w;
+      } else {
+        const uint2 w = ok ? *reinterpret_cast<const uint2*>(vb + (int64_t)tok * D) : make_uint2(0, 0);
+        vw[i][0] = w.x, vw[i][1] = w.y;
+      }
+      ksv[i] = ok ? ksb[tok] : 0.f;
+      vsv[i] = ok ? vsb[tok] : 0.f;
+    }
+  };
+
+  float o[ND][4];
+#pragma unroll
+  for (int i = 0; i < ND; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+  float m = -INFINITY, ell = 0.f, vref = kTiny;
+
+  int base = c0 + 16 * warp;
+  if (base < c1) load(base);
+  for (; base < c1; base += 64) {
+    // S of two eights of tokens
+    float sc[2][4];
+#pragma unroll
+    for (int nt = 0; nt < 2; ++nt) {
+      sc[nt][0] = sc[nt][1] = sc[nt][2] = sc[nt][3] = 0.f;
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        const uint4 q4 = kw[nt][s / 4];
+        const uint32_t w = (s % 4) == 0 ? q4.x : (s % 4) == 1 ? q4.y : (s % 4) == 2 ? q4.z : q4.w;
+        mma16816(sc[nt], qa[s], Codec<STORE>::template pair<false>(w), Codec<STORE>::template pair<true>(w));
+      }
+    }
+    float x[4], vsc[4];
+    uint32_t vcur[4][VB / 4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int tok = base + (i & 1) + 2 * t + 8 * (i >> 1);
+      float y = (sc[i >> 1][i & 1] + sc[i >> 1][2 + (i & 1)]) * (qf * ksv[i]);
+      if constexpr (CAP) y = kc * tanhf(y);  // a relative error: 1 - 2 / (e^2y + 1) is off by 3e-7 of the cap
+      x[i] = tok < c1 ? y : -INFINITY;
+      vsc[i] = vsv[i];
+#pragma unroll
+      for (int j = 0; j < VB / 4; ++j) vcur[i][j] = vw[i][j];
+    }
+    if (base + 64 < c1) load(base + 64);
+
+    float mx = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+    float vx = fmaxf(fmaxf(vsc[0], vsc[1]), fmaxf(vsc[2], vsc[3]));
+#pragma unroll
+    for (int d = 1; d <= 2; d <<= 1) {
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+      vx = fmaxf(vx, __shfl_xor_sync(0xffffffffu, vx, d));
+    }
+    const float mn = fmaxf(m, mx), vn = fmaxf(vref, vx);
+    if (__any_sync(0xffffffffu, mn > m || vn > vref)) {
+      const float cm = m == mn ? 1.f : ex2(m - mn);  // m -inf: 0
+      const float co = cm * (vref / vn);
+      ell *= cm;
+#pragma unroll
+      for (int i = 0; i < ND; ++i) o[i][0] *= co, o[i][1] *= co, o[i][2] *= co, o[i][3] *= co;
+      m = mn;
+      vref = vn;
+    }
+    const float vinv = kUp / vref;
+    const float me = m == -INFINITY ? 0.f : m;
+    float pr[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float e = ex2(x[i] - me);
+      ell += e;
+      pr[i] = e * (vsc[i] * vinv);
+    }
+    uint32_t pa[4];
+#pragma unroll
+    for (int nt = 0; nt < 2; ++nt) {
+      const uint32_t hi = pack_h2(pr[2 * nt], pr[2 * nt + 1]);
+      const float2 h2 = unpack_h2(hi);
+      pa[2 * nt] = hi;
+      pa[2 * nt + 1] = pack_h2(pr[2 * nt] - h2.x, pr[2 * nt + 1] - h2.y);
+    }
+    // O += P V: word j of the lane's four tokens holds output dims VB g + 4 j + 0..3
+#pragma unroll
+    for (int j = 0; j < VB / 4; ++j) {
+      const uint32_t a0 = __byte_perm(vcur[0][j], vcur[1][j], 0x5140), a1 = __byte_perm(vcur[0][j], vcur[1][j], 0x7362);
+      const uint32_t b0 = __byte_perm(vcur[2][j], vcur[3][j], 0x5140), b1 = __byte_perm(vcur[2][j], vcur[3][j], 0x7362);
+      mma16816(o[4 * j], pa, Codec<STORE>::template pair<false>(a0), Codec<STORE>::template pair<false>(b0));
+      mma16816(o[4 * j + 1], pa, Codec<STORE>::template pair<true>(a0), Codec<STORE>::template pair<true>(b0));
+      mma16816(o[4 * j + 2], pa, Codec<STORE>::template pair<false>(a1), Codec<STORE>::template pair<false>(b1));
+      mma16816(o[4 * j + 3], pa, Codec<STORE>::template pair<true>(a1), Codec<STORE>::template pair<true>(b1));
+    }
+  }
+
+  // join the warps: n column 2 t + c of tile i is output dim VB (2 t + c) + i
+  ell += __shfl_xor_sync(0xffffffffu, ell, 1);
+  ell += __shfl_xor_sync(0xffffffffu, ell, 2);
+  if (t == 0) {
+    m_s[warp][g] = m;
+    l_s[warp][g] = ell;
+  }
+  float* ow = sm.o + (warp * 8 + g) * OS;
+  const float vout = vref / kUp;
+#pragma unroll
+  for (int c = 0; c < 2; ++c)
+#pragma unroll
+    for (int i = 0; i < ND; i += 4) {
+      const int d = VB * (2 * t + c) + i;
+      float4 w;
+      w.x = (o[i][c] + o[i][2 + c]) * vout;
+      w.y = (o[i + 1][c] + o[i + 1][2 + c]) * vout;
+      w.z = (o[i + 2][c] + o[i + 2][2 + c]) * vout;
+      w.w = (o[i + 3][c] + o[i + 3][2 + c]) * vout;
+      *reinterpret_cast<float4*>(ow + d + d / 32 * 4) = w;
+    }
+  __syncthreads();
+  for (int i = threadIdx.x; i < nE * D; i += kAtThreads) {
+    const int e = i / D, d = i - e * D;
+    float M = m_s[0][e];
+#pragma unroll
+    for (int w = 1; w < 4; ++w) M = fmaxf(M, m_s[w][e]);
+    float l = 0.f, ov = 0.f;
+    if (M > -INFINITY) {
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const float c = ex2(m_s[w][e] - M);
+        l += c * l_s[w][e];
+        ov += c * sm.o[(w * 8 + e) * OS + d + d / 32 * 4];
+      }
+    }
+    if (active == 1) {
+      const int64_t hq = (int64_t)b * p.Hq + hkv * p.E + e0 + e;
+      static_cast<TQ*>(p.out)[hq * D + d] = from_f<TQ>(l != 0.f ? ov / l : 0.f);
+      if (d == 0) p.lse[hq] = l != 0.f ? (M + log2f(l)) * kLn2 : -INFINITY;
+    } else {
+      float* q = p.part + ((slot0 + split) * 8 + e) * (D + 2);
+      __stcg(q + 2 + d, ov);
+      if (d == 0) {
+        __stcg(q, M);
+        __stcg(q + 1, l);
+      }
+    }
+  }
+  close_split<TQ>(p, b, hg, e0, nE, slot0, active, pos, &flag);
+}
+
+// Any head dims up to 256 and any head count: fp32 on the CUDA cores, a warp per
+// token, lanes over dims; the same splits and the same join.
+constexpr int kAnyDims = 256 / 32;
+template <typename TQ, int STORE, bool STEP>
+__global__ void __launch_bounds__(kAtThreads) attend_any(AttendParams p) {
+  __shared__ float q_s[256], o_s[4][256], m_s[4], l_s[4];
+  __shared__ int flag;
+  const int split = blockIdx.x, hg = blockIdx.y, b = blockIdx.z;
+  const int hkv = hg / p.groups, e0 = (hg - hkv * p.groups) * 8;
+  const int nE = min(8, p.E - e0);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int pos = p.lengths[b];
+  const int ntok = (int)min((int64_t)(STEP ? pos + 1 : pos), p.cap);
+  const int active = max(1, min(p.splits, (ntok + p.chunk - 1) / p.chunk));
+  const int64_t slot0 = ((int64_t)b * p.Hkv * p.groups + hg) * p.splits;
+  if (split >= active) {
+    if (p.advance) close_split<TQ>(p, b, hg, e0, nE, slot0, active, pos, &flag);
+    return;
+  }
+  const int c0 = split * p.chunk, c1 = split == active - 1 ? ntok : c0 + p.chunk;
+  const int64_t head = (int64_t)b * p.Hkv + hkv;
+  if constexpr (STEP) {
+    if (split == active - 1 && pos < p.cap) {
+      if (warp == 0)
+        write_token<TQ, STORE>(p, static_cast<const TQ*>(p.k_t) + b * p.k_sb + hkv * p.k_sh, p.Dk, p.R, pos, head, p.k,
+                               p.ks, p.k_new);
+      if (warp == 1)
+        write_token<TQ, STORE>(p, static_cast<const TQ*>(p.v_t) + b * p.v_sb + hkv * p.v_sh, p.Dv, 0, pos, head, p.v,
+                               p.vs, p.v_new);
+    } else if (split == active - 1 && threadIdx.x == 0 && p.status) {
+      atomicOr(p.status, TC_DEV_BAD_INDEX);
+    }
+  }
+  for (int e = 0; e < nE; ++e) {
+    __syncthreads();
+    const TQ* x = static_cast<const TQ*>(p.q) + b * p.q_sb + (int64_t)(hkv * p.E + e0 + e) * p.q_sh;
+    for (int u = threadIdx.x; u < (p.Dk + 1) / 2; u += kAtThreads) {
+      int i1, i2;
+      float y1, y2;
+      load_pair(p, x, u, p.Dk, STEP ? p.R : 0, pos, &i1, &i2, &y1, &y2);
+      q_s[i1] = y1;
+      q_s[i2] = y2;
+    }
+    __syncthreads();
+    float m = -INFINITY, ell = 0.f, o[kAnyDims];
+#pragma unroll
+    for (int i = 0; i < kAnyDims; ++i) o[i] = 0.f;
+    for (int tok = c0 + warp; tok < c1; tok += 4) {
+      const int64_t at = head * p.cap + tok;
+      float s = 0.f;
+      for (int d = lane; d < p.Dk; d += 32) s += q_s[d] * Codec<STORE>::value(p.k[at * p.Dk + d]);
+      float xl = warp_sum(s) * p.ks[at] * p.qscale;
+      if (p.has_cap) xl = p.softcap * tanhf(xl / p.softcap);
+      xl *= kLog2e;
+      const float mn = fmaxf(m, xl);
+      const float cm = m == mn ? 1.f : exp2f(m - mn);
+      const float pr = exp2f(xl - mn);
+      ell = ell * cm + pr;
+      m = mn;
+      const float w = pr * p.vs[at];
+#pragma unroll
+      for (int i = 0; i < kAnyDims; ++i) {
+        const int d = lane + 32 * i;
+        if (d < p.Dv) o[i] = o[i] * cm + w * Codec<STORE>::value(p.v[at * p.Dv + d]);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kAnyDims; ++i) o_s[warp][lane + 32 * i] = o[i];
+    if (lane == 0) {
+      m_s[warp] = m;
+      l_s[warp] = ell;
+    }
+    __syncthreads();
+    float M = fmaxf(fmaxf(m_s[0], m_s[1]), fmaxf(m_s[2], m_s[3]));
+    for (int d = threadIdx.x; d < p.Dv; d += kAtThreads) {
+      float l = 0.f, ov = 0.f;
+      if (M > -INFINITY) {
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const float c = exp2f(m_s[w] - M);
+          l += c * l_s[w];
+          ov += c * o_s[w][d];
+        }
+      }
+      if (active == 1) {
+        const int64_t hq = (int64_t)b * p.Hq + hkv * p.E + e0 + e;
+        static_cast<TQ*>(p.out)[hq * p.Dv + d] = from_f<TQ>(l != 0.f ? ov / l : 0.f);
+        if (d == 0) p.lse[hq] = l != 0.f ? (M + log2f(l)) * kLn2 : -INFINITY;
+      } else {
+        float* q = p.part + ((slot0 + split) * 8 + e) * (p.Dv + 2);
+        __stcg(q + 2 + d, ov);
+        if (d == 0) {
+          __stcg(q, M);
+          __stcg(q + 1, l);
+        }
+      }
+    }
+  }
+  close_split<TQ>(p, b, hg, e0, nE, slot0, active, pos, &flag);
+}
+
+template <typename TQ, int STORE, int D, bool STEP>
+int launch_mma(const AttendParams& p, dim3 grid, cudaStream_t st) {
+  if (p.has_cap) attend_mma<TQ, STORE, D, true, STEP><<<grid, kAtThreads, 0, st>>>(p);
+  else attend_mma<TQ, STORE, D, false, STEP><<<grid, kAtThreads, 0, st>>>(p);
+  return launch_status();
+}
+
+template <typename TQ, int STORE, bool STEP>
+int launch_attend(const AttendParams& p, cudaStream_t st) {
+  const dim3 grid(p.splits, p.Hkv * p.groups, p.B);
+  const bool mma = p.Dk == p.Dv && (p.Dk == 64 || p.Dk == 128) && (uintptr_t)p.k % 16 == 0 && (uintptr_t)p.v % 16 == 0;
+  if (mma && p.Dk == 128) return launch_mma<TQ, STORE, 128, STEP>(p, grid, st);
+  if (mma) return launch_mma<TQ, STORE, 64, STEP>(p, grid, st);
+  attend_any<TQ, STORE, STEP><<<grid, kAtThreads, 0, st>>>(p);
+  return launch_status();
+}
+
+bool cache_ok(const tc_kv_cache* c) {
+  return c && c->rows >= 0 && c->Hkv > 0 && c->Dk > 0 && c->Dv > 0 && c->capacity > 0 &&
+         (c->store == TC_KV_INT8 || c->store == TC_KV_FP8) && c->k && c->v && c->k_scale && c->v_scale && c->lengths;
+}
+
+// Tokens per CTA and CTAs per (sequence, head group) over at most `most`
+// tokens.  The CTAs wanted are four waves of three per SM over 148 SMs, so that
+// sequences of different lengths even out; a chunk is at least 64 tokens (one
+// step of the four warps) and a multiple of 64.
+void split_rule(int64_t most, int64_t heads, int* chunk, int* splits) {
+  const int64_t want = (4 * 3 * 148 + heads - 1) / heads;
+  int64_t c = (most + want - 1) / want;
+  c = (c + 63) / 64 * 64;
+  if (c < 64) c = 64;
+  const int64_t s = (most + c - 1) / c;
+  *chunk = (int)c;
+  *splits = (int)(s < 1 ? 1 : s);
+}
+
+}  // namespace
+
+extern "C" int tc_kv_write(const tc_kv_cache* c, const tc_kv_write_args* a, void* stream) {
+  if (!cache_ok(c) || !a || a->B < 0 || a->N < 0) return TC_ERR_ARG;
+  if ((int64_t)a->B * a->N == 0) return TC_OK;
+  if (!a->k || !a->v || (a->seq_idx && !a->starts) || (!a->seq_idx && a->B > c->rows)) return TC_ERR_ARG;
+  WriteParams p;
+  p.B = a->B, p.N = a->N, p.H = c->Hkv, p.D = 0, p.rows = c->rows, p.fresh = a->fresh != 0;
+  p.cap = c->capacity;
+  p.src[0] = a->k, p.src[1] = a->v;
+  p.sb[0] = a->k_stride_b, p.sn[0] = a->k_stride_n, p.sh[0] = a->k_stride_h;
+  p.sb[1] = a->v_stride_b, p.sn[1] = a->v_stride_n, p.sh[1] = a->v_stride_h;
+  p.codes[0] = c->k, p.codes[1] = c->v;
+  p.scales[0] = c->k_scale, p.scales[1] = c->v_scale;
+  p.dim[0] = c->Dk, p.dim[1] = c->Dv;
+  p.lengths = c->lengths;
+  p.seq = a->seq_idx, p.starts = a->starts;
+  p.status = a->dev_status;
+  cudaStream_t st = (cudaStream_t)stream;
+  if (c->store == TC_KV_INT8) { TC_DISPATCH(a->dtype, T, return launch_write<T, TC_KV_INT8>(p, st)); }
+  else { TC_DISPATCH(a->dtype, T, return launch_write<T, TC_KV_FP8>(p, st)); }
+}
+
+extern "C" int tc_kv_read(const tc_kv_cache* c, int32_t length, int32_t dtype, void* k_out, void* v_out, void* stream) {
+  if (!cache_ok(c) || length < 0 || !k_out || !v_out) return TC_ERR_ARG;
+  if ((int64_t)c->rows * length == 0) return TC_OK;
+  ReadParams p;
+  p.rows = c->rows, p.H = c->Hkv, p.L = length, p.cap = c->capacity;
+  p.codes[0] = c->k, p.codes[1] = c->v;
+  p.scales[0] = c->k_scale, p.scales[1] = c->v_scale;
+  p.dim[0] = c->Dk, p.dim[1] = c->Dv;
+  p.lengths = c->lengths;
+  p.out[0] = k_out, p.out[1] = v_out;
+  cudaStream_t st = (cudaStream_t)stream;
+  if (c->store == TC_KV_INT8) { TC_DISPATCH(dtype, T, return launch_read<T, TC_KV_INT8>(p, st)); }
+  else { TC_DISPATCH(dtype, T, return launch_read<T, TC_KV_FP8>(p, st)); }
+}
+
+static int attend_shape(const tc_kv_cache* c, int32_t B, int32_t Hq, int32_t max_tokens, int* chunk, int* splits) {
+  if (!cache_ok(c) || B < 0 || Hq <= 0 || Hq % c->Hkv || max_tokens < 0) return TC_ERR_ARG;
+  const int groups = (Hq / c->Hkv + 7) / 8;
+  split_rule(max_tokens < 1 ? 1 : max_tokens, (int64_t)(B < 1 ? 1 : B) * c->Hkv * groups, chunk, splits);
+  return TC_OK;
+}
+
+extern "C" int64_t tc_kv_attend_scratch_floats(const tc_kv_cache* c, int32_t B, int32_t Hq, int32_t max_tokens) {
+  int chunk, splits;
+  if (attend_shape(c, B, Hq, max_tokens, &chunk, &splits)) return -1;
+  const int groups = (Hq / c->Hkv + 7) / 8;
+  return splits > 1 ? (int64_t)B * c->Hkv * groups * splits * 8 * (c->Dv + 2) : 0;
+}
+
+extern "C" int tc_kv_attend(const tc_kv_cache* c, const tc_kv_attend_args* a, void* stream) {
+  if (!a) return TC_ERR_ARG;
+  AttendParams p;
+  if (int rc = attend_shape(c, a->B, a->Hq, a->max_tokens, &p.chunk, &p.splits)) return rc;
+  if (a->B == 0) return TC_OK;
+  if (a->B > c->rows || !a->q || !a->out || !a->lse || a->max_tokens > c->capacity) return TC_ERR_ARG;
+  if (c->Dk > 256 || c->Dv > 256 || a->B > 65535) return TC_ERR_UNSUPPORTED;
+  const bool step = a->k_t != nullptr;
+  if (step && !a->v_t) return TC_ERR_ARG;
+  if (a->R < 0 || a->R % 2 || a->R > c->Dk || (a->R && (!a->rope_cos || !a->rope_sin || a->n_pos <= 0 || !step)))
+    return TC_ERR_ARG;
+  p.groups = (a->Hq / c->Hkv + 7) / 8;
+  if ((int64_t)c->Hkv * p.groups > 65535) return TC_ERR_UNSUPPORTED;
+  const int64_t need = p.splits > 1 ? (int64_t)a->B * c->Hkv * p.groups * p.splits * 8 * (c->Dv + 2) : 0;
+  if (need && (!a->scratch || a->scratch_floats < need)) return TC_ERR_ARG;
+  if ((p.splits > 1 || a->advance) && (!a->counters || a->num_counters < (int64_t)a->B * (c->Hkv * p.groups + 1)))
+    return TC_ERR_ARG;
+  p.B = a->B, p.Hq = a->Hq, p.Hkv = c->Hkv, p.E = a->Hq / c->Hkv;
+  p.Dk = c->Dk, p.Dv = c->Dv, p.cap = c->capacity;
+  p.k = c->k, p.v = c->v, p.ks = c->k_scale, p.vs = c->v_scale, p.lengths = c->lengths;
+  p.q = a->q, p.q_sb = a->q_stride_b, p.q_sh = a->q_stride_h;
+  p.k_t = a->k_t, p.v_t = a->v_t;
+  p.k_sb = a->k_stride_b, p.k_sh = a->k_stride_h, p.v_sb = a->v_stride_b, p.v_sh = a->v_stride_h;
+  p.cos_t = a->rope_cos, p.sin_t = a->rope_sin, p.R = a->R, p.interleaved = a->interleaved != 0, p.n_pos = a->n_pos;
+  p.qscale = a->scale, p.softcap = a->softcap, p.has_cap = a->has_softcap != 0;
+  p.advance = step && a->advance;
+  p.out = a->out, p.lse = a->lse, p.k_new = a->k_new, p.v_new = a->v_new, p.new_dtype = a->new_dtype;
+  p.part = a->scratch, p.done = a->counters, p.status = a->dev_status;
+  cudaStream_t st = (cudaStream_t)stream;
+#define TC_KV_GO(S, STEP) TC_DISPATCH(a->dtype, T, return launch_attend<T, S, STEP>(p, st))
+  if (c->store == TC_KV_INT8) {
+    if (step) { TC_KV_GO(TC_KV_INT8, true); }
+    else { TC_KV_GO(TC_KV_INT8, false); }
+  } else {
+    if (step) { TC_KV_GO(TC_KV_FP8, true); }
+    else { TC_KV_GO(TC_KV_FP8, false); }
+  }
+#undef TC_KV_GO
+}

@@ -73,3 +73,37 @@ def test_tree_bwd_scratch_plan():
     bad = args(8)
     bad.total += 1
     assert lib.tc_tree_bwd_scratch_bytes(ctypes.byref(bad)) == -1
+
+
+def test_full_attention_structs_and_bad_arguments():
+    """Sizes as a C compiler lays the header's structs out (LP64), and refusals
+    before any launch."""
+    sizes = dict(RotaryArgs=152, KVCacheArgs=64, KVWriteArgs=104, KVAttendArgs=216, CausalArgs=240)
+    assert {n: ctypes.sizeof(getattr(_lib, n)) for n in sizes} == sizes
+    lib = _lib.lib()
+    assert lib.tc_rotary(None, None) == _lib.TC_ERR_ARG
+    assert lib.tc_rotary(_lib.RotaryArgs(B=1, N=1, Hq=1, D=8, R=3), None) == _lib.TC_ERR_ARG  # R odd
+    assert lib.tc_segment_bounds(1, 1, None, None, None, None) == _lib.TC_ERR_ARG
+    assert lib.tc_causal_fwd(None, None) == _lib.TC_ERR_ARG
+    assert lib.tc_causal_fwd(_lib.CausalArgs(B=1, N=1, Hq=3, Hkv=2, Dk=8, Dv=8), None) == _lib.TC_ERR_ARG
+    assert lib.tc_causal_bwd(_lib.CausalArgs(B=1, N=1, Hq=2, Hkv=2, Dk=8, Dv=8, dtype=1), None) == _lib.TC_ERR_ARG
+    bad = _lib.KVCacheArgs(rows=1, Hkv=1, Dk=8, Dv=8, capacity=4)  # no tensors
+    assert lib.tc_kv_write(bad, _lib.KVWriteArgs(B=1, N=1), None) == _lib.TC_ERR_ARG
+    assert lib.tc_kv_read(bad, 1, 0, None, None, None) == _lib.TC_ERR_ARG
+    assert lib.tc_kv_attend(bad, _lib.KVAttendArgs(B=1, Hq=1), None) == _lib.TC_ERR_ARG
+    assert lib.tc_kv_attend_scratch_floats(bad, 1, 1, 4) == -1
+
+
+def test_cached_attention_split_plan():
+    """Chunks are multiples of 64 tokens, four waves of three CTAs per SM are
+    wanted, one chunk needs no scratch."""
+    lib = _lib.lib()
+    c = _lib.KVCacheArgs(rows=64, Hkv=4, Dk=128, Dv=128, capacity=40000, k=16, v=16, k_scale=16, v_scale=16,
+                         lengths=16)
+    floats = lambda B, Hq, n: lib.tc_kv_attend_scratch_floats(c, B, Hq, n)  # noqa: E731
+    assert floats(1, 4, 64) == 0 and floats(1, 4, 0) == 0
+    assert floats(1, 4, 65) == 4 * 2 * 8 * 130
+    want = -(-4 * 3 * 148 // (64 * 4))
+    chunk = -(-(-(-32768 // want)) // 64) * 64
+    assert floats(64, 16, 32768) == 64 * 4 * -(-32768 // chunk) * 8 * 130
+    assert floats(64, 4 * 9, 64) == 0 and floats(64, 4 * 9, 128) == 64 * 4 * 2 * 2 * 8 * 130  # nine heads: two eights
