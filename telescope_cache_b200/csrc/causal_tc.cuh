@@ -1,0 +1,56 @@
+// Pieces shared by the tensor-core kernels of packed causal attention.
+#pragma once
+
+#include "causal.cuh"
+#include "tc_common.cuh"
+
+namespace tc {
+namespace ctc {
+
+using namespace ptx;
+using namespace tcx;
+
+constexpr int KT = 128;  // keys per tile of the forward
+
+// [B, N, H, D] through its strides as a 4-D map (d, h, n, b) of 64 x 1 x rows x 1
+// boxes with the 128-byte swizzle; tokens past N read as zeros.  The stride of a
+// dimension of size one is never used: any valid one stands in.
+inline int make_map_strided(CUtensorMap* m, const void* base, int dt, int64_t B, int64_t N, int64_t H, int D, int64_t sb,
+                            int64_t sn, int64_t sh, int rows) {
+  auto fn = encode_fn();
+  if (!fn) return TC_ERR_CUDA;
+  const CUtensorMapDataType t = dt == TC_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  if (H == 1) sh = D;
+  if (N == 1) sn = D * H;
+  if (B == 1) sb = sn * N;
+  cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)H, (cuuint64_t)N, (cuuint64_t)B};
+  cuuint64_t strides[3] = {(cuuint64_t)sh * 2, (cuuint64_t)sn * 2, (cuuint64_t)sb * 2};
+  cuuint32_t box[4] = {64, 1, (cuuint32_t)rows, 1};
+  cuuint32_t estr[4] = {1, 1, 1, 1};
+  CUresult r = fn(m, t, 4, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? TC_OK : TC_ERR_CUDA;
+}
+
+// A rows x HD tile: HD / 64 swizzled blocks of rows x 64.
+template <int HD, int ROWS>
+__device__ __forceinline__ void load_rows(uint8_t* dst, const CUtensorMap* m, int h, int n, int b, uint64_t* bar) {
+#pragma unroll
+  for (int c = 0; c < HD / 64; ++c) tma_load_4d(dst + c * ROWS * 128, m, 64 * c, h, n, b, bar);
+}
+
+inline bool strides_ok(const void* p, int64_t sb, int64_t sn, int64_t sh, int64_t B, int64_t N, int64_t H) {
+  const int64_t most = int64_t(1) << 38;  // elements: a map's byte stride stays below 2^40
+  return (uintptr_t)p % 16 == 0 && (B == 1 || (sb % 8 == 0 && sb > 0 && sb < most)) &&
+         (N == 1 || (sn % 8 == 0 && sn > 0 && sn < most)) && (H == 1 || (sh % 8 == 0 && sh > 0 && sh < most));
+}
+
+inline bool tc_shape(const CausalParams& p, int dtype) {
+  return (dtype == TC_BF16 || dtype == TC_F16) && p.Dk == p.Dv && (p.Dk == 64 || p.Dk == 128) &&
+         strides_ok(p.q, p.q_sb, p.q_sn, p.q_sh, p.B, p.N, p.Hq) &&
+         strides_ok(p.k, p.k_sb, p.k_sn, p.k_sh, p.B, p.N, p.Hkv) &&
+         strides_ok(p.v, p.v_sb, p.v_sn, p.v_sh, p.B, p.N, p.Hkv);
+}
+
+}  // namespace ctc
+}  // namespace tc
