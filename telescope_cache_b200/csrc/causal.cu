@@ -73,18 +73,43 @@ __global__ void __launch_bounds__(kBoundThreads) bounds_kernel(int N, const int3
 // ---------------------------------------------------------------------------
 // Delta = rowsum(dO * out) - dlse
 // ---------------------------------------------------------------------------
-template <typename T>
+// LANES lanes per row, 16 bytes of dO and out each (LANES 0: a warp per row of
+// any length).  Bound by HBM.
+template <typename T, int LANES>
 __global__ void __launch_bounds__(256) delta_rows(CausalParams p, int64_t rows) {
-  const int64_t r = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
-  const int lane = threadIdx.x & 31;
-  if (r >= rows) return;
-  const T* o = static_cast<const T*>(p.o) + r * p.Dv;
-  const T* g = static_cast<const T*>(p.dout) + r * p.Dv;
+  constexpr int L = LANES ? LANES : 32, VE = 16 / sizeof(T);
+  const int64_t r = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) / L;
+  const int lane = threadIdx.x % L;
   float s = 0.f;
-  for (int d = lane; d < p.Dv; d += 32) s += to_f(o[d]) * to_f(g[d]);
+  if (r < rows) {
+    const T* o = static_cast<const T*>(p.o) + r * p.Dv;
+    const T* g = static_cast<const T*>(p.dout) + r * p.Dv;
+    if constexpr (LANES) {
+      const uint4 a = *reinterpret_cast<const uint4*>(o + lane * VE), c = *reinterpret_cast<const uint4*>(g + lane * VE);
 #pragma unroll
-  for (int x = 16; x; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
-  if (lane == 0) p.delta[r] = s - (p.dlse ? p.dlse[r] : 0.f);
+      for (int i = 0; i < VE; ++i) s += to_f(reinterpret_cast<const T*>(&a)[i]) * to_f(reinterpret_cast<const T*>(&c)[i]);
+    } else {
+      for (int d = lane; d < p.Dv; d += 32) s += to_f(o[d]) * to_f(g[d]);
+    }
+  }
+#pragma unroll
+  for (int x = L / 2; x; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
+  if (r < rows && lane == 0) p.delta[r] = s - (p.dlse ? p.dlse[r] : 0.f);
+}
+
+template <typename T>
+int launch_delta(const CausalParams& p, cudaStream_t st) {
+  const int64_t rows = (int64_t)p.B * p.N * p.Hq;
+  const bool vec = (uintptr_t)p.o % 16 == 0 && (uintptr_t)p.dout % 16 == 0;
+  const int lanes = vec ? p.Dv * (int)sizeof(T) / 16 : 0;
+  const bool fit = vec && p.Dv * (int)sizeof(T) % 16 == 0 && (lanes == 8 || lanes == 16 || lanes == 32);
+  const int64_t grid = (rows * (fit ? lanes : 32) + 255) / 256;
+  if (grid > INT32_MAX) return TC_ERR_UNSUPPORTED;
+  if (!fit) delta_rows<T, 0><<<(unsigned)grid, 256, 0, st>>>(p, rows);
+  else if (lanes == 8) delta_rows<T, 8><<<(unsigned)grid, 256, 0, st>>>(p, rows);
+  else if (lanes == 16) delta_rows<T, 16><<<(unsigned)grid, 256, 0, st>>>(p, rows);
+  else delta_rows<T, 32><<<(unsigned)grid, 256, 0, st>>>(p, rows);
+  return launch_status();
 }
 
 // ---------------------------------------------------------------------------
@@ -455,10 +480,7 @@ int make_params(const tc_causal_args* a, CausalParams* p) {
 
 namespace tc {
 int causal_delta(const CausalParams& p, int dtype, cudaStream_t st) {
-  const int64_t rows = (int64_t)p.B * p.N * p.Hq, grid = (rows + 7) / 8;
-  if (grid > INT32_MAX) return TC_ERR_UNSUPPORTED;
-  TC_DISPATCH(dtype, T, delta_rows<T><<<(unsigned)grid, 256, 0, st>>>(p, rows));
-  return launch_status();
+  TC_DISPATCH(dtype, T, return launch_delta<T>(p, st));
 }
 }  // namespace tc
 

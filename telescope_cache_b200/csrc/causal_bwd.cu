@@ -1,5 +1,595 @@
+// Packed causal attention backward on the tensor cores (sm_100a, bf16 / f16,
+// Dk = Dv = HD of 64 or 128), in two passes that each recompute S and dP:
+//
+//   dQ pass   CTA = 128 queries of one head over their 128-key tiles:
+//             S = Q K^T, dP = dO V^T, dQ += dX K.
+//   dKV pass  CTA = 128 keys of one key head over the 128-query tiles that see
+//             them, head by head of the group: S^T = K Q^T, dP^T = V dO^T,
+//             dV += P^T dO, dK += dX^T Q.
+//   P = exp2(logit2 - lse2),  dX = P softcap' (dP - Delta).
+//
+// Seven products instead of the five of a single pass, and nothing is summed by
+// atomics: the results do not depend on the order in which CTAs run.
+//
+// Both passes: warp 0 TMA producer, warp 1 MMA issuer, warps 4-11 compute: a
+// thread owns one TMEM lane (query, or key) and 64 of the tile's 128 columns.
+// P and dX leave as 16-bit pairs in the first 32 of the thread's own 64 columns
+// of S or dP and are the A operands of the accumulating products: they never
+// pass through shared memory.  The MMAs of one thread run in the order of their
+// issue, so the next tile's S (dP) is issued right behind the product that
+// reads P (dX) out of its columns.
+//
+// dKV pass, TMEM: S^T, dP^T, dV, dK.  Per tile the compute warps work in two
+// halves, exp of S then dX of dP, and the tensor core does the other half's
+// products meanwhile (dK of the last tile and dP during exp; dV and the next S
+// during dX).  dQ pass, TMEM: two S, dP, dQ; S is a tile ahead, dQ and the next
+// dP run during exp.
 #include "causal_tc.cuh"
+
 namespace tc {
-bool causal_bwd_tc_supported(const CausalParams&, int) { return false; }
-int causal_bwd_tc(const CausalParams&, int, cudaStream_t) { return TC_ERR_UNSUPPORTED; }
+namespace {
+
+using namespace ctc;
+
+constexpr int kBwdThreads = 384;
+constexpr int kCompute = 256;
+constexpr int BLK = 128 * 128;  // one 64-column block of a 128-row tile
+
+struct BwdParams {
+  CausalParams c;
+  float kq, kc;  // logit2 = kq s, or kc tanh(kq s)
+};
+
+template <int HD> struct BwdSmem {
+  static constexpr int kTile = 128 * HD * 2;
+  static constexpr int kNK = 3, kNV = 2, kNQ = 2;
+  static constexpr int kDq = (2 + kNK + kNV) * kTile + 256 + 1024;
+  static constexpr int kDkv = (2 + 2 * kNQ) * kTile + kNQ * 128 * 8 + 256 + 1024;
+  static_assert(kDq <= 227 * 1024 && kDkv <= 227 * 1024, "backward shared memory exceeds the per-CTA limit");
+};
+
+// 1 - 2 / (e^2x + 1): tanh to a few 1e-7
+__device__ __forceinline__ float tanh_exp(float x) {
+  return 1.f - __fdividef(2.f, exp2_fast(x * (2.f * kLog2e)) + 1.f);
+}
+
+// p = exp2(logit2(s) + nl2) and pg = p softcap' of two columns.
+template <bool CAP>
+__device__ __forceinline__ void p_pair(float2 s, float2 nl2, float kq, float kc, float2* p, float2* pg) {
+  if constexpr (CAP) {
+    const float2 y = fmul2(s, make_float2(kq, kq));
+    const float2 t = make_float2(tanh_exp(y.x), tanh_exp(y.y));
+    const float2 a = ffma2(t, make_float2(kc, kc), nl2);
+    *p = make_float2(exp2_fast(a.x), exp2_fast(a.y));
+    *pg = fmul2(*p, ffma2(make_float2(-t.x, -t.y), t, make_float2(1.f, 1.f)));
+  } else {
+    const float2 a = ffma2(s, make_float2(kq, kq), nl2);
+    *p = make_float2(exp2_fast(a.x), exp2_fast(a.y));
+    *pg = *p;
+  }
+}
+
+// Tile column base + i inside [jlo, jhi)?
+__device__ __forceinline__ bool inside(int i, int jlo, int jhi) { return i >= jlo && i < jhi; }
+
+// Row `r` of a 128-row fp32 accumulator in TMEM (zeros unless have) times mul, as T.
+template <typename T, int HD>
+__device__ __forceinline__ void store_row(uint32_t taddr, bool have, T* out, float mul, bool store) {
+#pragma unroll 1
+  for (int d = 0; d < HD; d += 32) {
+    float v[32];
+    if (have) {
+      tmem_ld32(taddr + d, v);
+      tmem_wait_ld();
+    } else {
+#pragma unroll
+      for (int i = 0; i < 32; ++i) v[i] = 0.f;
+    }
+    if (store) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(out + d + i * 8) = pack8<T>(v + i * 8, mul);
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// dQ
+// ---------------------------------------------------------------------------
+template <typename T, int HD, bool CAP>
+__global__ void __launch_bounds__(kBwdThreads, 1)
+    causal_dq_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__ CUtensorMap tmg,
+                     const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv,
+                     const __grid_constant__ BwdParams p) {
+  using Z = BwdSmem<HD>;
+  constexpr int TB = Z::kTile, NK = Z::kNK, NV = Z::kNV, KK = HD / 16;
+  constexpr uint32_t kColP = 256, kColQ = 384;  // S [0, 256), dP, dQ
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* q_s = sm;
+  uint8_t* g_s = q_s + TB;
+  uint8_t* k_s = g_s + TB;
+  uint8_t* v_s = k_s + NK * TB;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(v_s + NV * TB);
+  uint64_t* q_full = bars;           // Q
+  uint64_t* g_full = bars + 1;       // dO
+  uint64_t* k_full = g_full + 1;     // [NK]
+  uint64_t* k_empty = k_full + NK;
+  uint64_t* v_full = k_empty + NK;   // [NV]
+  uint64_t* v_empty = v_full + NV;
+  uint64_t* s_full = v_empty + NV;   // [2]
+  uint64_t* p_full = s_full + 2;     // dP computed
+  uint64_t* x_full = p_full + 1;     // dX written
+  uint64_t* q_done = x_full + 1;
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(q_done + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
+  static_assert((2 + 2 * NK + 2 * NV + 5) * 8 + 8 <= 256, "barrier area");
+
+  const CausalParams& c = p.c;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int q0 = (gridDim.x - 1 - blockIdx.x) * 128, hq = blockIdx.y, b = blockIdx.z, hkv = hq / c.E;
+  int32_t* status = c.status;
+  const int first0 = first_key(c, b, q0), last = min(q0 + 128, c.N) - 1;
+  const int j0 = first0 <= last ? first0 / 128 : 0, j1 = first0 <= last ? last / 128 + 1 : 0;
+
+  if (threadIdx.x == 0) {
+    mbar_init(q_full, 1);
+    mbar_init(g_full, 1);
+    for (int i = 0; i < NK; ++i) {
+      mbar_init(&k_full[i], 1);
+      mbar_init(&k_empty[i], 1);
+    }
+    for (int i = 0; i < NV; ++i) {
+      mbar_init(&v_full[i], 1);
+      mbar_init(&v_empty[i], 1);
+    }
+    mbar_init(&s_full[0], 1);
+    mbar_init(&s_full[1], 1);
+    mbar_init(p_full, 1);
+    mbar_init(x_full, kCompute);
+    mbar_init(q_done, 1);
+    *abort_flag = 0;
+    mbar_fence_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_holder, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_holder;
+
+  if (warp == 0) {
+    if (lane == 0 && j0 < j1) {
+      mbar_expect_tx(q_full, TB);
+      load_rows<HD, 128>(q_s, &tmq, hq, q0, b, q_full);
+      bool ok = true;
+      auto load_k = [&](int j) {
+        const int i = j - j0, st = i % NK;
+        if (i >= NK && !mbar_wait(&k_empty[st], ((i / NK) - 1) & 1, abort_flag, status)) return false;
+        mbar_expect_tx(&k_full[st], TB);
+        load_rows<HD, 128>(k_s + st * TB, &tmk, hkv, j * 128, b, &k_full[st]);
+        return true;
+      };
+      ok = load_k(j0);
+      mbar_expect_tx(g_full, TB);
+      load_rows<HD, 128>(g_s, &tmg, hq, q0, b, g_full);
+      for (int j = j0; ok && j < j1; ++j) {
+        const int i = j - j0, st = i % NV;
+        if (i >= NV && !mbar_wait(&v_empty[st], ((i / NV) - 1) & 1, abort_flag, status)) break;
+        mbar_expect_tx(&v_full[st], TB);
+        load_rows<HD, 128>(v_s + st * TB, &tmv, hkv, j * 128, b, &v_full[st]);
+        if (j + 1 < j1) ok = load_k(j + 1);
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && j0 < j1) {
+      constexpr uint32_t kIdS = idesc_f16(128, 128, Pack2<T>::kFmt, 0, 0);
+      constexpr uint32_t kIdQ = idesc_f16(128, HD, Pack2<T>::kFmt, 0, 1);
+      const uint64_t qd = sdesc_sw128(smem_addr(q_s), 16, 1024), gd = sdesc_sw128(smem_addr(g_s), 16, 1024);
+      const uint64_t kd0 = sdesc_sw128(smem_addr(k_s), 16, 1024), vd0 = sdesc_sw128(smem_addr(v_s), 16, 1024);
+      const uint64_t kt0 = sdesc_sw128(smem_addr(k_s), BLK, 1024);
+      const int n = j1 - j0;
+      auto issue_s = [&](int i) {
+        if (!mbar_wait(&k_full[i % NK], (i / NK) & 1, abort_flag, status)) return false;
+        const uint64_t kd = sdesc_add(kd0, (i % NK) * TB);
+        tc_fence_after();
+#pragma unroll
+        for (int kk = 0; kk < KK; ++kk) {
+          const uint32_t off = (kk >> 2) * BLK + (kk & 3) * 32;
+          mma_f16(tmem + (i & 1) * 128, sdesc_add(qd, off), sdesc_add(kd, off), kIdS, kk > 0 ? 1u : 0u);
+        }
+        mma_commit(&s_full[i & 1]);
+        return true;
+      };
+      auto issue_p = [&](int i) {
+        if (!mbar_wait(&v_full[i % NV], (i / NV) & 1, abort_flag, status)) return false;
+        const uint64_t vd = sdesc_add(vd0, (i % NV) * TB);
+        tc_fence_after();
+#pragma unroll
+        for (int kk = 0; kk < KK; ++kk) {
+          const uint32_t off = (kk >> 2) * BLK + (kk & 3) * 32;
+          mma_f16(tmem + kColP, sdesc_add(gd, off), sdesc_add(vd, off), kIdS, kk > 0 ? 1u : 0u);
+        }
+        mma_commit(p_full);
+        mma_commit(&v_empty[i % NV]);
+        return true;
+      };
+      bool ok = mbar_wait(q_full, 0, abort_flag, status) && issue_s(0) && mbar_wait(g_full, 0, abort_flag, status) &&
+                issue_p(0) && (n < 2 || issue_s(1));
+      for (int i = 0; ok && i < n; ++i) {
+        if (!mbar_wait(x_full, i & 1, abort_flag, status)) break;
+        tc_fence_after();
+        const uint64_t kt = sdesc_add(kt0, (i % NK) * TB);
+#pragma unroll
+        for (int kk = 0; kk < 8; ++kk)
+          mma_f16_ta(tmem + kColQ, tmem + kColP + (kk >> 2) * 64 + (kk & 3) * 8, sdesc_add(kt, kk * 2048), kIdQ,
+                     (i > 0 || kk > 0) ? 1u : 0u);
+        mma_commit(&k_empty[i % NK]);
+        if (i + 1 < n) ok = issue_p(i + 1);
+        if (ok && i + 2 < n) ok = issue_s(i + 2);
+        if (i + 1 == n) mma_commit(q_done);
+      }
+    }
+  } else if (warp >= 4) {
+    const int half = (warp - 4) >> 2;  // columns [64 half, 64 half + 64)
+    const int r = (threadIdx.x - 128) & 127, q = q0 + r;
+    const bool row_ok = q < c.N;
+    const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
+    const int64_t row = ((int64_t)b * c.N + q) * c.Hq + hq;
+    const int first = row_ok ? first_key(c, b, q) : 1, end = row_ok ? q + 1 : 0;
+    const float nl = row_ok ? -c.lse[row] * kLog2e : 0.f, nd = row_ok ? -c.delta[row] : 0.f;
+    const float2 nl2 = make_float2(nl, nl), nd2 = make_float2(nd, nd);
+    const uint32_t x_addr = tmem + lane_base + kColP + half * 64;
+    bool alive = true;
+    int i = 0;
+    for (int j = j0; j < j1; ++j, ++i) {
+      alive = __all_sync(0xffffffffu, mbar_wait(&s_full[i & 1], (i >> 1) & 1, abort_flag, status));
+      if (!alive) break;
+      tc_fence_after();
+      const uint32_t s_addr = tmem + lane_base + (i & 1) * 128 + half * 64;
+      const int jlo = first - j * 128 - half * 64, jhi = end - j * 128 - half * 64;
+      const bool interior = __all_sync(0xffffffffu, jlo <= 0 && jhi >= 64);
+      float pg[64];
+      tmem_ld32(s_addr, pg);
+      tmem_ld32(s_addr + 32, pg + 32);
+      tmem_wait_ld();
+#pragma unroll
+      for (int k = 0; k < 64; k += 2) {
+        float2 pr, g;
+        p_pair<CAP>(make_float2(pg[k], pg[k + 1]), nl2, p.kq, p.kc, &pr, &g);
+        pg[k] = g.x;
+        pg[k + 1] = g.y;
+      }
+      alive = __all_sync(0xffffffffu, mbar_wait(p_full, i & 1, abort_flag, status));
+      if (!alive) break;
+      tc_fence_after();
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float dp[32];
+        uint32_t w[16];
+        tmem_ld32(x_addr + 32 * h, dp);
+        tmem_wait_ld();
+#pragma unroll
+        for (int k = 0; k < 32; k += 2) {
+          float2 v = fmul2(make_float2(pg[32 * h + k], pg[32 * h + k + 1]), fadd2(make_float2(dp[k], dp[k + 1]), nd2));
+          if (!interior) {
+            v.x = inside(32 * h + k, jlo, jhi) ? v.x : 0.f;
+            v.y = inside(32 * h + k + 1, jlo, jhi) ? v.y : 0.f;
+          }
+          w[k >> 1] = Pack2<T>::pack(v.x, v.y);
+        }
+        tmem_st16u(x_addr + 16 * h, w);  // columns that this thread has read
+      }
+      tmem_wait_st();
+      tc_fence_before();
+      mbar_arrive(x_full);
+    }
+    if (alive && i > 0) alive = __all_sync(0xffffffffu, mbar_wait(q_done, 0, abort_flag, status));
+    if (alive) {
+      tc_fence_after();
+      if (half == 0)
+        store_row<T, HD>(tmem + lane_base + kColQ, i > 0, static_cast<T*>(c.dq) + row * HD, c.scale, row_ok);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    __syncwarp();
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// dK, dV
+// ---------------------------------------------------------------------------
+template <typename T, int HD, bool CAP>
+__global__ void __launch_bounds__(kBwdThreads, 1)
+    causal_dkv_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__ CUtensorMap tmg,
+                      const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv,
+                      const __grid_constant__ BwdParams p) {
+  using Z = BwdSmem<HD>;
+  constexpr int TB = Z::kTile, NQ = Z::kNQ, KK = HD / 16;
+  constexpr uint32_t kColP = 128, kColV = 256, kColK = 256 + HD;  // S^T, dP^T, dV, dK
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* k_s = sm;
+  uint8_t* v_s = k_s + TB;
+  uint8_t* q_s = v_s + TB;        // [NQ]
+  uint8_t* g_s = q_s + NQ * TB;   // [NQ]
+  float2* info = reinterpret_cast<float2*>(g_s + NQ * TB);  // [NQ][128] {-lse log2e, -Delta} of the tile's queries
+  uint64_t* bars = reinterpret_cast<uint64_t*>(info + NQ * 128);
+  uint64_t* k_full = bars;
+  uint64_t* v_full = bars + 1;
+  uint64_t* q_full = bars + 2;      // [NQ] Q
+  uint64_t* g_full = q_full + NQ;   // [NQ] dO
+  uint64_t* i_full = g_full + NQ;   // [NQ] info
+  uint64_t* q_empty = i_full + NQ;  // [NQ] Q, dO read by the last product
+  uint64_t* i_empty = q_empty + NQ; // [NQ]
+  uint64_t* s_full = i_empty + NQ;
+  uint64_t* p_full = s_full + 1;    // P^T written
+  uint64_t* d_full = p_full + 1;    // dP^T computed
+  uint64_t* x_full = d_full + 1;    // dX^T written
+  uint64_t* done = x_full + 1;
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(done + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
+  static_assert((2 + 5 * NQ + 5) * 8 + 8 <= 256, "barrier area");
+
+  const CausalParams& c = p.c;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int k0 = blockIdx.x * 128, hkv = blockIdx.y, b = blockIdx.z;  // the first keys are seen by the most queries
+  int32_t* status = c.status;
+  const int last = min(k0 + 128, c.N) - 1;
+  const int t0 = k0 / 128, t1 = (query_end(c, b, last) + 127) / 128;  // query tiles
+  const int nt = max(t1 - t0, 0);
+  const int n = query_end(c, b, last) > k0 ? nt * c.E : 0;  // nobody sees a tile of padding
+
+  if (threadIdx.x == 0) {
+    mbar_init(k_full, 1);
+    mbar_init(v_full, 1);
+    for (int i = 0; i < NQ; ++i) {
+      mbar_init(&q_full[i], 1);
+      mbar_init(&g_full[i], 1);
+      mbar_init(&i_full[i], 64);
+      mbar_init(&q_empty[i], 1);
+      mbar_init(&i_empty[i], kCompute);
+    }
+    mbar_init(s_full, 1);
+    mbar_init(p_full, kCompute);
+    mbar_init(d_full, 1);
+    mbar_init(x_full, kCompute);
+    mbar_init(done, 1);
+    *abort_flag = 0;
+    mbar_fence_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_holder, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_holder;
+
+  if (warp == 0) {
+    if (lane == 0 && n > 0) {
+      mbar_expect_tx(k_full, TB);
+      load_rows<HD, 128>(k_s, &tmk, hkv, k0, b, k_full);
+      for (int i = 0; i < n; ++i) {
+        const int st = i % NQ, hq = hkv * c.E + i / nt, qt = t0 + i % nt;
+        if (i >= NQ && !mbar_wait(&q_empty[st], ((i / NQ) - 1) & 1, abort_flag, status)) break;
+        mbar_expect_tx(&q_full[st], TB);
+        load_rows<HD, 128>(q_s + st * TB, &tmq, hq, qt * 128, b, &q_full[st]);
+        if (i == 0) {
+          mbar_expect_tx(v_full, TB);
+          load_rows<HD, 128>(v_s, &tmv, hkv, k0, b, v_full);
+        }
+        mbar_expect_tx(&g_full[st], TB);
+        load_rows<HD, 128>(g_s + st * TB, &tmg, hq, qt * 128, b, &g_full[st]);
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && n > 0) {
+      constexpr uint32_t kIdS = idesc_f16(128, 128, Pack2<T>::kFmt, 0, 0);
+      constexpr uint32_t kIdA = idesc_f16(128, HD, Pack2<T>::kFmt, 0, 1);
+      const uint64_t kd = sdesc_sw128(smem_addr(k_s), 16, 1024), vd = sdesc_sw128(smem_addr(v_s), 16, 1024);
+      const uint64_t qd0 = sdesc_sw128(smem_addr(q_s), 16, 1024), gd0 = sdesc_sw128(smem_addr(g_s), 16, 1024);
+      const uint64_t qt0 = sdesc_sw128(smem_addr(q_s), BLK, 1024), gt0 = sdesc_sw128(smem_addr(g_s), BLK, 1024);
+      auto issue_s = [&](int i) {
+        if (!mbar_wait(&q_full[i % NQ], (i / NQ) & 1, abort_flag, status)) return false;
+        tc_fence_after();
+        const uint64_t qd = sdesc_add(qd0, (i % NQ) * TB);
+#pragma unroll
+        for (int kk = 0; kk < KK; ++kk) {
+          const uint32_t off = (kk >> 2) * BLK + (kk & 3) * 32;
+          mma_f16(tmem, sdesc_add(kd, off), sdesc_add(qd, off), kIdS, kk > 0 ? 1u : 0u);
+        }
+        mma_commit(s_full);
+        return true;
+      };
+      auto issue_d = [&](int i) {
+        if (!mbar_wait(&g_full[i % NQ], (i / NQ) & 1, abort_flag, status)) return false;
+        tc_fence_after();
+        const uint64_t gd = sdesc_add(gd0, (i % NQ) * TB);
+#pragma unroll
+        for (int kk = 0; kk < KK; ++kk) {
+          const uint32_t off = (kk >> 2) * BLK + (kk & 3) * 32;
+          mma_f16(tmem + kColP, sdesc_add(vd, off), sdesc_add(gd, off), kIdS, kk > 0 ? 1u : 0u);
+        }
+        mma_commit(d_full);
+        return true;
+      };
+      // dst += A (16-bit pairs at `a`, 32 columns of each 64) x the tile at bt
+      auto issue_acc = [&](uint32_t dst, uint32_t a, uint64_t bt, int i) {
+#pragma unroll
+        for (int kk = 0; kk < 8; ++kk)
+          mma_f16_ta(dst, a + (kk >> 2) * 64 + (kk & 3) * 8, sdesc_add(bt, kk * 2048), kIdA, (i > 0 || kk > 0) ? 1u : 0u);
+      };
+      bool ok = mbar_wait(k_full, 0, abort_flag, status) && issue_s(0) && mbar_wait(v_full, 0, abort_flag, status) &&
+                issue_d(0);
+      for (int i = 0; ok && i < n; ++i) {
+        const int st = i % NQ;
+        if (!mbar_wait(p_full, i & 1, abort_flag, status)) break;
+        tc_fence_after();
+        issue_acc(tmem + kColV, tmem, sdesc_add(gt0, st * TB), i);
+        if (i + 1 < n && !issue_s(i + 1)) break;
+        if (!mbar_wait(x_full, i & 1, abort_flag, status)) break;
+        tc_fence_after();
+        issue_acc(tmem + kColK, tmem + kColP, sdesc_add(qt0, st * TB), i);
+        mma_commit(&q_empty[st]);
+        if (i + 1 < n) ok = issue_d(i + 1);
+        else mma_commit(done);
+      }
+    }
+  } else if (warp < 4) {
+    // the tile's per-query numbers, two queries a thread
+    const int t = threadIdx.x - 64;
+    for (int i = 0; i < n; ++i) {
+      const int st = i % NQ, hq = hkv * c.E + i / nt, qt = t0 + i % nt;
+      float2 v[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int q = qt * 128 + t + 64 * h;
+        v[h] = make_float2(0.f, 0.f);
+        if (q < c.N) {
+          const int64_t row = ((int64_t)b * c.N + q) * c.Hq + hq;
+          v[h] = make_float2(-c.lse[row] * kLog2e, -c.delta[row]);
+        }
+      }
+      if (i >= NQ && !__all_sync(0xffffffffu, mbar_wait(&i_empty[st], ((i / NQ) - 1) & 1, abort_flag, status))) break;
+      info[st * 128 + t] = v[0];
+      info[st * 128 + t + 64] = v[1];
+      mbar_arrive(&i_full[st]);
+    }
+  } else {
+    const int half = (warp - 4) >> 2;
+    const int r = (threadIdx.x - 128) & 127, k = k0 + r;
+    const bool row_ok = k < c.N;
+    const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t s_addr = tmem + lane_base + half * 64, x_addr = s_addr + kColP;
+    const int qend = row_ok ? query_end(c, b, k) : 0;
+    bool alive = true;
+    int i = 0;
+    for (; i < n; ++i) {
+      const int st = i % NQ, qt = t0 + i % nt;
+      const int jlo = k - qt * 128 - half * 64, jhi = qend - qt * 128 - half * 64;
+      const bool interior = __all_sync(0xffffffffu, jlo <= 0 && jhi >= 64);
+      alive = __all_sync(0xffffffffu, mbar_wait(&i_full[st], (i / NQ) & 1, abort_flag, status)) &&
+              __all_sync(0xffffffffu, mbar_wait(s_full, i & 1, abort_flag, status));
+      if (!alive) break;
+      tc_fence_after();
+      const float4* inf = reinterpret_cast<const float4*>(info + st * 128 + half * 64);
+      float pg[64];
+      tmem_ld32(s_addr, pg);
+      tmem_ld32(s_addr + 32, pg + 32);
+      tmem_wait_ld();
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        uint32_t w[16];
+#pragma unroll
+        for (int m = 0; m < 32; m += 2) {
+          const float4 v = inf[16 * h + (m >> 1)];
+          float2 pr, g;
+          p_pair<CAP>(make_float2(pg[32 * h + m], pg[32 * h + m + 1]), make_float2(v.x, v.z), p.kq, p.kc, &pr, &g);
+          if (!interior) {
+            pr.x = inside(32 * h + m, jlo, jhi) ? pr.x : 0.f;
+            pr.y = inside(32 * h + m + 1, jlo, jhi) ? pr.y : 0.f;
+          }
+          w[m >> 1] = Pack2<T>::pack(pr.x, pr.y);
+          pg[32 * h + m] = g.x;
+          pg[32 * h + m + 1] = g.y;
+        }
+        tmem_st16u(s_addr + 16 * h, w);
+      }
+      tmem_wait_st();
+      tc_fence_before();
+      mbar_arrive(p_full);
+      alive = __all_sync(0xffffffffu, mbar_wait(d_full, i & 1, abort_flag, status));
+      if (!alive) break;
+      tc_fence_after();
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float dp[32];
+        uint32_t w[16];
+        tmem_ld32(x_addr + 32 * h, dp);
+        tmem_wait_ld();
+#pragma unroll
+        for (int m = 0; m < 32; m += 2) {
+          const float4 v = inf[16 * h + (m >> 1)];
+          float2 x = fmul2(make_float2(pg[32 * h + m], pg[32 * h + m + 1]),
+                           fadd2(make_float2(dp[m], dp[m + 1]), make_float2(v.y, v.w)));
+          if (!interior) {
+            x.x = inside(32 * h + m, jlo, jhi) ? x.x : 0.f;
+            x.y = inside(32 * h + m + 1, jlo, jhi) ? x.y : 0.f;
+          }
+          w[m >> 1] = Pack2<T>::pack(x.x, x.y);
+        }
+        tmem_st16u(x_addr + 16 * h, w);
+      }
+      mbar_arrive(&i_empty[st]);
+      tmem_wait_st();
+      tc_fence_before();
+      mbar_arrive(x_full);
+    }
+    if (alive && n > 0) alive = __all_sync(0xffffffffu, mbar_wait(done, 0, abort_flag, status));
+    if (alive) {
+      tc_fence_after();
+      const int64_t row = ((int64_t)b * c.N + k) * c.Hkv + hkv;
+      if (half == 0)
+        store_row<T, HD>(tmem + lane_base + kColV, n > 0, static_cast<T*>(c.dv) + row * HD, 1.f, row_ok);
+      else
+        store_row<T, HD>(tmem + lane_base + kColK, n > 0, static_cast<T*>(c.dk) + row * HD, c.scale, row_ok);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    __syncwarp();
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+template <typename T, int HD, bool CAP>
+int launch_bwd(const CausalParams& a, int dtype, cudaStream_t st) {
+  CUtensorMap mq, mg, mk, mv;
+  const int64_t gh = HD, gn = (int64_t)a.Hq * HD, gb = gn * a.N;
+  if (int rc = make_map_strided(&mq, a.q, dtype, a.B, a.N, a.Hq, HD, a.q_sb, a.q_sn, a.q_sh, 128)) return rc;
+  if (int rc = make_map_strided(&mg, a.dout, dtype, a.B, a.N, a.Hq, HD, gb, gn, gh, 128)) return rc;
+  if (int rc = make_map_strided(&mk, a.k, dtype, a.B, a.N, a.Hkv, HD, a.k_sb, a.k_sn, a.k_sh, 128)) return rc;
+  if (int rc = make_map_strided(&mv, a.v, dtype, a.B, a.N, a.Hkv, HD, a.v_sb, a.v_sn, a.v_sh, 128)) return rc;
+  BwdParams p;
+  p.c = a;
+  p.kq = a.has_cap ? a.scale / a.cap : a.scale * kLog2e;
+  p.kc = a.cap * kLog2e;
+  auto kq = causal_dq_kernel<T, HD, CAP>;
+  auto kk = causal_dkv_kernel<T, HD, CAP>;
+  if (cudaFuncSetAttribute(kq, cudaFuncAttributeMaxDynamicSharedMemorySize, BwdSmem<HD>::kDq) != cudaSuccess ||
+      cudaFuncSetAttribute(kk, cudaFuncAttributeMaxDynamicSharedMemorySize, BwdSmem<HD>::kDkv) != cudaSuccess)
+    return TC_ERR_CUDA;
+  const int tiles = (a.N + 127) / 128;
+  kq<<<dim3(tiles, a.Hq, a.B), kBwdThreads, BwdSmem<HD>::kDq, st>>>(mq, mg, mk, mv, p);
+  if (int rc = launch_status()) return rc;
+  kk<<<dim3(tiles, a.Hkv, a.B), kBwdThreads, BwdSmem<HD>::kDkv, st>>>(mq, mg, mk, mv, p);
+  return launch_status();
+}
+
+template <typename T>
+int dispatch_bwd(const CausalParams& a, int dtype, cudaStream_t st) {
+  if (a.Dk == 128)
+    return a.has_cap ? launch_bwd<T, 128, true>(a, dtype, st) : launch_bwd<T, 128, false>(a, dtype, st);
+  return a.has_cap ? launch_bwd<T, 64, true>(a, dtype, st) : launch_bwd<T, 64, false>(a, dtype, st);
+}
+
+}  // namespace
+
+bool causal_bwd_tc_supported(const CausalParams& p, int dtype) {
+  return ctc::tc_shape(p, dtype) && (uintptr_t)p.dout % 16 == 0;
+}
+
+int causal_bwd_tc(const CausalParams& p, int dtype, cudaStream_t st) {
+  return dtype == TC_BF16 ? dispatch_bwd<__nv_bfloat16>(p, dtype, st) : dispatch_bwd<__half>(p, dtype, st);
+}
+
 }  // namespace tc
