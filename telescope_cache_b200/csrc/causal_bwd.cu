@@ -22,8 +22,9 @@
 // dKV pass, TMEM: S^T, dP^T, dV, dK.  Per tile the compute warps work in two
 // halves, exp of S then dX of dP, and the tensor core does the other half's
 // products meanwhile (dK of the last tile and dP during exp; dV and the next S
-// during dX).  dQ pass, TMEM: two S, dP, dQ; S is a tile ahead, dQ and the next
-// dP run during exp.
+// during dX).  dQ pass, TMEM: S, two dP, dQ.  S of the next tile is issued as soon
+// as this one's is in registers and dP a tile ahead, so the compute warps wait
+// for no product that depends on them.
 #include "causal_tc.cuh"
 
 namespace tc {
@@ -32,7 +33,7 @@ namespace {
 using namespace ctc;
 
 constexpr int kBwdThreads = 384;
-constexpr int kCompute = 256;
+constexpr int kComputeWarps = 8;
 constexpr int BLK = 128 * 128;  // one 64-column block of a 128-row tile
 
 struct BwdParams {
@@ -44,7 +45,7 @@ template <int HD> struct BwdSmem {
   static constexpr int kTile = 128 * HD * 2;
   static constexpr int kNK = 3, kNV = 2, kNQ = 2;
   static constexpr int kDq = (2 + kNK + kNV) * kTile + 256 + 1024;
-  static constexpr int kDkv = (2 + 2 * kNQ) * kTile + kNQ * 128 * 8 + 256 + 1024;
+  static constexpr int kDkv = (2 + 2 * kNQ) * kTile + 2 * kNQ * 128 * 4 + 256 + 1024;
   static_assert(kDq <= 227 * 1024 && kDkv <= 227 * 1024, "backward shared memory exceeds the per-CTA limit");
 };
 
@@ -71,6 +72,85 @@ __device__ __forceinline__ void p_pair(float2 s, float2 nl2, float kq, float kc,
 
 // Tile column base + i inside [jlo, jhi)?
 __device__ __forceinline__ bool inside(int i, int jlo, int jhi) { return i >= jlo && i < jhi; }
+
+// dX = pg (dP + nd) of a thread's 64 columns at x_addr, as 16-bit pairs over the
+// first 32 of them (each half is read before it is overwritten).
+template <typename T, bool MASK>
+__device__ __forceinline__ void dx_columns(uint32_t x_addr, const float* pg, float2 nd, int jlo, int jhi) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    float dp[32];
+    uint32_t w[16];
+    tmem_ld32(x_addr + 32 * h, dp);
+    tmem_wait_ld();
+#pragma unroll
+    for (int k = 0; k < 32; k += 2) {
+      float2 v = fmul2(make_float2(pg[32 * h + k], pg[32 * h + k + 1]), fadd2(make_float2(dp[k], dp[k + 1]), nd));
+      if constexpr (MASK) {
+        v.x = inside(32 * h + k, jlo, jhi) ? v.x : 0.f;
+        v.y = inside(32 * h + k + 1, jlo, jhi) ? v.y : 0.f;
+      }
+      w[k >> 1] = Pack2<T>::pack(v.x, v.y);
+    }
+    tmem_st16u(x_addr + 16 * h, w);
+  }
+}
+
+// The same with one Delta per column (nd, shared memory).
+template <typename T, bool MASK>
+__device__ __forceinline__ void dx_columns_t(uint32_t x_addr, const float* pg, const float* nd, int jlo, int jhi) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    float dp[32];
+    uint32_t w[16];
+    tmem_ld32(x_addr + 32 * h, dp);
+    tmem_wait_ld();
+#pragma unroll
+    for (int k = 0; k < 32; k += 4) {
+      const float4 d = *reinterpret_cast<const float4*>(nd + 32 * h + k);
+#pragma unroll
+      for (int m = 0; m < 4; m += 2) {
+        float2 v = fmul2(make_float2(pg[32 * h + k + m], pg[32 * h + k + m + 1]),
+                         fadd2(make_float2(dp[k + m], dp[k + m + 1]), m ? make_float2(d.z, d.w) : make_float2(d.x, d.y)));
+        if constexpr (MASK) {
+          v.x = inside(32 * h + k + m, jlo, jhi) ? v.x : 0.f;
+          v.y = inside(32 * h + k + m + 1, jlo, jhi) ? v.y : 0.f;
+        }
+        w[(k + m) >> 1] = Pack2<T>::pack(v.x, v.y);
+      }
+    }
+    tmem_st16u(x_addr + 16 * h, w);
+  }
+}
+
+// P of a thread's 64 columns at s_addr (scores already in pg), as 16-bit pairs over
+// the first 32 of them; pg becomes P softcap'.  nl: -lse2 per column.
+template <typename T, bool CAP, bool MASK>
+__device__ __forceinline__ void p_columns_t(uint32_t s_addr, float* pg, const float* nl, float kq, float kc, int jlo,
+                                            int jhi) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    uint32_t w[16];
+#pragma unroll
+    for (int k = 0; k < 32; k += 4) {
+      const float4 l = *reinterpret_cast<const float4*>(nl + 32 * h + k);
+#pragma unroll
+      for (int m = 0; m < 4; m += 2) {
+        float* x = pg + 32 * h + k + m;
+        float2 pr, g;
+        p_pair<CAP>(make_float2(x[0], x[1]), m ? make_float2(l.z, l.w) : make_float2(l.x, l.y), kq, kc, &pr, &g);
+        if constexpr (MASK) {
+          pr.x = inside(32 * h + k + m, jlo, jhi) ? pr.x : 0.f;
+          pr.y = inside(32 * h + k + m + 1, jlo, jhi) ? pr.y : 0.f;
+        }
+        w[(k + m) >> 1] = Pack2<T>::pack(pr.x, pr.y);
+        x[0] = g.x;
+        x[1] = g.y;
+      }
+    }
+    tmem_st16u(s_addr + 16 * h, w);
+  }
+}
 
 // Row `r` of a 128-row fp32 accumulator in TMEM (zeros unless have) times mul, as T.
 template <typename T, int HD>
@@ -102,7 +182,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
                      const __grid_constant__ BwdParams p) {
   using Z = BwdSmem<HD>;
   constexpr int TB = Z::kTile, NK = Z::kNK, NV = Z::kNV, KK = HD / 16;
-  constexpr uint32_t kColP = 256, kColQ = 384;  // S [0, 256), dP, dQ
+  constexpr uint32_t kColP = 128, kColQ = 384;  // S, dP [128, 384), dQ
   extern __shared__ uint8_t smem_raw[];
   uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* q_s = sm;
@@ -116,13 +196,14 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   uint64_t* k_empty = k_full + NK;
   uint64_t* v_full = k_empty + NK;   // [NV]
   uint64_t* v_empty = v_full + NV;
-  uint64_t* s_full = v_empty + NV;   // [2]
-  uint64_t* p_full = s_full + 2;     // dP computed
-  uint64_t* x_full = p_full + 1;     // dX written
+  uint64_t* s_full = v_empty + NV;
+  uint64_t* s_free = s_full + 1;     // S in registers
+  uint64_t* p_full = s_free + 1;     // [2] dP computed
+  uint64_t* x_full = p_full + 2;     // dX written
   uint64_t* q_done = x_full + 1;
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(q_done + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
-  static_assert((2 + 2 * NK + 2 * NV + 5) * 8 + 8 <= 256, "barrier area");
+  static_assert((2 + 2 * NK + 2 * NV + 6) * 8 + 8 <= 256, "barrier area");
 
   const CausalParams& c = p.c;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -142,10 +223,11 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       mbar_init(&v_full[i], 1);
       mbar_init(&v_empty[i], 1);
     }
-    mbar_init(&s_full[0], 1);
-    mbar_init(&s_full[1], 1);
-    mbar_init(p_full, 1);
-    mbar_init(x_full, kCompute);
+    mbar_init(s_full, 1);
+    mbar_init(s_free, kComputeWarps);
+    mbar_init(&p_full[0], 1);
+    mbar_init(&p_full[1], 1);
+    mbar_init(x_full, kComputeWarps);
     mbar_init(q_done, 1);
     *abort_flag = 0;
     mbar_fence_init();
@@ -197,9 +279,9 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
 #pragma unroll
         for (int kk = 0; kk < KK; ++kk) {
           const uint32_t off = (kk >> 2) * BLK + (kk & 3) * 32;
-          mma_f16(tmem + (i & 1) * 128, sdesc_add(qd, off), sdesc_add(kd, off), kIdS, kk > 0 ? 1u : 0u);
+          mma_f16(tmem, sdesc_add(qd, off), sdesc_add(kd, off), kIdS, kk > 0 ? 1u : 0u);
         }
-        mma_commit(&s_full[i & 1]);
+        mma_commit(s_full);
         return true;
       };
       auto issue_p = [&](int i) {
@@ -209,25 +291,28 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
 #pragma unroll
         for (int kk = 0; kk < KK; ++kk) {
           const uint32_t off = (kk >> 2) * BLK + (kk & 3) * 32;
-          mma_f16(tmem + kColP, sdesc_add(gd, off), sdesc_add(vd, off), kIdS, kk > 0 ? 1u : 0u);
+          mma_f16(tmem + kColP + (i & 1) * 128, sdesc_add(gd, off), sdesc_add(vd, off), kIdS, kk > 0 ? 1u : 0u);
         }
-        mma_commit(p_full);
+        mma_commit(&p_full[i & 1]);
         mma_commit(&v_empty[i % NV]);
         return true;
       };
       bool ok = mbar_wait(q_full, 0, abort_flag, status) && issue_s(0) && mbar_wait(g_full, 0, abort_flag, status) &&
-                issue_p(0) && (n < 2 || issue_s(1));
+                issue_p(0);
       for (int i = 0; ok && i < n; ++i) {
+        if (i + 1 < n) {
+          if (!mbar_wait(s_free, i & 1, abort_flag, status)) break;
+          // dP of i + 1 replaces dX of i - 1: behind the product that reads it
+          if (!issue_s(i + 1) || !issue_p(i + 1)) break;
+        }
         if (!mbar_wait(x_full, i & 1, abort_flag, status)) break;
         tc_fence_after();
         const uint64_t kt = sdesc_add(kt0, (i % NK) * TB);
 #pragma unroll
         for (int kk = 0; kk < 8; ++kk)
-          mma_f16_ta(tmem + kColQ, tmem + kColP + (kk >> 2) * 64 + (kk & 3) * 8, sdesc_add(kt, kk * 2048), kIdQ,
-                     (i > 0 || kk > 0) ? 1u : 0u);
+          mma_f16_ta(tmem + kColQ, tmem + kColP + (i & 1) * 128 + (kk >> 2) * 64 + (kk & 3) * 8, sdesc_add(kt, kk * 2048),
+                     kIdQ, (i > 0 || kk > 0) ? 1u : 0u);
         mma_commit(&k_empty[i % NK]);
-        if (i + 1 < n) ok = issue_p(i + 1);
-        if (ok && i + 2 < n) ok = issue_s(i + 2);
         if (i + 1 == n) mma_commit(q_done);
       }
     }
@@ -240,20 +325,21 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     const int first = row_ok ? first_key(c, b, q) : 1, end = row_ok ? q + 1 : 0;
     const float nl = row_ok ? -c.lse[row] * kLog2e : 0.f, nd = row_ok ? -c.delta[row] : 0.f;
     const float2 nl2 = make_float2(nl, nl), nd2 = make_float2(nd, nd);
-    const uint32_t x_addr = tmem + lane_base + kColP + half * 64;
+    const uint32_t s_addr = tmem + lane_base + half * 64;
     bool alive = true;
     int i = 0;
     for (int j = j0; j < j1; ++j, ++i) {
-      alive = __all_sync(0xffffffffu, mbar_wait(&s_full[i & 1], (i >> 1) & 1, abort_flag, status));
+      alive = __all_sync(0xffffffffu, mbar_wait(s_full, i & 1, abort_flag, status));
       if (!alive) break;
       tc_fence_after();
-      const uint32_t s_addr = tmem + lane_base + (i & 1) * 128 + half * 64;
+      const uint32_t x_addr = s_addr + kColP + (i & 1) * 128;
       const int jlo = first - j * 128 - half * 64, jhi = end - j * 128 - half * 64;
-      const bool interior = __all_sync(0xffffffffu, jlo <= 0 && jhi >= 64);
       float pg[64];
       tmem_ld32(s_addr, pg);
       tmem_ld32(s_addr + 32, pg + 32);
       tmem_wait_ld();
+      tc_fence_before();
+      warp_arrive(s_free, lane);
 #pragma unroll
       for (int k = 0; k < 64; k += 2) {
         float2 pr, g;
@@ -261,29 +347,14 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         pg[k] = g.x;
         pg[k + 1] = g.y;
       }
-      alive = __all_sync(0xffffffffu, mbar_wait(p_full, i & 1, abort_flag, status));
+      alive = __all_sync(0xffffffffu, mbar_wait(&p_full[i & 1], (i >> 1) & 1, abort_flag, status));
       if (!alive) break;
       tc_fence_after();
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        float dp[32];
-        uint32_t w[16];
-        tmem_ld32(x_addr + 32 * h, dp);
-        tmem_wait_ld();
-#pragma unroll
-        for (int k = 0; k < 32; k += 2) {
-          float2 v = fmul2(make_float2(pg[32 * h + k], pg[32 * h + k + 1]), fadd2(make_float2(dp[k], dp[k + 1]), nd2));
-          if (!interior) {
-            v.x = inside(32 * h + k, jlo, jhi) ? v.x : 0.f;
-            v.y = inside(32 * h + k + 1, jlo, jhi) ? v.y : 0.f;
-          }
-          w[k >> 1] = Pack2<T>::pack(v.x, v.y);
-        }
-        tmem_st16u(x_addr + 16 * h, w);  // columns that this thread has read
-      }
+      if (__all_sync(0xffffffffu, jlo <= 0 && jhi >= 64)) dx_columns<T, false>(x_addr, pg, nd2, jlo, jhi);
+      else dx_columns<T, true>(x_addr, pg, nd2, jlo, jhi);
       tmem_wait_st();
       tc_fence_before();
-      mbar_arrive(x_full);
+      warp_arrive(x_full, lane);
     }
     if (alive && i > 0) alive = __all_sync(0xffffffffu, mbar_wait(q_done, 0, abort_flag, status));
     if (alive) {
@@ -318,8 +389,9 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   uint8_t* v_s = k_s + TB;
   uint8_t* q_s = v_s + TB;        // [NQ]
   uint8_t* g_s = q_s + NQ * TB;   // [NQ]
-  float2* info = reinterpret_cast<float2*>(g_s + NQ * TB);  // [NQ][128] {-lse log2e, -Delta} of the tile's queries
-  uint64_t* bars = reinterpret_cast<uint64_t*>(info + NQ * 128);
+  float* nl_s = reinterpret_cast<float*>(g_s + NQ * TB);  // [NQ][128] -lse log2e of the tile's queries
+  float* nd_s = nl_s + NQ * 128;                          // [NQ][128] -Delta
+  uint64_t* bars = reinterpret_cast<uint64_t*>(nd_s + NQ * 128);
   uint64_t* k_full = bars;
   uint64_t* v_full = bars + 1;
   uint64_t* q_full = bars + 2;      // [NQ] Q
@@ -353,12 +425,12 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       mbar_init(&g_full[i], 1);
       mbar_init(&i_full[i], 64);
       mbar_init(&q_empty[i], 1);
-      mbar_init(&i_empty[i], kCompute);
+      mbar_init(&i_empty[i], kComputeWarps);
     }
     mbar_init(s_full, 1);
-    mbar_init(p_full, kCompute);
+    mbar_init(p_full, kComputeWarps);
     mbar_init(d_full, 1);
-    mbar_init(x_full, kCompute);
+    mbar_init(x_full, kComputeWarps);
     mbar_init(done, 1);
     *abort_flag = 0;
     mbar_fence_init();
@@ -458,8 +530,11 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         }
       }
       if (i >= NQ && !__all_sync(0xffffffffu, mbar_wait(&i_empty[st], ((i / NQ) - 1) & 1, abort_flag, status))) break;
-      info[st * 128 + t] = v[0];
-      info[st * 128 + t + 64] = v[1];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        nl_s[st * 128 + t + 64 * h] = v[h].x;
+        nd_s[st * 128 + t + 64 * h] = v[h].y;
+      }
       mbar_arrive(&i_full[st]);
     }
   } else {
@@ -479,58 +554,26 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
               __all_sync(0xffffffffu, mbar_wait(s_full, i & 1, abort_flag, status));
       if (!alive) break;
       tc_fence_after();
-      const float4* inf = reinterpret_cast<const float4*>(info + st * 128 + half * 64);
+      const float* nl = nl_s + st * 128 + half * 64;
+      const float* nd = nd_s + st * 128 + half * 64;
       float pg[64];
       tmem_ld32(s_addr, pg);
       tmem_ld32(s_addr + 32, pg + 32);
       tmem_wait_ld();
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        uint32_t w[16];
-#pragma unroll
-        for (int m = 0; m < 32; m += 2) {
-          const float4 v = inf[16 * h + (m >> 1)];
-          float2 pr, g;
-          p_pair<CAP>(make_float2(pg[32 * h + m], pg[32 * h + m + 1]), make_float2(v.x, v.z), p.kq, p.kc, &pr, &g);
-          if (!interior) {
-            pr.x = inside(32 * h + m, jlo, jhi) ? pr.x : 0.f;
-            pr.y = inside(32 * h + m + 1, jlo, jhi) ? pr.y : 0.f;
-          }
-          w[m >> 1] = Pack2<T>::pack(pr.x, pr.y);
-          pg[32 * h + m] = g.x;
-          pg[32 * h + m + 1] = g.y;
-        }
-        tmem_st16u(s_addr + 16 * h, w);
-      }
+      if (interior) p_columns_t<T, CAP, false>(s_addr, pg, nl, p.kq, p.kc, jlo, jhi);
+      else p_columns_t<T, CAP, true>(s_addr, pg, nl, p.kq, p.kc, jlo, jhi);
       tmem_wait_st();
       tc_fence_before();
-      mbar_arrive(p_full);
+      warp_arrive(p_full, lane);
       alive = __all_sync(0xffffffffu, mbar_wait(d_full, i & 1, abort_flag, status));
       if (!alive) break;
       tc_fence_after();
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        float dp[32];
-        uint32_t w[16];
-        tmem_ld32(x_addr + 32 * h, dp);
-        tmem_wait_ld();
-#pragma unroll
-        for (int m = 0; m < 32; m += 2) {
-          const float4 v = inf[16 * h + (m >> 1)];
-          float2 x = fmul2(make_float2(pg[32 * h + m], pg[32 * h + m + 1]),
-                           fadd2(make_float2(dp[m], dp[m + 1]), make_float2(v.y, v.w)));
-          if (!interior) {
-            x.x = inside(32 * h + m, jlo, jhi) ? x.x : 0.f;
-            x.y = inside(32 * h + m + 1, jlo, jhi) ? x.y : 0.f;
-          }
-          w[m >> 1] = Pack2<T>::pack(x.x, x.y);
-        }
-        tmem_st16u(x_addr + 16 * h, w);
-      }
-      mbar_arrive(&i_empty[st]);
+      if (interior) dx_columns_t<T, false>(x_addr, pg, nd, jlo, jhi);
+      else dx_columns_t<T, true>(x_addr, pg, nd, jlo, jhi);
       tmem_wait_st();
       tc_fence_before();
-      mbar_arrive(x_full);
+      warp_arrive(&i_empty[st], lane);
+      warp_arrive(x_full, lane);
     }
     if (alive && n > 0) alive = __all_sync(0xffffffffu, mbar_wait(done, 0, abort_flag, status));
     if (alive) {

@@ -165,7 +165,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
     for (int i = 0; i < 2; ++i) {
       mbar_init(&q_full[i], 1);
       mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i], 128);
+      mbar_init(&p_full[i], 4);
       mbar_init(&o_done[i], 1);
     }
     for (int i = 0; i < NS; ++i) {
@@ -372,7 +372,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
       ell += ts;
       tmem_wait_st();
       tc_fence_before();
-      mbar_arrive(&p_full[x]);
+      warp_arrive(&p_full[x], lane);
     }
     if (alive && n > 0) alive = __all_sync(0xffffffffu, mbar_wait(&o_done[x], 0, abort_flag, status));
     if (alive) {

@@ -39,6 +39,13 @@ __device__ __forceinline__ void load_rows(uint8_t* dst, const CUtensorMap* m, in
   for (int c = 0; c < HD / 64; ++c) tma_load_4d(dst + c * ROWS * 128, m, 64 * c, h, n, b, bar);
 }
 
+// One arrival for the warp, behind every lane's accesses (barriers of the compute
+// warps count warps: 32 arrivals on one address would be served one by one).
+__device__ __forceinline__ void warp_arrive(uint64_t* bar, int lane) {
+  __syncwarp();
+  if (lane == 0) mbar_arrive(bar);
+}
+
 inline bool strides_ok(const void* p, int64_t sb, int64_t sn, int64_t sh, int64_t B, int64_t N, int64_t H) {
   const int64_t most = int64_t(1) << 38;  // elements: a map's byte stride stays below 2^40
   return (uintptr_t)p % 16 == 0 && (B == 1 || (sb % 8 == 0 && sb > 0 && sb < most)) &&
