@@ -181,7 +181,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
                      const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv,
                      const __grid_constant__ BwdParams p) {
   using Z = BwdSmem<HD>;
-  constexpr int TB = Z::kTile, NK = Z::kNK, NV = Z::kNV, KK = HD / 16;
+  constexpr int TB = Z::kTile, NK = Z::kNK, NV = Z::kNV;
   constexpr uint32_t kColP = 128, kColQ = 384;  // S, dP [128, 384), dQ
   extern __shared__ uint8_t smem_raw[];
   uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -206,7 +206,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   static_assert((2 + 2 * NK + 2 * NV + 6) * 8 + 8 <= 256, "barrier area");
 
   const CausalParams& c = p.c;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   const int q0 = (gridDim.x - 1 - blockIdx.x) * 128, hq = blockIdx.y, b = blockIdx.z, hkv = hq / c.E;
   int32_t* status = c.status;
   const int first0 = first_key(c, b, q0), last = min(q0 + 128, c.N) - 1;
@@ -264,54 +264,45 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         if (j + 1 < j1) ok = load_k(j + 1);
       }
     }
-  } else if (warp == 1) {
-    if (lane == 0 && j0 < j1) {
-      constexpr uint32_t kIdS = idesc_f16(128, 128, Pack2<T>::kFmt, 0, 0);
-      constexpr uint32_t kIdQ = idesc_f16(128, HD, Pack2<T>::kFmt, 0, 1);
-      const uint64_t qd = sdesc_sw128(smem_addr(q_s), 16, 1024), gd = sdesc_sw128(smem_addr(g_s), 16, 1024);
-      const uint64_t kd0 = sdesc_sw128(smem_addr(k_s), 16, 1024), vd0 = sdesc_sw128(smem_addr(v_s), 16, 1024);
-      const uint64_t kt0 = sdesc_sw128(smem_addr(k_s), BLK, 1024);
-      const int n = j1 - j0;
-      auto issue_s = [&](int i) {
-        if (!mbar_wait(&k_full[i % NK], (i / NK) & 1, abort_flag, status)) return false;
-        const uint64_t kd = sdesc_add(kd0, (i % NK) * TB);
-        tc_fence_after();
-#pragma unroll
-        for (int kk = 0; kk < KK; ++kk) {
-          const uint32_t off = (kk >> 2) * BLK + (kk & 3) * 32;
-          mma_f16(tmem, sdesc_add(qd, off), sdesc_add(kd, off), kIdS, kk > 0 ? 1u : 0u);
-        }
+  } else if (warp == 1 && j0 < j1) {
+    constexpr uint32_t kIdS = idesc_f16(128, 128, Pack2<T>::kFmt, 0, 0);
+    constexpr uint32_t kIdQ = idesc_f16(128, HD, Pack2<T>::kFmt, 0, 1);
+    const uint32_t qd = desc_lo(q_s, 16), gd = desc_lo(g_s, 16), kd0 = desc_lo(k_s, 16), vd0 = desc_lo(v_s, 16),
+                   kt0 = desc_lo(k_s, BLK);
+    const uint32_t tm = uniform(tmem);
+    const int n = uniform(j1 - j0);
+    const bool leader = elect_one();
+    auto issue_s = [&](int i) {
+      if (!mbar_wait(&k_full[i % NK], (i / NK) & 1, abort_flag, status)) return false;
+      tc_fence_after();
+      if (leader) {
+        mma_tile_ss<HD>(tm, qd, kd0 + (((i % NK) * TB) >> 4), kIdS);
         mma_commit(s_full);
-        return true;
-      };
-      auto issue_p = [&](int i) {
-        if (!mbar_wait(&v_full[i % NV], (i / NV) & 1, abort_flag, status)) return false;
-        const uint64_t vd = sdesc_add(vd0, (i % NV) * TB);
-        tc_fence_after();
-#pragma unroll
-        for (int kk = 0; kk < KK; ++kk) {
-          const uint32_t off = (kk >> 2) * BLK + (kk & 3) * 32;
-          mma_f16(tmem + kColP + (i & 1) * 128, sdesc_add(gd, off), sdesc_add(vd, off), kIdS, kk > 0 ? 1u : 0u);
-        }
+      }
+      return true;
+    };
+    auto issue_p = [&](int i) {
+      if (!mbar_wait(&v_full[i % NV], (i / NV) & 1, abort_flag, status)) return false;
+      tc_fence_after();
+      if (leader) {
+        mma_tile_ss<HD>(tm + kColP + (i & 1) * 128, gd, vd0 + (((i % NV) * TB) >> 4), kIdS);
         mma_commit(&p_full[i & 1]);
         mma_commit(&v_empty[i % NV]);
-        return true;
-      };
-      bool ok = mbar_wait(q_full, 0, abort_flag, status) && issue_s(0) && mbar_wait(g_full, 0, abort_flag, status) &&
-                issue_p(0);
-      for (int i = 0; ok && i < n; ++i) {
-        if (i + 1 < n) {
-          if (!mbar_wait(s_free, i & 1, abort_flag, status)) break;
-          // dP of i + 1 replaces dX of i - 1: behind the product that reads it
-          if (!issue_s(i + 1) || !issue_p(i + 1)) break;
-        }
-        if (!mbar_wait(x_full, i & 1, abort_flag, status)) break;
-        tc_fence_after();
-        const uint64_t kt = sdesc_add(kt0, (i % NK) * TB);
-#pragma unroll
-        for (int kk = 0; kk < 8; ++kk)
-          mma_f16_ta(tmem + kColQ, tmem + kColP + (i & 1) * 128 + (kk >> 2) * 64 + (kk & 3) * 8, sdesc_add(kt, kk * 2048),
-                     kIdQ, (i > 0 || kk > 0) ? 1u : 0u);
+      }
+      return true;
+    };
+    bool ok = mbar_wait(q_full, 0, abort_flag, status) && issue_s(0) && mbar_wait(g_full, 0, abort_flag, status) &&
+              issue_p(0);
+    for (int i = 0; ok && i < n; ++i) {
+      if (i + 1 < n) {
+        if (!mbar_wait(s_free, i & 1, abort_flag, status)) break;
+        // dP of i + 1 replaces dX of i - 1: behind the product that reads it
+        if (!issue_s(i + 1) || !issue_p(i + 1)) break;
+      }
+      if (!mbar_wait(x_full, i & 1, abort_flag, status)) break;
+      tc_fence_after();
+      if (leader) {
+        mma_tile_ts(tm + kColQ, tm + kColP + (i & 1) * 128, 64, kt0 + (((i % NK) * TB) >> 4), kIdQ, i > 0 ? 1u : 0u);
         mma_commit(&k_empty[i % NK]);
         if (i + 1 == n) mma_commit(q_done);
       }
@@ -381,7 +372,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
                       const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv,
                       const __grid_constant__ BwdParams p) {
   using Z = BwdSmem<HD>;
-  constexpr int TB = Z::kTile, NQ = Z::kNQ, KK = HD / 16;
+  constexpr int TB = Z::kTile, NQ = Z::kNQ;
   constexpr uint32_t kColP = 128, kColV = 256, kColK = 256 + HD;  // S^T, dP^T, dV, dK
   extern __shared__ uint8_t smem_raw[];
   uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -409,7 +400,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   static_assert((2 + 5 * NQ + 5) * 8 + 8 <= 256, "barrier area");
 
   const CausalParams& c = p.c;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   const int k0 = blockIdx.x * 128, hkv = blockIdx.y, b = blockIdx.z;  // the first keys are seen by the most queries
   int32_t* status = c.status;
   const int last = min(k0 + 128, c.N) - 1;
@@ -462,57 +453,47 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       }
     }
   } else if (warp == 1) {
-    if (lane == 0 && n > 0) {
-      constexpr uint32_t kIdS = idesc_f16(128, 128, Pack2<T>::kFmt, 0, 0);
-      constexpr uint32_t kIdA = idesc_f16(128, HD, Pack2<T>::kFmt, 0, 1);
-      const uint64_t kd = sdesc_sw128(smem_addr(k_s), 16, 1024), vd = sdesc_sw128(smem_addr(v_s), 16, 1024);
-      const uint64_t qd0 = sdesc_sw128(smem_addr(q_s), 16, 1024), gd0 = sdesc_sw128(smem_addr(g_s), 16, 1024);
-      const uint64_t qt0 = sdesc_sw128(smem_addr(q_s), BLK, 1024), gt0 = sdesc_sw128(smem_addr(g_s), BLK, 1024);
-      auto issue_s = [&](int i) {
-        if (!mbar_wait(&q_full[i % NQ], (i / NQ) & 1, abort_flag, status)) return false;
-        tc_fence_after();
-        const uint64_t qd = sdesc_add(qd0, (i % NQ) * TB);
-#pragma unroll
-        for (int kk = 0; kk < KK; ++kk) {
-          const uint32_t off = (kk >> 2) * BLK + (kk & 3) * 32;
-          mma_f16(tmem, sdesc_add(kd, off), sdesc_add(qd, off), kIdS, kk > 0 ? 1u : 0u);
-        }
+    constexpr uint32_t kIdS = idesc_f16(128, 128, Pack2<T>::kFmt, 0, 0);
+    constexpr uint32_t kIdA = idesc_f16(128, HD, Pack2<T>::kFmt, 0, 1);
+    const uint32_t kd = desc_lo(k_s, 16), vd = desc_lo(v_s, 16), qd0 = desc_lo(q_s, 16), gd0 = desc_lo(g_s, 16),
+                   qt0 = desc_lo(q_s, BLK), gt0 = desc_lo(g_s, BLK);
+    const uint32_t tm = uniform(tmem);
+    const int un = uniform(n);
+    const bool leader = elect_one();
+    auto issue_s = [&](int i) {
+      if (!mbar_wait(&q_full[i % NQ], (i / NQ) & 1, abort_flag, status)) return false;
+      tc_fence_after();
+      if (leader) {
+        mma_tile_ss<HD>(tm, kd, qd0 + (((i % NQ) * TB) >> 4), kIdS);
         mma_commit(s_full);
-        return true;
-      };
-      auto issue_d = [&](int i) {
-        if (!mbar_wait(&g_full[i % NQ], (i / NQ) & 1, abort_flag, status)) return false;
-        tc_fence_after();
-        const uint64_t gd = sdesc_add(gd0, (i % NQ) * TB);
-#pragma unroll
-        for (int kk = 0; kk < KK; ++kk) {
-          const uint32_t off = (kk >> 2) * BLK + (kk & 3) * 32;
-          mma_f16(tmem + kColP, sdesc_add(vd, off), sdesc_add(gd, off), kIdS, kk > 0 ? 1u : 0u);
-        }
-        mma_commit(d_full);
-        return true;
-      };
-      // dst += A (16-bit pairs at `a`, 32 columns of each 64) x the tile at bt
-      auto issue_acc = [&](uint32_t dst, uint32_t a, uint64_t bt, int i) {
-#pragma unroll
-        for (int kk = 0; kk < 8; ++kk)
-          mma_f16_ta(dst, a + (kk >> 2) * 64 + (kk & 3) * 8, sdesc_add(bt, kk * 2048), kIdA, (i > 0 || kk > 0) ? 1u : 0u);
-      };
-      bool ok = mbar_wait(k_full, 0, abort_flag, status) && issue_s(0) && mbar_wait(v_full, 0, abort_flag, status) &&
-                issue_d(0);
-      for (int i = 0; ok && i < n; ++i) {
-        const int st = i % NQ;
-        if (!mbar_wait(p_full, i & 1, abort_flag, status)) break;
-        tc_fence_after();
-        issue_acc(tmem + kColV, tmem, sdesc_add(gt0, st * TB), i);
-        if (i + 1 < n && !issue_s(i + 1)) break;
-        if (!mbar_wait(x_full, i & 1, abort_flag, status)) break;
-        tc_fence_after();
-        issue_acc(tmem + kColK, tmem + kColP, sdesc_add(qt0, st * TB), i);
-        mma_commit(&q_empty[st]);
-        if (i + 1 < n) ok = issue_d(i + 1);
-        else mma_commit(done);
       }
+      return true;
+    };
+    auto issue_d = [&](int i) {
+      if (!mbar_wait(&g_full[i % NQ], (i / NQ) & 1, abort_flag, status)) return false;
+      tc_fence_after();
+      if (leader) {
+        mma_tile_ss<HD>(tm + kColP, vd, gd0 + (((i % NQ) * TB) >> 4), kIdS);
+        mma_commit(d_full);
+      }
+      return true;
+    };
+    bool ok = un > 0 && mbar_wait(k_full, 0, abort_flag, status) && issue_s(0) &&
+              mbar_wait(v_full, 0, abort_flag, status) && issue_d(0);
+    for (int i = 0; ok && i < un; ++i) {
+      const int st = i % NQ;
+      if (!mbar_wait(p_full, i & 1, abort_flag, status)) break;
+      tc_fence_after();
+      if (leader) mma_tile_ts(tm + kColV, tm, 64, gt0 + ((st * TB) >> 4), kIdA, i > 0 ? 1u : 0u);
+      if (i + 1 < un && !issue_s(i + 1)) break;
+      if (!mbar_wait(x_full, i & 1, abort_flag, status)) break;
+      tc_fence_after();
+      if (leader) {
+        mma_tile_ts(tm + kColK, tm + kColP, 64, qt0 + ((st * TB) >> 4), kIdA, i > 0 ? 1u : 0u);
+        mma_commit(&q_empty[st]);
+        if (i + 1 == un) mma_commit(done);
+      }
+      if (i + 1 < un) ok = issue_d(i + 1);
     }
   } else if (warp < 4) {
     // the tile's per-query numbers, two queries a thread

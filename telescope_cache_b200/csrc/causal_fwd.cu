@@ -131,7 +131,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
     causal_fwd_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__ CUtensorMap tmk,
                       const __grid_constant__ CUtensorMap tmv, const __grid_constant__ FwdParams p) {
   using Z = FwdSmem<HD>;
-  constexpr int TB = Z::kTile, NS = Z::kStages, BLK = 128 * 128, KK = HD / 16;
+  constexpr int TB = Z::kTile, NS = Z::kStages, BLK = 128 * 128;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* q_s = sm;             // [2] Q tiles
@@ -151,7 +151,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
   static_assert((8 + 4 * NS) * 8 + 8 <= 256, "barrier area");
 
   const CausalParams& c = p.c;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   const int q0 = (gridDim.x - 1 - blockIdx.x) * 256, hq = blockIdx.y, b = blockIdx.z;
   const int hkv = hq / c.E;
   int32_t* status = c.status;
@@ -213,56 +213,52 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
       }
     }
   } else if (warp == 1) {
-    if (lane == 0) {
-      constexpr uint32_t kIdS = idesc_f16(128, KT, Pack2<T>::kFmt, 0, 0);
-      constexpr uint32_t kIdO = idesc_f16(128, HD, Pack2<T>::kFmt, 0, 1);
-      const uint64_t qd0 = sdesc_sw128(smem_addr(q_s), 16, 1024);
-      const uint64_t kd0 = sdesc_sw128(smem_addr(k_s), 16, 1024);
-      const uint64_t vd0 = sdesc_sw128(smem_addr(v_s), BLK, 1024);
-      int nP[2] = {0, 0};
-      auto issue_s = [&](int x, int st) {
-        const uint64_t qd = sdesc_add(qd0, x * TB), kd = sdesc_add(kd0, st * TB);
-#pragma unroll
-        for (int kk = 0; kk < KK; ++kk) {
-          const uint32_t off = (kk >> 2) * BLK + (kk & 3) * 32;
-          mma_f16(tmem + x * 128, sdesc_add(qd, off), sdesc_add(kd, off), kIdS, kk > 0 ? 1u : 0u);
-        }
+    constexpr uint32_t kIdS = idesc_f16(128, KT, Pack2<T>::kFmt, 0, 0);
+    constexpr uint32_t kIdO = idesc_f16(128, HD, Pack2<T>::kFmt, 0, 1);
+    const uint32_t qd0 = desc_lo(q_s, 16), kd0 = desc_lo(k_s, 16), vd0 = desc_lo(v_s, BLK);
+    const uint32_t tm = uniform(tmem);
+    const int ua0 = uniform(has_a ? alo : 0), ua1 = uniform(has_a ? ahi : 0), ub0 = uniform(has_b ? blo : 0),
+              ub1 = uniform(has_b ? bhi : 0), u0 = uniform(j0), u1 = uniform(j1);
+    const bool leader = elect_one();
+    int np0 = 0, np1 = 0;
+    auto issue_s = [&](int x, int st) {
+      if (leader) {
+        mma_tile_ss<HD>(tm + x * 128, qd0 + ((x * TB) >> 4), kd0 + ((st * TB) >> 4), kIdS);
         mma_commit(&s_full[x]);
-      };
-      auto issue_pv = [&](int x, int st) -> bool {
-        if (!mbar_wait(&p_full[x], nP[x] & 1, abort_flag, status)) return false;
-        tc_fence_after();
-        const uint64_t vd = sdesc_add(vd0, st * TB);
-#pragma unroll
-        for (int kk = 0; kk < KT / 16; ++kk)
-          mma_f16_ta(tmem + 256 + x * HD, tmem + x * 128 + kk * 8, sdesc_add(vd, kk * 2048), kIdO,
-                     (nP[x] > 0 || kk > 0) ? 1u : 0u);
-        ++nP[x];
-        return true;
-      };
-      bool ok = j0 < j1;
-      if (ok) ok = mbar_wait(&k_full[0], 0, abort_flag, status);
-      if (ok && has_a) ok = mbar_wait(&q_full[0], 0, abort_flag, status);
-      if (ok && has_b) ok = mbar_wait(&q_full[1], 0, abort_flag, status);
+      }
+    };
+    auto issue_pv = [&](int x, int& np, int st) -> bool {
+      if (!mbar_wait(&p_full[x], np & 1, abort_flag, status)) return false;
       tc_fence_after();
-      if (ok) {
-        if (has_a && j0 == alo) issue_s(0, 0);
-        if (has_b && j0 == blo) issue_s(1, 0);
-        mma_commit(&k_empty[0]);
-      }
-      for (int j = j0, i = 0; ok && j < j1; ++j, ++i) {
-        const int st = i % NS, st1 = (i + 1) % NS;
-        if (j + 1 < j1 && !mbar_wait(&k_full[st1], ((i + 1) / NS) & 1, abort_flag, status)) break;
-        if (!mbar_wait(&v_full[st], (i / NS) & 1, abort_flag, status)) break;
-        if (has_a && j >= alo && j < ahi && !issue_pv(0, st)) break;
-        if (has_a && j + 1 >= alo && j + 1 < ahi) issue_s(0, st1);
-        if (has_a && j + 1 == ahi) mma_commit(&o_done[0]);
-        if (has_b && j >= blo && j < bhi && !issue_pv(1, st)) break;
-        mma_commit(&v_empty[st]);
-        if (has_b && j + 1 >= blo && j + 1 < bhi) issue_s(1, st1);
-        if (has_b && j + 1 == bhi) mma_commit(&o_done[1]);
-        if (j + 1 < j1) mma_commit(&k_empty[st1]);
-      }
+      if (leader) mma_tile_ts(tm + 256 + x * HD, tm + x * 128, 32, vd0 + ((st * TB) >> 4), kIdO, np > 0 ? 1u : 0u);
+      ++np;
+      return true;
+    };
+    auto commit = [&](uint64_t* bar) {
+      if (leader) mma_commit(bar);
+    };
+    bool ok = u0 < u1;
+    if (ok) ok = mbar_wait(&k_full[0], 0, abort_flag, status);
+    if (ok && ua0 < ua1) ok = mbar_wait(&q_full[0], 0, abort_flag, status);
+    if (ok && ub0 < ub1) ok = mbar_wait(&q_full[1], 0, abort_flag, status);
+    tc_fence_after();
+    if (ok) {
+      if (u0 >= ua0 && u0 < ua1) issue_s(0, 0);
+      if (u0 >= ub0 && u0 < ub1) issue_s(1, 0);
+      commit(&k_empty[0]);
+    }
+    for (int j = u0, i = 0; ok && j < u1; ++j, ++i) {
+      const int st = i % NS, st1 = (i + 1) % NS;
+      if (j + 1 < u1 && !mbar_wait(&k_full[st1], ((i + 1) / NS) & 1, abort_flag, status)) break;
+      if (!mbar_wait(&v_full[st], (i / NS) & 1, abort_flag, status)) break;
+      if (j >= ua0 && j < ua1 && !issue_pv(0, np0, st)) break;
+      if (j + 1 >= ua0 && j + 1 < ua1) issue_s(0, st1);
+      if (ua0 < ua1 && j + 1 == ua1) commit(&o_done[0]);
+      if (j >= ub0 && j < ub1 && !issue_pv(1, np1, st)) break;
+      commit(&v_empty[st]);
+      if (j + 1 >= ub0 && j + 1 < ub1) issue_s(1, st1);
+      if (ub0 < ub1 && j + 1 == ub1) commit(&o_done[1]);
+      if (j + 1 < u1) commit(&k_empty[st1]);
     }
   } else if (warp >= 4) {
     const int x = (warp - 4) >> 2;

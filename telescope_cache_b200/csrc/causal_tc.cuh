@@ -39,6 +39,64 @@ __device__ __forceinline__ void load_rows(uint8_t* dst, const CUtensorMap* m, in
   for (int c = 0; c < HD / 64; ++c) tma_load_4d(dst + c * ROWS * 128, m, 64 * c, h, n, b, bar);
 }
 
+// MMA issue by a converged warp: every lane walks the loop, so that descriptors
+// stay in uniform registers, and one elected lane issues.  (One lane alone in
+// the branch had the issue of 24 products take 2200 cycles: each operand moved
+// to a uniform register by itself.)  Descriptors: the low word holds the
+// address and the leading offset, the high word is the same for every operand
+// here (1024-byte stride of 8-row groups, 128-byte swizzle).
+constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t desc_lo(const void* s, uint32_t lbo) {
+  return ((smem_addr(s) & 0x3FFFFu) >> 4) | ((lbo >> 4) << 16);
+}
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.b32 %0, 1, 0, p;\n\t}"
+      : "=r"(r));
+  return r != 0;
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t alo, uint32_t blo, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\t"
+      "mov.b64 a, {%1, %5};\n\t"
+      "mov.b64 b, {%2, %5};\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t}" ::"r"(d),
+      "r"(alo), "r"(blo), "r"(idesc), "r"(acc), "n"(kDescHi)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t blo, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\t"
+      "mov.b64 b, {%2, %5};\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(blo), "r"(idesc), "r"(acc), "n"(kDescHi)
+      : "memory");
+}
+// d = A B^T of two K-major 128 x HD tiles.
+template <int HD>
+__device__ __forceinline__ void mma_tile_ss(uint32_t d, uint32_t alo, uint32_t blo, uint32_t idesc) {
+#pragma unroll
+  for (int kk = 0; kk < HD / 16; ++kk) {
+    const uint32_t off = ((kk >> 2) * 128 * 128 + (kk & 3) * 32) >> 4;
+    mma_ss(d, alo + off, blo + off, idesc, kk > 0 ? 1u : 0u);
+  }
+}
+// d (+)= A B of A [128 x 128] in TMEM (16-bit pairs: 32 columns from a and 32 from
+// a + second) and an MN-major 128 x HD tile.
+__device__ __forceinline__ void mma_tile_ts(uint32_t d, uint32_t a, uint32_t second, uint32_t blo, uint32_t idesc,
+                                            uint32_t acc) {
+#pragma unroll
+  for (int kk = 0; kk < 8; ++kk)
+    mma_ts(d, a + (kk >> 2) * second + (kk & 3) * 8, blo + ((kk * 2048) >> 4), idesc, kk > 0 ? 1u : acc);
+}
+// A value that every lane holds alike, known to be uniform.
+__device__ __forceinline__ int uniform(int v) { return __shfl_sync(0xffffffffu, v, 0); }
+
 // One arrival for the warp, behind every lane's accesses (barriers of the compute
 // warps count warps: 32 arrivals on one address would be served one by one).
 __device__ __forceinline__ void warp_arrive(uint64_t* bar, int lane) {
