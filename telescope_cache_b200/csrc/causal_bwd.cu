@@ -32,8 +32,14 @@ namespace {
 
 using namespace ctc;
 
-constexpr int kBwdThreads = 384;
-constexpr int kComputeWarps = 8;
+// Columns of a tile per compute thread, and the CTA's sizes that follow.
+template <int COLS> struct Shape {
+  static constexpr int kParts = 128 / COLS;             // threads per TMEM lane
+  static constexpr int kWarps = 4 * kParts;             // compute warps
+  static constexpr int kThreads = 128 + 32 * kWarps;
+  static constexpr int kSteps = COLS / 16;              // 16-column steps of an A operand per thread
+};
+constexpr int kDqCols = 64, kDkvCols = 32;
 constexpr int BLK = 128 * 128;  // one 64-column block of a 128-row tile
 
 struct BwdParams {
@@ -73,12 +79,12 @@ __device__ __forceinline__ void p_pair(float2 s, float2 nl2, float kq, float kc,
 // Tile column base + i inside [jlo, jhi)?
 __device__ __forceinline__ bool inside(int i, int jlo, int jhi) { return i >= jlo && i < jhi; }
 
-// dX = pg (dP + nd) of a thread's 64 columns at x_addr, as 16-bit pairs over the
-// first 32 of them (each half is read before it is overwritten).
-template <typename T, bool MASK>
+// dX = pg (dP + nd) of a thread's COLS columns at x_addr, as 16-bit pairs over the
+// first half of them (each 32 are read before they are overwritten).
+template <typename T, int COLS, bool MASK>
 __device__ __forceinline__ void dx_columns(uint32_t x_addr, const float* pg, float2 nd, int jlo, int jhi) {
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
+  for (int h = 0; h < COLS / 32; ++h) {
     float dp[32];
     uint32_t w[16];
     tmem_ld32(x_addr + 32 * h, dp);
@@ -97,10 +103,10 @@ __device__ __forceinline__ void dx_columns(uint32_t x_addr, const float* pg, flo
 }
 
 // The same with one Delta per column (nd, shared memory).
-template <typename T, bool MASK>
+template <typename T, int COLS, bool MASK>
 __device__ __forceinline__ void dx_columns_t(uint32_t x_addr, const float* pg, const float* nd, int jlo, int jhi) {
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
+  for (int h = 0; h < COLS / 32; ++h) {
     float dp[32];
     uint32_t w[16];
     tmem_ld32(x_addr + 32 * h, dp);
@@ -123,13 +129,13 @@ __device__ __forceinline__ void dx_columns_t(uint32_t x_addr, const float* pg, c
   }
 }
 
-// P of a thread's 64 columns at s_addr (scores already in pg), as 16-bit pairs over
-// the first 32 of them; pg becomes P softcap'.  nl: -lse2 per column.
-template <typename T, bool CAP, bool MASK>
+// P of a thread's COLS columns at s_addr (scores already in pg), as 16-bit pairs over
+// the first half of them; pg becomes P softcap'.  nl: -lse2 per column.
+template <typename T, int COLS, bool CAP, bool MASK>
 __device__ __forceinline__ void p_columns_t(uint32_t s_addr, float* pg, const float* nl, float kq, float kc, int jlo,
                                             int jhi) {
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
+  for (int h = 0; h < COLS / 32; ++h) {
     uint32_t w[16];
 #pragma unroll
     for (int k = 0; k < 32; k += 4) {
@@ -176,7 +182,7 @@ __device__ __forceinline__ void store_row(uint32_t taddr, bool have, T* out, flo
 // dQ
 // ---------------------------------------------------------------------------
 template <typename T, int HD, bool CAP>
-__global__ void __launch_bounds__(kBwdThreads, 1)
+__global__ void __launch_bounds__(Shape<kDqCols>::kThreads, 1)
     causal_dq_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__ CUtensorMap tmg,
                      const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv,
                      const __grid_constant__ BwdParams p) {
@@ -224,10 +230,10 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       mbar_init(&v_empty[i], 1);
     }
     mbar_init(s_full, 1);
-    mbar_init(s_free, kComputeWarps);
+    mbar_init(s_free, Shape<kDqCols>::kWarps);
     mbar_init(&p_full[0], 1);
     mbar_init(&p_full[1], 1);
-    mbar_init(x_full, kComputeWarps);
+    mbar_init(x_full, Shape<kDqCols>::kWarps);
     mbar_init(q_done, 1);
     *abort_flag = 0;
     mbar_fence_init();
@@ -302,13 +308,15 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       if (!mbar_wait(x_full, i & 1, abort_flag, status)) break;
       tc_fence_after();
       if (leader) {
-        mma_tile_ts(tm + kColQ, tm + kColP + (i & 1) * 128, 64, kt0 + (((i % NK) * TB) >> 4), kIdQ, i > 0 ? 1u : 0u);
+        mma_tile_ts<Shape<kDqCols>::kSteps, kDqCols>(tm + kColQ, tm + kColP + (i & 1) * 128,
+                                                     kt0 + (((i % NK) * TB) >> 4), kIdQ, i > 0 ? 1u : 0u);
         mma_commit(&k_empty[i % NK]);
         if (i + 1 == n) mma_commit(q_done);
       }
     }
   } else if (warp >= 4) {
-    const int half = (warp - 4) >> 2;  // columns [64 half, 64 half + 64)
+    constexpr int COLS = kDqCols;
+    const int part = (warp - 4) >> 2;  // columns [COLS part, COLS part + COLS)
     const int r = (threadIdx.x - 128) & 127, q = q0 + r;
     const bool row_ok = q < c.N;
     const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
@@ -316,7 +324,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     const int first = row_ok ? first_key(c, b, q) : 1, end = row_ok ? q + 1 : 0;
     const float nl = row_ok ? -c.lse[row] * kLog2e : 0.f, nd = row_ok ? -c.delta[row] : 0.f;
     const float2 nl2 = make_float2(nl, nl), nd2 = make_float2(nd, nd);
-    const uint32_t s_addr = tmem + lane_base + half * 64;
+    const uint32_t s_addr = tmem + lane_base + part * COLS;
     bool alive = true;
     int i = 0;
     for (int j = j0; j < j1; ++j, ++i) {
@@ -324,15 +332,14 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       if (!alive) break;
       tc_fence_after();
       const uint32_t x_addr = s_addr + kColP + (i & 1) * 128;
-      const int jlo = first - j * 128 - half * 64, jhi = end - j * 128 - half * 64;
-      float pg[64];
-      tmem_ld32(s_addr, pg);
-      tmem_ld32(s_addr + 32, pg + 32);
+      const int jlo = first - j * 128 - part * COLS, jhi = end - j * 128 - part * COLS;
+      float pg[COLS];
+      tmem_ld<COLS>(s_addr, pg);
       tmem_wait_ld();
       tc_fence_before();
       warp_arrive(s_free, lane);
 #pragma unroll
-      for (int k = 0; k < 64; k += 2) {
+      for (int k = 0; k < COLS; k += 2) {
         float2 pr, g;
         p_pair<CAP>(make_float2(pg[k], pg[k + 1]), nl2, p.kq, p.kc, &pr, &g);
         pg[k] = g.x;
@@ -341,8 +348,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       alive = __all_sync(0xffffffffu, mbar_wait(&p_full[i & 1], (i >> 1) & 1, abort_flag, status));
       if (!alive) break;
       tc_fence_after();
-      if (__all_sync(0xffffffffu, jlo <= 0 && jhi >= 64)) dx_columns<T, false>(x_addr, pg, nd2, jlo, jhi);
-      else dx_columns<T, true>(x_addr, pg, nd2, jlo, jhi);
+      if (__all_sync(0xffffffffu, jlo <= 0 && jhi >= COLS)) dx_columns<T, COLS, false>(x_addr, pg, nd2, jlo, jhi);
+      else dx_columns<T, COLS, true>(x_addr, pg, nd2, jlo, jhi);
       tmem_wait_st();
       tc_fence_before();
       warp_arrive(x_full, lane);
@@ -350,7 +357,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     if (alive && i > 0) alive = __all_sync(0xffffffffu, mbar_wait(q_done, 0, abort_flag, status));
     if (alive) {
       tc_fence_after();
-      if (half == 0)
+      if (part == 0)
         store_row<T, HD>(tmem + lane_base + kColQ, i > 0, static_cast<T*>(c.dq) + row * HD, c.scale, row_ok);
     }
   }
@@ -367,11 +374,12 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
 // dK, dV
 // ---------------------------------------------------------------------------
 template <typename T, int HD, bool CAP>
-__global__ void __launch_bounds__(kBwdThreads, 1)
+__global__ void __launch_bounds__(Shape<kDkvCols>::kThreads, 1)
     causal_dkv_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__ CUtensorMap tmg,
                       const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv,
                       const __grid_constant__ BwdParams p) {
   using Z = BwdSmem<HD>;
+  using Z2 = Shape<kDkvCols>;
   constexpr int TB = Z::kTile, NQ = Z::kNQ;
   constexpr uint32_t kColP = 128, kColV = 256, kColK = 256 + HD;  // S^T, dP^T, dV, dK
   extern __shared__ uint8_t smem_raw[];
@@ -416,12 +424,12 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       mbar_init(&g_full[i], 1);
       mbar_init(&i_full[i], 64);
       mbar_init(&q_empty[i], 1);
-      mbar_init(&i_empty[i], kComputeWarps);
+      mbar_init(&i_empty[i], Z2::kWarps);
     }
     mbar_init(s_full, 1);
-    mbar_init(p_full, kComputeWarps);
+    mbar_init(p_full, Z2::kWarps);
     mbar_init(d_full, 1);
-    mbar_init(x_full, kComputeWarps);
+    mbar_init(x_full, Z2::kWarps);
     mbar_init(done, 1);
     *abort_flag = 0;
     mbar_fence_init();
@@ -484,12 +492,12 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       const int st = i % NQ;
       if (!mbar_wait(p_full, i & 1, abort_flag, status)) break;
       tc_fence_after();
-      if (leader) mma_tile_ts(tm + kColV, tm, 64, gt0 + ((st * TB) >> 4), kIdA, i > 0 ? 1u : 0u);
+      if (leader) mma_tile_ts<Z2::kSteps, kDkvCols>(tm + kColV, tm, gt0 + ((st * TB) >> 4), kIdA, i > 0 ? 1u : 0u);
       if (i + 1 < un && !issue_s(i + 1)) break;
       if (!mbar_wait(x_full, i & 1, abort_flag, status)) break;
       tc_fence_after();
       if (leader) {
-        mma_tile_ts(tm + kColK, tm + kColP, 64, qt0 + ((st * TB) >> 4), kIdA, i > 0 ? 1u : 0u);
+        mma_tile_ts<Z2::kSteps, kDkvCols>(tm + kColK, tm + kColP, qt0 + ((st * TB) >> 4), kIdA, i > 0 ? 1u : 0u);
         mma_commit(&q_empty[st]);
         if (i + 1 == un) mma_commit(done);
       }
@@ -519,38 +527,38 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       mbar_arrive(&i_full[st]);
     }
   } else {
-    const int half = (warp - 4) >> 2;
+    constexpr int COLS = kDkvCols;
+    const int part = (warp - 4) >> 2;
     const int r = (threadIdx.x - 128) & 127, k = k0 + r;
     const bool row_ok = k < c.N;
     const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t s_addr = tmem + lane_base + half * 64, x_addr = s_addr + kColP;
+    const uint32_t s_addr = tmem + lane_base + part * COLS, x_addr = s_addr + kColP;
     const int qend = row_ok ? query_end(c, b, k) : 0;
     bool alive = true;
     int i = 0;
     for (; i < n; ++i) {
       const int st = i % NQ, qt = t0 + i % nt;
-      const int jlo = k - qt * 128 - half * 64, jhi = qend - qt * 128 - half * 64;
-      const bool interior = __all_sync(0xffffffffu, jlo <= 0 && jhi >= 64);
+      const int jlo = k - qt * 128 - part * COLS, jhi = qend - qt * 128 - part * COLS;
+      const bool interior = __all_sync(0xffffffffu, jlo <= 0 && jhi >= COLS);
       alive = __all_sync(0xffffffffu, mbar_wait(&i_full[st], (i / NQ) & 1, abort_flag, status)) &&
               __all_sync(0xffffffffu, mbar_wait(s_full, i & 1, abort_flag, status));
       if (!alive) break;
       tc_fence_after();
-      const float* nl = nl_s + st * 128 + half * 64;
-      const float* nd = nd_s + st * 128 + half * 64;
-      float pg[64];
-      tmem_ld32(s_addr, pg);
-      tmem_ld32(s_addr + 32, pg + 32);
+      const float* nl = nl_s + st * 128 + part * COLS;
+      const float* nd = nd_s + st * 128 + part * COLS;
+      float pg[COLS];
+      tmem_ld<COLS>(s_addr, pg);
       tmem_wait_ld();
-      if (interior) p_columns_t<T, CAP, false>(s_addr, pg, nl, p.kq, p.kc, jlo, jhi);
-      else p_columns_t<T, CAP, true>(s_addr, pg, nl, p.kq, p.kc, jlo, jhi);
+      if (interior) p_columns_t<T, COLS, CAP, false>(s_addr, pg, nl, p.kq, p.kc, jlo, jhi);
+      else p_columns_t<T, COLS, CAP, true>(s_addr, pg, nl, p.kq, p.kc, jlo, jhi);
       tmem_wait_st();
       tc_fence_before();
       warp_arrive(p_full, lane);
       alive = __all_sync(0xffffffffu, mbar_wait(d_full, i & 1, abort_flag, status));
       if (!alive) break;
       tc_fence_after();
-      if (interior) dx_columns_t<T, false>(x_addr, pg, nd, jlo, jhi);
-      else dx_columns_t<T, true>(x_addr, pg, nd, jlo, jhi);
+      if (interior) dx_columns_t<T, COLS, false>(x_addr, pg, nd, jlo, jhi);
+      else dx_columns_t<T, COLS, true>(x_addr, pg, nd, jlo, jhi);
       tmem_wait_st();
       tc_fence_before();
       warp_arrive(&i_empty[st], lane);
@@ -560,9 +568,9 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     if (alive) {
       tc_fence_after();
       const int64_t row = ((int64_t)b * c.N + k) * c.Hkv + hkv;
-      if (half == 0)
+      if (part == 0)
         store_row<T, HD>(tmem + lane_base + kColV, n > 0, static_cast<T*>(c.dv) + row * HD, 1.f, row_ok);
-      else
+      else if (part == 1)
         store_row<T, HD>(tmem + lane_base + kColK, n > 0, static_cast<T*>(c.dk) + row * HD, c.scale, row_ok);
     }
   }
@@ -593,9 +601,9 @@ int launch_bwd(const CausalParams& a, int dtype, cudaStream_t st) {
       cudaFuncSetAttribute(kk, cudaFuncAttributeMaxDynamicSharedMemorySize, BwdSmem<HD>::kDkv) != cudaSuccess)
     return TC_ERR_CUDA;
   const int tiles = (a.N + 127) / 128;
-  kq<<<dim3(tiles, a.Hq, a.B), kBwdThreads, BwdSmem<HD>::kDq, st>>>(mq, mg, mk, mv, p);
+  kq<<<dim3(tiles, a.Hq, a.B), Shape<kDqCols>::kThreads, BwdSmem<HD>::kDq, st>>>(mq, mg, mk, mv, p);
   if (int rc = launch_status()) return rc;
-  kk<<<dim3(tiles, a.Hkv, a.B), kBwdThreads, BwdSmem<HD>::kDkv, st>>>(mq, mg, mk, mv, p);
+  kk<<<dim3(tiles, a.Hkv, a.B), Shape<kDkvCols>::kThreads, BwdSmem<HD>::kDkv, st>>>(mq, mg, mk, mv, p);
   return launch_status();
 }
 

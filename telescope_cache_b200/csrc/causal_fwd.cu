@@ -230,7 +230,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
     auto issue_pv = [&](int x, int& np, int st) -> bool {
       if (!mbar_wait(&p_full[x], np & 1, abort_flag, status)) return false;
       tc_fence_after();
-      if (leader) mma_tile_ts(tm + 256 + x * HD, tm + x * 128, 32, vd0 + ((st * TB) >> 4), kIdO, np > 0 ? 1u : 0u);
+      if (leader) mma_tile_ts<8, 64>(tm + 256 + x * HD, tm + x * 128, vd0 + ((st * TB) >> 4), kIdO, np > 0 ? 1u : 0u);
       ++np;
       return true;
     };

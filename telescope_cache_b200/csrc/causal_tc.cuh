@@ -86,13 +86,13 @@ __device__ __forceinline__ void mma_tile_ss(uint32_t d, uint32_t alo, uint32_t b
     mma_ss(d, alo + off, blo + off, idesc, kk > 0 ? 1u : 0u);
   }
 }
-// d (+)= A B of A [128 x 128] in TMEM (16-bit pairs: 32 columns from a and 32 from
-// a + second) and an MN-major 128 x HD tile.
-__device__ __forceinline__ void mma_tile_ts(uint32_t d, uint32_t a, uint32_t second, uint32_t blo, uint32_t idesc,
-                                            uint32_t acc) {
+// d (+)= A B of A [128 x 128] in TMEM as 16-bit pairs, STEPS 16-element steps
+// (8 columns each) to every STRIDE columns, and an MN-major 128 x HD tile.
+template <int STEPS, int STRIDE>
+__device__ __forceinline__ void mma_tile_ts(uint32_t d, uint32_t a, uint32_t blo, uint32_t idesc, uint32_t acc) {
 #pragma unroll
   for (int kk = 0; kk < 8; ++kk)
-    mma_ts(d, a + (kk >> 2) * second + (kk & 3) * 8, blo + ((kk * 2048) >> 4), idesc, kk > 0 ? 1u : acc);
+    mma_ts(d, a + (kk / STEPS) * STRIDE + (kk % STEPS) * 8, blo + ((kk * 2048) >> 4), idesc, kk > 0 ? 1u : acc);
 }
 // A value that every lane holds alike, known to be uniform.
 __device__ __forceinline__ int uniform(int v) { return __shfl_sync(0xffffffffu, v, 0); }
