@@ -11,6 +11,14 @@
 // Seven products instead of the five of a single pass, and nothing is summed by
 // atomics: the results do not depend on the order in which CTAs run.
 //
+// -lse and -Delta: in the dQ pass a row's two numbers sit in its thread.  In the
+// dKV pass they belong to columns, and reading them from shared memory for every
+// element took half of the compute warps' time (128 words a warp and tile);
+// there they ride on the products instead: one more 16-dim step of ones times
+// three bf16 terms per query (24 bits) leaves s - lse / scale and dP - Delta in
+// the accumulators.  (With the softcap lse comes after the tanh: from shared
+// memory.)
+//
 // Both passes: warp 0 TMA producer, warp 1 MMA issuer, warps 4-11 compute: a
 // thread owns one TMEM lane (query, or key) and 64 of the tile's 128 columns.
 // P and dX leave as 16-bit pairs in the first 32 of the thread's own 64 columns
@@ -44,14 +52,16 @@ constexpr int BLK = 128 * 128;  // one 64-column block of a 128-row tile
 
 struct BwdParams {
   CausalParams c;
+  GridOrder order;
   float kq, kc;  // logit2 = kq s, or kc tanh(kq s)
 };
 
 template <int HD> struct BwdSmem {
   static constexpr int kTile = 128 * HD * 2;
   static constexpr int kNK = 3, kNV = 2, kNQ = 2;
+  static constexpr int kAug = (2 + kNQ) * kAugTile;
   static constexpr int kDq = (2 + kNK + kNV) * kTile + 256 + 1024;
-  static constexpr int kDkv = (2 + 2 * kNQ) * kTile + 2 * kNQ * 128 * 4 + 256 + 1024;
+  static constexpr int kDkv = (2 + 2 * kNQ) * kTile + kAug + kNQ * 128 * 4 + 256 + 1024;
   static_assert(kDq <= 227 * 1024 && kDkv <= 227 * 1024, "backward shared memory exceeds the per-CTA limit");
 };
 
@@ -79,9 +89,9 @@ __device__ __forceinline__ void p_pair(float2 s, float2 nl2, float kq, float kc,
 // Tile column base + i inside [jlo, jhi)?
 __device__ __forceinline__ bool inside(int i, int jlo, int jhi) { return i >= jlo && i < jhi; }
 
-// dX = pg (dP + nd) of a thread's COLS columns at x_addr, as 16-bit pairs over the
+// dX = pg (dP + nd), or pg dP unless DELTA, of a thread's COLS columns at x_addr, as 16-bit pairs over the
 // first half of them (each 32 are read before they are overwritten).
-template <typename T, int COLS, bool MASK>
+template <typename T, int COLS, bool MASK, bool DELTA>
 __device__ __forceinline__ void dx_columns(uint32_t x_addr, const float* pg, float2 nd, int jlo, int jhi) {
 #pragma unroll
   for (int h = 0; h < COLS / 32; ++h) {
@@ -91,7 +101,9 @@ __device__ __forceinline__ void dx_columns(uint32_t x_addr, const float* pg, flo
     tmem_wait_ld();
 #pragma unroll
     for (int k = 0; k < 32; k += 2) {
-      float2 v = fmul2(make_float2(pg[32 * h + k], pg[32 * h + k + 1]), fadd2(make_float2(dp[k], dp[k + 1]), nd));
+      float2 v = make_float2(dp[k], dp[k + 1]);
+      if constexpr (DELTA) v = fadd2(v, nd);
+      v = fmul2(make_float2(pg[32 * h + k], pg[32 * h + k + 1]), v);
       if constexpr (MASK) {
         v.x = inside(32 * h + k, jlo, jhi) ? v.x : 0.f;
         v.y = inside(32 * h + k + 1, jlo, jhi) ? v.y : 0.f;
@@ -102,35 +114,9 @@ __device__ __forceinline__ void dx_columns(uint32_t x_addr, const float* pg, flo
   }
 }
 
-// The same with one Delta per column (nd, shared memory).
-template <typename T, int COLS, bool MASK>
-__device__ __forceinline__ void dx_columns_t(uint32_t x_addr, const float* pg, const float* nd, int jlo, int jhi) {
-#pragma unroll
-  for (int h = 0; h < COLS / 32; ++h) {
-    float dp[32];
-    uint32_t w[16];
-    tmem_ld32(x_addr + 32 * h, dp);
-    tmem_wait_ld();
-#pragma unroll
-    for (int k = 0; k < 32; k += 4) {
-      const float4 d = *reinterpret_cast<const float4*>(nd + 32 * h + k);
-#pragma unroll
-      for (int m = 0; m < 4; m += 2) {
-        float2 v = fmul2(make_float2(pg[32 * h + k + m], pg[32 * h + k + m + 1]),
-                         fadd2(make_float2(dp[k + m], dp[k + m + 1]), m ? make_float2(d.z, d.w) : make_float2(d.x, d.y)));
-        if constexpr (MASK) {
-          v.x = inside(32 * h + k + m, jlo, jhi) ? v.x : 0.f;
-          v.y = inside(32 * h + k + m + 1, jlo, jhi) ? v.y : 0.f;
-        }
-        w[(k + m) >> 1] = Pack2<T>::pack(v.x, v.y);
-      }
-    }
-    tmem_st16u(x_addr + 16 * h, w);
-  }
-}
-
-// P of a thread's COLS columns at s_addr (scores already in pg), as 16-bit pairs over
-// the first half of them; pg becomes P softcap'.  nl: -lse2 per column.
+// P of a thread's COLS columns at s_addr (scores already in pg), as 16-bit pairs
+// over the first half of them; pg becomes P softcap'.  With the softcap nl holds
+// -lse2 per column; without it the scores come as s - lse / scale.
 template <typename T, int COLS, bool CAP, bool MASK>
 __device__ __forceinline__ void p_columns_t(uint32_t s_addr, float* pg, const float* nl, float kq, float kc, int jlo,
                                             int jhi) {
@@ -139,12 +125,18 @@ __device__ __forceinline__ void p_columns_t(uint32_t s_addr, float* pg, const fl
     uint32_t w[16];
 #pragma unroll
     for (int k = 0; k < 32; k += 4) {
-      const float4 l = *reinterpret_cast<const float4*>(nl + 32 * h + k);
+      float4 l = make_float4(0.f, 0.f, 0.f, 0.f);
+      if constexpr (CAP) l = *reinterpret_cast<const float4*>(nl + 32 * h + k);
 #pragma unroll
       for (int m = 0; m < 4; m += 2) {
         float* x = pg + 32 * h + k + m;
         float2 pr, g;
-        p_pair<CAP>(make_float2(x[0], x[1]), m ? make_float2(l.z, l.w) : make_float2(l.x, l.y), kq, kc, &pr, &g);
+        if constexpr (CAP) {
+          p_pair<true>(make_float2(x[0], x[1]), m ? make_float2(l.z, l.w) : make_float2(l.x, l.y), kq, kc, &pr, &g);
+        } else {
+          const float2 a = fmul2(make_float2(x[0], x[1]), make_float2(kq, kq));
+          pr = g = make_float2(exp2_fast(a.x), exp2_fast(a.y));
+        }
         if constexpr (MASK) {
           pr.x = inside(32 * h + k + m, jlo, jhi) ? pr.x : 0.f;
           pr.y = inside(32 * h + k + m + 1, jlo, jhi) ? pr.y : 0.f;
@@ -213,7 +205,9 @@ __global__ void __launch_bounds__(Shape<kDqCols>::kThreads, 1)
 
   const CausalParams& c = p.c;
   const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
-  const int q0 = (gridDim.x - 1 - blockIdx.x) * 128, hq = blockIdx.y, b = blockIdx.z, hkv = hq / c.E;
+  int block, hq, b;
+  grid_place(p.order, &block, &hq, &b);
+  const int q0 = (grid_blocks(p.order) - 1 - block) * 128, hkv = hq / c.E;
   int32_t* status = c.status;
   const int first0 = first_key(c, b, q0), last = min(q0 + 128, c.N) - 1;
   const int j0 = first0 <= last ? first0 / 128 : 0, j1 = first0 <= last ? last / 128 + 1 : 0;
@@ -348,8 +342,8 @@ __global__ void __launch_bounds__(Shape<kDqCols>::kThreads, 1)
       alive = __all_sync(0xffffffffu, mbar_wait(&p_full[i & 1], (i >> 1) & 1, abort_flag, status));
       if (!alive) break;
       tc_fence_after();
-      if (__all_sync(0xffffffffu, jlo <= 0 && jhi >= COLS)) dx_columns<T, COLS, false>(x_addr, pg, nd2, jlo, jhi);
-      else dx_columns<T, COLS, true>(x_addr, pg, nd2, jlo, jhi);
+      if (__all_sync(0xffffffffu, jlo <= 0 && jhi >= COLS)) dx_columns<T, COLS, false, true>(x_addr, pg, nd2, jlo, jhi);
+      else dx_columns<T, COLS, true, true>(x_addr, pg, nd2, jlo, jhi);
       tmem_wait_st();
       tc_fence_before();
       warp_arrive(x_full, lane);
@@ -384,13 +378,14 @@ __global__ void __launch_bounds__(Shape<kDkvCols>::kThreads, 1)
   constexpr uint32_t kColP = 128, kColV = 256, kColK = 256 + HD;  // S^T, dP^T, dV, dK
   extern __shared__ uint8_t smem_raw[];
   uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* k_s = sm;
+  uint8_t* one_s = sm;                // [2] ones that pick -lse / scale (dims 0-2) and -Delta (3-5) out of aug_s
+  uint8_t* aug_s = one_s + 2 * kAugTile;  // [NQ] per query: both, as three bf16 terms each
+  uint8_t* k_s = aug_s + NQ * kAugTile;
   uint8_t* v_s = k_s + TB;
   uint8_t* q_s = v_s + TB;        // [NQ]
   uint8_t* g_s = q_s + NQ * TB;   // [NQ]
-  float* nl_s = reinterpret_cast<float*>(g_s + NQ * TB);  // [NQ][128] -lse log2e of the tile's queries
-  float* nd_s = nl_s + NQ * 128;                          // [NQ][128] -Delta
-  uint64_t* bars = reinterpret_cast<uint64_t*>(nd_s + NQ * 128);
+  float* nl_s = reinterpret_cast<float*>(g_s + NQ * TB);  // softcap: [NQ][128] -lse log2e of the tile's queries
+  uint64_t* bars = reinterpret_cast<uint64_t*>(nl_s + NQ * 128);
   uint64_t* k_full = bars;
   uint64_t* v_full = bars + 1;
   uint64_t* q_full = bars + 2;      // [NQ] Q
@@ -409,7 +404,9 @@ __global__ void __launch_bounds__(Shape<kDkvCols>::kThreads, 1)
 
   const CausalParams& c = p.c;
   const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
-  const int k0 = blockIdx.x * 128, hkv = blockIdx.y, b = blockIdx.z;  // the first keys are seen by the most queries
+  int block, hkv, b;
+  grid_place(p.order, &block, &hkv, &b);
+  const int k0 = block * 128;  // the first keys are seen by the most queries
   int32_t* status = c.status;
   const int last = min(k0 + 128, c.N) - 1;
   const int t0 = k0 / 128, t1 = (query_end(c, b, last) + 127) / 128;  // query tiles
@@ -438,6 +435,15 @@ __global__ void __launch_bounds__(Shape<kDkvCols>::kThreads, 1)
     tmem_alloc(tmem_holder, 512);
     tmem_relinquish();
   }
+  if (threadIdx.x >= 128 && threadIdx.x < 256) {
+    const int r = threadIdx.x - 128;
+    const uint32_t one = 0x3f80u;  // bf16 1
+    *reinterpret_cast<uint4*>(one_s + r * 16) = make_uint4(one | one << 16, one, 0u, 0u);
+    *reinterpret_cast<uint4*>(one_s + kAugTile + r * 16) = make_uint4(0u, one << 16, one | one << 16, 0u);
+    for (int i = 0; i < 2 + NQ; ++i)  // dims 8-15
+      *reinterpret_cast<uint4*>(one_s + i * kAugTile + kAugHalf + r * 16) = make_uint4(0u, 0u, 0u, 0u);
+    fence_async_smem();
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -464,15 +470,18 @@ __global__ void __launch_bounds__(Shape<kDkvCols>::kThreads, 1)
     constexpr uint32_t kIdS = idesc_f16(128, 128, Pack2<T>::kFmt, 0, 0);
     constexpr uint32_t kIdA = idesc_f16(128, HD, Pack2<T>::kFmt, 0, 1);
     const uint32_t kd = desc_lo(k_s, 16), vd = desc_lo(v_s, 16), qd0 = desc_lo(q_s, 16), gd0 = desc_lo(g_s, 16),
-                   qt0 = desc_lo(q_s, BLK), gt0 = desc_lo(g_s, BLK);
+                   qt0 = desc_lo(q_s, BLK), gt0 = desc_lo(g_s, BLK), one0 = aug_lo(one_s), aug0 = aug_lo(aug_s);
     const uint32_t tm = uniform(tmem);
     const int un = uniform(n);
     const bool leader = elect_one();
     auto issue_s = [&](int i) {
-      if (!mbar_wait(&q_full[i % NQ], (i / NQ) & 1, abort_flag, status)) return false;
+      if (!mbar_wait(&q_full[i % NQ], (i / NQ) & 1, abort_flag, status) ||
+          !mbar_wait(&i_full[i % NQ], (i / NQ) & 1, abort_flag, status))
+        return false;
       tc_fence_after();
       if (leader) {
         mma_tile_ss<HD>(tm, kd, qd0 + (((i % NQ) * TB) >> 4), kIdS);
+        if constexpr (!CAP) mma_aug(tm, one0, aug0 + (((i % NQ) * kAugTile) >> 4));
         mma_commit(s_full);
       }
       return true;
@@ -482,6 +491,7 @@ __global__ void __launch_bounds__(Shape<kDkvCols>::kThreads, 1)
       tc_fence_after();
       if (leader) {
         mma_tile_ss<HD>(tm + kColP, vd, gd0 + (((i % NQ) * TB) >> 4), kIdS);
+        mma_aug(tm + kColP, one0 + (kAugTile >> 4), aug0 + (((i % NQ) * kAugTile) >> 4));
         mma_commit(d_full);
       }
       return true;
@@ -508,22 +518,37 @@ __global__ void __launch_bounds__(Shape<kDkvCols>::kThreads, 1)
     const int t = threadIdx.x - 64;
     for (int i = 0; i < n; ++i) {
       const int st = i % NQ, hq = hkv * c.E + i / nt, qt = t0 + i % nt;
-      float2 v[2];
+      float lse[2], nd[2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int q = qt * 128 + t + 64 * h;
-        v[h] = make_float2(0.f, 0.f);
+        lse[h] = nd[h] = 0.f;
         if (q < c.N) {
           const int64_t row = ((int64_t)b * c.N + q) * c.Hq + hq;
-          v[h] = make_float2(-c.lse[row] * kLog2e, -c.delta[row]);
+          lse[h] = c.lse[row];
+          nd[h] = -c.delta[row];
+          if (lse[h] == -INFINITY) lse[h] = 0.f;  // sees nothing: masked everywhere
         }
       }
-      if (i >= NQ && !__all_sync(0xffffffffu, mbar_wait(&i_empty[st], ((i / NQ) - 1) & 1, abort_flag, status))) break;
+      // the products of step i - NQ have read the buffer (and the compute warps nl_s)
+      if (i >= NQ && !(__all_sync(0xffffffffu, mbar_wait(&q_empty[st], ((i / NQ) - 1) & 1, abort_flag, status)) &&
+                       (!CAP || __all_sync(0xffffffffu, mbar_wait(&i_empty[st], ((i / NQ) - 1) & 1, abort_flag, status)))))
+        break;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        nl_s[st * 128 + t + 64 * h] = v[h].x;
-        nd_s[st * 128 + t + 64 * h] = v[h].y;
+        const int r = t + 64 * h;
+        if constexpr (CAP) nl_s[st * 128 + r] = -lse[h] * kLog2e;
+        const float x[2] = {-lse[h] / c.scale, nd[h]};
+        float y[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+          y[3 * w] = round_to<__nv_bfloat16>(x[w]);
+          y[3 * w + 1] = round_to<__nv_bfloat16>(x[w] - y[3 * w]);
+          y[3 * w + 2] = x[w] - y[3 * w] - y[3 * w + 1];
+        }
+        *reinterpret_cast<uint4*>(aug_s + st * kAugTile + r * 16) = pack8<__nv_bfloat16>(y, 1.f);
       }
+      fence_async_smem();
       mbar_arrive(&i_full[st]);
     }
   } else {
@@ -540,12 +565,11 @@ __global__ void __launch_bounds__(Shape<kDkvCols>::kThreads, 1)
       const int st = i % NQ, qt = t0 + i % nt;
       const int jlo = k - qt * 128 - part * COLS, jhi = qend - qt * 128 - part * COLS;
       const bool interior = __all_sync(0xffffffffu, jlo <= 0 && jhi >= COLS);
-      alive = __all_sync(0xffffffffu, mbar_wait(&i_full[st], (i / NQ) & 1, abort_flag, status)) &&
-              __all_sync(0xffffffffu, mbar_wait(s_full, i & 1, abort_flag, status));
+      if constexpr (CAP) alive = __all_sync(0xffffffffu, mbar_wait(&i_full[st], (i / NQ) & 1, abort_flag, status));
+      alive = alive && __all_sync(0xffffffffu, mbar_wait(s_full, i & 1, abort_flag, status));
       if (!alive) break;
       tc_fence_after();
       const float* nl = nl_s + st * 128 + part * COLS;
-      const float* nd = nd_s + st * 128 + part * COLS;
       float pg[COLS];
       tmem_ld<COLS>(s_addr, pg);
       tmem_wait_ld();
@@ -553,15 +577,15 @@ __global__ void __launch_bounds__(Shape<kDkvCols>::kThreads, 1)
       else p_columns_t<T, COLS, CAP, true>(s_addr, pg, nl, p.kq, p.kc, jlo, jhi);
       tmem_wait_st();
       tc_fence_before();
+      if constexpr (CAP) warp_arrive(&i_empty[st], lane);
       warp_arrive(p_full, lane);
       alive = __all_sync(0xffffffffu, mbar_wait(d_full, i & 1, abort_flag, status));
       if (!alive) break;
       tc_fence_after();
-      if (interior) dx_columns_t<T, COLS, false>(x_addr, pg, nd, jlo, jhi);
-      else dx_columns_t<T, COLS, true>(x_addr, pg, nd, jlo, jhi);
+      if (interior) dx_columns<T, COLS, false, false>(x_addr, pg, make_float2(0.f, 0.f), jlo, jhi);
+      else dx_columns<T, COLS, true, false>(x_addr, pg, make_float2(0.f, 0.f), jlo, jhi);
       tmem_wait_st();
       tc_fence_before();
-      warp_arrive(&i_empty[st], lane);
       warp_arrive(x_full, lane);
     }
     if (alive && n > 0) alive = __all_sync(0xffffffffu, mbar_wait(done, 0, abort_flag, status));
@@ -601,9 +625,12 @@ int launch_bwd(const CausalParams& a, int dtype, cudaStream_t st) {
       cudaFuncSetAttribute(kk, cudaFuncAttributeMaxDynamicSharedMemorySize, BwdSmem<HD>::kDkv) != cudaSuccess)
     return TC_ERR_CUDA;
   const int tiles = (a.N + 127) / 128;
-  kq<<<dim3(tiles, a.Hq, a.B), Shape<kDqCols>::kThreads, BwdSmem<HD>::kDq, st>>>(mq, mg, mk, mv, p);
+  const int64_t rows = (int64_t)a.B * a.N * HD * 4;  // bytes of a head's K and V, or Q and dO
+  dim3 grid = grid_order(tiles, a.Hq, a.B, rows * a.Hkv, &p.order);
+  kq<<<grid, Shape<kDqCols>::kThreads, BwdSmem<HD>::kDq, st>>>(mq, mg, mk, mv, p);
   if (int rc = launch_status()) return rc;
-  kk<<<dim3(tiles, a.Hkv, a.B), Shape<kDkvCols>::kThreads, BwdSmem<HD>::kDkv, st>>>(mq, mg, mk, mv, p);
+  grid = grid_order(tiles, a.Hkv, a.B, rows * a.Hq, &p.order);
+  kk<<<grid, Shape<kDkvCols>::kThreads, BwdSmem<HD>::kDkv, st>>>(mq, mg, mk, mv, p);
   return launch_status();
 }
 

@@ -21,7 +21,7 @@
 //
 // A query tile's keys run from the first key of its first row (starts do not
 // descend) to the diagonal; tiles in between need no mask.  The heaviest blocks
-// of a head come first in the grid.
+// come first in the grid.
 //
 // Softcap: with y = x / c and a the largest |y| of the warp's rows in the tile,
 // tanh comes from its odd Maclaurin series (through y^5 below 0.15, y^9 below
@@ -49,6 +49,7 @@ template <int HD> struct FwdSmem {
 
 struct FwdParams {
   CausalParams c;
+  GridOrder order;
   float kq, kc;              // logit2 = kq s, or kc tanh(kq s)
   float e1, e3, e5, e7, e9;  // its series in s
 };
@@ -152,8 +153,9 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
 
   const CausalParams& c = p.c;
   const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
-  const int q0 = (gridDim.x - 1 - blockIdx.x) * 256, hq = blockIdx.y, b = blockIdx.z;
-  const int hkv = hq / c.E;
+  int block, hq, b;
+  grid_place(p.order, &block, &hq, &b);
+  const int q0 = (grid_blocks(p.order) - 1 - block) * 256, hkv = hq / c.E;
   int32_t* status = c.status;
   int alo, ahi, blo, bhi;
   key_tiles(c, b, q0, &alo, &ahi);
@@ -426,7 +428,8 @@ int launch_fwd(const CausalParams& a, int dtype, cudaStream_t st) {
   auto k = causal_fwd_kernel<T, HD, CAP>;
   constexpr int smem = FwdSmem<HD>::kBytes;
   if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return TC_ERR_CUDA;
-  k<<<dim3((a.N + 255) / 256, a.Hq, a.B), kFwdThreads, smem, st>>>(mq, mk, mv, p);
+  const dim3 grid = grid_order((a.N + 255) / 256, a.Hq, a.B, (int64_t)a.B * a.N * a.Hkv * HD * 4, &p.order);
+  k<<<grid, kFwdThreads, smem, st>>>(mq, mk, mv, p);
   return launch_status();
 }
 

@@ -49,6 +49,13 @@ constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
 __device__ __forceinline__ uint32_t desc_lo(const void* s, uint32_t lbo) {
   return ((smem_addr(s) & 0x3FFFFu) >> 4) | ((lbo >> 4) << 16);
 }
+// K-major 128 x 16 tile without swizzle: element (r, k) at (k / 8) * kAugHalf +
+// r * 16 + (k % 8) * 2.
+constexpr uint32_t kAugHalf = 128 * 16, kAugTile = 2 * kAugHalf;
+constexpr uint32_t kAugHi = (128u >> 4) | (1u << 14);
+__device__ __forceinline__ uint32_t aug_lo(const void* s) {
+  return ((smem_addr(s) & 0x3FFFFu) >> 4) | ((kAugHalf >> 4) << 16);
+}
 __device__ __forceinline__ bool elect_one() {
   uint32_t r;
   asm volatile(
@@ -66,6 +73,16 @@ __device__ __forceinline__ void mma_ss(uint32_t d, uint32_t alo, uint32_t blo, u
       "setp.ne.b32 p, %4, 0;\n\t"
       "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t}" ::"r"(d),
       "r"(alo), "r"(blo), "r"(idesc), "r"(acc), "n"(kDescHi)
+      : "memory");
+}
+// d += A B^T of two such tiles, bf16 whatever the other operands' type.
+__device__ __forceinline__ void mma_aug(uint32_t d, uint32_t alo, uint32_t blo) {
+  asm volatile(
+      "{\n\t.reg .b64 a, b;\n\t"
+      "mov.b64 a, {%1, %4};\n\t"
+      "mov.b64 b, {%2, %4};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, 1;\n\t}" ::"r"(d),
+      "r"(alo), "r"(blo), "r"(idesc_f16(128, 128, 1, 0, 0)), "n"(kAugHi)
       : "memory");
 }
 __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t blo, uint32_t idesc, uint32_t acc) {
@@ -103,6 +120,26 @@ __device__ __forceinline__ void warp_arrive(uint64_t* bar, int lane) {
   __syncwarp();
   if (lane == 0) mbar_arrive(bar);
 }
+
+// Grid of a pass whose CTAs are (block, head, sequence): blocks first, so that
+// the heaviest blocks of every head start before any light one (the long
+// training case ends 12% earlier), while what the heads stream, `bytes`, stays
+// in half of the L2; else head by head, so that a head's blocks share it.
+constexpr int64_t kShareBytes = int64_t(64) << 20;
+struct GridOrder {
+  int heads, by_block;
+};
+inline dim3 grid_order(int blocks, int heads, int B, int64_t bytes, GridOrder* o) {
+  o->heads = heads;
+  o->by_block = bytes <= kShareBytes && blocks <= 65535;
+  return o->by_block ? dim3((unsigned)heads * B, blocks, 1) : dim3(blocks, heads, B);
+}
+__device__ __forceinline__ void grid_place(const GridOrder& o, int* block, int* head, int* b) {
+  *block = o.by_block ? blockIdx.y : blockIdx.x;
+  *head = o.by_block ? blockIdx.x % o.heads : blockIdx.y;
+  *b = o.by_block ? blockIdx.x / o.heads : blockIdx.z;
+}
+__device__ __forceinline__ int grid_blocks(const GridOrder& o) { return o.by_block ? gridDim.y : gridDim.x; }
 
 inline bool strides_ok(const void* p, int64_t sb, int64_t sn, int64_t sh, int64_t B, int64_t N, int64_t H) {
   const int64_t most = int64_t(1) << 38;  // elements: a map's byte stride stays below 2^40
