@@ -15,16 +15,17 @@
 
 #include <type_traits>
 
-#include "common.cuh"
 #include "rotary.cuh"
+#include "tc_common.cuh"
 
 using namespace tc;
+using namespace tc::ptx;
+using tc::tcx::kLn2;
+using tc::tcx::kLog2e;
 
 namespace {
 
 constexpr float kTiny = 1e-30f;
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLn2 = 0.6931471805599453f;
 
 template <int STORE> struct Codec;
 template <> struct Codec<TC_KV_INT8> {
@@ -33,6 +34,14 @@ template <> struct Codec<TC_KV_INT8> {
     return (uint32_t)(min(max(__float2int_rn(y), -127), 127) + 128);
   }
   static __device__ __forceinline__ float value(uint32_t c) { return (float)((int)c - 128); }
+  // The same two bytes as f16 subnormals u 2^-24, u = code + 128: a sum of their
+  // products is (sum code q + 128 sum q) 2^-24.  One instruction where pair takes
+  // two; for the keys, where the second sum is of the first one's size.  (For the
+  // values it would be: 128 sum p against a sum of p v that averages out.)
+  static constexpr float kMul = 16777216.f, kOff = 128.f;
+  template <bool HI> static __device__ __forceinline__ uint32_t raw_pair(uint32_t x) {
+    return __byte_perm(x, 0u, HI ? 0x4342 : 0x4140);
+  }
   // bytes 0, 1 (hi: 2, 3) of x as two f16 values: 0x6400 | u is 1024 + u exactly
   template <bool HI> static __device__ __forceinline__ uint32_t pair(uint32_t x) {
     const uint32_t r = __byte_perm(x, 0x64646464u, HI ? 0x4342 : 0x4140);
@@ -42,6 +51,8 @@ template <> struct Codec<TC_KV_INT8> {
 };
 template <> struct Codec<TC_KV_FP8> {
   static constexpr float kTop = 448.f;
+  static constexpr float kMul = 1.f, kOff = 0.f;
+  template <bool HI> static __device__ __forceinline__ uint32_t raw_pair(uint32_t x) { return pair<HI>(x); }
   static __device__ __forceinline__ uint32_t code(float y) {
     return __nv_cvt_float_to_fp8(y, __NV_SATFINITE, __NV_E4M3);
   }
@@ -258,47 +269,54 @@ struct ReadParams {
   void* out[2];  // [rows, L, H, D]
 };
 
-// A thread per V codes of one row (V = 16 / element size, or 1), heads fastest
-// in the output; slots past a row's length are zeros and read nothing.
+// A thread per V codes of one row (V = 16 / element size, or 1) and kReadTok
+// tokens; a CTA's threads run over the heads and dims of a token, so the output
+// is written in order.  Slots past a row's length are zeros and read nothing.
+constexpr int kReadTok = 4;
 template <typename T, int STORE, int V>
 __global__ void __launch_bounds__(256) read_kernel(ReadParams p) {
-  const int which = blockIdx.y, D = p.dim[which], per = D / V;
+  const int which = blockIdx.y, D = p.dim[which], per = p.H * (D / V);  // threads per token
+  const int b = blockIdx.z, len = (int)min((int64_t)p.lengths[b], p.cap);
   const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-  if (i >= (int64_t)p.rows * p.L * p.H * per) return;
-  const int d = (int)(i % per) * V;
-  const int64_t rh = i / per;
-  const int h = (int)(rh % p.H);
-  const int64_t bt = rh / p.H;
-  const int n = (int)(bt % p.L), b = (int)(bt / p.L);
-  T* out = static_cast<T*>(p.out[which]) + rh * D + d;
-  float v[V];
-  if (n < p.lengths[b] && n < p.cap) {
-    const int64_t at = ((int64_t)b * p.H + h) * p.cap + n;
-    const float s = p.scales[which][at];
-    const uint8_t* c = p.codes[which] + at * D + d;
-    if constexpr (V == 8) {
-      const uint2 w = *reinterpret_cast<const uint2*>(c);
+  const int tile = (int)(i / per), rest = (int)(i - (int64_t)tile * per);
+  const int h = rest / (D / V), d = (rest - h * (D / V)) * V;
+  const int n0 = tile * kReadTok;
+  using Raw = typename std::conditional<V == 8, uint2, typename std::conditional<V == 4, uint32_t, uint8_t>::type>::type;
+  Raw raw[kReadTok];
+  float sc[kReadTok];
+  const int64_t at0 = ((int64_t)b * p.H + h) * p.cap;
 #pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] = dequant<STORE>(((k < 4 ? w.x : w.y) >> (8 * (k & 3))) & 255u, s);
-    } else if constexpr (V == 4) {
-      const uint32_t w = *reinterpret_cast<const uint32_t*>(c);
-#pragma unroll
-      for (int k = 0; k < 4; ++k) v[k] = dequant<STORE>((w >> (8 * k)) & 255u, s);
-    } else {
-      v[0] = dequant<STORE>(c[0], s);
+  for (int j = 0; j < kReadTok; ++j) {
+    const int n = n0 + j;
+    sc[j] = 0.f;
+    if (n < len && n < p.L) {
+      raw[j] = *reinterpret_cast<const Raw*>(p.codes[which] + (at0 + n) * D + d);
+      sc[j] = p.scales[which][at0 + n];
     }
-  } else {
-#pragma unroll
-    for (int k = 0; k < V; ++k) v[k] = 0.f;
   }
-  if constexpr (V == 1) {
-    out[0] = from_f<T>(v[0]);
-  } else {
-    uint4 w;
-    T* e = reinterpret_cast<T*>(&w);
 #pragma unroll
-    for (int k = 0; k < V; ++k) e[k] = from_f<T>(v[k]);
-    *reinterpret_cast<uint4*>(out) = w;
+  for (int j = 0; j < kReadTok; ++j) {
+    const int n = n0 + j;
+    if (n >= p.L) return;
+    T* out = static_cast<T*>(p.out[which]) + (((int64_t)b * p.L + n) * p.H + h) * D + d;
+    float v[V];
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+      uint32_t c;
+      if constexpr (V == 8) c = ((k < 4 ? raw[j].x : raw[j].y) >> (8 * (k & 3))) & 255u;
+      else if constexpr (V == 4) c = (raw[j] >> (8 * k)) & 255u;
+      else c = raw[j];
+      v[k] = n < len ? dequant<STORE>(c, sc[j]) : 0.f;
+    }
+    if constexpr (V == 1) {
+      out[0] = from_f<T>(v[0]);
+    } else {
+      uint4 w;
+      T* e = reinterpret_cast<T*>(&w);
+#pragma unroll
+      for (int k = 0; k < V; ++k) e[k] = from_f<T>(v[k]);
+      *reinterpret_cast<uint4*>(out) = w;
+    }
   }
 }
 
@@ -309,11 +327,12 @@ int launch_read(const ReadParams& p, cudaStream_t st) {
   for (int w = 0; w < 2; ++w)
     vec = vec && p.dim[w] % V == 0 && (uintptr_t)p.codes[w] % V == 0 && (uintptr_t)p.out[w] % 16 == 0;
   const int D = p.dim[0] > p.dim[1] ? p.dim[0] : p.dim[1];
-  const int64_t units = (int64_t)p.rows * p.L * p.H * (vec ? D / V : D);
+  const int64_t units = (int64_t)((p.L + kReadTok - 1) / kReadTok) * p.H * (vec ? D / V : D);
   const int64_t grid = (units + 255) / 256;
-  if (grid > INT32_MAX) return TC_ERR_UNSUPPORTED;
-  if (vec) read_kernel<T, STORE, V><<<dim3((unsigned)grid, 2), 256, 0, st>>>(p);
-  else read_kernel<T, STORE, 1><<<dim3((unsigned)grid, 2), 256, 0, st>>>(p);
+  if (grid > INT32_MAX || p.rows > 65535) return TC_ERR_UNSUPPORTED;
+  const dim3 g((unsigned)grid, 2, p.rows);
+  if (vec) read_kernel<T, STORE, V><<<g, 256, 0, st>>>(p);
+  else read_kernel<T, STORE, 1><<<g, 256, 0, st>>>(p);
   return launch_status();
 }
 
@@ -409,10 +428,11 @@ __device__ __forceinline__ void load_pair(const AttendParams& p, const T* x, int
   }
 }
 
-// One warp quantises the new token's row into slot `pos` of its head.
-template <typename T, int STORE>
+// One warp quantises the new token's row into slot `pos` of its head, and into
+// `copy` (byte place(d) for dim d) with its scale.
+template <typename T, int STORE, typename F>
 __device__ void write_token(const AttendParams& p, const T* x, int D, int R, int pos, int64_t head, uint8_t* codes,
-                            float* scales, void* stored) {
+                            float* scales, void* stored, uint8_t* copy, float* copy_scale, F place) {
   const int lane = threadIdx.x & 31, pairs = (D + 1) / 2;
   uint32_t m = 0;
   for (int u = lane; u < pairs; u += 32) {
@@ -427,42 +447,68 @@ __device__ void write_token(const AttendParams& p, const T* x, int D, int R, int
   row_scale<STORE>(__uint_as_float(m), &scale, &inv);
   const int64_t at = head * p.cap + pos;
   for (int u = lane; u < pairs; u += 32) {
-    int i1, i2;
-    float y1, y2;
-    load_pair(p, x, u, D, R, pos, &i1, &i2, &y1, &y2);
-    const uint32_t c1 = Codec<STORE>::code(__fmul_rn(y1, inv)), c2 = Codec<STORE>::code(__fmul_rn(y2, inv));
-    codes[at * D + i1] = (uint8_t)c1;
-    codes[at * D + i2] = (uint8_t)c2;
-    if (stored) {
-      store_any(stored, head * D + i1, p.new_dtype, dequant<STORE>(c1, scale));
-      store_any(stored, head * D + i2, p.new_dtype, dequant<STORE>(c2, scale));
+    int i[2];
+    float y[2];
+    load_pair(p, x, u, D, R, pos, &i[0], &i[1], &y[0], &y[1]);
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const uint32_t c = Codec<STORE>::code(__fmul_rn(y[k], inv));
+      codes[at * D + i[k]] = (uint8_t)c;
+      if (copy) copy[place(i[k])] = (uint8_t)c;
+      if (stored) store_any(stored, head * D + i[k], p.new_dtype, dequant<STORE>(c, scale));
     }
   }
-  if (lane == 0) scales[at] = scale;
+  if (lane == 0) {
+    scales[at] = scale;
+    if (copy) *copy_scale = scale;
+  }
 }
 
 // Joins the partial (m, l, O) of `active` splits of nE heads and writes out, lse.
+// The warps share the splits (a lane reads VE consecutive dims of one), then
+// join in shared memory: a chain of `active` / 4 reads instead of `active`.
+constexpr int kAtWarps = 4;
 template <typename TQ>
-__device__ void join_splits(const AttendParams& p, int b, int hkv, int e0, int nE, int64_t slot0, int active) {
+__device__ void join_splits(const AttendParams& p, int b, int hkv, int e0, int nE, int64_t slot0, int active,
+                            float* buf /* [kAtWarps][Dv + 2] */) {
   const int D = p.Dv, stride = D + 2;
-  for (int i = threadIdx.x; i < nE * D; i += blockDim.x) {
-    const int e = i / D, d = i - e * D;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int e = 0; e < nE; ++e) {
     const float* base = p.part + (slot0 * 8 + e) * stride;
     float M = -INFINITY;
-    for (int s = 0; s < active; ++s) M = fmaxf(M, __ldcg(base + (int64_t)s * 8 * stride));
-    float l = 0.f, o = 0.f;
-    if (M > -INFINITY) {
+    for (int s = lane; s < active; s += 32) M = fmaxf(M, __ldcg(base + (int64_t)s * 8 * stride));
+    M = warp_max(M);
+    float l = 0.f, o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (M > -INFINITY && warp < kAtWarps) {
 #pragma unroll 4
-      for (int s = 0; s < active; ++s) {
+      for (int s = warp; s < active; s += kAtWarps) {
         const float* q = base + (int64_t)s * 8 * stride;
         const float w = ex2(__ldcg(q) - M);
         l += w * __ldcg(q + 1);
-        o += w * __ldcg(q + 2 + d);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (lane + 32 * i < D) o[i] += w * __ldcg(q + 2 + lane + 32 * i);
       }
     }
+    __syncthreads();
+    if (warp < kAtWarps) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (lane + 32 * i < D) buf[warp * stride + 2 + lane + 32 * i] = o[i];
+      if (lane == 0) buf[warp * stride] = l;
+    }
+    __syncthreads();
+    float lt = 0.f;
+#pragma unroll
+    for (int w = 0; w < kAtWarps; ++w) lt += buf[w * stride];
     const int64_t head = (int64_t)b * p.Hq + hkv * p.E + e0 + e;
-    static_cast<TQ*>(p.out)[head * D + d] = from_f<TQ>(l != 0.f ? o / l : 0.f);
-    if (d == 0) p.lse[head] = l != 0.f ? (M + log2f(l)) * kLn2 : -INFINITY;
+    for (int d = threadIdx.x; d < D; d += blockDim.x) {
+      float ot = 0.f;
+#pragma unroll
+      for (int w = 0; w < kAtWarps; ++w) ot += buf[w * stride + 2 + d];
+      static_cast<TQ*>(p.out)[head * D + d] = from_f<TQ>(lt != 0.f ? ot / lt : 0.f);
+    }
+    if (threadIdx.x == 0) p.lse[head] = lt != 0.f ? (M + log2f(lt)) * kLn2 : -INFINITY;
   }
 }
 
@@ -473,7 +519,7 @@ __device__ void join_splits(const AttendParams& p, int b, int hkv, int e0, int n
 // The counts return to zero.
 template <typename TQ>
 __device__ void close_split(const AttendParams& p, int b, int hg, int e0, int nE, int64_t slot0, int active, int pos,
-                            int* flag) {
+                            int* flag, float* buf) {
   const int total = p.advance ? p.splits : active, per = p.Hkv * p.groups;
   if (total > 1) {
     __threadfence();
@@ -487,7 +533,7 @@ __device__ void close_split(const AttendParams& p, int b, int hg, int e0, int nE
     __syncthreads();
     if (!*flag) return;
     __threadfence();
-    if (active > 1) join_splits<TQ>(p, b, hg / p.groups, e0, nE, slot0, active);
+    if (active > 1) join_splits<TQ>(p, b, hg / p.groups, e0, nE, slot0, active, buf);
   }
   if (p.advance && threadIdx.x == 0) {
     int32_t* d = p.done + (int64_t)p.B * per + b;
@@ -498,36 +544,81 @@ __device__ void close_split(const AttendParams& p, int b, int hg, int e0, int nE
   }
 }
 
+// tanh to 1e-6 of its value: the Maclaurin series through y^13 up to 1/2 (next
+// term 1e-7 of the sum), beyond it 1 - 2 / (e^2y + 1) (3e-7 of at least 0.46).
+__device__ __forceinline__ float tanh_rel(float y) {
+  const float w = y * y;
+  float s = fmaf(w, 21844.f / 6081075.f, -1382.f / 155925.f);
+  s = fmaf(w, s, 62.f / 2835.f);
+  s = fmaf(w, s, -17.f / 315.f);
+  s = fmaf(w, s, 2.f / 15.f);
+  s = fmaf(w, s, -1.f / 3.f);
+  s = fmaf(y * w, s, y);
+  const float t = 1.f - __fdividef(2.f, ex2(fabsf(y) * (2.f * kLog2e)) + 1.f);
+  return fabsf(y) <= 0.5f ? s : copysignf(t, y);
+}
+
 // Tensor-core path, Dk = Dv = D (64 or 128).  CTA = one chunk of one sequence
-// and up to eight query heads of one key head; four warps, sixteen tokens a
-// warp and step, m16n8k16 f16 products with fp32 accumulators:
+// and up to eight query heads of one key head.  The chunk's codes stream into a
+// ring of 64-token stages by TMA (16 KB at D = 128, 48 KB in flight per CTA, three
+// CTAs per SM): the last of the four warps to finish a stage refills it.  (A fifth
+// warp for that would cost a third of the registers: ten warps leave 168 each as
+// twelve do.)  A warp takes sixteen tokens of a stage, with m16n8k16 f16 products
+// and fp32 accumulators:
 //   S[head, token] = q K^T:  A = q, rows 0-7 the f16 roundings of the heads'
 //     q and rows 8-15 what the roundings left over, so S = row h + row h + 8
 //     has q to 22 bits; B = codes, exact in f16.
 //   O[head, dim] += P V:     A = P, split in two the same way, with the value
 //     rows' scales folded into it (relative to their largest so far, times 2^14:
 //     the f16 leftovers of a weight 2^-k keep 22 - max(0, k - 17) bits).
-// A dot product does not care about the order of its terms, so a lane loads 16
-// consecutive codes of a token (64 or 128 bytes of a row per four lanes) and
-// the A operand follows that order; likewise output dims follow the value
-// loads.  P leaves S's accumulator layout as the A operand without a shuffle.
-// Codes go from global memory straight to registers, one step ahead.
-constexpr int kAtThreads = 128;
+// A dot product does not care about the order of its terms, so a lane reads 16
+// consecutive codes of a token and the A operand follows that order; likewise
+// output dims follow the value reads.  P leaves S's accumulator layout as the A
+// operand without a shuffle.  Column n of an eight of tokens is token n or, for
+// odd n, (n - 1 ^ 4) + 1: with the 128-byte swizzle the eight lanes of a shared
+// memory phase then meet eight different bank groups, for keys and for values.
+//
+// Bound by HBM in principle (2 (D + 4) bytes a token and key head); per sixteen
+// tokens a warp issues some 280 instructions, half of them code conversions.
+constexpr int kAtThreads = 32 * kAtWarps;
 constexpr float kUp = 16384.f;
+constexpr int kStage = 64;  // tokens per stage
+
+template <int D> struct AtSmem {
+  static constexpr int kTile = kStage * D;  // codes of one stage, keys or values
+  static constexpr int kNS = D == 128 ? 3 : 4;
+  static constexpr int QS = D + 8;             // q row stride (halves)
+  static constexpr int OS = D + D / 32 * 4;    // O row stride (floats)
+  static constexpr int kBytes = 2 * kNS * kTile + 1024;
+};
+
+// Byte of 16-byte chunk `c` of row `r` in a stage (TMA swizzle of D-byte rows).
+template <int D>
+__device__ __forceinline__ int stage_at(int r, int c) {
+  return r * D + ((D == 128 ? c ^ (r & 7) : c ^ ((r >> 1) & 3)) << 4);
+}
+// Token of column n (0..7) of an eight.
+__device__ __forceinline__ int tok_of(int n) { return n & 1 ? ((n - 1) ^ 4) | 1 : n; }
+
 template <typename TQ, int STORE, int D, bool CAP, bool STEP>
-__global__ void __launch_bounds__(kAtThreads, 3) attend_mma(AttendParams p) {
-  constexpr int KS = D / 16;        // k steps of S
-  constexpr int NC = D / 64;        // 16-byte key chunks per lane and token
-  constexpr int ND = D / 8;         // n tiles of O
-  constexpr int VB = D / 8;         // value codes per lane and token
-  constexpr int QS = D + 8;         // q row stride in shared memory (halves)
-  constexpr int OS = D + D / 32 * 4;  // O row stride (floats)
+__global__ void __launch_bounds__(kAtThreads, 3)
+    attend_mma(const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv,
+               const __grid_constant__ AttendParams p) {
+  using Z = AtSmem<D>;
+  constexpr int KS = D / 16;  // k steps of S
+  constexpr int ND = D / 8;   // n tiles of O
+  constexpr int VB = D / 8;   // value codes per lane and token
+  constexpr int NS = Z::kNS, QS = Z::QS, OS = Z::OS;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   __shared__ __align__(16) union {
     __half q[16 * QS];
-    float o[4 * 8 * OS];
-  } sm;
-  __shared__ float qf_s[8], m_s[4][8], l_s[4][8];
-  __shared__ int flag;
+    float o[kAtWarps * 8 * OS];
+  } u;
+  __shared__ __align__(128) uint8_t new_s[2][128];  // the new token's codes, as a stage row of its slot holds them
+  __shared__ float new_scale[2], qf_s[8], qs_s[8], m_s[kAtWarps][8], l_s[kAtWarps][8];
+  __shared__ uint64_t full[NS];
+  __shared__ int flag, abort_s, taken[NS];  // taken: warps done with the stage so far
 
   const int split = blockIdx.x;
   const int hg = blockIdx.y, b = blockIdx.z;
@@ -539,24 +630,44 @@ __global__ void __launch_bounds__(kAtThreads, 3) attend_mma(AttendParams p) {
   const int active = max(1, min(p.splits, (ntok + p.chunk - 1) / p.chunk));
   const int64_t slot0 = ((int64_t)b * p.Hkv * p.groups + hg) * p.splits;
   if (split >= active) {
-    if (p.advance) close_split<TQ>(p, b, hg, e0, nE, slot0, active, pos, &flag);
+    if (p.advance) close_split<TQ>(p, b, hg, e0, nE, slot0, active, pos, &flag, u.o);
     return;
   }
   const int c0 = split * p.chunk, c1 = split == active - 1 ? ntok : c0 + p.chunk;
+  const int stages = (c1 - c0 + kStage - 1) / kStage;
   const int64_t head = (int64_t)b * p.Hkv + hkv;
+  const bool owner = STEP && split == active - 1 && pos < p.cap;  // its chunk holds the new slot
+  volatile int* abort_flag = &abort_s;
 
+  auto fill = [&](int i) {  // one thread: stage i of the chunk
+    const int st = i % NS;
+    mbar_expect_tx(&full[st], 2 * Z::kTile);
+    tma_load_3d(sm + 2 * st * Z::kTile, &tmk, 0, c0 + i * kStage, (int)head, &full[st]);
+    tma_load_3d(sm + (2 * st + 1) * Z::kTile, &tmv, 0, c0 + i * kStage, (int)head, &full[st]);
+  };
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < NS; ++i) {
+      mbar_init(&full[i], 1);
+      taken[i] = 0;
+    }
+    abort_s = 0;
+    mbar_fence_init();
+    fence_async_smem();
+    for (int i = 0; i < NS && i < stages; ++i) fill(i);
+  }
   // q: rotate, bring each head's largest element to [2^13, 2^14), split in two
-  for (int e = warp; e < 8; e += 4) {
+  for (int e = warp; e < 8; e += kAtWarps) {
     const TQ* x = static_cast<const TQ*>(p.q) + b * p.q_sb + (int64_t)(hkv * p.E + e0 + e) * p.q_sh;
     float y1[D / 64], y2[D / 64];
     int i1[D / 64], i2[D / 64];
     uint32_t m = 0;
+    float sum = 0.f;
 #pragma unroll
     for (int j = 0; j < D / 64; ++j) {
-      const int u = lane + 32 * j;
+      const int v = lane + 32 * j;
       y1[j] = y2[j] = 0.f;
-      if (e < nE) load_pair(p, x, u, D, STEP ? p.R : 0, pos, &i1[j], &i2[j], &y1[j], &y2[j]);
-      else pair_dims(u, STEP ? p.R : 0, p.interleaved, D, &i1[j], &i2[j]);
+      if (e < nE) load_pair(p, x, v, D, STEP ? p.R : 0, pos, &i1[j], &i2[j], &y1[j], &y2[j]);
+      else pair_dims(v, STEP ? p.R : 0, p.interleaved, D, &i1[j], &i2[j]);
       m = max(m, max(abs_bits(y1[j]), abs_bits(y2[j])));
     }
 #pragma unroll
@@ -567,190 +678,221 @@ __global__ void __launch_bounds__(kAtThreads, 3) attend_mma(AttendParams p) {
 #pragma unroll
     for (int j = 0; j < D / 64; ++j) {
       const float a = y1[j] * up, c = y2[j] * up;
+      sum += a + c;
       const __half ah = __float2half_rn(a), ch = __float2half_rn(c);
-      sm.q[e * QS + i1[j]] = ah;
-      sm.q[e * QS + i2[j]] = ch;
-      sm.q[(e + 8) * QS + i1[j]] = __float2half_rn(a - __half2float(ah));
-      sm.q[(e + 8) * QS + i2[j]] = __float2half_rn(c - __half2float(ch));
+      u.q[e * QS + i1[j]] = ah;
+      u.q[e * QS + i2[j]] = ch;
+      u.q[(e + 8) * QS + i1[j]] = __float2half_rn(a - __half2float(ah));
+      u.q[(e + 8) * QS + i2[j]] = __float2half_rn(c - __half2float(ch));
     }
-    if (lane == 0) qf_s[e] = down * p.qscale * (CAP ? 1.f / p.softcap : kLog2e);
+    sum = warp_sum(sum);
+    if (lane == 0) {
+      qf_s[e] = down * p.qscale * (CAP ? 1.f / p.softcap : kLog2e);
+      qs_s[e] = -Codec<STORE>::kOff * sum;
+    }
   }
   if constexpr (STEP) {
-    // the CTA whose chunk holds the new slot writes it before it reads its chunk
-    // (head groups of one key head write the same bytes)
-    if (split == active - 1 && pos < p.cap) {
-      if (warp == 2)
-        write_token<TQ, STORE>(p, static_cast<const TQ*>(p.k_t) + b * p.k_sb + hkv * p.k_sh, D, p.R, pos, head, p.k, p.ks,
-                               p.k_new);
-      if (warp == 3)
-        write_token<TQ, STORE>(p, static_cast<const TQ*>(p.v_t) + b * p.v_sb + hkv * p.v_sh, D, 0, pos, head, p.v, p.vs,
-                               p.v_new);
-    } else if (split == active - 1 && threadIdx.x == 0 && p.status) {
-      atomicOr(p.status, TC_DEV_BAD_INDEX);
+    // The new token's row goes to the cache and, for this chunk's attention, to
+    // new_s: the stage may have been loaded before the row was written.  (Head
+    // groups of one key head write the same bytes.)
+    if (owner && warp >= 2) {
+      const int which = warp - 2;
+      const int r = (pos - c0) % kStage;
+      const TQ* x = which ? static_cast<const TQ*>(p.v_t) + b * p.v_sb + hkv * p.v_sh
+                          : static_cast<const TQ*>(p.k_t) + b * p.k_sb + hkv * p.k_sh;
+      write_token<TQ, STORE>(p, x, D, which ? 0 : p.R, pos, head, which ? p.v : p.k, which ? p.vs : p.ks,
+                             which ? p.v_new : p.k_new, new_s[which], &new_scale[which],
+                             [&](int d) { return stage_at<D>(r, d >> 4) - r * D + (d & 15); });
     }
+    if (split == active - 1 && !owner && threadIdx.x == 0 && p.status) atomicOr(p.status, TC_DEV_BAD_INDEX);
   }
   __syncthreads();
 
-  // A operand of S: k step 4 c + w covers, for lane t, the codes of word w of
-  // its 16-byte chunk c, dims 64 c + 16 t + 4 w + {0, 1 | 2, 3}
-  uint32_t qa[KS][4];
+  {
+    // A operand of S: k step 4 c + w covers, for lane t, the codes of word w of
+    // its 16-byte chunk 4 c + t, dims 64 c + 16 t + 4 w + {0, 1 | 2, 3}
+    uint32_t qa[KS][4];
 #pragma unroll
-  for (int s = 0; s < KS; ++s) {
-    const int d = 64 * (s / 4) + 16 * t + 4 * (s % 4);
-    const uint2 hi = *reinterpret_cast<const uint2*>(sm.q + g * QS + d);
-    const uint2 lo = *reinterpret_cast<const uint2*>(sm.q + (g + 8) * QS + d);
-    qa[s][0] = hi.x, qa[s][1] = lo.x, qa[s][2] = hi.y, qa[s][3] = lo.y;
-  }
-  const float qf = qf_s[g];
-  const float kc = p.softcap * kLog2e;
-  __syncthreads();  // sm.o takes q's place below
-
-  const uint8_t* kb = p.k + head * p.cap * D + 16 * t;
-  const uint8_t* vb = p.v + head * p.cap * D + VB * g;
-  const float* ksb = p.ks + head * p.cap;
-  const float* vsb = p.vs + head * p.cap;
-
-  uint4 kw[2][NC];
-  uint32_t vw[4][VB / 4];
-  float ksv[4], vsv[4];
-  auto load = [&](int base) {
-#pragma unroll
-    for (int nt = 0; nt < 2; ++nt) {
-      const int tok = base + 8 * nt + g;
-#pragma unroll
-      for (int c = 0; c < NC; ++c)
-        kw[nt][c] = tok < c1 ? *reinterpret_cast<const uint4*>(kb + (int64_t)tok * D + 64 * c) : make_uint4(0, 0, 0, 0);
+    for (int s = 0; s < KS; ++s) {
+      const int d = 64 * (s / 4) + 16 * t + 4 * (s % 4);
+      const uint2 hi = *reinterpret_cast<const uint2*>(u.q + g * QS + d);
+      const uint2 lo = *reinterpret_cast<const uint2*>(u.q + (g + 8) * QS + d);
+      qa[s][0] = hi.x, qa[s][1] = lo.x, qa[s][2] = hi.y, qa[s][3] = lo.y;
     }
+    const float qf = qf_s[g], qoff = qs_s[g];
+    const float kc = p.softcap * kLog2e;
+    const int kr = 16 * warp + tok_of(g);                               // rows of the stage this lane reads
+    const int tv[4] = {2 * t, tok_of(2 * t + 1), 8 + 2 * t, 8 + tok_of(2 * t + 1)};
+    float o[ND][4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int tok = base + (i & 1) + 2 * t + 8 * (i >> 1);
-      const bool ok = tok < c1;
-      if constexpr (VB == 16) {
-        const uint4 w = ok ? *reinterpret_cast<const uint4*>(vb + (int64_t)tok * D) : make_uint4(0, 0, 0, 0);
-        vw[i][0] = w.x, vw[i][1] = w.y, vw[i][2] = w.z, vw[i][3] = w.w;
-      } else {
-        const uint2 w = ok ? *reinterpret_cast<const uint2*>(vb + (int64_t)tok * D) : make_uint2(0, 0);
-        vw[i][0] = w.x, vw[i][1] = w.y;
+    for (int i = 0; i < ND; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+    float m = -INFINITY, ell = 0.f, vref = kTiny;
+    // lanes 0-15 hold the key scales of the warp's sixteen tokens, 16-31 the value scales
+    const float* scb = (lane < 16 ? p.ks : p.vs) + head * p.cap + c0 + 16 * warp + (lane & 15);
+    auto load_scales = [&](int at) { return c0 + 16 * warp + at + (lane & 15) < c1 ? scb[at] : 0.f; };
+    float scales = load_scales(0);
+
+    auto sixteen = [&](auto tail, int st, int at) {
+      constexpr bool TAIL = decltype(tail)::value;
+      const uint8_t* kt = sm + 2 * st * Z::kTile;
+      const uint8_t* vt = kt + Z::kTile;
+      const int left = c1 - (c0 + 16 * warp + at);         // tokens of the sixteen that count
+      const int np = TAIL && owner ? pos - (c0 + 16 * warp + at) : -1;  // the new one among them
+      float sc[2][4];
+#pragma unroll
+      for (int nt = 0; nt < 2; ++nt) {
+        const int r = kr + 8 * nt;
+        const uint8_t* row = kt;
+        int at0 = stage_at<D>(r, t), at1 = D == 128 ? stage_at<D>(r, 4 + t) : 0;
+        if (TAIL && np == r - 16 * warp) {
+          row = new_s[0];
+          at0 -= r * D;
+          at1 -= r * D;
+        }
+        uint4 kw[D / 64];
+        kw[0] = *reinterpret_cast<const uint4*>(row + at0);
+        if constexpr (D == 128) kw[1] = *reinterpret_cast<const uint4*>(row + at1);
+        sc[nt][0] = sc[nt][1] = sc[nt][2] = sc[nt][3] = 0.f;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+          const uint4 q4 = kw[s / 4];
+          const uint32_t w = (s % 4) == 0 ? q4.x : (s % 4) == 1 ? q4.y : (s % 4) == 2 ? q4.z : q4.w;
+          mma16816(sc[nt], qa[s], Codec<STORE>::template raw_pair<false>(w), Codec<STORE>::template raw_pair<true>(w));
+        }
       }
-      ksv[i] = ok ? ksb[tok] : 0.f;
-      vsv[i] = ok ? vsb[tok] : 0.f;
-    }
-  };
+      float x[4], vsc[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float ks = __shfl_sync(0xffffffffu, scales, tv[i]);
+        vsc[i] = __shfl_sync(0xffffffffu, scales, 16 + tv[i]);
+        if (TAIL && np == tv[i]) {
+          ks = new_scale[0];
+          vsc[i] = new_scale[1];
+        }
+        float y = fmaf(sc[i >> 1][i & 1] + sc[i >> 1][2 + (i & 1)], Codec<STORE>::kMul, qoff) * (qf * ks);
+        if constexpr (CAP) y = kc * tanh_rel(y);
+        x[i] = !TAIL || tv[i] < left ? y : -INFINITY;
+        if (TAIL && tv[i] >= left) vsc[i] = 0.f;
+      }
+      if (!TAIL) scales = load_scales(at + kStage);  // the next stage's, a stage ahead
 
-  float o[ND][4];
+      float mx = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+      float vx = fmaxf(fmaxf(vsc[0], vsc[1]), fmaxf(vsc[2], vsc[3]));
 #pragma unroll
-  for (int i = 0; i < ND; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-  float m = -INFINITY, ell = 0.f, vref = kTiny;
+      for (int d = 1; d <= 2; d <<= 1) {
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+        vx = fmaxf(vx, __shfl_xor_sync(0xffffffffu, vx, d));
+      }
+      const float mn = fmaxf(m, mx), vn = fmaxf(vref, vx);
+      if (__any_sync(0xffffffffu, mn > m || vn > vref)) {
+        const float cm = m == mn ? 1.f : ex2(m - mn);  // m -inf: 0
+        const float co = cm * (vref / vn);
+        ell *= cm;
+#pragma unroll
+        for (int i = 0; i < ND; ++i) o[i][0] *= co, o[i][1] *= co, o[i][2] *= co, o[i][3] *= co;
+        m = mn;
+        vref = vn;
+      }
+      const float vinv = __fdividef(kUp, vref);
+      const float me = m == -INFINITY ? 0.f : m;
+      float pr[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float e = ex2(x[i] - me);
+        ell += e;
+        pr[i] = e * (vsc[i] * vinv);
+      }
+      uint32_t pa[4];
+#pragma unroll
+      for (int nt = 0; nt < 2; ++nt) {
+        const uint32_t hi = pack_h2(pr[2 * nt], pr[2 * nt + 1]);
+        const float2 h2 = unpack_h2(hi);
+        pa[2 * nt] = hi;
+        pa[2 * nt + 1] = pack_h2(pr[2 * nt] - h2.x, pr[2 * nt + 1] - h2.y);
+      }
+      uint32_t vw[4][VB / 4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int r = 16 * warp + tv[i];
+        const uint8_t* row = vt + stage_at<D>(r, D == 128 ? g : g >> 1) + (D == 128 ? 0 : (g & 1) * 8);
+        if (TAIL && np == tv[i]) row = new_s[1] + (row - vt) - r * D;
+        if constexpr (VB == 16) {
+          uint4 w = *reinterpret_cast<const uint4*>(row);
+          if (TAIL && tv[i] >= left) w = make_uint4(0, 0, 0, 0);  // an e4m3 NaN times 0 is one
+          vw[i][0] = w.x, vw[i][1] = w.y, vw[i][2] = w.z, vw[i][3] = w.w;
+        } else {
+          uint2 w = *reinterpret_cast<const uint2*>(row);
+          if (TAIL && tv[i] >= left) w = make_uint2(0, 0);
+          vw[i][0] = w.x, vw[i][1] = w.y;
+        }
+      }
+      // O += P V: word j of the lane's four tokens holds output dims VB g + 4 j + 0..3
+#pragma unroll
+      for (int j = 0; j < VB / 4; ++j) {
+        const uint32_t a0 = __byte_perm(vw[0][j], vw[1][j], 0x5140), a1 = __byte_perm(vw[0][j], vw[1][j], 0x7362);
+        const uint32_t b0 = __byte_perm(vw[2][j], vw[3][j], 0x5140), b1 = __byte_perm(vw[2][j], vw[3][j], 0x7362);
+        mma16816(o[4 * j], pa, Codec<STORE>::template pair<false>(a0), Codec<STORE>::template pair<false>(b0));
+        mma16816(o[4 * j + 1], pa, Codec<STORE>::template pair<true>(a0), Codec<STORE>::template pair<true>(b0));
+        mma16816(o[4 * j + 2], pa, Codec<STORE>::template pair<false>(a1), Codec<STORE>::template pair<false>(b1));
+        mma16816(o[4 * j + 3], pa, Codec<STORE>::template pair<true>(a1), Codec<STORE>::template pair<true>(b1));
+      }
+    };
 
-  int base = c0 + 16 * warp;
-  if (base < c1) load(base);
-  for (; base < c1; base += 64) {
-    // S of two eights of tokens
-    float sc[2][4];
-#pragma unroll
-    for (int nt = 0; nt < 2; ++nt) {
-      sc[nt][0] = sc[nt][1] = sc[nt][2] = sc[nt][3] = 0.f;
-#pragma unroll
-      for (int s = 0; s < KS; ++s) {
-        const uint4 q4 = kw[nt][s / 4];
-        const uint32_t w = (s % 4) == 0 ? q4.x : (s % 4) == 1 ? q4.y : (s % 4) == 2 ? q4.z : q4.w;
-        mma16816(sc[nt], qa[s], Codec<STORE>::template pair<false>(w), Codec<STORE>::template pair<true>(w));
+    bool alive = true;
+    for (int i = 0; i < stages; ++i) {
+      const int st = i % NS;
+      alive = __all_sync(0xffffffffu, mbar_wait(&full[st], (i / NS) & 1, abort_flag, p.status));
+      if (!alive) break;
+      const int left = c1 - (c0 + 16 * warp + i * kStage);
+      // the last stage may end inside the sixteen and hold the new token
+      if (i + 1 < stages) sixteen(std::false_type{}, st, i * kStage);
+      else if (left > 0) sixteen(std::true_type{}, st, i * kStage);
+      __syncwarp();
+      if (lane == 0 && i + NS < stages) {
+        __threadfence_block();
+        if ((atomicAdd(&taken[st], 1) & (kAtWarps - 1)) == kAtWarps - 1) {
+          __threadfence_block();
+          fill(i + NS);
+        }
       }
     }
-    float x[4], vsc[4];
-    uint32_t vcur[4][VB / 4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int tok = base + (i & 1) + 2 * t + 8 * (i >> 1);
-      float y = (sc[i >> 1][i & 1] + sc[i >> 1][2 + (i & 1)]) * (qf * ksv[i]);
-      if constexpr (CAP) y = kc * tanhf(y);  // a relative error: 1 - 2 / (e^2y + 1) is off by 3e-7 of the cap
-      x[i] = tok < c1 ? y : -INFINITY;
-      vsc[i] = vsv[i];
-#pragma unroll
-      for (int j = 0; j < VB / 4; ++j) vcur[i][j] = vw[i][j];
-    }
-    if (base + 64 < c1) load(base + 64);
 
-    float mx = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
-    float vx = fmaxf(fmaxf(vsc[0], vsc[1]), fmaxf(vsc[2], vsc[3]));
-#pragma unroll
-    for (int d = 1; d <= 2; d <<= 1) {
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
-      vx = fmaxf(vx, __shfl_xor_sync(0xffffffffu, vx, d));
+    // join the warps: n column 2 t + c of tile i is output dim VB (2 t + c) + i
+    __syncthreads();  // every warp has its q operand: u.o takes its place
+    ell += __shfl_xor_sync(0xffffffffu, ell, 1);
+    ell += __shfl_xor_sync(0xffffffffu, ell, 2);
+    if (t == 0) {
+      m_s[warp][g] = m;
+      l_s[warp][g] = ell;
     }
-    const float mn = fmaxf(m, mx), vn = fmaxf(vref, vx);
-    if (__any_sync(0xffffffffu, mn > m || vn > vref)) {
-      const float cm = m == mn ? 1.f : ex2(m - mn);  // m -inf: 0
-      const float co = cm * (vref / vn);
-      ell *= cm;
+    float* ow = u.o + (warp * 8 + g) * OS;
+    const float vout = vref / kUp;
 #pragma unroll
-      for (int i = 0; i < ND; ++i) o[i][0] *= co, o[i][1] *= co, o[i][2] *= co, o[i][3] *= co;
-      m = mn;
-      vref = vn;
-    }
-    const float vinv = kUp / vref;
-    const float me = m == -INFINITY ? 0.f : m;
-    float pr[4];
+    for (int c = 0; c < 2; ++c)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float e = ex2(x[i] - me);
-      ell += e;
-      pr[i] = e * (vsc[i] * vinv);
-    }
-    uint32_t pa[4];
-#pragma unroll
-    for (int nt = 0; nt < 2; ++nt) {
-      const uint32_t hi = pack_h2(pr[2 * nt], pr[2 * nt + 1]);
-      const float2 h2 = unpack_h2(hi);
-      pa[2 * nt] = hi;
-      pa[2 * nt + 1] = pack_h2(pr[2 * nt] - h2.x, pr[2 * nt + 1] - h2.y);
-    }
-    // O += P V: word j of the lane's four tokens holds output dims VB g + 4 j + 0..3
-#pragma unroll
-    for (int j = 0; j < VB / 4; ++j) {
-      const uint32_t a0 = __byte_perm(vcur[0][j], vcur[1][j], 0x5140), a1 = __byte_perm(vcur[0][j], vcur[1][j], 0x7362);
-      const uint32_t b0 = __byte_perm(vcur[2][j], vcur[3][j], 0x5140), b1 = __byte_perm(vcur[2][j], vcur[3][j], 0x7362);
-      mma16816(o[4 * j], pa, Codec<STORE>::template pair<false>(a0), Codec<STORE>::template pair<false>(b0));
-      mma16816(o[4 * j + 1], pa, Codec<STORE>::template pair<true>(a0), Codec<STORE>::template pair<true>(b0));
-      mma16816(o[4 * j + 2], pa, Codec<STORE>::template pair<false>(a1), Codec<STORE>::template pair<false>(b1));
-      mma16816(o[4 * j + 3], pa, Codec<STORE>::template pair<true>(a1), Codec<STORE>::template pair<true>(b1));
-    }
+      for (int i = 0; i < ND; i += 4) {
+        const int d = VB * (2 * t + c) + i;
+        float4 w;
+        w.x = (o[i][c] + o[i][2 + c]) * vout;
+        w.y = (o[i + 1][c] + o[i + 1][2 + c]) * vout;
+        w.z = (o[i + 2][c] + o[i + 2][2 + c]) * vout;
+        w.w = (o[i + 3][c] + o[i + 3][2 + c]) * vout;
+        *reinterpret_cast<float4*>(ow + d + d / 32 * 4) = w;
+      }
   }
-
-  // join the warps: n column 2 t + c of tile i is output dim VB (2 t + c) + i
-  ell += __shfl_xor_sync(0xffffffffu, ell, 1);
-  ell += __shfl_xor_sync(0xffffffffu, ell, 2);
-  if (t == 0) {
-    m_s[warp][g] = m;
-    l_s[warp][g] = ell;
-  }
-  float* ow = sm.o + (warp * 8 + g) * OS;
-  const float vout = vref / kUp;
-#pragma unroll
-  for (int c = 0; c < 2; ++c)
-#pragma unroll
-    for (int i = 0; i < ND; i += 4) {
-      const int d = VB * (2 * t + c) + i;
-      float4 w;
-      w.x = (o[i][c] + o[i][2 + c]) * vout;
-      w.y = (o[i + 1][c] + o[i + 1][2 + c]) * vout;
-      w.z = (o[i + 2][c] + o[i + 2][2 + c]) * vout;
-      w.w = (o[i + 3][c] + o[i + 3][2 + c]) * vout;
-      *reinterpret_cast<float4*>(ow + d + d / 32 * 4) = w;
-    }
   __syncthreads();
   for (int i = threadIdx.x; i < nE * D; i += kAtThreads) {
     const int e = i / D, d = i - e * D;
     float M = m_s[0][e];
 #pragma unroll
-    for (int w = 1; w < 4; ++w) M = fmaxf(M, m_s[w][e]);
+    for (int w = 1; w < kAtWarps; ++w) M = fmaxf(M, m_s[w][e]);
     float l = 0.f, ov = 0.f;
     if (M > -INFINITY) {
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
+      for (int w = 0; w < kAtWarps; ++w) {
         const float c = ex2(m_s[w][e] - M);
         l += c * l_s[w][e];
-        ov += c * sm.o[(w * 8 + e) * OS + d + d / 32 * 4];
+        ov += c * u.o[(w * 8 + e) * OS + d + d / 32 * 4];
       }
     }
     if (active == 1) {
@@ -766,15 +908,15 @@ __global__ void __launch_bounds__(kAtThreads, 3) attend_mma(AttendParams p) {
       }
     }
   }
-  close_split<TQ>(p, b, hg, e0, nE, slot0, active, pos, &flag);
+  close_split<TQ>(p, b, hg, e0, nE, slot0, active, pos, &flag, u.o);
 }
 
 // Any head dims up to 256 and any head count: fp32 on the CUDA cores, a warp per
 // token, lanes over dims; the same splits and the same join.
-constexpr int kAnyDims = 256 / 32;
+constexpr int kAnyDims = 256 / 32, kAnyThreads = 128;
 template <typename TQ, int STORE, bool STEP>
-__global__ void __launch_bounds__(kAtThreads) attend_any(AttendParams p) {
-  __shared__ float q_s[256], o_s[4][256], m_s[4], l_s[4];
+__global__ void __launch_bounds__(kAnyThreads) attend_any(AttendParams p) {
+  __shared__ float q_s[256], o_s[4][256 + 2], m_s[4], l_s[4];
   __shared__ int flag;
   const int split = blockIdx.x, hg = blockIdx.y, b = blockIdx.z;
   const int hkv = hg / p.groups, e0 = (hg - hkv * p.groups) * 8;
@@ -785,7 +927,7 @@ __global__ void __launch_bounds__(kAtThreads) attend_any(AttendParams p) {
   const int active = max(1, min(p.splits, (ntok + p.chunk - 1) / p.chunk));
   const int64_t slot0 = ((int64_t)b * p.Hkv * p.groups + hg) * p.splits;
   if (split >= active) {
-    if (p.advance) close_split<TQ>(p, b, hg, e0, nE, slot0, active, pos, &flag);
+    if (p.advance) close_split<TQ>(p, b, hg, e0, nE, slot0, active, pos, &flag, &o_s[0][0]);
     return;
   }
   const int c0 = split * p.chunk, c1 = split == active - 1 ? ntok : c0 + p.chunk;
@@ -794,10 +936,10 @@ __global__ void __launch_bounds__(kAtThreads) attend_any(AttendParams p) {
     if (split == active - 1 && pos < p.cap) {
       if (warp == 0)
         write_token<TQ, STORE>(p, static_cast<const TQ*>(p.k_t) + b * p.k_sb + hkv * p.k_sh, p.Dk, p.R, pos, head, p.k,
-                               p.ks, p.k_new);
+                               p.ks, p.k_new, nullptr, nullptr, [](int) { return 0; });
       if (warp == 1)
         write_token<TQ, STORE>(p, static_cast<const TQ*>(p.v_t) + b * p.v_sb + hkv * p.v_sh, p.Dv, 0, pos, head, p.v,
-                               p.vs, p.v_new);
+                               p.vs, p.v_new, nullptr, nullptr, [](int) { return 0; });
     } else if (split == active - 1 && threadIdx.x == 0 && p.status) {
       atomicOr(p.status, TC_DEV_BAD_INDEX);
     }
@@ -805,7 +947,7 @@ __global__ void __launch_bounds__(kAtThreads) attend_any(AttendParams p) {
   for (int e = 0; e < nE; ++e) {
     __syncthreads();
     const TQ* x = static_cast<const TQ*>(p.q) + b * p.q_sb + (int64_t)(hkv * p.E + e0 + e) * p.q_sh;
-    for (int u = threadIdx.x; u < (p.Dk + 1) / 2; u += kAtThreads) {
+    for (int u = threadIdx.x; u < (p.Dk + 1) / 2; u += kAnyThreads) {
       int i1, i2;
       float y1, y2;
       load_pair(p, x, u, p.Dk, STEP ? p.R : 0, pos, &i1, &i2, &y1, &y2);
@@ -843,7 +985,7 @@ __global__ void __launch_bounds__(kAtThreads) attend_any(AttendParams p) {
     }
     __syncthreads();
     float M = fmaxf(fmaxf(m_s[0], m_s[1]), fmaxf(m_s[2], m_s[3]));
-    for (int d = threadIdx.x; d < p.Dv; d += kAtThreads) {
+    for (int d = threadIdx.x; d < p.Dv; d += kAnyThreads) {
       float l = 0.f, ov = 0.f;
       if (M > -INFINITY) {
 #pragma unroll
@@ -867,23 +1009,50 @@ __global__ void __launch_bounds__(kAtThreads) attend_any(AttendParams p) {
       }
     }
   }
-  close_split<TQ>(p, b, hg, e0, nE, slot0, active, pos, &flag);
+  close_split<TQ>(p, b, hg, e0, nE, slot0, active, pos, &flag, &o_s[0][0]);
 }
 
-template <typename TQ, int STORE, int D, bool STEP>
-int launch_mma(const AttendParams& p, dim3 grid, cudaStream_t st) {
-  if (p.has_cap) attend_mma<TQ, STORE, D, true, STEP><<<grid, kAtThreads, 0, st>>>(p);
-  else attend_mma<TQ, STORE, D, false, STEP><<<grid, kAtThreads, 0, st>>>(p);
+// Codes [rows * Hkv, capacity, D] as a 3-D map of kStage-token boxes, slots past the
+// capacity reading as zeros.
+template <int D>
+int code_map(CUtensorMap* m, const void* base, const AttendParams& p, int64_t heads) {
+  auto fn = tcx::encode_fn();
+  if (!fn) return TC_ERR_CUDA;
+  cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)p.cap, (cuuint64_t)heads};
+  cuuint64_t strides[2] = {(cuuint64_t)D, (cuuint64_t)D * p.cap};
+  cuuint32_t box[3] = {(cuuint32_t)D, (cuuint32_t)kStage, 1};
+  cuuint32_t estr[3] = {1, 1, 1};
+  const CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(base), dims, strides, box, estr,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, D == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? TC_OK : TC_ERR_CUDA;
+}
+
+template <typename TQ, int STORE, int D, bool CAP, bool STEP>
+int launch_mma(const AttendParams& p, int64_t heads, dim3 grid, cudaStream_t st) {
+  CUtensorMap mk, mv;
+  if (int rc = code_map<D>(&mk, p.k, p, heads)) return rc;
+  if (int rc = code_map<D>(&mv, p.v, p, heads)) return rc;
+  auto k = attend_mma<TQ, STORE, D, CAP, STEP>;
+  constexpr int smem = AtSmem<D>::kBytes;
+  if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return TC_ERR_CUDA;
+  k<<<grid, kAtThreads, smem, st>>>(mk, mv, p);
   return launch_status();
 }
 
 template <typename TQ, int STORE, bool STEP>
-int launch_attend(const AttendParams& p, cudaStream_t st) {
+int launch_attend(const AttendParams& p, int64_t rows, cudaStream_t st) {
   const dim3 grid(p.splits, p.Hkv * p.groups, p.B);
-  const bool mma = p.Dk == p.Dv && (p.Dk == 64 || p.Dk == 128) && (uintptr_t)p.k % 16 == 0 && (uintptr_t)p.v % 16 == 0;
-  if (mma && p.Dk == 128) return launch_mma<TQ, STORE, 128, STEP>(p, grid, st);
-  if (mma) return launch_mma<TQ, STORE, 64, STEP>(p, grid, st);
-  attend_any<TQ, STORE, STEP><<<grid, kAtThreads, 0, st>>>(p);
+  const int64_t heads = rows * p.Hkv;
+  const bool mma = p.Dk == p.Dv && (p.Dk == 64 || p.Dk == 128) && (uintptr_t)p.k % 16 == 0 && (uintptr_t)p.v % 16 == 0 &&
+                   heads <= INT32_MAX && p.cap * p.Dk < (int64_t(1) << 40);
+  if (mma && p.Dk == 128)
+    return p.has_cap ? launch_mma<TQ, STORE, 128, true, STEP>(p, heads, grid, st)
+                     : launch_mma<TQ, STORE, 128, false, STEP>(p, heads, grid, st);
+  if (mma)
+    return p.has_cap ? launch_mma<TQ, STORE, 64, true, STEP>(p, heads, grid, st)
+                     : launch_mma<TQ, STORE, 64, false, STEP>(p, heads, grid, st);
+  attend_any<TQ, STORE, STEP><<<grid, kAnyThreads, 0, st>>>(p);
   return launch_status();
 }
 
@@ -892,12 +1061,12 @@ bool cache_ok(const tc_kv_cache* c) {
          (c->store == TC_KV_INT8 || c->store == TC_KV_FP8) && c->k && c->v && c->k_scale && c->v_scale && c->lengths;
 }
 
-// Tokens per CTA and CTAs per (sequence, head group) over at most `most`
-// tokens.  The CTAs wanted are four waves of three per SM over 148 SMs, so that
-// sequences of different lengths even out; a chunk is at least 64 tokens (one
-// step of the four warps) and a multiple of 64.
-void split_rule(int64_t most, int64_t heads, int* chunk, int* splits) {
-  const int64_t want = (4 * 3 * 148 + heads - 1) / heads;
+// Tokens per CTA and CTAs per (sequence, head group) over at most `most` tokens.
+// One sequence: one wave of three CTAs per SM over 148 SMs.  Several may differ
+// in length: four waves, so that they even out.  A chunk is a multiple of 64
+// tokens (one stage).
+void split_rule(int64_t most, int64_t heads, int B, int* chunk, int* splits) {
+  const int64_t want = ((B > 1 ? 4 : 1) * 3 * 148 + heads - 1) / heads;
   int64_t c = (most + want - 1) / want;
   c = (c + 63) / 64 * 64;
   if (c < 64) c = 64;
@@ -947,7 +1116,7 @@ extern "C" int tc_kv_read(const tc_kv_cache* c, int32_t length, int32_t dtype, v
 static int attend_shape(const tc_kv_cache* c, int32_t B, int32_t Hq, int32_t max_tokens, int* chunk, int* splits) {
   if (!cache_ok(c) || B < 0 || Hq <= 0 || Hq % c->Hkv || max_tokens < 0) return TC_ERR_ARG;
   const int groups = (Hq / c->Hkv + 7) / 8;
-  split_rule(max_tokens < 1 ? 1 : max_tokens, (int64_t)(B < 1 ? 1 : B) * c->Hkv * groups, chunk, splits);
+  split_rule(max_tokens < 1 ? 1 : max_tokens, (int64_t)(B < 1 ? 1 : B) * c->Hkv * groups, B, chunk, splits);
   return TC_OK;
 }
 
@@ -987,7 +1156,7 @@ extern "C" int tc_kv_attend(const tc_kv_cache* c, const tc_kv_attend_args* a, vo
   p.out = a->out, p.lse = a->lse, p.k_new = a->k_new, p.v_new = a->v_new, p.new_dtype = a->new_dtype;
   p.part = a->scratch, p.done = a->counters, p.status = a->dev_status;
   cudaStream_t st = (cudaStream_t)stream;
-#define TC_KV_GO(S, STEP) TC_DISPATCH(a->dtype, T, return launch_attend<T, S, STEP>(p, st))
+#define TC_KV_GO(S, STEP) TC_DISPATCH(a->dtype, T, return launch_attend<T, S, STEP>(p, c->rows, st))
   if (c->store == TC_KV_INT8) {
     if (step) { TC_KV_GO(TC_KV_INT8, true); }
     else { TC_KV_GO(TC_KV_INT8, false); }

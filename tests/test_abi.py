@@ -95,8 +95,8 @@ def test_full_attention_structs_and_bad_arguments():
 
 
 def test_cached_attention_split_plan():
-    """Chunks are multiples of 64 tokens, four waves of three CTAs per SM are
-    wanted, one chunk needs no scratch."""
+    """Chunks are multiples of 64 tokens, one wave of three CTAs per SM is wanted
+    for one sequence and four for several, one chunk needs no scratch."""
     lib = _lib.lib()
     c = _lib.KVCacheArgs(rows=64, Hkv=4, Dk=128, Dv=128, capacity=40000, k=16, v=16, k_scale=16, v_scale=16,
                          lengths=16)
