@@ -594,7 +594,8 @@ typedef struct tc_kv_attend_args {
   void* k_new;               /* step: the key and value as stored [B, Hkv, D] */
   void* v_new;               /* of new_dtype, or NULL                        */
   int32_t new_dtype;
-  float* scratch;            /* tc_kv_attend_scratch_floats floats           */
+  float* scratch;            /* tc_kv_attend_scratch_floats floats, 16-byte
+                                aligned                                      */
   int64_t scratch_floats;
   int32_t* counters;         /* B (Hkv ceil(Hq / Hkv / 8) + 1) int32, zeros
                                 before the first call; every call leaves zeros */

@@ -364,7 +364,8 @@ struct AttendParams {
   void* v_new;
   int new_dtype;
   int chunk, splits;           // tokens per CTA, CTAs per (sequence, head group)
-  float* part;                 // [B * Hkv * groups * splits][8][Dv + 2]
+  float* part;                 // [B * Hkv * groups * splits][8][Dv] unnormalised O
+  float2* ml;                  // [B * Hkv * groups * splits][8] their maximum (log2 units) and sum
   int32_t* done;               // [B * Hkv * groups + B] arrival counts, zero between calls
   int32_t* status;
 };
@@ -464,51 +465,60 @@ __device__ void write_token(const AttendParams& p, const T* x, int D, int R, int
   }
 }
 
-// Joins the partial (m, l, O) of `active` splits of nE heads and writes out, lse.
-// The warps share the splits (a lane reads VE consecutive dims of one), then
-// join in shared memory: a chain of `active` / 4 reads instead of `active`.
+// Joins the partials of `active` splits of nE heads and writes out, lse: a warp
+// per head; a lane reads the (m, l) of every 32nd split, then consecutive dims of
+// one split after another, eight loads in flight.  (All warps on one head after
+// another left the last CTA 24 us of dependent loads over 54 splits.)
 constexpr int kAtWarps = 4;
 template <typename TQ>
-__device__ void join_splits(const AttendParams& p, int b, int hkv, int e0, int nE, int64_t slot0, int active,
-                            float* buf /* [kAtWarps][Dv + 2] */) {
-  const int D = p.Dv, stride = D + 2;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  for (int e = 0; e < nE; ++e) {
-    const float* base = p.part + (slot0 * 8 + e) * stride;
+__device__ void join_splits(const AttendParams& p, int b, int hkv, int e0, int nE, int64_t slot0, int active) {
+  const int D = p.Dv, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int e = warp; e < nE; e += kAtWarps) {
+    const float2* ml = p.ml + slot0 * 8 + e;
+    const float* part = p.part + (slot0 * 8 + e) * D;
     float M = -INFINITY;
-    for (int s = lane; s < active; s += 32) M = fmaxf(M, __ldcg(base + (int64_t)s * 8 * stride));
+    for (int s = lane; s < active; s += 32) M = fmaxf(M, __ldcg(ml + (int64_t)s * 8).x);
     M = warp_max(M);
-    float l = 0.f, o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (M > -INFINITY && warp < kAtWarps) {
-#pragma unroll 4
-      for (int s = warp; s < active; s += kAtWarps) {
-        const float* q = base + (int64_t)s * 8 * stride;
-        const float w = ex2(__ldcg(q) - M);
-        l += w * __ldcg(q + 1);
+    const float ref = M == -INFINITY ? 0.f : M;
+    float l = 0.f;
+    for (int s = lane; s < active; s += 32) {
+      const float2 v = __ldcg(ml + (int64_t)s * 8);
+      l += ex2(v.x - ref) * v.y;
+    }
+    l = warp_sum(l);
+    const float inv = l != 0.f ? 1.f / l : 0.f;
+    const int64_t head = (int64_t)b * p.Hq + hkv * p.E + e0 + e;
+    TQ* out = static_cast<TQ*>(p.out) + head * D;
+    for (int d0 = 0; d0 < D; d0 += 128) {
+      // dims d0 + 4 lane .. + 3 where D divides by four, else d0 + lane + 32 i
+      const bool quad = D % 4 == 0;
+      float o[4] = {0.f, 0.f, 0.f, 0.f};
+      for (int s0 = 0; s0 < active; s0 += 32) {
+        const int n = min(32, active - s0);
+        const float w = lane < n ? ex2(__ldcg(ml + (int64_t)(s0 + lane) * 8).x - ref) : 0.f;
+#pragma unroll 8
+        for (int j = 0; j < n; ++j) {
+          const float wj = __shfl_sync(0xffffffffu, w, j);
+          const float* q = part + (int64_t)(s0 + j) * 8 * D + d0;
+          if (quad) {
+            if (d0 + 4 * lane < D) {
+              const float4 v = __ldcg(reinterpret_cast<const float4*>(q) + lane);
+              o[0] += wj * v.x, o[1] += wj * v.y, o[2] += wj * v.z, o[3] += wj * v.w;
+            }
+          } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (lane + 32 * i < D) o[i] += w * __ldcg(q + 2 + lane + 32 * i);
+            for (int i = 0; i < 4; ++i)
+              if (d0 + lane + 32 * i < D) o[i] += wj * __ldcg(q + lane + 32 * i);
+          }
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int d = quad ? d0 + 4 * lane + i : d0 + lane + 32 * i;
+        if (d < D) out[d] = from_f<TQ>(l != 0.f ? o[i] * inv : 0.f);
       }
     }
-    __syncthreads();
-    if (warp < kAtWarps) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (lane + 32 * i < D) buf[warp * stride + 2 + lane + 32 * i] = o[i];
-      if (lane == 0) buf[warp * stride] = l;
-    }
-    __syncthreads();
-    float lt = 0.f;
-#pragma unroll
-    for (int w = 0; w < kAtWarps; ++w) lt += buf[w * stride];
-    const int64_t head = (int64_t)b * p.Hq + hkv * p.E + e0 + e;
-    for (int d = threadIdx.x; d < D; d += blockDim.x) {
-      float ot = 0.f;
-#pragma unroll
-      for (int w = 0; w < kAtWarps; ++w) ot += buf[w * stride + 2 + d];
-      static_cast<TQ*>(p.out)[head * D + d] = from_f<TQ>(lt != 0.f ? ot / lt : 0.f);
-    }
-    if (threadIdx.x == 0) p.lse[head] = lt != 0.f ? (M + log2f(lt)) * kLn2 : -INFINITY;
+    if (lane == 0) p.lse[head] = l != 0.f ? (M + log2f(l)) * kLn2 : -INFINITY;
   }
 }
 
@@ -519,7 +529,7 @@ __device__ void join_splits(const AttendParams& p, int b, int hkv, int e0, int n
 // The counts return to zero.
 template <typename TQ>
 __device__ void close_split(const AttendParams& p, int b, int hg, int e0, int nE, int64_t slot0, int active, int pos,
-                            int* flag, float* buf) {
+                            int* flag) {
   const int total = p.advance ? p.splits : active, per = p.Hkv * p.groups;
   if (total > 1) {
     __threadfence();
@@ -533,7 +543,7 @@ __device__ void close_split(const AttendParams& p, int b, int hg, int e0, int nE
     __syncthreads();
     if (!*flag) return;
     __threadfence();
-    if (active > 1) join_splits<TQ>(p, b, hg / p.groups, e0, nE, slot0, active, buf);
+    if (active > 1) join_splits<TQ>(p, b, hg / p.groups, e0, nE, slot0, active);
   }
   if (p.advance && threadIdx.x == 0) {
     int32_t* d = p.done + (int64_t)p.B * per + b;
@@ -569,8 +579,9 @@ __device__ __forceinline__ float tanh_rel(float y) {
 //     q and rows 8-15 what the roundings left over, so S = row h + row h + 8
 //     has q to 22 bits; B = codes, exact in f16.
 //   O[head, dim] += P V:     A = P, split in two the same way, with the value
-//     rows' scales folded into it (relative to their largest so far, times 2^14:
-//     the f16 leftovers of a weight 2^-k keep 22 - max(0, k - 17) bits).
+//     rows' scales folded into it (relative to their largest so far, times 2^9,
+//     so that a weight of 2^5 and a scale of 2 fit: the f16 leftovers of a weight
+//     2^-k keep 22 - max(0, k - 12) bits).
 // A dot product does not care about the order of its terms, so a lane reads 16
 // consecutive codes of a token and the A operand follows that order; likewise
 // output dims follow the value reads.  P leaves S's accumulator layout as the A
@@ -581,7 +592,7 @@ __device__ __forceinline__ float tanh_rel(float y) {
 // Bound by HBM in principle (2 (D + 4) bytes a token and key head); per sixteen
 // tokens a warp issues some 280 instructions, half of them code conversions.
 constexpr int kAtThreads = 32 * kAtWarps;
-constexpr float kUp = 16384.f;
+constexpr float kUp = 512.f, kLazy = 5.f;
 constexpr int kStage = 64;  // tokens per stage
 
 template <int D> struct AtSmem {
@@ -630,7 +641,7 @@ __global__ void __launch_bounds__(kAtThreads, 3)
   const int active = max(1, min(p.splits, (ntok + p.chunk - 1) / p.chunk));
   const int64_t slot0 = ((int64_t)b * p.Hkv * p.groups + hg) * p.splits;
   if (split >= active) {
-    if (p.advance) close_split<TQ>(p, b, hg, e0, nE, slot0, active, pos, &flag, u.o);
+    if (p.advance) close_split<TQ>(p, b, hg, e0, nE, slot0, active, pos, &flag);
     return;
   }
   const int c0 = split * p.chunk, c1 = split == active - 1 ? ntok : c0 + p.chunk;
@@ -687,8 +698,9 @@ __global__ void __launch_bounds__(kAtThreads, 3)
     }
     sum = warp_sum(sum);
     if (lane == 0) {
-      qf_s[e] = down * p.qscale * (CAP ? 1.f / p.softcap : kLog2e);
-      qs_s[e] = -Codec<STORE>::kOff * sum;
+      const float f = down * p.qscale * (CAP ? 1.f / p.softcap : kLog2e);
+      qf_s[e] = Codec<STORE>::kMul * f;
+      qs_s[e] = -Codec<STORE>::kOff * sum * f;
     }
   }
   if constexpr (STEP) {
@@ -769,7 +781,7 @@ __global__ void __launch_bounds__(kAtThreads, 3)
           ks = new_scale[0];
           vsc[i] = new_scale[1];
         }
-        float y = fmaf(sc[i >> 1][i & 1] + sc[i >> 1][2 + (i & 1)], Codec<STORE>::kMul, qoff) * (qf * ks);
+        float y = fmaf(sc[i >> 1][i & 1] + sc[i >> 1][2 + (i & 1)], qf, qoff) * ks;
         if constexpr (CAP) y = kc * tanh_rel(y);
         x[i] = !TAIL || tv[i] < left ? y : -INFINITY;
         if (TAIL && tv[i] >= left) vsc[i] = 0.f;
@@ -783,8 +795,10 @@ __global__ void __launch_bounds__(kAtThreads, 3)
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
         vx = fmaxf(vx, __shfl_xor_sync(0xffffffffu, vx, d));
       }
-      const float mn = fmaxf(m, mx), vn = fmaxf(vref, vx);
-      if (__any_sync(0xffffffffu, mn > m || vn > vref)) {
+      // m and vref move only where a weight could pass 2^5 of them (vref 2): most
+      // sixteens after the first leave the accumulators alone
+      if (__any_sync(0xffffffffu, mx > m + kLazy || vx > 2.f * vref)) {
+        const float mn = fmaxf(m, mx), vn = fmaxf(vref, vx);
         const float cm = m == mn ? 1.f : ex2(m - mn);  // m -inf: 0
         const float co = cm * (vref / vn);
         ell *= cm;
@@ -900,15 +914,12 @@ __global__ void __launch_bounds__(kAtThreads, 3)
       static_cast<TQ*>(p.out)[hq * D + d] = from_f<TQ>(l != 0.f ? ov / l : 0.f);
       if (d == 0) p.lse[hq] = l != 0.f ? (M + log2f(l)) * kLn2 : -INFINITY;
     } else {
-      float* q = p.part + ((slot0 + split) * 8 + e) * (D + 2);
-      __stcg(q + 2 + d, ov);
-      if (d == 0) {
-        __stcg(q, M);
-        __stcg(q + 1, l);
-      }
+      const int64_t at = (slot0 + split) * 8 + e;
+      __stcg(p.part + at * D + d, ov);
+      if (d == 0) __stcg(p.ml + at, make_float2(M, l));
     }
   }
-  close_split<TQ>(p, b, hg, e0, nE, slot0, active, pos, &flag, u.o);
+  close_split<TQ>(p, b, hg, e0, nE, slot0, active, pos, &flag);
 }
 
 // Any head dims up to 256 and any head count: fp32 on the CUDA cores, a warp per
@@ -916,7 +927,7 @@ __global__ void __launch_bounds__(kAtThreads, 3)
 constexpr int kAnyDims = 256 / 32, kAnyThreads = 128;
 template <typename TQ, int STORE, bool STEP>
 __global__ void __launch_bounds__(kAnyThreads) attend_any(AttendParams p) {
-  __shared__ float q_s[256], o_s[4][256 + 2], m_s[4], l_s[4];
+  __shared__ float q_s[256], o_s[4][256], m_s[4], l_s[4];
   __shared__ int flag;
   const int split = blockIdx.x, hg = blockIdx.y, b = blockIdx.z;
   const int hkv = hg / p.groups, e0 = (hg - hkv * p.groups) * 8;
@@ -927,7 +938,7 @@ __global__ void __launch_bounds__(kAnyThreads) attend_any(AttendParams p) {
   const int active = max(1, min(p.splits, (ntok + p.chunk - 1) / p.chunk));
   const int64_t slot0 = ((int64_t)b * p.Hkv * p.groups + hg) * p.splits;
   if (split >= active) {
-    if (p.advance) close_split<TQ>(p, b, hg, e0, nE, slot0, active, pos, &flag, &o_s[0][0]);
+    if (p.advance) close_split<TQ>(p, b, hg, e0, nE, slot0, active, pos, &flag);
     return;
   }
   const int c0 = split * p.chunk, c1 = split == active - 1 ? ntok : c0 + p.chunk;
@@ -1000,16 +1011,13 @@ __global__ void __launch_bounds__(kAnyThreads) attend_any(AttendParams p) {
         static_cast<TQ*>(p.out)[hq * p.Dv + d] = from_f<TQ>(l != 0.f ? ov / l : 0.f);
         if (d == 0) p.lse[hq] = l != 0.f ? (M + log2f(l)) * kLn2 : -INFINITY;
       } else {
-        float* q = p.part + ((slot0 + split) * 8 + e) * (p.Dv + 2);
-        __stcg(q + 2 + d, ov);
-        if (d == 0) {
-          __stcg(q, M);
-          __stcg(q + 1, l);
-        }
+        const int64_t at = (slot0 + split) * 8 + e;
+        __stcg(p.part + at * p.Dv + d, ov);
+        if (d == 0) __stcg(p.ml + at, make_float2(M, l));
       }
     }
   }
-  close_split<TQ>(p, b, hg, e0, nE, slot0, active, pos, &flag, &o_s[0][0]);
+  close_split<TQ>(p, b, hg, e0, nE, slot0, active, pos, &flag);
 }
 
 // Codes [rows * Hkv, capacity, D] as a 3-D map of kStage-token boxes, slots past the
@@ -1063,10 +1071,12 @@ bool cache_ok(const tc_kv_cache* c) {
 
 // Tokens per CTA and CTAs per (sequence, head group) over at most `most` tokens.
 // One sequence: one wave of three CTAs per SM over 148 SMs.  Several may differ
-// in length: four waves, so that they even out.  A chunk is a multiple of 64
-// tokens (one stage).
+// in length: eight waves, so that they even out (64 sequences of 1 to 32768
+// tokens: 360 us with two, 302 with four, 294 with eight, 301 with sixteen).  A
+// chunk is a multiple of 64 tokens (one stage).
 void split_rule(int64_t most, int64_t heads, int B, int* chunk, int* splits) {
-  const int64_t want = ((B > 1 ? 4 : 1) * 3 * 148 + heads - 1) / heads;
+  const int64_t resident = 3 * 148;
+  const int64_t want = B > 1 ? (8 * resident + heads - 1) / heads : heads < resident ? resident / heads : 1;
   int64_t c = (most + want - 1) / want;
   c = (c + 63) / 64 * 64;
   if (c < 64) c = 64;
@@ -1141,7 +1151,7 @@ extern "C" int tc_kv_attend(const tc_kv_cache* c, const tc_kv_attend_args* a, vo
   p.groups = (a->Hq / c->Hkv + 7) / 8;
   if ((int64_t)c->Hkv * p.groups > 65535) return TC_ERR_UNSUPPORTED;
   const int64_t need = p.splits > 1 ? (int64_t)a->B * c->Hkv * p.groups * p.splits * 8 * (c->Dv + 2) : 0;
-  if (need && (!a->scratch || a->scratch_floats < need)) return TC_ERR_ARG;
+  if (need && (!a->scratch || (uintptr_t)a->scratch % 16 || a->scratch_floats < need)) return TC_ERR_ARG;
   if ((p.splits > 1 || a->advance) && (!a->counters || a->num_counters < (int64_t)a->B * (c->Hkv * p.groups + 1)))
     return TC_ERR_ARG;
   p.B = a->B, p.Hq = a->Hq, p.Hkv = c->Hkv, p.E = a->Hq / c->Hkv;
@@ -1154,7 +1164,9 @@ extern "C" int tc_kv_attend(const tc_kv_cache* c, const tc_kv_attend_args* a, vo
   p.qscale = a->scale, p.softcap = a->softcap, p.has_cap = a->has_softcap != 0;
   p.advance = step && a->advance;
   p.out = a->out, p.lse = a->lse, p.k_new = a->k_new, p.v_new = a->v_new, p.new_dtype = a->new_dtype;
-  p.part = a->scratch, p.done = a->counters, p.status = a->dev_status;
+  const int64_t slots = (int64_t)a->B * c->Hkv * p.groups * p.splits;
+  p.ml = reinterpret_cast<float2*>(a->scratch), p.part = a->scratch + slots * 16;
+  p.done = a->counters, p.status = a->dev_status;
   cudaStream_t st = (cudaStream_t)stream;
 #define TC_KV_GO(S, STEP) TC_DISPATCH(a->dtype, T, return launch_attend<T, S, STEP>(p, c->rows, st))
   if (c->store == TC_KV_INT8) {

@@ -96,14 +96,14 @@ def test_full_attention_structs_and_bad_arguments():
 
 def test_cached_attention_split_plan():
     """Chunks are multiples of 64 tokens, one wave of three CTAs per SM is wanted
-    for one sequence and four for several, one chunk needs no scratch."""
+    for one sequence and eight for several, one chunk needs no scratch."""
     lib = _lib.lib()
     c = _lib.KVCacheArgs(rows=64, Hkv=4, Dk=128, Dv=128, capacity=40000, k=16, v=16, k_scale=16, v_scale=16,
                          lengths=16)
     floats = lambda B, Hq, n: lib.tc_kv_attend_scratch_floats(c, B, Hq, n)  # noqa: E731
     assert floats(1, 4, 64) == 0 and floats(1, 4, 0) == 0
     assert floats(1, 4, 65) == 4 * 2 * 8 * 130
-    want = -(-4 * 3 * 148 // (64 * 4))
+    want = -(-8 * 3 * 148 // (64 * 4))
     chunk = -(-(-(-32768 // want)) // 64) * 64
     assert floats(64, 16, 32768) == 64 * 4 * -(-32768 // chunk) * 8 * 130
     assert floats(64, 4 * 9, 64) == 0 and floats(64, 4 * 9, 128) == 64 * 4 * 2 * 2 * 8 * 130  # nine heads: two eights
