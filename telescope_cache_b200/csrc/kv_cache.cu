@@ -465,60 +465,85 @@ __device__ void write_token(const AttendParams& p, const T* x, int D, int R, int
   }
 }
 
-// Joins the partials of `active` splits of nE heads and writes out, lse: a warp
-// per head; a lane reads the (m, l) of every 32nd split, then consecutive dims of
-// one split after another, eight loads in flight.  (All warps on one head after
-// another left the last CTA 24 us of dependent loads over 54 splits.)
+// Joins the partials of `active` splits of nE heads and writes out, lse.  A warp
+// takes a head (with fewer than four heads, the warps of one share its splits): it
+// finds the joint maximum and sum, then reads the splits' O, four consecutive dims
+// a lane and sixteen splits in flight.  The last CTA runs this alone, so what
+// counts is how few rounds of loads follow one another.
 constexpr int kAtWarps = 4;
 template <typename TQ>
-__device__ void join_splits(const AttendParams& p, int b, int hkv, int e0, int nE, int64_t slot0, int active) {
+__device__ void join_splits(const AttendParams& p, int b, int hkv, int e0, int nE, int64_t slot0, int active,
+                            float* red /* [kAtWarps][Dv] */) {
+  constexpr int kFly = 16;
+  __shared__ float inv_s[kAtWarps];
   const int D = p.Dv, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  for (int e = warp; e < nE; e += kAtWarps) {
-    const float2* ml = p.ml + slot0 * 8 + e;
-    const float* part = p.part + (slot0 * 8 + e) * D;
-    float M = -INFINITY;
-    for (int s = lane; s < active; s += 32) M = fmaxf(M, __ldcg(ml + (int64_t)s * 8).x);
-    M = warp_max(M);
-    const float ref = M == -INFINITY ? 0.f : M;
-    float l = 0.f;
-    for (int s = lane; s < active; s += 32) {
-      const float2 v = __ldcg(ml + (int64_t)s * 8);
-      l += ex2(v.x - ref) * v.y;
-    }
-    l = warp_sum(l);
-    const float inv = l != 0.f ? 1.f / l : 0.f;
-    const int64_t head = (int64_t)b * p.Hq + hkv * p.E + e0 + e;
-    TQ* out = static_cast<TQ*>(p.out) + head * D;
-    for (int d0 = 0; d0 < D; d0 += 128) {
-      // dims d0 + 4 lane .. + 3 where D divides by four, else d0 + lane + 32 i
-      const bool quad = D % 4 == 0;
-      float o[4] = {0.f, 0.f, 0.f, 0.f};
-      for (int s0 = 0; s0 < active; s0 += 32) {
-        const int n = min(32, active - s0);
-        const float w = lane < n ? ex2(__ldcg(ml + (int64_t)(s0 + lane) * 8).x - ref) : 0.f;
-#pragma unroll 8
-        for (int j = 0; j < n; ++j) {
-          const float wj = __shfl_sync(0xffffffffu, w, j);
-          const float* q = part + (int64_t)(s0 + j) * 8 * D + d0;
-          if (quad) {
-            if (d0 + 4 * lane < D) {
-              const float4 v = __ldcg(reinterpret_cast<const float4*>(q) + lane);
-              o[0] += wj * v.x, o[1] += wj * v.y, o[2] += wj * v.z, o[3] += wj * v.w;
-            }
-          } else {
+  const int heads = nE >= 3 ? 4 : nE, shares = kAtWarps / heads, share = warp / heads;  // heads at a time
+  const int64_t head0 = (int64_t)b * p.Hq + hkv * p.E + e0;
+  const bool quad = D % 4 == 0;
+  for (int e1 = 0; e1 < nE; e1 += heads) {
+    const int e = e1 + warp % heads;
+    if (e < nE) {
+      const float2* ml = p.ml + slot0 * 8 + e;
+      const float* part = p.part + (slot0 * 8 + e) * D;
+      float m = -INFINITY, l = 0.f;  // over this lane's splits
+      for (int s = lane; s < active; s += 32) {
+        const float2 v = __ldcg(ml + (int64_t)s * 8);
+        const float mn = fmaxf(m, v.x), ref = mn == -INFINITY ? 0.f : mn;
+        l = l * ex2(m - ref) + v.y * ex2(v.x - ref);
+        m = mn;
+      }
+      const float top = warp_max(m), M = top == -INFINITY ? 0.f : top;
+      l = warp_sum(l * ex2(m - M));
+      if (lane == 0 && share == 0) {
+        inv_s[warp] = l != 0.f ? 1.f / l : 0.f;
+        p.lse[head0 + e] = l != 0.f ? (top + log2f(l)) * kLn2 : -INFINITY;
+      }
+      for (int d0 = 0; d0 < D; d0 += 128) {
+        const int d = quad ? d0 + 4 * lane : d0 + lane;
+        float o[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int s0 = share; s0 < active; s0 += kFly * shares) {
+          float4 v[kFly];
+          float w[kFly];
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-              if (d0 + lane + 32 * i < D) o[i] += wj * __ldcg(q + lane + 32 * i);
+          for (int j = 0; j < kFly; ++j) {
+            const int s = s0 + j * shares;
+            v[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+            w[j] = -INFINITY;
+            if (s < active) {
+              w[j] = __ldcg(ml + (int64_t)s * 8).x;
+              const float* q = part + (int64_t)s * 8 * D + d;
+              if (quad) {
+                if (d < D) v[j] = __ldcg(reinterpret_cast<const float4*>(q));
+              } else {
+                if (d < D) v[j].x = __ldcg(q);
+                if (d + 32 < D) v[j].y = __ldcg(q + 32);
+                if (d + 64 < D) v[j].z = __ldcg(q + 64);
+                if (d + 96 < D) v[j].w = __ldcg(q + 96);
+              }
+            }
+          }
+#pragma unroll
+          for (int j = 0; j < kFly; ++j) {
+            const float c = ex2(w[j] - M);
+            o[0] += c * v[j].x, o[1] += c * v[j].y, o[2] += c * v[j].z, o[3] += c * v[j].w;
           }
         }
-      }
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int d = quad ? d0 + 4 * lane + i : d0 + lane + 32 * i;
-        if (d < D) out[d] = from_f<TQ>(l != 0.f ? o[i] * inv : 0.f);
+        for (int i = 0; i < 4; ++i) {
+          const int di = quad ? d + i : d + 32 * i;
+          if (di < D) red[warp * D + di] = o[i];
+        }
       }
     }
-    if (lane == 0) p.lse[head] = l != 0.f ? (M + log2f(l)) * kLn2 : -INFINITY;
+    __syncthreads();
+    for (int i = threadIdx.x; i < heads * D; i += kAtWarps * 32) {
+      const int h = i / D, d = i - h * D;
+      if (e1 + h >= nE) break;
+      float o = 0.f;
+      for (int k = 0; k < shares; ++k) o += red[(h + k * heads) * D + d];
+      static_cast<TQ*>(p.out)[(head0 + e1 + h) * D + d] = from_f<TQ>(inv_s[h] != 0.f ? o * inv_s[h] : 0.f);
+    }
+    __syncthreads();
   }
 }
 
@@ -529,7 +554,7 @@ __device__ void join_splits(const AttendParams& p, int b, int hkv, int e0, int n
 // The counts return to zero.
 template <typename TQ>
 __device__ void close_split(const AttendParams& p, int b, int hg, int e0, int nE, int64_t slot0, int active, int pos,
-                            int* flag) {
+                            int* flag, float* red) {
   const int total = p.advance ? p.splits : active, per = p.Hkv * p.groups;
   if (total > 1) {
     __threadfence();
@@ -543,7 +568,7 @@ __device__ void close_split(const AttendParams& p, int b, int hg, int e0, int nE
     __syncthreads();
     if (!*flag) return;
     __threadfence();
-    if (active > 1) join_splits<TQ>(p, b, hg / p.groups, e0, nE, slot0, active);
+    if (active > 1) join_splits<TQ>(p, b, hg / p.groups, e0, nE, slot0, active, red);
   }
   if (p.advance && threadIdx.x == 0) {
     int32_t* d = p.done + (int64_t)p.B * per + b;
@@ -569,12 +594,13 @@ __device__ __forceinline__ float tanh_rel(float y) {
 }
 
 // Tensor-core path, Dk = Dv = D (64 or 128).  CTA = one chunk of one sequence
-// and up to eight query heads of one key head.  The chunk's codes stream into a
-// ring of 64-token stages by TMA (16 KB at D = 128, 48 KB in flight per CTA, three
-// CTAs per SM): the last of the four warps to finish a stage refills it.  (A fifth
-// warp for that would cost a third of the registers: ten warps leave 168 each as
-// twelve do.)  A warp takes sixteen tokens of a stage, with m16n8k16 f16 products
-// and fp32 accumulators:
+// and up to eight query heads of one key head; its four warps take the chunk's
+// 32-token units in turn, each through a ring of its own that TMA fills (8 KB a
+// unit at D = 128; two in flight or in use per warp, twelve warps per SM), so that
+// no warp waits for another.  (Stages of 64 tokens shared by the four warps cost a
+// quarter of the time in their hand-over, and 16 tokens a step left a warp 3200
+// clocks of dependent instructions for them.)  Products are m16n8k16 f16 with fp32
+// accumulators:
 //   S[head, token] = q K^T:  A = q, rows 0-7 the f16 roundings of the heads'
 //     q and rows 8-15 what the roundings left over, so S = row h + row h + 8
 //     has q to 22 bits; B = codes, exact in f16.
@@ -589,18 +615,17 @@ __device__ __forceinline__ float tanh_rel(float y) {
 // odd n, (n - 1 ^ 4) + 1: with the 128-byte swizzle the eight lanes of a shared
 // memory phase then meet eight different bank groups, for keys and for values.
 //
-// Bound by HBM in principle (2 (D + 4) bytes a token and key head); per sixteen
-// tokens a warp issues some 280 instructions, half of them code conversions.
+// Bound by HBM in principle (2 (D + 4) bytes a token and key head).
 constexpr int kAtThreads = 32 * kAtWarps;
 constexpr float kUp = 512.f, kLazy = 5.f;
-constexpr int kStage = 64;  // tokens per stage
+constexpr int kUnit = 32;  // tokens per stage
 
 template <int D> struct AtSmem {
-  static constexpr int kTile = kStage * D;  // codes of one stage, keys or values
-  static constexpr int kNS = D == 128 ? 3 : 4;
+  static constexpr int kTile = kUnit * D;  // codes of one stage, keys or values
+  static constexpr int kNS = D == 128 ? 2 : 3;   // stages per warp
   static constexpr int QS = D + 8;             // q row stride (halves)
   static constexpr int OS = D + D / 32 * 4;    // O row stride (floats)
-  static constexpr int kBytes = 2 * kNS * kTile + 1024;
+  static constexpr int kBytes = kAtWarps * 2 * kNS * kTile + 1024;
 };
 
 // Byte of 16-byte chunk `c` of row `r` in a stage (TMA swizzle of D-byte rows).
@@ -622,14 +647,13 @@ __global__ void __launch_bounds__(kAtThreads, 3)
   constexpr int NS = Z::kNS, QS = Z::QS, OS = Z::OS;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  __shared__ __align__(16) union {
-    __half q[16 * QS];
-    float o[kAtWarps * 8 * OS];
-  } u;
+  __shared__ __align__(16) __half q_s[16 * QS];
+  float* o_s = reinterpret_cast<float*>(sm);  // the warps' O, once every unit has been read
+  static_assert(kAtWarps * 8 * OS * 4 <= kAtWarps * 2 * NS * Z::kTile, "O does not fit the ring");
   __shared__ __align__(128) uint8_t new_s[2][128];  // the new token's codes, as a stage row of its slot holds them
   __shared__ float new_scale[2], qf_s[8], qs_s[8], m_s[kAtWarps][8], l_s[kAtWarps][8];
-  __shared__ uint64_t full[NS];
-  __shared__ int flag, abort_s, taken[NS];  // taken: warps done with the stage so far
+  __shared__ uint64_t full_s[kAtWarps][NS];
+  __shared__ int flag, abort_s;
 
   const int split = blockIdx.x;
   const int hg = blockIdx.y, b = blockIdx.z;
@@ -637,48 +661,78 @@ __global__ void __launch_bounds__(kAtThreads, 3)
   const int nE = min(8, p.E - e0);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int pos = p.lengths[b];
+  if (threadIdx.x == 0) {
+    prefetch_tmap(&tmk);
+    prefetch_tmap(&tmv);
+  }
+  // the warp's query heads warp and warp + 4, on their way before the length is known
+  constexpr int NP = D / 64;  // pairs per lane
+  const int R = STEP ? p.R : 0;
+  TQ qx[2][NP][2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int e = warp + 4 * h;
+    const TQ* x = static_cast<const TQ*>(p.q) + b * p.q_sb + (int64_t)(hkv * p.E + e0 + e) * p.q_sh;
+#pragma unroll
+    for (int j = 0; j < NP; ++j) {
+      int i1, i2;
+      pair_dims(lane + 32 * j, R, p.interleaved, D, &i1, &i2);
+      qx[h][j][0] = e < nE ? x[i1] : from_f<TQ>(0.f);
+      qx[h][j][1] = e < nE ? x[i2] : from_f<TQ>(0.f);
+    }
+  }
   const int ntok = (int)min((int64_t)(STEP ? pos + 1 : pos), p.cap);
   const int active = max(1, min(p.splits, (ntok + p.chunk - 1) / p.chunk));
   const int64_t slot0 = ((int64_t)b * p.Hkv * p.groups + hg) * p.splits;
   if (split >= active) {
-    if (p.advance) close_split<TQ>(p, b, hg, e0, nE, slot0, active, pos, &flag);
+    if (p.advance) close_split<TQ>(p, b, hg, e0, nE, slot0, active, pos, &flag, o_s);
     return;
   }
   const int c0 = split * p.chunk, c1 = split == active - 1 ? ntok : c0 + p.chunk;
-  const int stages = (c1 - c0 + kStage - 1) / kStage;
+  const int units = (c1 - c0 + kUnit - 1) / kUnit, mine = (units - warp + kAtWarps - 1) / kAtWarps;
   const int64_t head = (int64_t)b * p.Hkv + hkv;
   const bool owner = STEP && split == active - 1 && pos < p.cap;  // its chunk holds the new slot
   volatile int* abort_flag = &abort_s;
+  uint8_t* ring = sm + warp * NS * 2 * Z::kTile;
+  uint64_t* full = full_s[warp];
 
-  auto fill = [&](int i) {  // one thread: stage i of the chunk
-    const int st = i % NS;
+  auto fill = [&](int i) {  // one lane: the warp's i-th unit
+    const int st = i % NS, at = c0 + (warp + i * kAtWarps) * kUnit;
     mbar_expect_tx(&full[st], 2 * Z::kTile);
-    tma_load_3d(sm + 2 * st * Z::kTile, &tmk, 0, c0 + i * kStage, (int)head, &full[st]);
-    tma_load_3d(sm + (2 * st + 1) * Z::kTile, &tmv, 0, c0 + i * kStage, (int)head, &full[st]);
+    tma_load_3d(ring + 2 * st * Z::kTile, &tmk, 0, at, (int)head, &full[st]);
+    tma_load_3d(ring + (2 * st + 1) * Z::kTile, &tmv, 0, at, (int)head, &full[st]);
   };
-  if (threadIdx.x == 0) {
-    for (int i = 0; i < NS; ++i) {
-      mbar_init(&full[i], 1);
-      taken[i] = 0;
-    }
-    abort_s = 0;
+  if (lane == 0) {
+    for (int i = 0; i < NS; ++i) mbar_init(&full[i], 1);
+    if (warp == 0) abort_s = 0;
     mbar_fence_init();
     fence_async_smem();
-    for (int i = 0; i < NS && i < stages; ++i) fill(i);
+    for (int i = 0; i < NS && i < mine; ++i) fill(i);
   }
   // q: rotate, bring each head's largest element to [2^13, 2^14), split in two
-  for (int e = warp; e < 8; e += kAtWarps) {
-    const TQ* x = static_cast<const TQ*>(p.q) + b * p.q_sb + (int64_t)(hkv * p.E + e0 + e) * p.q_sh;
-    float y1[D / 64], y2[D / 64];
-    int i1[D / 64], i2[D / 64];
+  float cs[NP], sn[NP];
+#pragma unroll
+  for (int j = 0; j < NP; ++j) {
+    const int v = lane + 32 * j;
+    cs[j] = 1.f;
+    sn[j] = 0.f;
+    if (STEP && v < R / 2) {
+      cs[j] = pos < p.n_pos ? p.cos_t[(int64_t)pos * (R / 2) + v] : NAN;
+      sn[j] = pos < p.n_pos ? p.sin_t[(int64_t)pos * (R / 2) + v] : NAN;
+    }
+  }
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int e = warp + 4 * h;
+    float y1[NP], y2[NP];
     uint32_t m = 0;
     float sum = 0.f;
 #pragma unroll
-    for (int j = 0; j < D / 64; ++j) {
-      const int v = lane + 32 * j;
-      y1[j] = y2[j] = 0.f;
-      if (e < nE) load_pair(p, x, v, D, STEP ? p.R : 0, pos, &i1[j], &i2[j], &y1[j], &y2[j]);
-      else pair_dims(v, STEP ? p.R : 0, p.interleaved, D, &i1[j], &i2[j]);
+    for (int j = 0; j < NP; ++j) {
+      y1[j] = to_f(qx[h][j][0]);
+      y2[j] = to_f(qx[h][j][1]);
+      if (STEP && lane + 32 * j < R / 2) rotate_pair(y1[j], y2[j], cs[j], sn[j], &y1[j], &y2[j]);
+      if (e >= nE) y1[j] = y2[j] = 0.f;
       m = max(m, max(abs_bits(y1[j]), abs_bits(y2[j])));
     }
 #pragma unroll
@@ -687,14 +741,16 @@ __global__ void __launch_bounds__(kAtThreads, 3)
     const float up = m ? __int_as_float((127 + 13 - ex) << 23) : 1.f;
     const float down = m ? __int_as_float((127 - 13 + ex) << 23) : 1.f;
 #pragma unroll
-    for (int j = 0; j < D / 64; ++j) {
+    for (int j = 0; j < NP; ++j) {
+      int i1, i2;
+      pair_dims(lane + 32 * j, R, p.interleaved, D, &i1, &i2);
       const float a = y1[j] * up, c = y2[j] * up;
       sum += a + c;
       const __half ah = __float2half_rn(a), ch = __float2half_rn(c);
-      u.q[e * QS + i1[j]] = ah;
-      u.q[e * QS + i2[j]] = ch;
-      u.q[(e + 8) * QS + i1[j]] = __float2half_rn(a - __half2float(ah));
-      u.q[(e + 8) * QS + i2[j]] = __float2half_rn(c - __half2float(ch));
+      q_s[e * QS + i1] = ah;
+      q_s[e * QS + i2] = ch;
+      q_s[(e + 8) * QS + i1] = __float2half_rn(a - __half2float(ah));
+      q_s[(e + 8) * QS + i2] = __float2half_rn(c - __half2float(ch));
     }
     sum = warp_sum(sum);
     if (lane == 0) {
@@ -709,7 +765,7 @@ __global__ void __launch_bounds__(kAtThreads, 3)
     // groups of one key head write the same bytes.)
     if (owner && warp >= 2) {
       const int which = warp - 2;
-      const int r = (pos - c0) % kStage;
+      const int r = (pos - c0) % kUnit;
       const TQ* x = which ? static_cast<const TQ*>(p.v_t) + b * p.v_sb + hkv * p.v_sh
                           : static_cast<const TQ*>(p.k_t) + b * p.k_sb + hkv * p.k_sh;
       write_token<TQ, STORE>(p, x, D, which ? 0 : p.R, pos, head, which ? p.v : p.k, which ? p.vs : p.ks,
@@ -727,36 +783,43 @@ __global__ void __launch_bounds__(kAtThreads, 3)
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
       const int d = 64 * (s / 4) + 16 * t + 4 * (s % 4);
-      const uint2 hi = *reinterpret_cast<const uint2*>(u.q + g * QS + d);
-      const uint2 lo = *reinterpret_cast<const uint2*>(u.q + (g + 8) * QS + d);
+      const uint2 hi = *reinterpret_cast<const uint2*>(q_s + g * QS + d);
+      const uint2 lo = *reinterpret_cast<const uint2*>(q_s + (g + 8) * QS + d);
       qa[s][0] = hi.x, qa[s][1] = lo.x, qa[s][2] = hi.y, qa[s][3] = lo.y;
     }
     const float qf = qf_s[g], qoff = qs_s[g];
     const float kc = p.softcap * kLog2e;
-    const int kr = 16 * warp + tok_of(g);                               // rows of the stage this lane reads
-    const int tv[4] = {2 * t, tok_of(2 * t + 1), 8 + 2 * t, 8 + tok_of(2 * t + 1)};
     float o[ND][4];
 #pragma unroll
     for (int i = 0; i < ND; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
     float m = -INFINITY, ell = 0.f, vref = kTiny;
-    // lanes 0-15 hold the key scales of the warp's sixteen tokens, 16-31 the value scales
-    const float* scb = (lane < 16 ? p.ks : p.vs) + head * p.cap + c0 + 16 * warp + (lane & 15);
-    auto load_scales = [&](int at) { return c0 + 16 * warp + at + (lane & 15) < c1 ? scb[at] : 0.f; };
-    float scales = load_scales(0);
+    // a lane holds the key and value scale of token `lane` of the warp's unit
+    const float* ksb = p.ks + head * p.cap + c0 + warp * kUnit + lane;
+    const float* vsb = p.vs + head * p.cap + c0 + warp * kUnit + lane;
+    float kscale = 0.f, vscale = 0.f;
+    auto load_scales = [&](int i) {
+      const int at = i * kAtWarps * kUnit;
+      const bool ok = c0 + warp * kUnit + lane + at < c1;
+      kscale = ok ? ksb[at] : 0.f;
+      vscale = ok ? vsb[at] : 0.f;
+    };
+    // tokens of an eight that this lane's accumulator columns 2 t, 2 t + 1 stand for
+    const int tk[2] = {2 * t, tok_of(2 * t + 1)};
 
-    auto sixteen = [&](auto tail, int st, int at) {
+    auto unit = [&](auto tail, int i) {
       constexpr bool TAIL = decltype(tail)::value;
-      const uint8_t* kt = sm + 2 * st * Z::kTile;
+      const uint8_t* kt = ring + 2 * (i % NS) * Z::kTile;
       const uint8_t* vt = kt + Z::kTile;
-      const int left = c1 - (c0 + 16 * warp + at);         // tokens of the sixteen that count
-      const int np = TAIL && owner ? pos - (c0 + 16 * warp + at) : -1;  // the new one among them
-      float sc[2][4];
+      const int u0 = c0 + (warp + i * kAtWarps) * kUnit;
+      const int left = c1 - u0;                     // tokens of the unit that count
+      const int np = TAIL && owner ? pos - u0 : -1;  // the new one among them
+      float sc[4][4];
 #pragma unroll
-      for (int nt = 0; nt < 2; ++nt) {
-        const int r = kr + 8 * nt;
+      for (int nt = 0; nt < 4; ++nt) {
+        const int r = 8 * nt + tok_of(g);
         const uint8_t* row = kt;
         int at0 = stage_at<D>(r, t), at1 = D == 128 ? stage_at<D>(r, 4 + t) : 0;
-        if (TAIL && np == r - 16 * warp) {
+        if (TAIL && np == r) {
           row = new_s[0];
           at0 -= r * D;
           at1 -= r * D;
@@ -772,114 +835,116 @@ __global__ void __launch_bounds__(kAtThreads, 3)
           mma16816(sc[nt], qa[s], Codec<STORE>::template raw_pair<false>(w), Codec<STORE>::template raw_pair<true>(w));
         }
       }
-      float x[4], vsc[4];
+      float x[8], vsc[8];  // index 2 nt + c: token 8 nt + tk[c]
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        float ks = __shfl_sync(0xffffffffu, scales, tv[i]);
-        vsc[i] = __shfl_sync(0xffffffffu, scales, 16 + tv[i]);
-        if (TAIL && np == tv[i]) {
+      for (int j = 0; j < 8; ++j) {
+        const int tok = 8 * (j >> 1) + tk[j & 1];
+        float ks = __shfl_sync(0xffffffffu, kscale, tok);
+        vsc[j] = __shfl_sync(0xffffffffu, vscale, tok);
+        if (TAIL && np == tok) {
           ks = new_scale[0];
-          vsc[i] = new_scale[1];
+          vsc[j] = new_scale[1];
         }
-        float y = fmaf(sc[i >> 1][i & 1] + sc[i >> 1][2 + (i & 1)], qf, qoff) * ks;
+        float y = fmaf(sc[j >> 1][j & 1] + sc[j >> 1][2 + (j & 1)], qf, qoff) * ks;
         if constexpr (CAP) y = kc * tanh_rel(y);
-        x[i] = !TAIL || tv[i] < left ? y : -INFINITY;
-        if (TAIL && tv[i] >= left) vsc[i] = 0.f;
+        x[j] = !TAIL || tok < left ? y : -INFINITY;
+        if (TAIL && tok >= left) vsc[j] = 0.f;
       }
-      if (!TAIL) scales = load_scales(at + kStage);  // the next stage's, a stage ahead
+      if (i + 1 < mine) load_scales(i + 1);
 
-      float mx = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
-      float vx = fmaxf(fmaxf(vsc[0], vsc[1]), fmaxf(vsc[2], vsc[3]));
+      float mx = x[0], vx = vsc[0];
+#pragma unroll
+      for (int j = 1; j < 8; ++j) {
+        mx = fmaxf(mx, x[j]);
+        vx = fmaxf(vx, vsc[j]);
+      }
 #pragma unroll
       for (int d = 1; d <= 2; d <<= 1) {
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
         vx = fmaxf(vx, __shfl_xor_sync(0xffffffffu, vx, d));
       }
       // m and vref move only where a weight could pass 2^5 of them (vref 2): most
-      // sixteens after the first leave the accumulators alone
+      // units after the first leave the accumulators alone
       if (__any_sync(0xffffffffu, mx > m + kLazy || vx > 2.f * vref)) {
         const float mn = fmaxf(m, mx), vn = fmaxf(vref, vx);
         const float cm = m == mn ? 1.f : ex2(m - mn);  // m -inf: 0
         const float co = cm * (vref / vn);
         ell *= cm;
 #pragma unroll
-        for (int i = 0; i < ND; ++i) o[i][0] *= co, o[i][1] *= co, o[i][2] *= co, o[i][3] *= co;
+        for (int d = 0; d < ND; ++d) o[d][0] *= co, o[d][1] *= co, o[d][2] *= co, o[d][3] *= co;
         m = mn;
         vref = vn;
       }
       const float vinv = __fdividef(kUp, vref);
       const float me = m == -INFINITY ? 0.f : m;
-      float pr[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float e = ex2(x[i] - me);
-        ell += e;
-        pr[i] = e * (vsc[i] * vinv);
-      }
-      uint32_t pa[4];
+      for (int h = 0; h < 2; ++h) {  // sixteen tokens: one k step of the second product
+        uint32_t pa[4];
 #pragma unroll
-      for (int nt = 0; nt < 2; ++nt) {
-        const uint32_t hi = pack_h2(pr[2 * nt], pr[2 * nt + 1]);
-        const float2 h2 = unpack_h2(hi);
-        pa[2 * nt] = hi;
-        pa[2 * nt + 1] = pack_h2(pr[2 * nt] - h2.x, pr[2 * nt + 1] - h2.y);
-      }
-      uint32_t vw[4][VB / 4];
+        for (int c = 0; c < 2; ++c) {
+          float pr[2];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int r = 16 * warp + tv[i];
-        const uint8_t* row = vt + stage_at<D>(r, D == 128 ? g : g >> 1) + (D == 128 ? 0 : (g & 1) * 8);
-        if (TAIL && np == tv[i]) row = new_s[1] + (row - vt) - r * D;
-        if constexpr (VB == 16) {
-          uint4 w = *reinterpret_cast<const uint4*>(row);
-          if (TAIL && tv[i] >= left) w = make_uint4(0, 0, 0, 0);  // an e4m3 NaN times 0 is one
-          vw[i][0] = w.x, vw[i][1] = w.y, vw[i][2] = w.z, vw[i][3] = w.w;
-        } else {
-          uint2 w = *reinterpret_cast<const uint2*>(row);
-          if (TAIL && tv[i] >= left) w = make_uint2(0, 0);
-          vw[i][0] = w.x, vw[i][1] = w.y;
+          for (int k = 0; k < 2; ++k) {
+            const int j = 4 * h + 2 * c + k;
+            const float e = ex2(x[j] - me);
+            ell += e;
+            pr[k] = e * (vsc[j] * vinv);
+          }
+          const uint32_t hi = pack_h2(pr[0], pr[1]);
+          const float2 h2 = unpack_h2(hi);
+          pa[2 * c] = hi;
+          pa[2 * c + 1] = pack_h2(pr[0] - h2.x, pr[1] - h2.y);
         }
-      }
-      // O += P V: word j of the lane's four tokens holds output dims VB g + 4 j + 0..3
+        uint32_t vw[4][VB / 4];
 #pragma unroll
-      for (int j = 0; j < VB / 4; ++j) {
-        const uint32_t a0 = __byte_perm(vw[0][j], vw[1][j], 0x5140), a1 = __byte_perm(vw[0][j], vw[1][j], 0x7362);
-        const uint32_t b0 = __byte_perm(vw[2][j], vw[3][j], 0x5140), b1 = __byte_perm(vw[2][j], vw[3][j], 0x7362);
-        mma16816(o[4 * j], pa, Codec<STORE>::template pair<false>(a0), Codec<STORE>::template pair<false>(b0));
-        mma16816(o[4 * j + 1], pa, Codec<STORE>::template pair<true>(a0), Codec<STORE>::template pair<true>(b0));
-        mma16816(o[4 * j + 2], pa, Codec<STORE>::template pair<false>(a1), Codec<STORE>::template pair<false>(b1));
-        mma16816(o[4 * j + 3], pa, Codec<STORE>::template pair<true>(a1), Codec<STORE>::template pair<true>(b1));
+        for (int k = 0; k < 4; ++k) {
+          const int r = 16 * h + 8 * (k >> 1) + tk[k & 1];
+          const uint8_t* row = vt + stage_at<D>(r, D == 128 ? g : g >> 1) + (D == 128 ? 0 : (g & 1) * 8);
+          if (TAIL && np == r) row = new_s[1] + (row - vt) - r * D;
+          if constexpr (VB == 16) {
+            uint4 w = *reinterpret_cast<const uint4*>(row);
+            if (TAIL && r >= left) w = make_uint4(0, 0, 0, 0);  // an e4m3 NaN times 0 is one
+            vw[k][0] = w.x, vw[k][1] = w.y, vw[k][2] = w.z, vw[k][3] = w.w;
+          } else {
+            uint2 w = *reinterpret_cast<const uint2*>(row);
+            if (TAIL && r >= left) w = make_uint2(0, 0);
+            vw[k][0] = w.x, vw[k][1] = w.y;
+          }
+        }
+        // word j of the lane's four tokens holds output dims VB g + 4 j + 0..3
+#pragma unroll
+        for (int j = 0; j < VB / 4; ++j) {
+          const uint32_t a0 = __byte_perm(vw[0][j], vw[1][j], 0x5140), a1 = __byte_perm(vw[0][j], vw[1][j], 0x7362);
+          const uint32_t b0 = __byte_perm(vw[2][j], vw[3][j], 0x5140), b1 = __byte_perm(vw[2][j], vw[3][j], 0x7362);
+          mma16816(o[4 * j], pa, Codec<STORE>::template pair<false>(a0), Codec<STORE>::template pair<false>(b0));
+          mma16816(o[4 * j + 1], pa, Codec<STORE>::template pair<true>(a0), Codec<STORE>::template pair<true>(b0));
+          mma16816(o[4 * j + 2], pa, Codec<STORE>::template pair<false>(a1), Codec<STORE>::template pair<false>(b1));
+          mma16816(o[4 * j + 3], pa, Codec<STORE>::template pair<true>(a1), Codec<STORE>::template pair<true>(b1));
+        }
       }
     };
 
+    load_scales(0);
     bool alive = true;
-    for (int i = 0; i < stages; ++i) {
-      const int st = i % NS;
-      alive = __all_sync(0xffffffffu, mbar_wait(&full[st], (i / NS) & 1, abort_flag, p.status));
+    for (int i = 0; i < mine; ++i) {
+      alive = __all_sync(0xffffffffu, mbar_wait(&full[i % NS], (i / NS) & 1, abort_flag, p.status));
       if (!alive) break;
-      const int left = c1 - (c0 + 16 * warp + i * kStage);
-      // the last stage may end inside the sixteen and hold the new token
-      if (i + 1 < stages) sixteen(std::false_type{}, st, i * kStage);
-      else if (left > 0) sixteen(std::true_type{}, st, i * kStage);
+      // the chunk's last unit may end inside and hold the new token
+      if (warp + i * kAtWarps + 1 < units) unit(std::false_type{}, i);
+      else unit(std::true_type{}, i);
       __syncwarp();
-      if (lane == 0 && i + NS < stages) {
-        __threadfence_block();
-        if ((atomicAdd(&taken[st], 1) & (kAtWarps - 1)) == kAtWarps - 1) {
-          __threadfence_block();
-          fill(i + NS);
-        }
-      }
+      if (lane == 0 && i + NS < mine) fill(i + NS);
     }
 
     // join the warps: n column 2 t + c of tile i is output dim VB (2 t + c) + i
-    __syncthreads();  // every warp has its q operand: u.o takes its place
+    __syncthreads();  // every warp is through with its ring
     ell += __shfl_xor_sync(0xffffffffu, ell, 1);
     ell += __shfl_xor_sync(0xffffffffu, ell, 2);
     if (t == 0) {
       m_s[warp][g] = m;
       l_s[warp][g] = ell;
     }
-    float* ow = u.o + (warp * 8 + g) * OS;
+    float* ow = o_s + (warp * 8 + g) * OS;
     const float vout = vref / kUp;
 #pragma unroll
     for (int c = 0; c < 2; ++c)
@@ -895,31 +960,39 @@ __global__ void __launch_bounds__(kAtThreads, 3)
       }
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < nE * D; i += kAtThreads) {
-    const int e = i / D, d = i - e * D;
-    float M = m_s[0][e];
+  // the warps' shares of each head's joint O: exp2(m_w - M) (and 1 / l where this
+  // chunk is the sequence's only one)
+  if (threadIdx.x < 8) {
+    const int e = threadIdx.x;
+    float M = m_s[0][e], l = 0.f;
 #pragma unroll
     for (int w = 1; w < kAtWarps; ++w) M = fmaxf(M, m_s[w][e]);
-    float l = 0.f, ov = 0.f;
-    if (M > -INFINITY) {
+    const float ref = M == -INFINITY ? 0.f : M;
+    float c[kAtWarps];
 #pragma unroll
-      for (int w = 0; w < kAtWarps; ++w) {
-        const float c = ex2(m_s[w][e] - M);
-        l += c * l_s[w][e];
-        ov += c * u.o[(w * 8 + e) * OS + d + d / 32 * 4];
-      }
+    for (int w = 0; w < kAtWarps; ++w) {
+      c[w] = ex2(m_s[w][e] - ref);
+      l += c[w] * l_s[w][e];
     }
-    if (active == 1) {
-      const int64_t hq = (int64_t)b * p.Hq + hkv * p.E + e0 + e;
-      static_cast<TQ*>(p.out)[hq * D + d] = from_f<TQ>(l != 0.f ? ov / l : 0.f);
-      if (d == 0) p.lse[hq] = l != 0.f ? (M + log2f(l)) * kLn2 : -INFINITY;
-    } else {
-      const int64_t at = (slot0 + split) * 8 + e;
-      __stcg(p.part + at * D + d, ov);
-      if (d == 0) __stcg(p.ml + at, make_float2(M, l));
+    const float f = active > 1 ? 1.f : l != 0.f ? 1.f / l : 0.f;
+#pragma unroll
+    for (int w = 0; w < kAtWarps; ++w) m_s[w][e] = c[w] * f;
+    l_s[0][e] = l;
+    if (e < nE) {
+      if (active > 1) __stcg(p.ml + (slot0 + split) * 8 + e, make_float2(M, l));
+      else p.lse[(int64_t)b * p.Hq + hkv * p.E + e0 + e] = l != 0.f ? (M + log2f(l)) * kLn2 : -INFINITY;
     }
   }
-  close_split<TQ>(p, b, hg, e0, nE, slot0, active, pos, &flag);
+  __syncthreads();
+  for (int i = threadIdx.x; i < nE * D; i += kAtThreads) {
+    const int e = i / D, d = i - e * D;
+    float ov = 0.f;
+#pragma unroll
+    for (int w = 0; w < kAtWarps; ++w) ov += m_s[w][e] * o_s[(w * 8 + e) * OS + d + d / 32 * 4];
+    if (active > 1) __stcg(p.part + ((slot0 + split) * 8 + e) * D + d, ov);
+    else static_cast<TQ*>(p.out)[((int64_t)b * p.Hq + hkv * p.E + e0 + e) * D + d] = from_f<TQ>(l_s[0][e] != 0.f ? ov : 0.f);
+  }
+  close_split<TQ>(p, b, hg, e0, nE, slot0, active, pos, &flag, o_s);
 }
 
 // Any head dims up to 256 and any head count: fp32 on the CUDA cores, a warp per
@@ -938,7 +1011,7 @@ __global__ void __launch_bounds__(kAnyThreads) attend_any(AttendParams p) {
   const int active = max(1, min(p.splits, (ntok + p.chunk - 1) / p.chunk));
   const int64_t slot0 = ((int64_t)b * p.Hkv * p.groups + hg) * p.splits;
   if (split >= active) {
-    if (p.advance) close_split<TQ>(p, b, hg, e0, nE, slot0, active, pos, &flag);
+    if (p.advance) close_split<TQ>(p, b, hg, e0, nE, slot0, active, pos, &flag, &o_s[0][0]);
     return;
   }
   const int c0 = split * p.chunk, c1 = split == active - 1 ? ntok : c0 + p.chunk;
@@ -1017,10 +1090,10 @@ __global__ void __launch_bounds__(kAnyThreads) attend_any(AttendParams p) {
       }
     }
   }
-  close_split<TQ>(p, b, hg, e0, nE, slot0, active, pos, &flag);
+  close_split<TQ>(p, b, hg, e0, nE, slot0, active, pos, &flag, &o_s[0][0]);
 }
 
-// Codes [rows * Hkv, capacity, D] as a 3-D map of kStage-token boxes, slots past the
+// Codes [rows * Hkv, capacity, D] as a 3-D map of kUnit-token boxes, slots past the
 // capacity reading as zeros.
 template <int D>
 int code_map(CUtensorMap* m, const void* base, const AttendParams& p, int64_t heads) {
@@ -1028,7 +1101,7 @@ int code_map(CUtensorMap* m, const void* base, const AttendParams& p, int64_t he
   if (!fn) return TC_ERR_CUDA;
   cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)p.cap, (cuuint64_t)heads};
   cuuint64_t strides[2] = {(cuuint64_t)D, (cuuint64_t)D * p.cap};
-  cuuint32_t box[3] = {(cuuint32_t)D, (cuuint32_t)kStage, 1};
+  cuuint32_t box[3] = {(cuuint32_t)D, (cuuint32_t)kUnit, 1};
   cuuint32_t estr[3] = {1, 1, 1};
   const CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(base), dims, strides, box, estr,
                         CU_TENSOR_MAP_INTERLEAVE_NONE, D == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
@@ -1073,7 +1146,7 @@ bool cache_ok(const tc_kv_cache* c) {
 // One sequence: one wave of three CTAs per SM over 148 SMs.  Several may differ
 // in length: eight waves, so that they even out (64 sequences of 1 to 32768
 // tokens: 360 us with two, 302 with four, 294 with eight, 301 with sixteen).  A
-// chunk is a multiple of 64 tokens (one stage).
+// chunk is a multiple of 64 tokens.
 void split_rule(int64_t most, int64_t heads, int B, int* chunk, int* splits) {
   const int64_t resident = 3 * 148;
   const int64_t want = B > 1 ? (8 * resident + heads - 1) / heads : heads < resident ? resident / heads : 1;
