@@ -15,28 +15,60 @@ namespace {
 // ---------------------------------------------------------------------------
 // example bounds
 // ---------------------------------------------------------------------------
-// One CTA per row; a thread owns consecutive tokens, so the largest run start
-// behind it and the smallest ahead of it come from one scan over the threads.
-// Bound by its two passes' latency (a few us at 16384 tokens, against the
-// attention that it precedes).
-constexpr int kBoundThreads = 1024;
-__global__ void __launch_bounds__(kBoundThreads) bounds_kernel(int N, const int32_t* seq, int32_t* starts, int32_t* ends) {
-  __shared__ int last_w[32], first_w[32];
-  const int64_t row = (int64_t)blockIdx.x * N;
-  const int32_t* id = seq + row;
-  const int per = (N + kBoundThreads - 1) / kBoundThreads;
-  const int n0 = min(N, (int)threadIdx.x * per), n1 = min(N, n0 + per);
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int first = N, last = -1;  // run starts among this thread's tokens
-  int prev = n0 > 0 && n0 < N ? id[n0 - 1] : 0;
-  for (int n = n0; n < n1; ++n) {
-    const int cur = id[n];
-    if (n == 0 || cur != prev) {
-      if (first == N) first = n;
-      last = n;
-    }
-    prev = cur;
+// A CTA covers kBoundTok tokens of a row, four consecutive ones a thread.  The run
+// that enters it (and the one that leaves it) may be long: the CTA looks for its
+// start (end) 16 tokens a thread at a time.  A few us at 16384 tokens.  (One CTA
+// per row: 31 us.)
+constexpr int kBoundThreads = 512, kBoundTok = 4 * kBoundThreads, kReach = 16;
+// Largest (FORWARD: smallest) run start over [lo, hi), -1 (N) where there is none;
+// the same for every thread.
+template <bool FORWARD>
+__device__ int edge(const int32_t* id, int lo, int hi, int N, int* box) {
+  int best = FORWARD ? N : -1;
+  int v[kReach], w[kReach];
+#pragma unroll
+  for (int k = 0; k < kReach; ++k) {
+    const int n = lo + threadIdx.x + k * kBoundThreads;
+    const bool in = n < hi;
+    v[k] = in ? id[n] : 0;
+    w[k] = in && n > 0 ? id[n - 1] : 0;
   }
+#pragma unroll
+  for (int k = 0; k < kReach; ++k) {
+    const int n = lo + threadIdx.x + k * kBoundThreads;
+    if (n < hi && (n == 0 || v[k] != w[k])) best = FORWARD ? min(best, n) : max(best, n);
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) *box = FORWARD ? N : -1;
+  __syncthreads();
+  if (FORWARD ? best < N : best >= 0) {
+    if (FORWARD) atomicMin(box, best);
+    else atomicMax(box, best);
+  }
+  __syncthreads();
+  return *box;
+}
+
+__global__ void __launch_bounds__(kBoundThreads) bounds_kernel(int N, const int32_t* seq, int32_t* starts, int32_t* ends) {
+  __shared__ int last_w[kBoundThreads / 32], first_w[kBoundThreads / 32], box;
+  const int64_t row = (int64_t)blockIdx.y * N;
+  const int32_t* id = seq + row;
+  const int c0 = blockIdx.x * kBoundTok, c1 = min(N, c0 + kBoundTok);
+  const int n0 = c0 + 4 * threadIdx.x;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int v[5];  // id[n0 - 1 .. n0 + 3]
+#pragma unroll
+  for (int k = 0; k < 5; ++k) {
+    const int n = n0 - 1 + k;
+    v[k] = n >= 0 && n < N ? id[n] : 0;
+  }
+  int first = N, last = -1;  // run starts among the thread's tokens
+#pragma unroll
+  for (int k = 3; k >= 0; --k)
+    if (n0 + k < c1 && (n0 + k == 0 || v[k + 1] != v[k])) first = n0 + k;
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    if (n0 + k < c1 && (n0 + k == 0 || v[k + 1] != v[k])) last = n0 + k;
   // exclusive scans: the largest start before this thread, the smallest after it
   int before = last, after = first;
 #pragma unroll
@@ -53,20 +85,39 @@ __global__ void __launch_bounds__(kBoundThreads) bounds_kernel(int N, const int3
   if (lane == 31) after = N;
   __syncthreads();
   for (int w = 0; w < warp; ++w) before = max(before, last_w[w]);
-  for (int w = warp + 1; w < 32; ++w) after = min(after, first_w[w]);
-  int start = before;
-  prev = n0 > 0 && n0 < N ? id[n0 - 1] : 0;
-  for (int n = n0; n < n1; ++n) {
-    const int cur = id[n];
-    if (n == 0 || cur != prev) start = n;
-    prev = cur;
-    starts[row + n] = cur < 0 ? n + 1 : start;
+  for (int w = warp + 1; w < kBoundThreads / 32; ++w) after = min(after, first_w[w]);
+  int first_all = N;
+  for (int w = 0; w < kBoundThreads / 32; ++w) first_all = min(first_all, first_w[w]);
+  // the run that enters the CTA
+  int enter = -1;
+  if (first_all > c0)  // uniform
+    for (int hi = c0; hi > 0 && enter < 0;) {
+      const int lo = max(0, hi - kReach * kBoundThreads);
+      enter = edge<false>(id, lo, hi, N, &box);
+      hi = lo;
+    }
+  // and where the last one ends
+  int leave = N;
+  for (int lo = c1; lo < N && leave == N;) {
+    const int hi = min(N, lo + kReach * kBoundThreads);
+    leave = edge<true>(id, lo, hi, N, &box);
+    lo = hi;
   }
-  int end = after;
-  for (int n = n1 - 1; n >= n0; --n) {
-    const int cur = id[n];
-    ends[row + n] = cur < 0 ? n : end;
-    if (n == 0 || id[n - 1] != cur) end = n;
+  int start = before >= 0 ? before : enter;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int n = n0 + k;
+    if (n >= c1) break;
+    if (n == 0 || v[k + 1] != v[k]) start = n;
+    starts[row + n] = v[k + 1] < 0 ? n + 1 : start;
+  }
+  int end = after < N ? after : leave;
+#pragma unroll
+  for (int k = 3; k >= 0; --k) {
+    const int n = n0 + k;
+    if (n >= c1) continue;
+    ends[row + n] = v[k + 1] < 0 ? n : end;
+    if (n == 0 || v[k + 1] != v[k]) end = n;
   }
 }
 
@@ -489,7 +540,8 @@ extern "C" int tc_segment_bounds(int32_t B, int32_t N, const int32_t* seq_idx, i
   if (B < 0 || N < 0) return TC_ERR_ARG;
   if ((int64_t)B * N == 0) return TC_OK;
   if (!seq_idx || !starts || !ends) return TC_ERR_ARG;
-  bounds_kernel<<<B, kBoundThreads, 0, (cudaStream_t)stream>>>(N, seq_idx, starts, ends);
+  if (B > 65535) return TC_ERR_UNSUPPORTED;
+  bounds_kernel<<<dim3((N + kBoundTok - 1) / kBoundTok, B), kBoundThreads, 0, (cudaStream_t)stream>>>(N, seq_idx, starts, ends);
   return launch_status();
 }
 

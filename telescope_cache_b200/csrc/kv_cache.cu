@@ -30,10 +30,23 @@ constexpr float kTiny = 1e-30f;
 template <int STORE> struct Codec;
 template <> struct Codec<TC_KV_INT8> {
   static constexpr float kTop = 127.f;
-  static __device__ __forceinline__ uint32_t code(float y) {
-    return (uint32_t)(min(max(__float2int_rn(y), -127), 127) + 128);
+  // y + 1.5 2^23 rounds y to an integer (nearest even) into the low mantissa bits:
+  // an add where the float-to-int conversion runs at a quarter of its rate
+  static __device__ __forceinline__ uint32_t code(float y) { return __float_as_uint(y + (12582912.f + 128.f)) & 255u; }
+  static __device__ __forceinline__ uint32_t code4(const float* y) {
+    uint32_t b[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) b[i] = __float_as_uint(y[i] + (12582912.f + 128.f));
+    return __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
   }
-  static __device__ __forceinline__ float value(uint32_t c) { return (float)((int)c - 128); }
+  // byte i of w: 2^23 + u exactly, then u - 128
+  static __device__ __forceinline__ float value(uint32_t c) { return __uint_as_float(0x4B000000u | c) - (8388608.f + 128.f); }
+  static __device__ __forceinline__ void value4(uint32_t w, float* v) {
+    v[0] = __uint_as_float(__byte_perm(w, 0x4B000000u, 0x7440)) - (8388608.f + 128.f);
+    v[1] = __uint_as_float(__byte_perm(w, 0x4B000000u, 0x7441)) - (8388608.f + 128.f);
+    v[2] = __uint_as_float(__byte_perm(w, 0x4B000000u, 0x7442)) - (8388608.f + 128.f);
+    v[3] = __uint_as_float(__byte_perm(w, 0x4B000000u, 0x7443)) - (8388608.f + 128.f);
+  }
   // The same two bytes as f16 subnormals u 2^-24, u = code + 128: a sum of their
   // products is (sum code q + 128 sum q) 2^-24.  One instruction where pair takes
   // two; for the keys, where the second sum is of the first one's size.  (For the
@@ -56,8 +69,18 @@ template <> struct Codec<TC_KV_FP8> {
   static __device__ __forceinline__ uint32_t code(float y) {
     return __nv_cvt_float_to_fp8(y, __NV_SATFINITE, __NV_E4M3);
   }
+  static __device__ __forceinline__ uint32_t code4(const float* y) {
+    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(y[0], y[1]), __NV_SATFINITE, __NV_E4M3);
+    const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(y[2], y[3]), __NV_SATFINITE, __NV_E4M3);
+    return lo | hi << 16;
+  }
   static __device__ __forceinline__ float value(uint32_t c) {
     return __half2float(__half(__nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)c, __NV_E4M3)));
+  }
+  static __device__ __forceinline__ void value4(uint32_t w, float* v) {
+    const uint32_t lo = pair<false>(w), hi = pair<true>(w);
+    const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&lo)), b = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+    v[0] = a.x, v[1] = a.y, v[2] = b.x, v[3] = b.y;
   }
   template <bool HI> static __device__ __forceinline__ uint32_t pair(uint32_t x) {
     const __half2_raw v = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(HI ? x >> 16 : x & 0xffffu), __NV_E4M3);
@@ -73,28 +96,60 @@ __device__ __forceinline__ void row_scale(float amax, float* scale, float* inv) 
   *inv = tiny ? 0.f : __fdiv_rn(Codec<STORE>::kTop, amax);
 }
 
+// The 16 bytes of w as floats, and floats as 16 bytes.
+template <typename T>
+__device__ __forceinline__ void unpack16(const uint4& w, float* x) {
+  const uint32_t v[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (std::is_same<T, float>::value) {
+      x[i] = __uint_as_float(v[i]);
+    } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+      x[2 * i] = __uint_as_float(v[i] << 16);
+      x[2 * i + 1] = __uint_as_float(v[i] & 0xffff0000u);
+    } else {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&v[i]));
+      x[2 * i] = f.x;
+      x[2 * i + 1] = f.y;
+    }
+  }
+}
+template <typename T>
+__device__ __forceinline__ uint4 pack16(const float* x) {
+  if constexpr (std::is_same<T, float>::value)
+    return make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
+  else
+    return tcx::pack8<T>(x, 1.f);
+}
+
 // |x| as bits: ordered as the floats are, with every NaN above infinity.
 __device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 
 // The value of a code: infinite or NaN only where the scale is (127 times a
 // scale that was rounded up may pass the largest float).
+__device__ __forceinline__ float held(float v, float scale) {
+  v *= scale;
+  return scale <= FLT_MAX ? fminf(fmaxf(v, -FLT_MAX), FLT_MAX) : v;
+}
 template <int STORE>
 __device__ __forceinline__ float dequant(uint32_t c, float scale) {
-  const float v = Codec<STORE>::value(c) * scale;
-  return scale <= FLT_MAX ? fminf(fmaxf(v, -FLT_MAX), FLT_MAX) : v;
+  return held(Codec<STORE>::value(c), scale);
 }
 
 // ---------------------------------------------------------------------------
 // write
 // ---------------------------------------------------------------------------
+struct WriteSide {  // keys or values
+  const void* src;
+  int64_t sb, sn, sh;
+  uint8_t* codes;
+  float* scales;
+  int dim;
+};
 struct WriteParams {
-  int B, N, H, D, rows, fresh;
+  int B, N, H, rows, fresh;
   int64_t cap;
-  const void* src[2];  // k, v
-  int64_t sb[2], sn[2], sh[2];
-  uint8_t* codes[2];
-  float* scales[2];
-  int dim[2];
+  WriteSide k, v;
   int32_t* lengths;
   const int32_t* seq;     // [B, N] or null: token (b, n) belongs to cache row b
   const int32_t* starts;  // [B, N] first token of each run of equal ids (with seq)
@@ -146,67 +201,66 @@ __global__ void __launch_bounds__(256) advance_kernel(WriteParams p) {
 
 // LANES lanes per row, 16 bytes each; blockIdx.y: 0 keys, 1 values.  Bound by
 // HBM: the row is read once, its maximum goes round the lanes by shuffles, and
-// the codes leave as 8-byte (fp32: 4-byte) pieces of whole 32-byte sectors.
-// kTok consecutive tokens of one head per lane group keep as many loads in
-// flight.
-constexpr int kTok = 4;
+// the codes leave as 8-byte (fp32: 4-byte) pieces of whole 32-byte sectors.  A
+// lane group takes kTok consecutive tokens of one head: lane j finds token j's
+// place, then kTok loads a lane are in flight (tokens without a place load
+// nothing).
+constexpr int kTok = 8;
 template <typename T, int STORE, int LANES>
-__global__ void __launch_bounds__(256) write_vec(WriteParams p) {
+__global__ void __launch_bounds__(256) write_vec(const __grid_constant__ WriteParams p) {
   constexpr int VE = 16 / sizeof(T);
-  const int which = blockIdx.y;
-  const int lane = threadIdx.x % LANES;
-  const int64_t group = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) / LANES;
-  const int tiles = (p.N + kTok - 1) / kTok;
-  const int h = (int)(group % p.H);
-  const int64_t bt = group / p.H;
-  if (bt >= (int64_t)p.B * tiles) return;  // whole lane groups leave; the shuffles below name their own lanes
-  const int b = (int)(bt / tiles), n0 = (int)(bt % tiles) * kTok;
+  const bool keys = blockIdx.y == 0;
+  const WriteSide& w = keys ? p.k : p.v;
+  const int b = blockIdx.z, lane = threadIdx.x % LANES;
+  const int group = blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
+  const int tile = group / p.H, h = group - tile * p.H, n0 = tile * kTok;
+  if (n0 >= p.N) return;  // whole lane groups leave; the shuffles below name their own lanes
   const uint32_t mask = LANES == 32 ? 0xffffffffu : ((1u << LANES) - 1u) << ((threadIdx.x & 31) / LANES * LANES);
-  const T* src = static_cast<const T*>(p.src[which]) + b * p.sb[which] + h * p.sh[which] + lane * VE;
-  uint4 raw[kTok];
-#pragma unroll
-  for (int j = 0; j < kTok; ++j)
-    if (n0 + j < p.N) raw[j] = *reinterpret_cast<const uint4*>(src + (int64_t)(n0 + j) * p.sn[which]);
-#pragma unroll
-  for (int j = 0; j < kTok; ++j) {
-    const int n = n0 + j;
-    if (n >= p.N) break;
+  int64_t at = -1;  // lane j: row of codes of token n0 + j
+  if (lane < kTok && n0 + lane < p.N) {
     int row;
     int64_t slot = 0;
-    place(p, b, n, &row, &slot);
-    if (p.fresh && which == 0 && h == 0 && lane == 0) advance_row(p, b, n);
-    if (row < 0) continue;
-    const T* e = reinterpret_cast<const T*>(&raw[j]);
+    place(p, b, n0 + lane, &row, &slot);
+    if (row >= 0) at = ((int64_t)row * p.H + h) * p.cap + slot;
+    if (p.fresh && keys && h == 0) advance_row(p, b, n0 + lane);
+  }
+  const T* src = static_cast<const T*>(w.src) + b * w.sb + h * w.sh + lane * VE;
+  uint4 raw[kTok];
+  int64_t to[kTok];
+  float mine = 0.f;  // lane j: token j's scale, so that they leave in one store
+#pragma unroll
+  for (int j = 0; j < kTok; ++j) {
+    to[j] = __shfl_sync(mask, at, j, LANES);
+    if (to[j] >= 0) raw[j] = *reinterpret_cast<const uint4*>(src + (int64_t)(n0 + j) * w.sn);
+  }
+#pragma unroll
+  for (int j = 0; j < kTok; ++j) {
+    if (to[j] < 0) continue;
     float x[VE];
+    unpack16<T>(raw[j], x);
     uint32_t m = 0;
 #pragma unroll
-    for (int i = 0; i < VE; ++i) {
-      x[i] = to_f(e[i]);
-      m = max(m, abs_bits(x[i]));
-    }
+    for (int i = 0; i < VE; ++i) m = max(m, abs_bits(x[i]));
 #pragma unroll
     for (int o = LANES / 2; o; o >>= 1) m = max(m, __shfl_xor_sync(mask, m, o));
     float scale, inv;
     row_scale<STORE>(__uint_as_float(m), &scale, &inv);
-    uint32_t w[VE / 4];
 #pragma unroll
-    for (int i = 0; i < VE / 4; ++i) {
-      w[i] = 0;
-#pragma unroll
-      for (int k = 0; k < 4; ++k) w[i] |= Codec<STORE>::code(__fmul_rn(x[4 * i + k], inv)) << (8 * k);
-    }
-    const int64_t at = ((int64_t)row * p.H + h) * p.cap + slot;
-    uint8_t* dst = p.codes[which] + at * p.dim[which] + lane * VE;
-    if constexpr (VE == 8) *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);
-    else *reinterpret_cast<uint32_t*>(dst) = w[0];
-    if (lane == 0) p.scales[which][at] = scale;
+    for (int i = 0; i < VE; ++i) x[i] = __fmul_rn(x[i], inv);
+    uint8_t* dst = w.codes + to[j] * (LANES * VE) + lane * VE;
+    if constexpr (VE == 8) *reinterpret_cast<uint2*>(dst) = make_uint2(Codec<STORE>::code4(x), Codec<STORE>::code4(x + 4));
+    else *reinterpret_cast<uint32_t*>(dst) = Codec<STORE>::code4(x);
+    if (lane == j) mine = scale;
   }
+  if (at >= 0) w.scales[at] = mine;
 }
 
 // Any head dim and strides: a warp per row, two passes over it.
 template <typename T, int STORE>
-__global__ void __launch_bounds__(256) write_any(WriteParams p) {
-  const int which = blockIdx.y, lane = threadIdx.x & 31;
+__global__ void __launch_bounds__(256) write_any(const __grid_constant__ WriteParams p) {
+  const bool keys = blockIdx.y == 0;
+  const WriteSide& w = keys ? p.k : p.v;
+  const int lane = threadIdx.x & 31;
   const int64_t i = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
   const int h = (int)(i % p.H);
   const int64_t tok = i / p.H;
@@ -215,10 +269,10 @@ __global__ void __launch_bounds__(256) write_any(WriteParams p) {
   int row;
   int64_t slot = 0;
   place(p, b, n, &row, &slot);
-  if (p.fresh && which == 0 && h == 0 && lane == 0) advance_row(p, b, n);
+  if (p.fresh && keys && h == 0 && lane == 0) advance_row(p, b, n);
   if (row < 0) return;
-  const T* src = static_cast<const T*>(p.src[which]) + b * p.sb[which] + (int64_t)n * p.sn[which] + h * p.sh[which];
-  const int D = p.dim[which];
+  const T* src = static_cast<const T*>(w.src) + b * w.sb + (int64_t)n * w.sn + h * w.sh;
+  const int D = w.dim;
   uint32_t m = 0;
   for (int d = lane; d < D; d += 32) m = max(m, abs_bits(to_f(src[d])));
 #pragma unroll
@@ -226,24 +280,24 @@ __global__ void __launch_bounds__(256) write_any(WriteParams p) {
   float scale, inv;
   row_scale<STORE>(__uint_as_float(m), &scale, &inv);
   const int64_t at = ((int64_t)row * p.H + h) * p.cap + slot;
-  for (int d = lane; d < D; d += 32) p.codes[which][at * D + d] = (uint8_t)Codec<STORE>::code(__fmul_rn(to_f(src[d]), inv));
-  if (lane == 0) p.scales[which][at] = scale;
+  for (int d = lane; d < D; d += 32) w.codes[at * D + d] = (uint8_t)Codec<STORE>::code(__fmul_rn(to_f(src[d]), inv));
+  if (lane == 0) w.scales[at] = scale;
 }
 
 template <typename T, int STORE>
 int launch_write(const WriteParams& p, cudaStream_t st) {
   constexpr int VE = 16 / sizeof(T);
-  bool vec = p.dim[0] == p.dim[1];
-  for (int w = 0; w < 2; ++w) {
-    vec = vec && (uintptr_t)p.src[w] % 16 == 0 && p.sb[w] % VE == 0 && p.sn[w] % VE == 0 && p.sh[w] % VE == 0 &&
-          (uintptr_t)p.codes[w] % 8 == 0;
-  }
-  const int lanes = p.dim[0] / VE;
-  vec = vec && p.dim[0] % VE == 0 && (lanes == 8 || lanes == 16 || lanes == 32);
-  const int64_t units = vec ? (int64_t)p.B * ((p.N + kTok - 1) / kTok) * p.H * lanes : (int64_t)p.B * p.N * p.H * 32;
+  bool vec = p.k.dim == p.v.dim;
+  for (const WriteSide* w : {&p.k, &p.v})
+    vec = vec && (uintptr_t)w->src % 16 == 0 && w->sb % VE == 0 && w->sn % VE == 0 && w->sh % VE == 0 &&
+          (uintptr_t)w->codes % 8 == 0;
+  const int lanes = p.k.dim / VE;
+  vec = vec && p.k.dim % VE == 0 && (lanes == 8 || lanes == 16 || lanes == 32);
+  vec = vec && p.B <= 65535;
+  const int64_t units = vec ? (int64_t)((p.N + kTok - 1) / kTok) * p.H * lanes : (int64_t)p.B * p.N * p.H * 32;
   const int64_t grid = (units + 255) / 256;
   if (grid > INT32_MAX) return TC_ERR_UNSUPPORTED;
-  const dim3 g((unsigned)grid, 2);
+  const dim3 g((unsigned)grid, 2, vec ? p.B : 1);
   if (!vec) write_any<T, STORE><<<g, 256, 0, st>>>(p);
   else if (lanes == 8) write_vec<T, STORE, 8><<<g, 256, 0, st>>>(p);
   else if (lanes == 16) write_vec<T, STORE, 16><<<g, 256, 0, st>>>(p);
@@ -259,26 +313,31 @@ int launch_write(const WriteParams& p, cudaStream_t st) {
 // ---------------------------------------------------------------------------
 // read back
 // ---------------------------------------------------------------------------
+struct ReadSide {
+  const uint8_t* codes;
+  const float* scales;
+  int dim;
+  void* out;  // [rows, L, H, D]
+};
 struct ReadParams {
   int rows, H, L;
   int64_t cap;
-  const uint8_t* codes[2];
-  const float* scales[2];
-  int dim[2];
+  ReadSide k, v;
   const int32_t* lengths;
-  void* out[2];  // [rows, L, H, D]
 };
 
 // A thread per V codes of one row (V = 16 / element size, or 1) and kReadTok
 // tokens; a CTA's threads run over the heads and dims of a token, so the output
 // is written in order.  Slots past a row's length are zeros and read nothing.
-constexpr int kReadTok = 4;
+constexpr int kReadTok = 8;
 template <typename T, int STORE, int V>
-__global__ void __launch_bounds__(256) read_kernel(ReadParams p) {
-  const int which = blockIdx.y, D = p.dim[which], per = p.H * (D / V);  // threads per token
+__global__ void __launch_bounds__(256) read_kernel(const __grid_constant__ ReadParams p) {
+  const ReadSide& w = blockIdx.y == 0 ? p.k : p.v;
+  const int D = w.dim, per = p.H * (D / V);  // threads per token
   const int b = blockIdx.z, len = (int)min((int64_t)p.lengths[b], p.cap);
-  const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-  const int tile = (int)(i / per), rest = (int)(i - (int64_t)tile * per);
+  const int64_t first = (int64_t)blockIdx.x * blockDim.x;
+  const int t0 = (int)(first / per), off = (int)(first - (int64_t)t0 * per) + threadIdx.x;  // one wide division a CTA
+  const int tile = t0 + off / per, rest = off % per;
   const int h = rest / (D / V), d = (rest - h * (D / V)) * V;
   const int n0 = tile * kReadTok;
   using Raw = typename std::conditional<V == 8, uint2, typename std::conditional<V == 4, uint32_t, uint8_t>::type>::type;
@@ -290,33 +349,32 @@ __global__ void __launch_bounds__(256) read_kernel(ReadParams p) {
     const int n = n0 + j;
     sc[j] = 0.f;
     if (n < len && n < p.L) {
-      raw[j] = *reinterpret_cast<const Raw*>(p.codes[which] + (at0 + n) * D + d);
-      sc[j] = p.scales[which][at0 + n];
+      raw[j] = *reinterpret_cast<const Raw*>(w.codes + (at0 + n) * D + d);
+      sc[j] = w.scales[at0 + n];
     }
   }
 #pragma unroll
   for (int j = 0; j < kReadTok; ++j) {
     const int n = n0 + j;
     if (n >= p.L) return;
-    T* out = static_cast<T*>(p.out[which]) + (((int64_t)b * p.L + n) * p.H + h) * D + d;
+    T* out = static_cast<T*>(w.out) + (((int64_t)b * p.L + n) * p.H + h) * D + d;
     float v[V];
 #pragma unroll
-    for (int k = 0; k < V; ++k) {
-      uint32_t c;
-      if constexpr (V == 8) c = ((k < 4 ? raw[j].x : raw[j].y) >> (8 * (k & 3))) & 255u;
-      else if constexpr (V == 4) c = (raw[j] >> (8 * k)) & 255u;
-      else c = raw[j];
-      v[k] = n < len ? dequant<STORE>(c, sc[j]) : 0.f;
-    }
-    if constexpr (V == 1) {
-      out[0] = from_f<T>(v[0]);
-    } else {
-      uint4 w;
-      T* e = reinterpret_cast<T*>(&w);
+    for (int k = 0; k < V; ++k) v[k] = 0.f;
+    if (n < len) {
+      if constexpr (V == 8) {
+        Codec<STORE>::value4(raw[j].x, v);
+        Codec<STORE>::value4(raw[j].y, v + 4);
+      } else if constexpr (V == 4) {
+        Codec<STORE>::value4(raw[j], v);
+      } else {
+        v[0] = Codec<STORE>::value(raw[j]);
+      }
 #pragma unroll
-      for (int k = 0; k < V; ++k) e[k] = from_f<T>(v[k]);
-      *reinterpret_cast<uint4*>(out) = w;
+      for (int k = 0; k < V; ++k) v[k] = held(v[k], sc[j]);
     }
+    if constexpr (V == 1) out[0] = from_f<T>(v[0]);
+    else *reinterpret_cast<uint4*>(out) = pack16<T>(v);
   }
 }
 
@@ -324,9 +382,9 @@ template <typename T, int STORE>
 int launch_read(const ReadParams& p, cudaStream_t st) {
   constexpr int V = 16 / sizeof(T);
   bool vec = true;
-  for (int w = 0; w < 2; ++w)
-    vec = vec && p.dim[w] % V == 0 && (uintptr_t)p.codes[w] % V == 0 && (uintptr_t)p.out[w] % 16 == 0;
-  const int D = p.dim[0] > p.dim[1] ? p.dim[0] : p.dim[1];
+  for (const ReadSide* w : {&p.k, &p.v})
+    vec = vec && w->dim % V == 0 && (uintptr_t)w->codes % V == 0 && (uintptr_t)w->out % 16 == 0;
+  const int D = p.k.dim > p.v.dim ? p.k.dim : p.v.dim;
   const int64_t units = (int64_t)((p.L + kReadTok - 1) / kReadTok) * p.H * (vec ? D / V : D);
   const int64_t grid = (units + 255) / 256;
   if (grid > INT32_MAX || p.rows > 65535) return TC_ERR_UNSUPPORTED;
@@ -1165,14 +1223,10 @@ extern "C" int tc_kv_write(const tc_kv_cache* c, const tc_kv_write_args* a, void
   if ((int64_t)a->B * a->N == 0) return TC_OK;
   if (!a->k || !a->v || (a->seq_idx && !a->starts) || (!a->seq_idx && a->B > c->rows)) return TC_ERR_ARG;
   WriteParams p;
-  p.B = a->B, p.N = a->N, p.H = c->Hkv, p.D = 0, p.rows = c->rows, p.fresh = a->fresh != 0;
+  p.B = a->B, p.N = a->N, p.H = c->Hkv, p.rows = c->rows, p.fresh = a->fresh != 0;
   p.cap = c->capacity;
-  p.src[0] = a->k, p.src[1] = a->v;
-  p.sb[0] = a->k_stride_b, p.sn[0] = a->k_stride_n, p.sh[0] = a->k_stride_h;
-  p.sb[1] = a->v_stride_b, p.sn[1] = a->v_stride_n, p.sh[1] = a->v_stride_h;
-  p.codes[0] = c->k, p.codes[1] = c->v;
-  p.scales[0] = c->k_scale, p.scales[1] = c->v_scale;
-  p.dim[0] = c->Dk, p.dim[1] = c->Dv;
+  p.k = {a->k, a->k_stride_b, a->k_stride_n, a->k_stride_h, c->k, c->k_scale, c->Dk};
+  p.v = {a->v, a->v_stride_b, a->v_stride_n, a->v_stride_h, c->v, c->v_scale, c->Dv};
   p.lengths = c->lengths;
   p.seq = a->seq_idx, p.starts = a->starts;
   p.status = a->dev_status;
@@ -1186,11 +1240,9 @@ extern "C" int tc_kv_read(const tc_kv_cache* c, int32_t length, int32_t dtype, v
   if ((int64_t)c->rows * length == 0) return TC_OK;
   ReadParams p;
   p.rows = c->rows, p.H = c->Hkv, p.L = length, p.cap = c->capacity;
-  p.codes[0] = c->k, p.codes[1] = c->v;
-  p.scales[0] = c->k_scale, p.scales[1] = c->v_scale;
-  p.dim[0] = c->Dk, p.dim[1] = c->Dv;
+  p.k = {c->k, c->k_scale, c->Dk, k_out};
+  p.v = {c->v, c->v_scale, c->Dv, v_out};
   p.lengths = c->lengths;
-  p.out[0] = k_out, p.out[1] = v_out;
   cudaStream_t st = (cudaStream_t)stream;
   if (c->store == TC_KV_INT8) { TC_DISPATCH(dtype, T, return launch_read<T, TC_KV_INT8>(p, st)); }
   else { TC_DISPATCH(dtype, T, return launch_read<T, TC_KV_FP8>(p, st)); }
