@@ -6,6 +6,7 @@ not available the calls raise; there is no CPU fallback.
 """
 
 import ctypes
+import importlib.util
 import os
 
 import torch
@@ -209,6 +210,38 @@ def lib():
         handle.tc_kv_attend_scratch_floats.restype = ctypes.c_int64
         _LIB = handle
     return _LIB
+
+
+HOST_PATH = os.path.join(_HERE, "_lib", "_full_attention.so")
+_HOST = None
+_HOST_DEVICES = set()  # devices whose status word the host extension has
+
+
+def _load_host():
+    global _HOST
+    lib()
+    if not os.path.exists(HOST_PATH):
+        raise RuntimeError(
+            f"telescope_cache_b200: host extension {HOST_PATH} is missing; build it with "
+            "`python -m telescope_cache_b200.build_lib`")
+    spec = importlib.util.spec_from_file_location("_full_attention", HOST_PATH)
+    module = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(module)
+    _HOST = module
+
+
+def host(t):
+    """The host extension (csrc/host), for a call on CUDA tensor t: it checks the
+    arguments, allocates the outputs and calls the library's C entries."""
+    if t.get_device() not in _HOST_DEVICES:
+        if _HOST is None:
+            _load_host()
+        require_cuda(t)
+        from .telescoping_attn.attention import device_status
+
+        _HOST.set_status(device_status(t.device))
+        _HOST_DEVICES.add(t.get_device())
+    return _HOST
 
 
 _ERRORS = {

@@ -22,18 +22,21 @@ reference's RoPE at summary positions) and the unweighted scan
 (``weight_mode=None``).
 """
 
-from typing import Dict, Optional, Tuple
+from typing import Any, Dict, Optional, Tuple
 
 import torch
 from torch import nn
 
 from .range_spec import activation_times_from_fmap
+from .telescoping_attn.causal import causal_attention, segment_bounds
 from .telescoping_attn.decode import decode_step
 from .telescoping_attn.decode_state import DecodeState, init_decode_state
+from .telescoping_attn.kv_cache import KVCache, cached_attention_step, init_kv_cache, write_kv_cache
 from .telescoping_attn.linear import project
 from .telescoping_attn.attention import multilevel_attention_forward
 from .telescoping_attn.packing import pack_levels
 from .telescoping_attn.position import compute_relative_states, rope_tables
+from .telescoping_attn.rotary import LAYOUTS, rotary, rotary_tables
 from .telescoping_attn.sink_gate import apply_attention_sink, apply_output_gate
 from .telescoping_attn.summaries import build_dyadic_summaries, short_conv
 
@@ -236,4 +239,107 @@ class MultiHeadAttention(nn.Module):
         return self._linear(out.reshape(B, 1, self.nheads * self.emb_v_per_head), self.dense)
 
 
-__all__ = ["MultiHeadAttention", "ShortConv1d", "DEFAULT_FMAP", "DEFAULT_CACHE_SIZE"]
+class FullMultiHeadAttention(nn.Module):
+    """The layer that a hybrid stack keeps at full attention between its
+    telescoping ones: rotary positions, causal attention over packed examples,
+    and an 8-bit cache for single tokens, with MultiHeadAttention's projections,
+    parameter names, sinks and gate.
+
+    Keyword-only: ``softcap``; ``rope_base``, ``rope_layout`` ('half' |
+    'interleaved'), ``rope_dim`` (dims of a head that rotate, all by default),
+    ``rope_scaling`` (rotary_tables' scaling arguments); ``cache_store`` ('int8'
+    | 'fp8'); ``use_sinks``, ``use_gate``."""
+
+    def __init__(self, emb_dim: int, emb_kq: int, emb_v: int, nheads: int, kvheads: int, use_bias: bool = False, *,
+                 softcap: Optional[float] = None, rope_base: float = 10000.0, rope_layout: str = "half",
+                 rope_dim: Optional[int] = None, rope_scaling: Optional[Dict[str, Any]] = None,
+                 cache_store: str = "int8", use_sinks: bool = False, use_gate: bool = False):
+        super().__init__()
+        if nheads % kvheads:
+            raise ValueError(f"nheads {nheads} is not a multiple of kvheads {kvheads}")
+        if rope_layout not in LAYOUTS:
+            raise ValueError(f"rope_layout must be one of {LAYOUTS}, got {rope_layout!r}")
+        rope_dim = emb_kq if rope_dim is None else int(rope_dim)
+        if not 0 < rope_dim <= emb_kq or rope_dim % 2:
+            raise ValueError(f"rope_dim must be even and in (0, {emb_kq}], got {rope_dim}")
+        self.emb_dim, self.nheads, self.kvheads = emb_dim, nheads, kvheads
+        self.emb_kq_per_head, self.emb_v_per_head = emb_kq, emb_v
+        self.softcap, self.cache_store = softcap, cache_store
+        self.rope_base, self.rope_layout, self.rope_dim = rope_base, rope_layout, rope_dim
+        self.rope_scaling = dict(rope_scaling or {})
+        self._split = (nheads * emb_kq, kvheads * emb_kq, kvheads * emb_v)
+        self.in_proj = nn.Linear(emb_dim, sum(self._split), bias=use_bias)
+        self.dense = nn.Linear(nheads * emb_v, emb_dim, bias=use_bias)
+        self.use_sinks, self.use_gate = use_sinks, use_gate
+        if use_sinks:
+            self.sinks = nn.Parameter(torch.zeros(nheads))
+        if use_gate:
+            self.gate_proj = nn.Linear(emb_dim, nheads * emb_v, bias=False)
+        self._rope: Tuple[int, Optional[torch.Tensor], Optional[torch.Tensor]] = (0, None, None)
+        self.reset_parameters()
+
+    def reset_parameters(self):
+        for m in self.modules():
+            if isinstance(m, nn.Linear):
+                nn.init.trunc_normal_(m.weight, mean=0.0, std=0.02)
+                if m.bias is not None:
+                    m.bias.data.zero_()
+        if self.use_sinks:
+            self.sinks.data.zero_()
+
+    def _tables(self, n_pos, device):
+        have, cos, sin = self._rope
+        if cos is None or have < n_pos or cos.device != device:
+            have = max(n_pos, 2 * have)
+            cos, sin = rotary_tables(have, self.rope_dim, self.rope_base, device=device, **self.rope_scaling)
+            self._rope = (have, cos, sin)
+        return cos, sin
+
+    def _qkv(self, x):
+        """q, k, v as views of the fused projection: rotary and the attention read
+        them in place."""
+        B, N, _ = x.shape
+        q, k, v = torch.split(MultiHeadAttention._linear(x, self.in_proj), self._split, dim=-1)
+        return (q.view(B, N, self.nheads, self.emb_kq_per_head), k.view(B, N, self.kvheads, self.emb_kq_per_head),
+                v.view(B, N, self.kvheads, self.emb_v_per_head))
+
+    def _finish(self, out, lse, x):
+        if self.use_sinks:
+            out = apply_attention_sink(out, lse, self.sinks)
+        if self.use_gate:
+            out = apply_output_gate(out, x, self.gate_proj.weight)
+        return MultiHeadAttention._linear(out.reshape(x.shape[0], x.shape[1], -1), self.dense)
+
+    def forward(self, x: torch.Tensor, seq_idx: Optional[torch.Tensor] = None, *, cache: Optional[KVCache] = None):
+        """x [B, N, emb_dim] -> [B, N, emb_dim].  seq_idx [B, N]: ids of packed
+        examples (negative: padding); positions restart with each.  With a cache
+        (new_cache), its rows start anew with these prompts: batch row b in cache
+        row b, or the example with id i in cache row i."""
+        B, N, _ = x.shape
+        q, k, v = self._qkv(x)
+        cos, sin = self._tables(N, x.device)
+        seg = None if seq_idx is None else segment_bounds(seq_idx)
+        q, k = rotary(q, k, cos, sin, positions=None if seg is None else seg.positions(), layout=self.rope_layout)
+        out, lse = causal_attention(q, k, v, seq_idx=seg, softcap=self.softcap)
+        if cache is not None:
+            with torch.no_grad():
+                write_kv_cache(cache, k.detach(), v.detach(), seq_idx=seq_idx, fresh=True)
+        return self._finish(out, lse, x)
+
+    def new_cache(self, rows: int, capacity: int, dtype: torch.dtype = torch.bfloat16, device=None) -> KVCache:
+        """An empty cache of this layer for `rows` sequences of up to `capacity` tokens."""
+        return init_kv_cache(rows, capacity, self.kvheads, self.emb_kq_per_head, self.emb_v_per_head,
+                             store=self.cache_store, dtype=dtype, device=device)
+
+    @torch.no_grad()
+    def decode(self, x_t: torch.Tensor, cache: KVCache) -> torch.Tensor:
+        """One token of every sequence, x_t [B, 1, emb_dim] -> [B, 1, emb_dim]: its
+        key and value join the cache, at the end of each row."""
+        q, k, v = self._qkv(x_t)
+        cos, sin = self._tables(cache.max_length + 1, x_t.device)
+        out, lse = cached_attention_step(q, k, v, cache, rope_cos=cos, rope_sin=sin, layout=self.rope_layout,
+                                         softcap=self.softcap)
+        return self._finish(out, lse, x_t)
+
+
+__all__ = ["MultiHeadAttention", "FullMultiHeadAttention", "ShortConv1d", "DEFAULT_FMAP", "DEFAULT_CACHE_SIZE"]

@@ -64,35 +64,6 @@ def rotary_tables(n_pos: int, dim: int, base: float = 10000.0, *, scaling: str =
     return (torch.cos(ang) * magnitude).float(), (torch.sin(ang) * magnitude).float()
 
 
-def _table(t):
-    return t if t.dtype == torch.float32 and t.is_contiguous() else t.float().contiguous()
-
-
-def _dense_head(t):
-    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
-
-
-def _launch(q, k, cos, sin, positions, layout, inverse):
-    B, N, Hq, D = q.shape
-    q = _dense_head(q)
-    a = _lib.RotaryArgs(B=B, N=N, Hq=Hq, Hk=0, D=D, R=2 * cos.shape[1], dtype=_lib.dtype_code(q.dtype),
-                        interleaved=layout == "interleaved", inverse=bool(inverse), n_pos=cos.shape[0],
-                        cos_t=cos.data_ptr(), sin_t=sin.data_ptr())
-    qo = torch.empty(q.shape, device=q.device, dtype=q.dtype)
-    a.q, a.q_out = q.data_ptr(), qo.data_ptr()
-    a.q_stride_b, a.q_stride_n, a.q_stride_h = q.stride(0), q.stride(1), q.stride(2)
-    ko = None
-    if k is not None:
-        k = _dense_head(k)
-        ko = torch.empty(k.shape, device=k.device, dtype=k.dtype)
-        a.Hk, a.k, a.k_out = k.shape[2], k.data_ptr(), ko.data_ptr()
-        a.k_stride_b, a.k_stride_n, a.k_stride_h = k.stride(0), k.stride(1), k.stride(2)
-    if positions is not None:
-        a.positions, a.pos_stride_b = positions.data_ptr(), positions.stride(0) if positions.dim() == 2 else 0
-    _lib.launch("tc_rotary", q.device, a, _lib.stream_of(q))
-    return qo, ko
-
-
 class _Rotary(torch.autograd.Function):
     """The rotation is linear: its VJP is the rotation by the negative angle
     (with the tables' magnitude), in the same kernel."""
@@ -101,17 +72,14 @@ class _Rotary(torch.autograd.Function):
     def forward(ctx, q, k, cos, sin, positions, layout, inverse):
         ctx.save_for_backward(cos, sin, positions)
         ctx.cfg = (layout, inverse, q.dtype)
-        qo, ko = _launch(q, k, cos, sin, positions, layout, inverse)
-        return qo, ko
+        return _lib.host(q).rotary(q, k, cos, sin, positions, layout, inverse)
 
     @staticmethod
     def backward(ctx, gq, gk):
         cos, sin, positions = ctx.saved_tensors
         layout, inverse, dtype = ctx.cfg
-        if gk is None:
-            dq, dk = _launch(gq.to(dtype), None, cos, sin, positions, layout, not inverse)
-        else:
-            dq, dk = _launch(gq.to(dtype), gk.to(dtype), cos, sin, positions, layout, not inverse)
+        dq, dk = _lib.host(gq).rotary(gq.to(dtype), None if gk is None else gk.to(dtype), cos, sin, positions, layout,
+                                      not inverse)
         return dq, dk, None, None, None, None, None
 
 
@@ -126,35 +94,15 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], cos: torch.Tensor, sin: t
     position outside the tables makes the rotated dims of its rows NaN (no
     device value is read on the host).  Differentiable in q and k; inverse=True
     rotates back.  Any strides with a dense head dim are read in place."""
-    if q.dim() != 4:
-        raise ValueError(f"q must be [B, N, H, D], got {tuple(q.shape)}")
-    B, N, _, D = q.shape
-    if k is not None and (k.dim() != 4 or tuple(k.shape[:2]) != (B, N) or k.shape[3] != D):
-        raise ValueError(f"k shape {tuple(k.shape)} incompatible with q {tuple(q.shape)}")
-    if k is not None and k.dtype != q.dtype:
-        raise ValueError(f"k dtype {k.dtype} must match q dtype {q.dtype}")
-    if cos.shape != sin.shape or cos.dim() != 2:
-        raise ValueError(f"cos {tuple(cos.shape)} and sin {tuple(sin.shape)} must be one [n_pos, R / 2] shape")
-    if 2 * cos.shape[1] > D:
-        raise ValueError(f"rotary tables cover dim {2 * cos.shape[1]}, the heads have {D}")
     if layout not in LAYOUTS:
         raise ValueError(f"layout must be one of {LAYOUTS}, got {layout!r}")
-    if positions is None:
-        if cos.shape[0] < N:
-            raise ValueError(f"rotary tables cover {cos.shape[0]} positions, q has {N}")
-    else:
-        if positions.dtype.is_floating_point or tuple(positions.shape) not in ((N,), (B, N)):
-            raise ValueError(f"positions must be integers [{N}] or [{B}, {N}], got {tuple(positions.shape)} "
-                             f"{positions.dtype}")
-        if positions.dtype != torch.int32 or positions.stride(-1) != 1:
-            positions = positions.to(torch.int32).contiguous()
-    _lib.require_cuda(q, k, cos, sin, positions)
+    interleaved = layout == "interleaved"
     if torch.is_grad_enabled():
         if cos.requires_grad or sin.requires_grad:
             raise NotImplementedError("gradients with respect to the rotary tables are not supported")
         if q.requires_grad or (k is not None and k.requires_grad):
-            return _Rotary.apply(q, k, _table(cos), _table(sin), positions, layout, bool(inverse))
-    return _launch(q, k, _table(cos), _table(sin), positions, layout, inverse)
+            return _Rotary.apply(q, k, cos, sin, positions, interleaved, inverse)
+    return _lib.host(q).rotary(q, k, cos, sin, positions, interleaved, inverse)
 
 
 __all__ = ["rotary_tables", "rotary"]
