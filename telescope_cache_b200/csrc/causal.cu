@@ -165,7 +165,7 @@ int launch_delta(const CausalParams& p, cudaStream_t st) {
 
 // ---------------------------------------------------------------------------
 // CUDA-core tiles: 256 threads as 16 x 16; thread (ty, tx) owns rows ty + 16 i
-// and columns tx + 16 j of a TM x TM score tile, and output rows ty + 16 i with
+// and columns tx + 16 j of a TM x TN score tile, and output rows ty + 16 i with
 // the four-wide columns 4 tx + 64 j of a DM-wide row.  Shared rows are DM + 4
 // floats, so that 16 lanes reading float4s of 16 rows meet no bank twice.
 // fp32 throughout with the accurate expf / tanhf; bound by FMA issue and shared
@@ -173,53 +173,73 @@ int launch_delta(const CausalParams& p, cudaStream_t st) {
 // ---------------------------------------------------------------------------
 constexpr int NT = 256;
 
-template <int TM, int DM> struct Tile {
+template <int TM, int TN, int DM> struct Tile {
   static constexpr int RS = DM + 4;     // operand row stride
-  static constexpr int PS = TM + 4;     // score row stride
-  static constexpr int R = TM / 16;     // rows (and score columns) per thread
+  static constexpr int PS = TN + 4;     // score row stride
+  static constexpr int R = TM / 16;     // rows per thread
+  static constexpr int S = TN / 16;     // score columns per thread
   static constexpr int C = DM / 64;     // float4 output columns per thread
 };
 
-// rows [r0, r0 + TM) of head h of x, zeros outside [0, N) x [0, D)
-template <typename T, int TM, int DM>
-__device__ __forceinline__ void load_tile(float* s, const void* x, int64_t base, int64_t sn, int r0, int N, int D) {
+// Rows [r0, r0 + ROWS) of a head, zeros outside [0, N) x [0, D): fetched into
+// registers, so that the next tile's loads run under this one's products, and
+// put into shared memory.
+template <int ROWS, int DM> constexpr int kFetch = ROWS * DM / NT;
+template <typename T, int ROWS, int DM>
+__device__ __forceinline__ void fetch_tile(float* r, const void* x, int64_t base, int64_t sn, int r0, int N, int D) {
   const T* src = static_cast<const T*>(x) + base;
-  for (int i = threadIdx.x; i < TM * DM; i += NT) {
-    const int r = i / DM, d = i - r * DM;
-    s[r * Tile<TM, DM>::RS + d] = (r0 + r < N && d < D) ? to_f(src[(int64_t)(r0 + r) * sn + d]) : 0.f;
+#pragma unroll
+  for (int j = 0; j < kFetch<ROWS, DM>; ++j) {
+    const int i = threadIdx.x + j * NT, row = r0 + i / DM, d = i % DM;
+    r[j] = row < N && d < D ? to_f(src[(int64_t)row * sn + d]) : 0.f;
   }
+}
+template <int ROWS, int DM>
+__device__ __forceinline__ void put_tile(float* s, const float* r) {
+#pragma unroll
+  for (int j = 0; j < kFetch<ROWS, DM>; ++j) {
+    const int i = threadIdx.x + j * NT;
+    s[i / DM * (DM + 4) + i % DM] = r[j];
+  }
+}
+template <typename T, int ROWS, int DM>
+__device__ __forceinline__ void load_tile(float* s, const void* x, int64_t base, int64_t sn, int r0, int N, int D) {
+  float r[kFetch<ROWS, DM>];
+  fetch_tile<T, ROWS, DM>(r, x, base, sn, r0, N, D);
+  put_tile<ROWS, DM>(s, r);
 }
 
 // acc[i][j] = a row (ty + 16 i) . b row (tx + 16 j)
-template <int TM, int DM>
-__device__ __forceinline__ void dot_tile(const float* a, const float* b, int D, float (*acc)[Tile<TM, DM>::R]) {
-  using Z = Tile<TM, DM>;
+template <int TM, int TN, int DM>
+__device__ __forceinline__ void dot_tile(const float* a, const float* b, int D, float (*acc)[Tile<TM, TN, DM>::S]) {
+  using Z = Tile<TM, TN, DM>;
   const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
 #pragma unroll
   for (int i = 0; i < Z::R; ++i)
 #pragma unroll
-    for (int j = 0; j < Z::R; ++j) acc[i][j] = 0.f;
+    for (int j = 0; j < Z::S; ++j) acc[i][j] = 0.f;
+#pragma unroll TM == 32 ? 4 : 2
   for (int d = 0; d < D; d += 4) {
-    float4 x[Z::R], y[Z::R];
+    float4 x[Z::R], y[Z::S];
 #pragma unroll
-    for (int i = 0; i < Z::R; ++i) {
-      x[i] = *reinterpret_cast<const float4*>(a + (ty + 16 * i) * Z::RS + d);
-      y[i] = *reinterpret_cast<const float4*>(b + (tx + 16 * i) * Z::RS + d);
-    }
+    for (int i = 0; i < Z::R; ++i) x[i] = *reinterpret_cast<const float4*>(a + (ty + 16 * i) * Z::RS + d);
+#pragma unroll
+    for (int j = 0; j < Z::S; ++j) y[j] = *reinterpret_cast<const float4*>(b + (tx + 16 * j) * Z::RS + d);
 #pragma unroll
     for (int i = 0; i < Z::R; ++i)
 #pragma unroll
-      for (int j = 0; j < Z::R; ++j)
+      for (int j = 0; j < Z::S; ++j)
         acc[i][j] += x[i].x * y[j].x + x[i].y * y[j].y + x[i].z * y[j].z + x[i].w * y[j].w;
   }
 }
 
 // acc[i][j] += sum_c w[ty + 16 i][c] m[c][4 tx + 64 j ..]
-template <int TM, int DM>
-__device__ __forceinline__ void mul_tile(const float* w, const float* m, float4 (*acc)[Tile<TM, DM>::C]) {
-  using Z = Tile<TM, DM>;
+template <int TM, int TN, int DM>
+__device__ __forceinline__ void mul_tile(const float* w, const float* m, float4 (*acc)[Tile<TM, TN, DM>::C]) {
+  using Z = Tile<TM, TN, DM>;
   const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
-  for (int c = 0; c < TM; c += 4) {
+#pragma unroll TM == 32 ? 2 : 1
+  for (int c = 0; c < TN; c += 4) {
     float4 x[Z::R];
 #pragma unroll
     for (int i = 0; i < Z::R; ++i) x[i] = *reinterpret_cast<const float4*>(w + (ty + 16 * i) * Z::PS + c);
@@ -241,10 +261,10 @@ __device__ __forceinline__ void mul_tile(const float* w, const float* m, float4 
   }
 }
 
-template <typename T, int TM, int DM>
+template <typename T, int TM, int TN, int DM>
 __device__ __forceinline__ void store_rows(T* out, int64_t row_stride, int r0, int N, int D, float mul,
-                                           float4 (*acc)[Tile<TM, DM>::C]) {
-  using Z = Tile<TM, DM>;
+                                           float4 (*acc)[Tile<TM, TN, DM>::C]) {
+  using Z = Tile<TM, TN, DM>;
   const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
 #pragma unroll
   for (int i = 0; i < Z::R; ++i) {
@@ -262,13 +282,13 @@ __device__ __forceinline__ void store_rows(T* out, int64_t row_stride, int r0, i
   }
 }
 
-template <typename T, int TM, int DM>
+template <typename T, int TM, int TN, int DM>
 __global__ void __launch_bounds__(NT) fwd_cores(CausalParams p) {
-  using Z = Tile<TM, DM>;
+  using Z = Tile<TM, TN, DM>;
   extern __shared__ __align__(16) float sm[];
   float* q_s = sm;                   // [TM][RS]
-  float* kv_s = q_s + TM * Z::RS;    // keys, then values
-  float* p_s = kv_s + TM * Z::RS;    // [TM][PS]
+  float* kv_s = q_s + TM * Z::RS;    // [TN][RS] keys, then values
+  float* p_s = kv_s + TN * Z::RS;    // [TM][PS]
   const int q0 = (gridDim.x - 1 - blockIdx.x) * TM, hq = blockIdx.y, b = blockIdx.z, hkv = hq / p.E;
   const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
   load_tile<T, TM, DM>(q_s, p.q, b * p.q_sb + hq * p.q_sh, p.q_sn, q0, p.N, p.Dk);
@@ -284,19 +304,26 @@ __global__ void __launch_bounds__(NT) fwd_cores(CausalParams p) {
 #pragma unroll
     for (int j = 0; j < Z::C; ++j) o[i][j] = make_float4(0.f, 0.f, 0.f, 0.f);
   }
-  const int end = min(q0 + TM, p.N);
-  for (int k0 = first_key(p, b, q0) / TM * TM; k0 < end; k0 += TM) {
+  const int end = min(q0 + TM, p.N), begin = first_key(p, b, q0) / 16 * 16;
+  const int64_t kb = b * p.k_sb + hkv * p.k_sh, vb = b * p.v_sb + hkv * p.v_sh;
+  float kr[kFetch<TN, DM>], vr[kFetch<TN, DM>];
+  if (begin < end) {
+    fetch_tile<T, TN, DM>(kr, p.k, kb, p.k_sn, begin, p.N, p.Dk);
+    fetch_tile<T, TN, DM>(vr, p.v, vb, p.v_sn, begin, p.N, p.Dv);
+  }
+  for (int k0 = begin; k0 < end; k0 += TN) {
     __syncthreads();
-    load_tile<T, TM, DM>(kv_s, p.k, b * p.k_sb + hkv * p.k_sh, p.k_sn, k0, p.N, p.Dk);
+    put_tile<TN, DM>(kv_s, kr);
     __syncthreads();
-    float s[Z::R][Z::R];
-    dot_tile<TM, DM>(q_s, kv_s, p.Dk, s);
+    if (k0 + TN < end) fetch_tile<T, TN, DM>(kr, p.k, kb, p.k_sn, k0 + TN, p.N, p.Dk);
+    float s[Z::R][Z::S];
+    dot_tile<TM, TN, DM>(q_s, kv_s, p.Dk, s);
 #pragma unroll
     for (int i = 0; i < Z::R; ++i) {
       const int q = q0 + ty + 16 * i;
       float mx = -INFINITY;
 #pragma unroll
-      for (int j = 0; j < Z::R; ++j) {
+      for (int j = 0; j < Z::S; ++j) {
         const int k = k0 + tx + 16 * j;
         float x = s[i][j] * p.scale;
         if (p.has_cap) x = p.cap * tanhf(x / p.cap);
@@ -309,7 +336,7 @@ __global__ void __launch_bounds__(NT) fwd_cores(CausalParams p) {
       const float c = expf(m[i] - me);
       float sum = 0.f;
 #pragma unroll
-      for (int j = 0; j < Z::R; ++j) {
+      for (int j = 0; j < Z::S; ++j) {
         // a NaN score (a NaN in a visible key) stays one; a masked one is 0
         const float e = expf(s[i][j] - me);
         sum += e;
@@ -323,9 +350,10 @@ __global__ void __launch_bounds__(NT) fwd_cores(CausalParams p) {
       for (int j = 0; j < Z::C; ++j) o[i][j].x *= c, o[i][j].y *= c, o[i][j].z *= c, o[i][j].w *= c;
     }
     __syncthreads();
-    load_tile<T, TM, DM>(kv_s, p.v, b * p.v_sb + hkv * p.v_sh, p.v_sn, k0, p.N, p.Dv);
+    put_tile<TN, DM>(kv_s, vr);
     __syncthreads();
-    mul_tile<TM, DM>(p_s, kv_s, o);
+    if (k0 + TN < end) fetch_tile<T, TN, DM>(vr, p.v, vb, p.v_sn, k0 + TN, p.N, p.Dv);
+    mul_tile<TM, TN, DM>(p_s, kv_s, o);
   }
 #pragma unroll
   for (int i = 0; i < Z::R; ++i) {
@@ -336,7 +364,7 @@ __global__ void __launch_bounds__(NT) fwd_cores(CausalParams p) {
     if (tx == 0 && q < p.N)
       p.lse[((int64_t)b * p.N + q) * p.Hq + hq] = l[i] != 0.f ? m[i] + logf(l[i]) : -INFINITY;
   }
-  store_rows<T, TM, DM>(static_cast<T*>(p.out) + ((int64_t)b * p.N * p.Hq + hq) * p.Dv, (int64_t)p.Hq * p.Dv, q0, p.N,
+  store_rows<T, TM, TN, DM>(static_cast<T*>(p.out) + ((int64_t)b * p.N * p.Hq + hq) * p.Dv, (int64_t)p.Hq * p.Dv, q0, p.N,
                         p.Dv, 1.f, o);
 }
 
@@ -369,16 +397,15 @@ __device__ __forceinline__ void grad_of(const CausalParams& p, const RowStat& r,
   *dx = see ? *pr * (dp - r.delta) * g : 0.f;
 }
 
-template <typename T, int TM, int DM>
-__global__ void __launch_bounds__(NT) dq_cores(CausalParams p) {
-  using Z = Tile<TM, DM>;
-  extern __shared__ __align__(16) float sm[];
+template <typename T, int TM, int TN, int DM>
+__device__ __forceinline__ void dq_cores(const CausalParams& p, float* sm, int q0, int hq, int b) {
+  using Z = Tile<TM, TN, DM>;
   float* q_s = sm;
   float* g_s = q_s + TM * Z::RS;
   float* k_s = g_s + TM * Z::RS;
-  float* v_s = k_s + TM * Z::RS;
-  float* x_s = v_s + TM * Z::RS;
-  const int q0 = (gridDim.x - 1 - blockIdx.x) * TM, hq = blockIdx.y, b = blockIdx.z, hkv = hq / p.E;
+  float* v_s = k_s + TN * Z::RS;
+  float* x_s = v_s + TN * Z::RS;
+  const int hkv = hq / p.E;
   const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
   load_tile<T, TM, DM>(q_s, p.q, b * p.q_sb + hq * p.q_sh, p.q_sn, q0, p.N, p.Dk);
   load_tile<T, TM, DM>(g_s, p.dout, ((int64_t)b * p.N * p.Hq + hq) * p.Dv, (int64_t)p.Hq * p.Dv, q0, p.N, p.Dv);
@@ -390,44 +417,52 @@ __global__ void __launch_bounds__(NT) dq_cores(CausalParams p) {
 #pragma unroll
     for (int j = 0; j < Z::C; ++j) acc[i][j] = make_float4(0.f, 0.f, 0.f, 0.f);
   }
-  const int end = min(q0 + TM, p.N);
-  for (int k0 = first_key(p, b, q0) / TM * TM; k0 < end; k0 += TM) {
+  const int end = min(q0 + TM, p.N), begin = first_key(p, b, q0) / 16 * 16;
+  const int64_t kb = b * p.k_sb + hkv * p.k_sh, vb = b * p.v_sb + hkv * p.v_sh;
+  float kr[kFetch<TN, DM>], vr[kFetch<TN, DM>];
+  if (begin < end) {
+    fetch_tile<T, TN, DM>(kr, p.k, kb, p.k_sn, begin, p.N, p.Dk);
+    fetch_tile<T, TN, DM>(vr, p.v, vb, p.v_sn, begin, p.N, p.Dv);
+  }
+  for (int k0 = begin; k0 < end; k0 += TN) {
     __syncthreads();
-    load_tile<T, TM, DM>(k_s, p.k, b * p.k_sb + hkv * p.k_sh, p.k_sn, k0, p.N, p.Dk);
-    load_tile<T, TM, DM>(v_s, p.v, b * p.v_sb + hkv * p.v_sh, p.v_sn, k0, p.N, p.Dv);
+    put_tile<TN, DM>(k_s, kr);
+    put_tile<TN, DM>(v_s, vr);
     __syncthreads();
-    float s[Z::R][Z::R], d[Z::R][Z::R];
-    dot_tile<TM, DM>(q_s, k_s, p.Dk, s);
-    dot_tile<TM, DM>(g_s, v_s, p.Dv, d);
+    if (k0 + TN < end) {
+      fetch_tile<T, TN, DM>(kr, p.k, kb, p.k_sn, k0 + TN, p.N, p.Dk);
+      fetch_tile<T, TN, DM>(vr, p.v, vb, p.v_sn, k0 + TN, p.N, p.Dv);
+    }
+    float s[Z::R][Z::S], d[Z::R][Z::S];
+    dot_tile<TM, TN, DM>(q_s, k_s, p.Dk, s);
+    dot_tile<TM, TN, DM>(g_s, v_s, p.Dv, d);
 #pragma unroll
     for (int i = 0; i < Z::R; ++i)
 #pragma unroll
-      for (int j = 0; j < Z::R; ++j) {
+      for (int j = 0; j < Z::S; ++j) {
         float pr, dx;
         grad_of(p, st[i], k0 + tx + 16 * j, s[i][j], d[i][j], &pr, &dx);
         x_s[(ty + 16 * i) * Z::PS + tx + 16 * j] = dx;
       }
     __syncthreads();
-    mul_tile<TM, DM>(x_s, k_s, acc);
+    mul_tile<TM, TN, DM>(x_s, k_s, acc);
   }
-  store_rows<T, TM, DM>(static_cast<T*>(p.dq) + ((int64_t)b * p.N * p.Hq + hq) * p.Dk, (int64_t)p.Hq * p.Dk, q0, p.N,
+  store_rows<T, TM, TN, DM>(static_cast<T*>(p.dq) + ((int64_t)b * p.N * p.Hq + hq) * p.Dk, (int64_t)p.Hq * p.Dk, q0, p.N,
                         p.Dk, p.scale, acc);
 }
 
 // dK, dV of TM keys of one key head: the queries that see them, head by head of
 // the group, in order (no atomics: the sum's order is fixed).
-template <typename T, int TM, int DM>
-__global__ void __launch_bounds__(NT) dkv_cores(CausalParams p) {
-  using Z = Tile<TM, DM>;
-  extern __shared__ __align__(16) float sm[];
+template <typename T, int TM, int TN, int DM>
+__device__ __forceinline__ void dkv_cores(const CausalParams& p, float* sm, int k0, int hkv, int b) {
+  using Z = Tile<TM, TN, DM>;
   float* k_s = sm;
   float* v_s = k_s + TM * Z::RS;
   float* q_s = v_s + TM * Z::RS;
-  float* g_s = q_s + TM * Z::RS;
-  float* p_s = g_s + TM * Z::RS;
+  float* g_s = q_s + TN * Z::RS;
+  float* p_s = g_s + TN * Z::RS;
   float* x_s = p_s + TM * Z::PS;
-  __shared__ RowStat st_s[TM];
-  const int k0 = blockIdx.x * TM, hkv = blockIdx.y, b = blockIdx.z;
+  __shared__ RowStat st_s[TN];
   const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
   load_tile<T, TM, DM>(k_s, p.k, b * p.k_sb + hkv * p.k_sh, p.k_sn, k0, p.N, p.Dk);
   load_tile<T, TM, DM>(v_s, p.v, b * p.v_sb + hkv * p.v_sh, p.v_sn, k0, p.N, p.Dv);
@@ -436,36 +471,59 @@ __global__ void __launch_bounds__(NT) dkv_cores(CausalParams p) {
   for (int i = 0; i < Z::R; ++i)
 #pragma unroll
     for (int j = 0; j < Z::C; ++j) dk[i][j] = dv[i][j] = make_float4(0.f, 0.f, 0.f, 0.f);
-  const int end = query_end(p, b, min(k0 + TM, p.N) - 1);
+  const int end = query_end(p, b, min(k0 + TN, p.N) - 1);
+  float qr[kFetch<TN, DM>], gr[kFetch<TN, DM>];
+  auto fetch = [&](int hq, int q0) {
+    fetch_tile<T, TN, DM>(qr, p.q, b * p.q_sb + hq * p.q_sh, p.q_sn, q0, p.N, p.Dk);
+    fetch_tile<T, TN, DM>(gr, p.dout, ((int64_t)b * p.N * p.Hq + hq) * p.Dv, (int64_t)p.Hq * p.Dv, q0, p.N, p.Dv);
+  };
+  if (k0 < end) fetch(hkv * p.E, k0);
   for (int e = 0; e < p.E; ++e) {
     const int hq = hkv * p.E + e;
-    for (int q0 = k0; q0 < end; q0 += TM) {
+    for (int q0 = k0; q0 < end; q0 += TN) {
       __syncthreads();
-      load_tile<T, TM, DM>(q_s, p.q, b * p.q_sb + hq * p.q_sh, p.q_sn, q0, p.N, p.Dk);
-      load_tile<T, TM, DM>(g_s, p.dout, ((int64_t)b * p.N * p.Hq + hq) * p.Dv, (int64_t)p.Hq * p.Dv, q0, p.N, p.Dv);
-      if (threadIdx.x < TM) st_s[threadIdx.x] = row_stat(p, b, hq, q0 + threadIdx.x);
+      put_tile<TN, DM>(q_s, qr);
+      put_tile<TN, DM>(g_s, gr);
+      if (threadIdx.x < TN) st_s[threadIdx.x] = row_stat(p, b, hq, q0 + threadIdx.x);
       __syncthreads();
-      float s[Z::R][Z::R], d[Z::R][Z::R];
-      dot_tile<TM, DM>(k_s, q_s, p.Dk, s);
-      dot_tile<TM, DM>(v_s, g_s, p.Dv, d);
+      if (q0 + TN < end) fetch(hq, q0 + TN);
+      else if (e + 1 < p.E) fetch(hq + 1, k0);
+      float s[Z::R][Z::S], d[Z::R][Z::S];
+      dot_tile<TM, TN, DM>(k_s, q_s, p.Dk, s);
+      dot_tile<TM, TN, DM>(v_s, g_s, p.Dv, d);
 #pragma unroll
       for (int i = 0; i < Z::R; ++i)
 #pragma unroll
-        for (int j = 0; j < Z::R; ++j) {
+        for (int j = 0; j < Z::S; ++j) {
           float pr, dx;
           grad_of(p, st_s[tx + 16 * j], k0 + ty + 16 * i, s[i][j], d[i][j], &pr, &dx);
           p_s[(ty + 16 * i) * Z::PS + tx + 16 * j] = pr;
           x_s[(ty + 16 * i) * Z::PS + tx + 16 * j] = dx;
         }
       __syncthreads();
-      mul_tile<TM, DM>(p_s, g_s, dv);
-      mul_tile<TM, DM>(x_s, q_s, dk);
+      mul_tile<TM, TN, DM>(p_s, g_s, dv);
+      mul_tile<TM, TN, DM>(x_s, q_s, dk);
     }
   }
-  store_rows<T, TM, DM>(static_cast<T*>(p.dk) + ((int64_t)b * p.N * p.Hkv + hkv) * p.Dk, (int64_t)p.Hkv * p.Dk, k0, p.N,
+  store_rows<T, TM, TN, DM>(static_cast<T*>(p.dk) + ((int64_t)b * p.N * p.Hkv + hkv) * p.Dk, (int64_t)p.Hkv * p.Dk, k0, p.N,
                         p.Dk, p.scale, dk);
-  store_rows<T, TM, DM>(static_cast<T*>(p.dv) + ((int64_t)b * p.N * p.Hkv + hkv) * p.Dv, (int64_t)p.Hkv * p.Dv, k0, p.N,
+  store_rows<T, TM, TN, DM>(static_cast<T*>(p.dv) + ((int64_t)b * p.N * p.Hkv + hkv) * p.Dv, (int64_t)p.Hkv * p.Dv, k0, p.N,
                         p.Dv, 1.f, dv);
+}
+
+// Both passes in one launch, the dK/dV blocks first (they do four products a tile
+// to the other's three), each from its longest: a small problem's blocks of both
+// share the SMs.
+template <typename T, int TM, int TN, int DM>
+__global__ void __launch_bounds__(NT, TM == 32 && DM <= 64 ? 2 : 1) bwd_cores(const __grid_constant__ CausalParams p) {
+  extern __shared__ __align__(16) float sm[];
+  const int tiles = (p.N + TM - 1) / TM, x = blockIdx.x, b = blockIdx.y;
+  if (x < tiles * p.Hkv) {
+    dkv_cores<T, TM, TN, DM>(p, sm, x / p.Hkv * TM, x % p.Hkv, b);
+  } else {
+    const int y = x - tiles * p.Hkv;
+    dq_cores<T, TM, TN, DM>(p, sm, (tiles - 1 - y / p.Hq) * TM, y % p.Hq, b);
+  }
 }
 
 template <typename K>
@@ -476,34 +534,40 @@ int launch_cores(K kernel, dim3 grid, size_t smem, const CausalParams& p, cudaSt
   return launch_status();
 }
 
-template <typename T, int TM, int DM>
+template <typename T, int TM, int TN, int DM>
 int fwd_cores_launch(const CausalParams& p, cudaStream_t st) {
-  using Z = Tile<TM, DM>;
-  const size_t smem = sizeof(float) * (2 * TM * Z::RS + TM * Z::PS);
-  return launch_cores(fwd_cores<T, TM, DM>, dim3((p.N + TM - 1) / TM, p.Hq, p.B), smem, p, st);
+  using Z = Tile<TM, TN, DM>;
+  const size_t smem = sizeof(float) * ((TM + TN) * Z::RS + TM * Z::PS);
+  return launch_cores(fwd_cores<T, TM, TN, DM>, dim3((p.N + TM - 1) / TM, p.Hq, p.B), smem, p, st);
 }
-template <typename T, int TM, int DM>
+template <typename T, int TM, int TN, int DM>
 int bwd_cores_launch(const CausalParams& p, cudaStream_t st) {
-  using Z = Tile<TM, DM>;
-  const size_t sa = sizeof(float) * (4 * TM * Z::RS + TM * Z::PS), sb = sa + sizeof(float) * TM * Z::PS;
-  if (int rc = launch_cores(dq_cores<T, TM, DM>, dim3((p.N + TM - 1) / TM, p.Hq, p.B), sa, p, st)) return rc;
-  return launch_cores(dkv_cores<T, TM, DM>, dim3((p.N + TM - 1) / TM, p.Hkv, p.B), sb, p, st);
+  using Z = Tile<TM, TN, DM>;
+  const size_t smem = sizeof(float) * (2 * (TM + TN) * Z::RS + 2 * TM * Z::PS);
+  const int64_t blocks = (int64_t)((p.N + TM - 1) / TM) * (p.Hq + p.Hkv);
+  if (blocks > INT32_MAX) return TC_ERR_UNSUPPORTED;
+  return launch_cores(bwd_cores<T, TM, TN, DM>, dim3((unsigned)blocks, p.B), smem, p, st);
 }
 
-// 64 x 64 tiles while the operands of a head dim fit the shared memory.
+// 64 rows to a block where the blocks give every SM two, else 32 (and 64 columns:
+// fewer, longer steps).  4 heads of 64 and 1024 tokens, both directions: 553 us in
+// blocks of 64 (64 of them walk up to 16 tiles each on 148 SMs), 363 us in 32 x 32,
+// 308 us in 32 x 64, 262 us with both backward passes in one launch.
 template <typename T>
 int fwd_cores_any(const CausalParams& p, cudaStream_t st) {
   const int D = imax(p.Dk, p.Dv);
-  if (D <= 64) return fwd_cores_launch<T, 64, 64>(p, st);
-  if (D <= 128) return fwd_cores_launch<T, 64, 128>(p, st);
-  return fwd_cores_launch<T, 32, 256>(p, st);
+  const bool wide = (int64_t)((p.N + 63) / 64) * p.Hq * p.B >= 2 * 148;
+  if (D <= 64) return wide ? fwd_cores_launch<T, 64, 64, 64>(p, st) : fwd_cores_launch<T, 32, 64, 64>(p, st);
+  if (D <= 128) return wide ? fwd_cores_launch<T, 64, 64, 128>(p, st) : fwd_cores_launch<T, 32, 64, 128>(p, st);
+  return fwd_cores_launch<T, 32, 32, 256>(p, st);
 }
 template <typename T>
 int bwd_cores_any(const CausalParams& p, cudaStream_t st) {
   const int D = imax(p.Dk, p.Dv);
-  if (D <= 64) return bwd_cores_launch<T, 64, 64>(p, st);
-  if (D <= 128) return bwd_cores_launch<T, 64, 128>(p, st);
-  return bwd_cores_launch<T, 32, 256>(p, st);
+  const bool wide = (int64_t)((p.N + 63) / 64) * p.Hkv * p.B >= 2 * 148;
+  if (D <= 64) return wide ? bwd_cores_launch<T, 64, 64, 64>(p, st) : bwd_cores_launch<T, 32, 64, 64>(p, st);
+  if (D <= 128) return wide ? bwd_cores_launch<T, 64, 64, 128>(p, st) : bwd_cores_launch<T, 32, 64, 128>(p, st);
+  return bwd_cores_launch<T, 32, 32, 256>(p, st);
 }
 
 int make_params(const tc_causal_args* a, CausalParams* p) {
