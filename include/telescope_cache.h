@@ -621,8 +621,11 @@ typedef struct tc_causal_args {
   void* out;                 /* [B, N, Hq, Dv] dense                         */
   float* lse;                /* [B, N, Hq] natural log; -inf, out 0 for a
                                 token of no example                          */
+  void* out_low;             /* 16-bit types: what out's rounding left over,
+                                [B, N, Hq, Dv], or NULL                      */
   /* backward only */
   const void* o;             /* forward out, dense                           */
+  const void* o_low;         /* its out_low, or NULL: Delta from out alone   */
   const void* dout;          /* [B, N, Hq, Dv] dense                         */
   const float* dlse;         /* [B, N, Hq] or NULL                           */
   float* delta;              /* scratch [B, N, Hq]                           */

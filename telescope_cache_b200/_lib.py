@@ -130,7 +130,7 @@ class KVAttendArgs(ctypes.Structure):
 class CausalArgs(ctypes.Structure):
     _fields_ = _fields("i B N Hq Hkv Dk Dv dtype has_softcap; f softcap scale; p q; l q_stride_b q_stride_n q_stride_h;"
                        "p k; l k_stride_b k_stride_n k_stride_h; p v; l v_stride_b v_stride_n v_stride_h;"
-                       "p starts ends out lse o dout dlse delta dq dk dv dev_status; i impl")
+                       "p starts ends out lse out_low o o_low dout dlse delta dq dk dv dev_status; i impl")
 
 
 # (name, argtypes) of every exported symbol; the CPU test checks that each one

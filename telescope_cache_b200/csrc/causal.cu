@@ -122,7 +122,10 @@ __global__ void __launch_bounds__(kBoundThreads) bounds_kernel(int N, const int3
 }
 
 // ---------------------------------------------------------------------------
-// Delta = rowsum(dO * out) - dlse
+// Delta = rowsum(dO * out) - dlse, with out to twice its bits where its rounding's
+// leftovers were kept: the rounding of out alone puts an error of 2^-9 of a row's
+// |dO| |out| into every dX of the row (bf16, normal data: dQ off by 2.5e-3 of its
+// norm without, 2.3e-3 with, of which 1.7e-3 are its own rounding and as much dX's)
 // ---------------------------------------------------------------------------
 // LANES lanes per row, 16 bytes of dO and out each (LANES 0: a warp per row of
 // any length).  Bound by HBM.
@@ -135,12 +138,17 @@ __global__ void __launch_bounds__(256) delta_rows(CausalParams p, int64_t rows) 
   if (r < rows) {
     const T* o = static_cast<const T*>(p.o) + r * p.Dv;
     const T* g = static_cast<const T*>(p.dout) + r * p.Dv;
+    const T* low = p.o_low ? static_cast<const T*>(p.o_low) + r * p.Dv : nullptr;
     if constexpr (LANES) {
       const uint4 a = *reinterpret_cast<const uint4*>(o + lane * VE), c = *reinterpret_cast<const uint4*>(g + lane * VE);
+      uint4 r = make_uint4(0u, 0u, 0u, 0u);
+      if (low) r = *reinterpret_cast<const uint4*>(low + lane * VE);
 #pragma unroll
-      for (int i = 0; i < VE; ++i) s += to_f(reinterpret_cast<const T*>(&a)[i]) * to_f(reinterpret_cast<const T*>(&c)[i]);
+      for (int i = 0; i < VE; ++i)
+        s += (to_f(reinterpret_cast<const T*>(&a)[i]) + to_f(reinterpret_cast<const T*>(&r)[i])) *
+             to_f(reinterpret_cast<const T*>(&c)[i]);
     } else {
-      for (int d = lane; d < p.Dv; d += 32) s += to_f(o[d]) * to_f(g[d]);
+      for (int d = lane; d < p.Dv; d += 32) s += (to_f(o[d]) + (low ? to_f(low[d]) : 0.f)) * to_f(g[d]);
     }
   }
 #pragma unroll
@@ -151,7 +159,7 @@ __global__ void __launch_bounds__(256) delta_rows(CausalParams p, int64_t rows) 
 template <typename T>
 int launch_delta(const CausalParams& p, cudaStream_t st) {
   const int64_t rows = (int64_t)p.B * p.N * p.Hq;
-  const bool vec = (uintptr_t)p.o % 16 == 0 && (uintptr_t)p.dout % 16 == 0;
+  const bool vec = (uintptr_t)p.o % 16 == 0 && (uintptr_t)p.dout % 16 == 0 && (uintptr_t)p.o_low % 16 == 0;
   const int lanes = vec ? p.Dv * (int)sizeof(T) / 16 : 0;
   const bool fit = vec && p.Dv * (int)sizeof(T) % 16 == 0 && (lanes == 8 || lanes == 16 || lanes == 32);
   const int64_t grid = (rows * (fit ? lanes : 32) + 255) / 256;
@@ -263,7 +271,7 @@ __device__ __forceinline__ void mul_tile(const float* w, const float* m, float4 
 
 template <typename T, int TM, int TN, int DM>
 __device__ __forceinline__ void store_rows(T* out, int64_t row_stride, int r0, int N, int D, float mul,
-                                           float4 (*acc)[Tile<TM, TN, DM>::C]) {
+                                           float4 (*acc)[Tile<TM, TN, DM>::C], T* low = nullptr) {
   using Z = Tile<TM, TN, DM>;
   const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
 #pragma unroll
@@ -276,7 +284,10 @@ __device__ __forceinline__ void store_rows(T* out, int64_t row_stride, int r0, i
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const int d = 4 * tx + 64 * j + k;
-        if (d < D) out[(int64_t)r * row_stride + d] = from_f<T>(v[k] * mul);
+        if (d >= D) continue;
+        const T y = from_f<T>(v[k] * mul);
+        out[(int64_t)r * row_stride + d] = y;
+        if (low) low[(int64_t)r * row_stride + d] = from_f<T>(v[k] * mul - to_f(y));
       }
     }
   }
@@ -364,8 +375,9 @@ __global__ void __launch_bounds__(NT) fwd_cores(CausalParams p) {
     if (tx == 0 && q < p.N)
       p.lse[((int64_t)b * p.N + q) * p.Hq + hq] = l[i] != 0.f ? m[i] + logf(l[i]) : -INFINITY;
   }
-  store_rows<T, TM, TN, DM>(static_cast<T*>(p.out) + ((int64_t)b * p.N * p.Hq + hq) * p.Dv, (int64_t)p.Hq * p.Dv, q0, p.N,
-                        p.Dv, 1.f, o);
+  const int64_t at = ((int64_t)b * p.N * p.Hq + hq) * p.Dv;
+  store_rows<T, TM, TN, DM>(static_cast<T*>(p.out) + at, (int64_t)p.Hq * p.Dv, q0, p.N, p.Dv, 1.f, o,
+                            p.out_low ? static_cast<T*>(p.out_low) + at : nullptr);
 }
 
 // P and dX of a score tile whose rows are queries (ROWS_Q) or keys.
@@ -584,8 +596,8 @@ int make_params(const tc_causal_args* a, CausalParams* p) {
   p->k_sb = a->k_stride_b, p->k_sn = a->k_stride_n, p->k_sh = a->k_stride_h;
   p->v_sb = a->v_stride_b, p->v_sn = a->v_stride_n, p->v_sh = a->v_stride_h;
   p->starts = a->starts, p->ends = a->ends;
-  p->out = a->out, p->lse = a->lse;
-  p->o = a->o, p->dout = a->dout, p->dlse = a->dlse, p->delta = a->delta;
+  p->out = a->out, p->lse = a->lse, p->out_low = a->out_low;
+  p->o = a->o, p->o_low = a->o_low, p->dout = a->dout, p->dlse = a->dlse, p->delta = a->delta;
   p->dq = a->dq, p->dk = a->dk, p->dv = a->dv;
   p->status = a->dev_status;
   return TC_OK;

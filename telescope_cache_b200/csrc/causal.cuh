@@ -17,7 +17,9 @@ struct CausalParams {
   const int32_t* ends;
   void* out;
   float* lse;
+  void* out_low;
   const void* o;
+  const void* o_low;
   const void* dout;
   const float* dlse;
   float* delta;

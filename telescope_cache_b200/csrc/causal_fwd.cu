@@ -376,7 +376,9 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
     if (alive) {
       tc_fence_after();
       const float inv = ell != 0.f ? 1.f / ell : 0.f;
-      T* out = static_cast<T*>(c.out) + (((int64_t)b * c.N + q) * c.Hq + hq) * HD;
+      const int64_t at = (((int64_t)b * c.N + q) * c.Hq + hq) * HD;
+      T* out = static_cast<T*>(c.out) + at;
+      T* low = c.out_low ? static_cast<T*>(c.out_low) + at : nullptr;
 #pragma unroll 1
       for (int d = 0; d < HD; d += 32) {
         float ov[32];
@@ -392,6 +394,12 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
         if (row_ok) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(out + d + i * 8) = pack8<T>(ov + i * 8, inv);
+          if (low) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) ov[i] = ov[i] * inv - round_to<T>(ov[i] * inv);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(low + d + i * 8) = pack8<T>(ov + i * 8, 1.f);
+          }
         }
       }
       if (row_ok)

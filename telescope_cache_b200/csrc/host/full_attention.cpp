@@ -211,21 +211,28 @@ void causal_args(Causal& c, const Tensor& q, const Tensor& k, const Tensor& v, c
   a.impl = impl;
 }
 
-std::tuple<Tensor, Tensor> causal_forward(const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& seq,
+// keep_low: also what out's rounding left over (16-bit types), for the backward.
+std::tuple<Tensor, Tensor, OptTensor> causal_forward(const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& seq,
                                           const OptTensor& starts, const OptTensor& ends, std::optional<double> softcap,
-                                          std::optional<double> scale, int impl) {
+                                          std::optional<double> scale, int impl, bool keep_low) {
   Causal c;
   causal_args(c, q, k, v, seq, starts, ends, softcap, scale, impl);
   Call call(q);
   Tensor out = at::empty({q.size(0), q.size(1), q.size(2), v.size(3)}, q.options());
   Tensor lse = at::empty({q.size(0), q.size(1), q.size(2)}, q.options().dtype(at::kFloat));
   c.a.out = out.data_ptr(), c.a.lse = lse.data_ptr<float>();
+  Tensor low;
+  if (keep_low && q.scalar_type() != at::kFloat) {
+    low = at::empty(out.sizes(), out.options());
+    c.a.out_low = low.data_ptr();
+  }
   done(tc_causal_fwd(&c.a, call.stream), "tc_causal_fwd");
-  return {out, lse};
+  return {out, lse, low.defined() ? OptTensor(low) : std::nullopt};
 }
 
 std::tuple<Tensor, Tensor, Tensor> causal_backward(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& out0,
-                                                   const Tensor& lse0, const Tensor& dout0, const OptTensor& dlse0,
+                                                   const OptTensor& low0, const Tensor& lse0, const Tensor& dout0,
+                                                   const OptTensor& dlse0,
                                                    const OptTensor& seq, const OptTensor& starts, const OptTensor& ends,
                                                    std::optional<double> softcap, std::optional<double> scale, int impl) {
   Causal c;
@@ -241,17 +248,21 @@ std::tuple<Tensor, Tensor, Tensor> causal_backward(const Tensor& q, const Tensor
   CHECK_VALUE(lse0.sizes() == rows && lse0.scalar_type() == at::kFloat, "lse must be float32 [B, N, Hq]");
   CHECK_VALUE(!dlse0 || (dlse0->sizes() == rows && dlse0->is_floating_point()), "dlse must be floating [", B, ", ", N,
                     ", ", Hq, "], got ", dlse0 ? dlse0->sizes() : rows);
+  CHECK_VALUE(!low0 || (low0->sizes() == out0.sizes() && low0->scalar_type() == out0.scalar_type()), "out_low ",
+              low0 ? low0->sizes() : rows, " must match out ", out0.sizes());
   same_device(q, out0);
+  if (low0) same_device(q, *low0);
   same_device(q, dout0);
   same_device(q, lse0);
   if (dlse0) same_device(q, *dlse0);
   Call call(q);
   const Tensor out = out0.contiguous(), lse = lse0.contiguous(), dout = dout0.contiguous();
-  Tensor dlse;
+  Tensor dlse, low;
   if (dlse0) dlse = table(*dlse0);
+  if (low0) low = low0->contiguous();
   Tensor delta = at::empty(rows, q.options().dtype(at::kFloat));
   Tensor dq = at::empty(q.sizes(), q.options()), dk = at::empty(k.sizes(), q.options()), dv = at::empty(v.sizes(), q.options());
-  c.a.lse = lse.data_ptr<float>(), c.a.o = out.data_ptr(), c.a.dout = dout.data_ptr();
+  c.a.lse = lse.data_ptr<float>(), c.a.o = out.data_ptr(), c.a.o_low = low.defined() ? low.data_ptr() : nullptr, c.a.dout = dout.data_ptr();
   c.a.dlse = dlse.defined() ? dlse.data_ptr<float>() : nullptr;
   c.a.delta = delta.data_ptr<float>(), c.a.dq = dq.data_ptr(), c.a.dk = dk.data_ptr(), c.a.dv = dv.data_ptr();
   done(tc_causal_bwd(&c.a, call.stream), "tc_causal_bwd");

@@ -45,19 +45,19 @@ def _split(seq_idx):
 class _Causal(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, starts, ends, softcap, scale, impl):
-        out, lse = _lib.host(q).causal_forward(q, k, v, None, starts, ends, softcap, scale, impl)
-        ctx.save_for_backward(q, k, v, out, lse, starts, ends)
+        out, lse, low = _lib.host(q).causal_forward(q, k, v, None, starts, ends, softcap, scale, impl, True)
+        ctx.save_for_backward(q, k, v, out, low, lse, starts, ends)
         ctx.cfg = (softcap, scale, impl)
         ctx.set_materialize_grads(False)
         return out, lse
 
     @staticmethod
     def backward(ctx, dout, dlse):
-        q, k, v, out, lse, starts, ends = ctx.saved_tensors
+        q, k, v, out, low, lse, starts, ends = ctx.saved_tensors
         if dout is None and dlse is None:
             return (None,) * 8
         dout = torch.zeros_like(out) if dout is None else dout.to(out.dtype)
-        return _lib.host(q).causal_backward(q, k, v, out, lse, dout, dlse, None, starts, ends, *ctx.cfg) + (None,) * 5
+        return _lib.host(q).causal_backward(q, k, v, out, low, lse, dout, dlse, None, starts, ends, *ctx.cfg) + (None,) * 5
 
 
 def causal_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *,
@@ -73,7 +73,8 @@ def causal_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *,
     (out 0, lse -inf, zero gradients).  The bounds of segment_bounds may be
     given in its place, so that the layers of a model form them once.
 
-    Differentiable in q, k, v through both results.  bf16 / f16 with Dk = Dv of
+    Differentiable in q, k, v through both results (for 16-bit types the graph also
+    keeps what the rounding of out left over, a tensor of its size).  bf16 / f16 with Dk = Dv of
     64 or 128 run on the tensor cores (strided q, k, v in place where strides
     and addresses are multiples of 16 bytes), other types and head dims up to
     256 on the CUDA cores.  Products with tokens outside a row's view are formed
@@ -86,7 +87,7 @@ def causal_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *,
             seq_idx = segment_bounds(seq_idx)  # once for both directions
         _, starts, ends = _split(seq_idx)
         return _Causal.apply(q, k, v, starts, ends, softcap, scale, code)
-    return _lib.host(q).causal_forward(q, k, v, *_split(seq_idx), softcap, scale, code)
+    return _lib.host(q).causal_forward(q, k, v, *_split(seq_idx), softcap, scale, code, False)[:2]
 
 
 @torch.no_grad()
@@ -95,8 +96,10 @@ def causal_attention_backward(q, k, v, out, lse, dout, *, dlse: Optional[torch.T
                               scale: Optional[float] = None, impl: Optional[str] = None):
     """(dq, dk, dv) at the (out, lse) boundary of causal_attention, with the
     gradient of lse folded into Delta (the seam that attention_sink_backward
-    feeds).  Bit-for-bit repeatable."""
-    return _lib.host(q).causal_backward(q, k, v, out, lse, dout, dlse, *_split(seq_idx), softcap, scale, _impl_code(impl))
+    feeds); Delta is taken from the rounded out, where autograd has its leftovers
+    too.  Bit-for-bit repeatable."""
+    return _lib.host(q).causal_backward(q, k, v, out, None, lse, dout, dlse, *_split(seq_idx), softcap, scale,
+                                        _impl_code(impl))
 
 
 __all__ = ["Segments", "segment_bounds", "causal_attention", "causal_attention_backward"]

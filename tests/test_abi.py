@@ -78,7 +78,7 @@ def test_tree_bwd_scratch_plan():
 def test_full_attention_structs_and_bad_arguments():
     """Sizes as a C compiler lays the header's structs out (LP64), and refusals
     before any launch."""
-    sizes = dict(RotaryArgs=152, KVCacheArgs=64, KVWriteArgs=104, KVAttendArgs=216, CausalArgs=240)
+    sizes = dict(RotaryArgs=152, KVCacheArgs=64, KVWriteArgs=104, KVAttendArgs=216, CausalArgs=256)
     assert {n: ctypes.sizeof(getattr(_lib, n)) for n in sizes} == sizes
     lib = _lib.lib()
     assert lib.tc_rotary(None, None) == _lib.TC_ERR_ARG

@@ -90,14 +90,14 @@ def test_host_extension_checks_shapes_first():
             h.rotary(*args, None, False, False)
     for args in ((q[0], k, k), (q, k[:1], k[:1]), (q, k, k[:, :, :1]), (q[:, :, :3], k, k), (q, k.half(), k)):
         with pytest.raises(ValueError):
-            h.causal_forward(*args, None, None, None, None, None, 0)
+            h.causal_forward(*args, None, None, None, None, None, 0, False)
     with pytest.raises(ValueError, match="softcap"):
-        h.causal_forward(q, k, k, None, None, None, -1.0, None, 0)
+        h.causal_forward(q, k, k, None, None, None, -1.0, None, 0, False)
     for seq in (torch.zeros(2, 4), torch.zeros(4, dtype=torch.int32)):
         with pytest.raises(ValueError):
             h.segment_bounds(seq)
     with pytest.raises(RuntimeError, match="no CPU fallback"):
-        h.causal_forward(q, k, k, None, None, None, None, None, 0)
+        h.causal_forward(q, k, k, None, None, None, None, None, 0, False)
 
 
 def test_layer_parameters():

@@ -123,9 +123,14 @@ def test_gradients(dtype, B, N, Hq, Hkv, Dk, Dv, softcap):
     x = [t.detach().double().requires_grad_() for t in (q, k, v)]
     o, l, _, _ = causal(*x, visible(None, B, N, "cuda"), softcap, 0.11)
     want = torch.autograd.grad((o * gout.double()).sum() + (l * glse.double()).sum(), x)
-    check_grads(got, want, gradient_terms(q, k, v, visible(None, B, N, "cuda"), gout, glse, softcap, 0.11), dt)
-    for a, c in zip(got, explicit):
-        assert torch.equal(a, c)  # and the same bits from call to call
+    terms = gradient_terms(q, k, v, visible(None, B, N, "cuda"), gout, glse, softcap, 0.11)
+    check_grads(got, want, terms, dt)
+    check_grads(explicit, want, terms, dt)  # from the rounded out alone
+    # and the same bits from call to call
+    for a, c in zip(explicit, causal_attention_backward(q, k, v, out, lse, gout, dlse=glse, softcap=softcap, scale=0.11)):
+        assert torch.equal(a, c)
+    for a, c in zip(got, torch.autograd.grad(causal_attention(q, k, v, softcap=softcap, scale=0.11), (q, k, v), (gout, glse))):
+        assert torch.equal(a, c)
 
 
 def test_gradients_against_differences():
