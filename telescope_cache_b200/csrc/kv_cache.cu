@@ -122,6 +122,30 @@ __device__ __forceinline__ uint4 pack16(const float* x) {
     return tcx::pack8<T>(x, 1.f);
 }
 
+// Largest |x| of the 16 bytes of w, as the bits of its type (16-bit types: two to
+// a register, joined at the end), and as float bits.
+template <typename T>
+__device__ __forceinline__ uint32_t amax16(const uint4& w) {
+  if constexpr (std::is_same<T, float>::value) {
+    const uint32_t m = 0x7fffffffu;
+    return max(max(w.x & m, w.y & m), max(w.z & m, w.w & m));
+  } else {
+    const uint32_t m = 0x7fff7fffu;
+    return __vmaxu2(__vmaxu2(w.x & m, w.y & m), __vmaxu2(w.z & m, w.w & m));
+  }
+}
+template <typename T>
+__device__ __forceinline__ uint32_t amax_join(uint32_t a, uint32_t b) {
+  return std::is_same<T, float>::value ? max(a, b) : __vmaxu2(a, b);
+}
+template <typename T>
+__device__ __forceinline__ float amax_float(uint32_t a) {
+  if constexpr (std::is_same<T, float>::value) return __uint_as_float(a);
+  const uint32_t h = max(a & 0xffffu, a >> 16);
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) return __uint_as_float(h << 16);
+  return __half2float(__ushort_as_half((unsigned short)h));
+}
+
 // |x| as bits: ordered as the floats are, with every NaN above infinity.
 __device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 
@@ -205,7 +229,7 @@ __global__ void __launch_bounds__(256) advance_kernel(WriteParams p) {
 // lane group takes kTok consecutive tokens of one head: lane j finds token j's
 // place, then kTok loads a lane are in flight (tokens without a place load
 // nothing).
-constexpr int kTok = 8;
+constexpr int kTok = 4;
 template <typename T, int STORE, int LANES>
 __global__ void __launch_bounds__(256) write_vec(const __grid_constant__ WriteParams p) {
   constexpr int VE = 16 / sizeof(T);
@@ -216,43 +240,42 @@ __global__ void __launch_bounds__(256) write_vec(const __grid_constant__ WritePa
   const int tile = group / p.H, h = group - tile * p.H, n0 = tile * kTok;
   if (n0 >= p.N) return;  // whole lane groups leave; the shuffles below name their own lanes
   const uint32_t mask = LANES == 32 ? 0xffffffffu : ((1u << LANES) - 1u) << ((threadIdx.x & 31) / LANES * LANES);
-  int64_t at = -1;  // lane j: row of codes of token n0 + j
+  // lane j: row of codes of token n0 + j (rows of 64 or more bytes: 32 bits count
+  // more of them than the memory holds)
+  uint32_t at = 0xffffffffu;
   if (lane < kTok && n0 + lane < p.N) {
     int row;
     int64_t slot = 0;
     place(p, b, n0 + lane, &row, &slot);
-    if (row >= 0) at = ((int64_t)row * p.H + h) * p.cap + slot;
+    if (row >= 0) at = (uint32_t)(((int64_t)row * p.H + h) * p.cap + slot);
     if (p.fresh && keys && h == 0) advance_row(p, b, n0 + lane);
   }
   const T* src = static_cast<const T*>(w.src) + b * w.sb + h * w.sh + lane * VE;
   uint4 raw[kTok];
-  int64_t to[kTok];
+  uint32_t to[kTok];
   float mine = 0.f;  // lane j: token j's scale, so that they leave in one store
 #pragma unroll
   for (int j = 0; j < kTok; ++j) {
     to[j] = __shfl_sync(mask, at, j, LANES);
-    if (to[j] >= 0) raw[j] = *reinterpret_cast<const uint4*>(src + (int64_t)(n0 + j) * w.sn);
+    if (to[j] != 0xffffffffu) raw[j] = *reinterpret_cast<const uint4*>(src + (int64_t)(n0 + j) * w.sn);
   }
 #pragma unroll
   for (int j = 0; j < kTok; ++j) {
-    if (to[j] < 0) continue;
-    float x[VE];
+    if (to[j] == 0xffffffffu) continue;
+    uint32_t m = amax16<T>(raw[j]);
+#pragma unroll
+    for (int o = LANES / 2; o; o >>= 1) m = amax_join<T>(m, __shfl_xor_sync(mask, m, o));
+    float scale, inv, x[VE];
+    row_scale<STORE>(amax_float<T>(m), &scale, &inv);
     unpack16<T>(raw[j], x);
-    uint32_t m = 0;
-#pragma unroll
-    for (int i = 0; i < VE; ++i) m = max(m, abs_bits(x[i]));
-#pragma unroll
-    for (int o = LANES / 2; o; o >>= 1) m = max(m, __shfl_xor_sync(mask, m, o));
-    float scale, inv;
-    row_scale<STORE>(__uint_as_float(m), &scale, &inv);
 #pragma unroll
     for (int i = 0; i < VE; ++i) x[i] = __fmul_rn(x[i], inv);
-    uint8_t* dst = w.codes + to[j] * (LANES * VE) + lane * VE;
+    uint8_t* dst = w.codes + (int64_t)to[j] * (LANES * VE) + lane * VE;
     if constexpr (VE == 8) *reinterpret_cast<uint2*>(dst) = make_uint2(Codec<STORE>::code4(x), Codec<STORE>::code4(x + 4));
     else *reinterpret_cast<uint32_t*>(dst) = Codec<STORE>::code4(x);
     if (lane == j) mine = scale;
   }
-  if (at >= 0) w.scales[at] = mine;
+  if (at != 0xffffffffu) w.scales[at] = mine;
 }
 
 // Any head dim and strides: a warp per row, two passes over it.
