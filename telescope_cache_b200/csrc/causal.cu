@@ -172,67 +172,116 @@ int launch_delta(const CausalParams& p, cudaStream_t st) {
 }
 
 // ---------------------------------------------------------------------------
-// CUDA-core tiles: 256 threads as 16 x 16; thread (ty, tx) owns rows ty + 16 i
-// and columns tx + 16 j of a TM x TN score tile, and output rows ty + 16 i with
-// the four-wide columns 4 tx + 64 j of a DM-wide row.  Shared rows are DM + 4
-// floats, so that 16 lanes reading float4s of 16 rows meet no bank twice.
-// fp32 throughout with the accurate expf / tanhf; bound by FMA issue and shared
-// memory reads (8 float4 loads for 64 multiply-adds of a thread's 4 x 4 scores).
+// CUDA-core tiles.  A group of GT threads (16 across) works a TM x TN score tile:
+// thread (ty, tx) owns its rows ty + GT/16 i and columns tx + 16 j, and output rows
+// ty + GT/16 i with the four-wide columns 4 tx + 64 j of a DM-wide row.  Shared
+// rows are DM + 4 floats, so that 16 lanes reading float4s of 16 rows meet no bank
+// twice.  fp32 throughout with the accurate expf / tanhf.
+//
+// A CTA's G groups take the tiles of its block in turn, each with operands, a
+// barrier and sums of its own, and the first one joins them at the end in the order
+// of the groups: one group's products run while another loads or waits.  Bound by
+// FMA issue and shared memory reads: 12 wavefronts of float4 reads for a warp's 64
+// multiply-adds of 4 x 4 scores a thread (2 x 4: 10 for 32).  8.5 ms = 57 TFLOP/s
+// for the backward of 32 heads of 64 and 4096 tokens (seven products of a triangle).
 // ---------------------------------------------------------------------------
-constexpr int NT = 256;
-
-template <int TM, int TN, int DM> struct Tile {
+template <int TM_, int TN_, int DM_, int GT_, int G_> struct Tile {
+  static constexpr int TM = TM_, TN = TN_, DM = DM_, GT = GT_, G = G_;
   static constexpr int RS = DM + 4;     // operand row stride
   static constexpr int PS = TN + 4;     // score row stride
-  static constexpr int R = TM / 16;     // rows per thread
+  static constexpr int RW = GT / 16;    // rows a step of i covers
+  static constexpr int R = TM / RW;     // rows per thread
   static constexpr int S = TN / 16;     // score columns per thread
   static constexpr int C = DM / 64;     // float4 output columns per thread
+  static constexpr int NT = GT * G;
+  static constexpr int kFetch = TN * DM / GT;  // elements of an operand tile per thread
+  // floats of shared memory: of the CTA, and of each group
+  static constexpr int fwd_all() { return TM * RS; }
+  static constexpr int fwd_group() { return TN * RS + TM * PS; }
+  static constexpr int bwd_all() { return 2 * TM * RS; }
+  static constexpr int bwd_group() { return 2 * TN * RS + 2 * TM * PS; }
 };
 
-// Rows [r0, r0 + ROWS) of a head, zeros outside [0, N) x [0, D): fetched into
-// registers, so that the next tile's loads run under this one's products, and
-// put into shared memory.
-template <int ROWS, int DM> constexpr int kFetch = ROWS * DM / NT;
-template <typename T, int ROWS, int DM>
-__device__ __forceinline__ void fetch_tile(float* r, const void* x, int64_t base, int64_t sn, int r0, int N, int D) {
-  const T* src = static_cast<const T*>(x) + base;
-#pragma unroll
-  for (int j = 0; j < kFetch<ROWS, DM>; ++j) {
-    const int i = threadIdx.x + j * NT, row = r0 + i / DM, d = i % DM;
-    r[j] = row < N && d < D ? to_f(src[(int64_t)row * sn + d]) : 0.f;
-  }
+struct Place {
+  int g, t, ty, tx;  // group, thread in it, its row and column
+};
+template <typename Z>
+__device__ __forceinline__ Place place() {
+  const int t = threadIdx.x % Z::GT;
+  return {(int)threadIdx.x / Z::GT, t, t >> 4, t & 15};
 }
-template <int ROWS, int DM>
-__device__ __forceinline__ void put_tile(float* s, const float* r) {
-#pragma unroll
-  for (int j = 0; j < kFetch<ROWS, DM>; ++j) {
-    const int i = threadIdx.x + j * NT;
-    s[i / DM * (DM + 4) + i % DM] = r[j];
-  }
-}
-template <typename T, int ROWS, int DM>
-__device__ __forceinline__ void load_tile(float* s, const void* x, int64_t base, int64_t sn, int r0, int N, int D) {
-  float r[kFetch<ROWS, DM>];
-  fetch_tile<T, ROWS, DM>(r, x, base, sn, r0, N, D);
-  put_tile<ROWS, DM>(s, r);
+template <typename Z>
+__device__ __forceinline__ void group_sync(int g) {
+  if constexpr (Z::G == 1) __syncthreads();
+  else asm volatile("bar.sync %0, %1;" ::"r"(1 + g), "n"(Z::GT) : "memory");
 }
 
-// acc[i][j] = a row (ty + 16 i) . b row (tx + 16 j)
-template <int TM, int TN, int DM>
-__device__ __forceinline__ void dot_tile(const float* a, const float* b, int D, float (*acc)[Tile<TM, TN, DM>::S]) {
-  using Z = Tile<TM, TN, DM>;
-  const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
+// Elements d .. d + 3 of a D-element row, zeros past its end (and for a row that is
+// not there); vec: rows start on 4 elements and are a multiple of 4 long.
+template <typename T>
+__device__ __forceinline__ float4 load4(const T* x, int d, int D, bool there, bool vec) {
+  float v[4] = {0.f, 0.f, 0.f, 0.f};
+  if (vec) {
+    if (there && d < D) {
+      using Raw = typename std::conditional<sizeof(T) == 4, uint4, uint2>::type;
+      const Raw r = *reinterpret_cast<const Raw*>(x + d);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = to_f(reinterpret_cast<const T*>(&r)[i]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (there && d + i < D) v[i] = to_f(x[d + i]);
+  }
+  return make_float4(v[0], v[1], v[2], v[3]);
+}
+
+// Rows [r0, r0 + ROWS) of a head, zeros outside [0, N) x [0, D), by THREADS threads.
+// fetch_tile and put_tile: into registers, so that the loads run under products, and
+// from there into shared memory.
+template <typename T, typename Z>
+__device__ __forceinline__ void fetch_tile(float4* r, const void* x, int64_t base, int64_t sn, int r0, int N, int D, int t,
+                                           bool vec) {
+  const T* src = static_cast<const T*>(x) + base;
+#pragma unroll
+  for (int j = 0; j < Z::kFetch / 4; ++j) {
+    const int i = (t + j * Z::GT) * 4, row = r0 + i / Z::DM;
+    r[j] = load4<T>(src + (int64_t)row * sn, i % Z::DM, D, row < N, vec);
+  }
+}
+template <typename Z>
+__device__ __forceinline__ void put_tile(float* s, const float4* r, int t) {
+#pragma unroll
+  for (int j = 0; j < Z::kFetch / 4; ++j) {
+    const int i = (t + j * Z::GT) * 4;
+    *reinterpret_cast<float4*>(s + i / Z::DM * Z::RS + i % Z::DM) = r[j];
+  }
+}
+template <typename T, int ROWS, int DM, int THREADS>
+__device__ __forceinline__ void load_tile(float* s, const void* x, int64_t base, int64_t sn, int r0, int N, int D, int t,
+                                          bool vec) {
+  const T* src = static_cast<const T*>(x) + base;
+#pragma unroll 8
+  for (int i = 4 * t; i < ROWS * DM; i += 4 * THREADS) {
+    const int row = r0 + i / DM, d = i % DM;
+    *reinterpret_cast<float4*>(s + i / DM * (DM + 4) + d) = load4<T>(src + (int64_t)row * sn, d, D, row < N, vec);
+  }
+}
+
+// acc[i][j] = a row (ty + RW i) . b row (tx + 16 j)
+template <typename Z>
+__device__ __forceinline__ void dot_tile(const float* a, const float* b, int D, const Place& w, float (*acc)[Z::S]) {
 #pragma unroll
   for (int i = 0; i < Z::R; ++i)
 #pragma unroll
     for (int j = 0; j < Z::S; ++j) acc[i][j] = 0.f;
-#pragma unroll TM == 32 ? 4 : 2
+#pragma unroll 2
   for (int d = 0; d < D; d += 4) {
     float4 x[Z::R], y[Z::S];
 #pragma unroll
-    for (int i = 0; i < Z::R; ++i) x[i] = *reinterpret_cast<const float4*>(a + (ty + 16 * i) * Z::RS + d);
+    for (int i = 0; i < Z::R; ++i) x[i] = *reinterpret_cast<const float4*>(a + (w.ty + Z::RW * i) * Z::RS + d);
 #pragma unroll
-    for (int j = 0; j < Z::S; ++j) y[j] = *reinterpret_cast<const float4*>(b + (tx + 16 * j) * Z::RS + d);
+    for (int j = 0; j < Z::S; ++j) y[j] = *reinterpret_cast<const float4*>(b + (w.tx + 16 * j) * Z::RS + d);
 #pragma unroll
     for (int i = 0; i < Z::R; ++i)
 #pragma unroll
@@ -241,49 +290,84 @@ __device__ __forceinline__ void dot_tile(const float* a, const float* b, int D, 
   }
 }
 
-// acc[i][j] += sum_c w[ty + 16 i][c] m[c][4 tx + 64 j ..]
-template <int TM, int TN, int DM>
-__device__ __forceinline__ void mul_tile(const float* w, const float* m, float4 (*acc)[Tile<TM, TN, DM>::C]) {
-  using Z = Tile<TM, TN, DM>;
-  const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
-#pragma unroll TM == 32 ? 2 : 1
-  for (int c = 0; c < TN; c += 4) {
+// acc[i][j] += sum_c f[ty + RW i][c] m[c][4 tx + 64 j ..]
+template <typename Z>
+__device__ __forceinline__ void mul_tile(const float* f, const float* m, const Place& w, float4 (*acc)[Z::C]) {
+#pragma unroll 1
+  for (int c = 0; c < Z::TN; c += 4) {
     float4 x[Z::R];
 #pragma unroll
-    for (int i = 0; i < Z::R; ++i) x[i] = *reinterpret_cast<const float4*>(w + (ty + 16 * i) * Z::PS + c);
+    for (int i = 0; i < Z::R; ++i) x[i] = *reinterpret_cast<const float4*>(f + (w.ty + Z::RW * i) * Z::PS + c);
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
 #pragma unroll
       for (int j = 0; j < Z::C; ++j) {
-        const float4 y = *reinterpret_cast<const float4*>(m + (c + k) * Z::RS + 4 * tx + 64 * j);
+        const float4 y = *reinterpret_cast<const float4*>(m + (c + k) * Z::RS + 4 * w.tx + 64 * j);
 #pragma unroll
         for (int i = 0; i < Z::R; ++i) {
-          const float f = k == 0 ? x[i].x : k == 1 ? x[i].y : k == 2 ? x[i].z : x[i].w;
-          acc[i][j].x += f * y.x;
-          acc[i][j].y += f * y.y;
-          acc[i][j].z += f * y.z;
-          acc[i][j].w += f * y.w;
+          const float e = k == 0 ? x[i].x : k == 1 ? x[i].y : k == 2 ? x[i].z : x[i].w;
+          acc[i][j].x += e * y.x;
+          acc[i][j].y += e * y.y;
+          acc[i][j].z += e * y.z;
+          acc[i][j].w += e * y.w;
         }
       }
     }
   }
 }
 
-template <typename T, int TM, int TN, int DM>
-__device__ __forceinline__ void store_rows(T* out, int64_t row_stride, int r0, int N, int D, float mul,
-                                           float4 (*acc)[Tile<TM, TN, DM>::C], T* low = nullptr) {
-  using Z = Tile<TM, TN, DM>;
-  const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
+// Group g > 0 leaves `n` floats a thread in its own shared memory; behind a CTA
+// barrier the first group reads them: value i of thread t at [i][t].
+template <typename Z>
+__device__ __forceinline__ float& left(float* group, int i, int t) { return group[i * Z::GT + t]; }
+
+// Adds the other groups' acc to the first's, in order.  true: this thread is in
+// the first group.
+template <typename Z, int PER>
+__device__ __forceinline__ bool join_sums(float* groups, int stride, const Place& w, float4 (*acc)[Z::C], int at) {
+  if constexpr (Z::G > 1) {
+    static_assert((PER + 1) * Z::R * Z::C * 4 * Z::GT <= Z::bwd_group(), "sums fit the group's operands");
+    if (w.g > 0) {
+      float* s = groups + w.g * stride;
+#pragma unroll
+      for (int i = 0; i < Z::R; ++i)
+#pragma unroll
+        for (int j = 0; j < Z::C; ++j) {
+          const int k = at + (i * Z::C + j) * 4;
+          left<Z>(s, k, w.t) = acc[i][j].x, left<Z>(s, k + 1, w.t) = acc[i][j].y;
+          left<Z>(s, k + 2, w.t) = acc[i][j].z, left<Z>(s, k + 3, w.t) = acc[i][j].w;
+        }
+    }
+    __syncthreads();
+    if (w.g > 0) return false;
+    for (int g = 1; g < Z::G; ++g) {
+      float* s = groups + g * stride;
+#pragma unroll
+      for (int i = 0; i < Z::R; ++i)
+#pragma unroll
+        for (int j = 0; j < Z::C; ++j) {
+          const int k = at + (i * Z::C + j) * 4;
+          acc[i][j].x += left<Z>(s, k, w.t), acc[i][j].y += left<Z>(s, k + 1, w.t);
+          acc[i][j].z += left<Z>(s, k + 2, w.t), acc[i][j].w += left<Z>(s, k + 3, w.t);
+        }
+    }
+  }
+  return true;
+}
+
+template <typename T, typename Z>
+__device__ __forceinline__ void store_rows(T* out, int64_t row_stride, int r0, int N, int D, float mul, const Place& w,
+                                           float4 (*acc)[Z::C], T* low = nullptr) {
 #pragma unroll
   for (int i = 0; i < Z::R; ++i) {
-    const int r = r0 + ty + 16 * i;
+    const int r = r0 + w.ty + Z::RW * i;
     if (r >= N) continue;
 #pragma unroll
     for (int j = 0; j < Z::C; ++j) {
       const float v[4] = {acc[i][j].x, acc[i][j].y, acc[i][j].z, acc[i][j].w};
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        const int d = 4 * tx + 64 * j + k;
+        const int d = 4 * w.tx + 64 * j + k;
         if (d >= D) continue;
         const T y = from_f<T>(v[k] * mul);
         out[(int64_t)r * row_stride + d] = y;
@@ -293,49 +377,53 @@ __device__ __forceinline__ void store_rows(T* out, int64_t row_stride, int r0, i
   }
 }
 
-template <typename T, int TM, int TN, int DM>
-__global__ void __launch_bounds__(NT) fwd_cores(CausalParams p) {
-  using Z = Tile<TM, TN, DM>;
+template <typename T, typename Z>
+__global__ void __launch_bounds__(Z::NT) fwd_cores(CausalParams p) {
+  constexpr int TM = Z::TM, TN = Z::TN, DM = Z::DM;
+  constexpr bool kAhead = Z::kFetch <= 16;  // the next tile's loads under this one's products
   extern __shared__ __align__(16) float sm[];
-  float* q_s = sm;                   // [TM][RS]
-  float* kv_s = q_s + TM * Z::RS;    // [TN][RS] keys, then values
-  float* p_s = kv_s + TN * Z::RS;    // [TM][PS]
+  const Place w = place<Z>();
+  float* groups = sm + Z::fwd_all();
+  float* q_s = sm;                               // [TM][RS]
+  float* kv_s = groups + w.g * Z::fwd_group();     // [TN][RS] keys, then values
+  float* p_s = kv_s + TN * Z::RS;                // [TM][PS]
   const int q0 = (gridDim.x - 1 - blockIdx.x) * TM, hq = blockIdx.y, b = blockIdx.z, hkv = hq / p.E;
-  const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
-  load_tile<T, TM, DM>(q_s, p.q, b * p.q_sb + hq * p.q_sh, p.q_sn, q0, p.N, p.Dk);
+  load_tile<T, TM, DM, Z::NT>(q_s, p.q, b * p.q_sb + hq * p.q_sh, p.q_sn, q0, p.N, p.Dk, threadIdx.x, p.vec4);
   int lo[Z::R];
   float m[Z::R], l[Z::R];
   float4 o[Z::R][Z::C];
 #pragma unroll
   for (int i = 0; i < Z::R; ++i) {
-    const int q = q0 + ty + 16 * i;
+    const int q = q0 + w.ty + Z::RW * i;
     lo[i] = q < p.N ? first_key(p, b, q) : p.N;
     m[i] = -INFINITY;
     l[i] = 0.f;
 #pragma unroll
     for (int j = 0; j < Z::C; ++j) o[i][j] = make_float4(0.f, 0.f, 0.f, 0.f);
   }
-  const int end = min(q0 + TM, p.N), begin = first_key(p, b, q0) / 16 * 16;
+  const int end = min(q0 + TM, p.N), begin = first_key(p, b, q0) / 16 * 16 + w.g * TN, step = Z::G * TN;
   const int64_t kb = b * p.k_sb + hkv * p.k_sh, vb = b * p.v_sb + hkv * p.v_sh;
-  float kr[kFetch<TN, DM>], vr[kFetch<TN, DM>];
-  if (begin < end) {
-    fetch_tile<T, TN, DM>(kr, p.k, kb, p.k_sn, begin, p.N, p.Dk);
-    fetch_tile<T, TN, DM>(vr, p.v, vb, p.v_sn, begin, p.N, p.Dv);
+  float4 kr[kAhead ? Z::kFetch / 4 : 1], vr[kAhead ? Z::kFetch / 4 : 1];
+  if (kAhead && begin < end) {
+    fetch_tile<T, Z>(kr, p.k, kb, p.k_sn, begin, p.N, p.Dk, w.t, p.vec4);
+    fetch_tile<T, Z>(vr, p.v, vb, p.v_sn, begin, p.N, p.Dv, w.t, p.vec4);
   }
-  for (int k0 = begin; k0 < end; k0 += TN) {
-    __syncthreads();
-    put_tile<TN, DM>(kv_s, kr);
-    __syncthreads();
-    if (k0 + TN < end) fetch_tile<T, TN, DM>(kr, p.k, kb, p.k_sn, k0 + TN, p.N, p.Dk);
+  __syncthreads();
+  for (int k0 = begin; k0 < end; k0 += step) {
+    group_sync<Z>(w.g);
+    if constexpr (kAhead) put_tile<Z>(kv_s, kr, w.t);
+    else load_tile<T, TN, DM, Z::GT>(kv_s, p.k, kb, p.k_sn, k0, p.N, p.Dk, w.t, p.vec4);
+    group_sync<Z>(w.g);
+    if (kAhead && k0 + step < end) fetch_tile<T, Z>(kr, p.k, kb, p.k_sn, k0 + step, p.N, p.Dk, w.t, p.vec4);
     float s[Z::R][Z::S];
-    dot_tile<TM, TN, DM>(q_s, kv_s, p.Dk, s);
+    dot_tile<Z>(q_s, kv_s, p.Dk, w, s);
 #pragma unroll
     for (int i = 0; i < Z::R; ++i) {
-      const int q = q0 + ty + 16 * i;
+      const int row = w.ty + Z::RW * i, q = q0 + row;
       float mx = -INFINITY;
 #pragma unroll
       for (int j = 0; j < Z::S; ++j) {
-        const int k = k0 + tx + 16 * j;
+        const int k = k0 + w.tx + 16 * j;
         float x = s[i][j] * p.scale;
         if (p.has_cap) x = p.cap * tanhf(x / p.cap);
         s[i][j] = k >= lo[i] && k <= q ? x : -INFINITY;
@@ -351,7 +439,7 @@ __global__ void __launch_bounds__(NT) fwd_cores(CausalParams p) {
         // a NaN score (a NaN in a visible key) stays one; a masked one is 0
         const float e = expf(s[i][j] - me);
         sum += e;
-        p_s[(ty + 16 * i) * Z::PS + tx + 16 * j] = e;
+        p_s[row * Z::PS + w.tx + 16 * j] = e;
       }
 #pragma unroll
       for (int x = 8; x; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
@@ -360,24 +448,67 @@ __global__ void __launch_bounds__(NT) fwd_cores(CausalParams p) {
 #pragma unroll
       for (int j = 0; j < Z::C; ++j) o[i][j].x *= c, o[i][j].y *= c, o[i][j].z *= c, o[i][j].w *= c;
     }
+    group_sync<Z>(w.g);
+    if constexpr (kAhead) put_tile<Z>(kv_s, vr, w.t);
+    else load_tile<T, TN, DM, Z::GT>(kv_s, p.v, vb, p.v_sn, k0, p.N, p.Dv, w.t, p.vec4);
+    group_sync<Z>(w.g);
+    if (kAhead && k0 + step < end) fetch_tile<T, Z>(vr, p.v, vb, p.v_sn, k0 + step, p.N, p.Dv, w.t, p.vec4);
+    mul_tile<Z>(p_s, kv_s, w, o);
+  }
+  if constexpr (Z::G > 1) {
+    // joint maximum, then sums and O weighted by it, in the order of the groups
+    constexpr int kPer = 2 + 4 * Z::C;
+    static_assert(Z::R * kPer * Z::GT <= Z::fwd_group(), "a group's state fits its operands");
+    group_sync<Z>(w.g);
+    if (w.g > 0) {
+#pragma unroll
+      for (int i = 0; i < Z::R; ++i) {
+        left<Z>(kv_s, i * kPer, w.t) = m[i], left<Z>(kv_s, i * kPer + 1, w.t) = l[i];
+#pragma unroll
+        for (int j = 0; j < Z::C; ++j) {
+          const int k = i * kPer + 2 + 4 * j;
+          left<Z>(kv_s, k, w.t) = o[i][j].x, left<Z>(kv_s, k + 1, w.t) = o[i][j].y;
+          left<Z>(kv_s, k + 2, w.t) = o[i][j].z, left<Z>(kv_s, k + 3, w.t) = o[i][j].w;
+        }
+      }
+    }
     __syncthreads();
-    put_tile<TN, DM>(kv_s, vr);
-    __syncthreads();
-    if (k0 + TN < end) fetch_tile<T, TN, DM>(vr, p.v, vb, p.v_sn, k0 + TN, p.N, p.Dv);
-    mul_tile<TM, TN, DM>(p_s, kv_s, o);
+    if (w.g > 0) return;
+#pragma unroll
+    for (int i = 0; i < Z::R; ++i) {
+      float mn = m[i];
+      for (int g = 1; g < Z::G; ++g) mn = fmaxf(mn, left<Z>(groups + g * Z::fwd_group(), i * kPer, w.t));
+      const float me = mn == -INFINITY ? 0.f : mn;
+      const float c = expf(m[i] - me);
+      l[i] *= c;
+#pragma unroll
+      for (int j = 0; j < Z::C; ++j) o[i][j].x *= c, o[i][j].y *= c, o[i][j].z *= c, o[i][j].w *= c;
+      for (int g = 1; g < Z::G; ++g) {
+        float* s = groups + g * Z::fwd_group();
+        const float e = expf(left<Z>(s, i * kPer, w.t) - me);
+        l[i] += e * left<Z>(s, i * kPer + 1, w.t);
+#pragma unroll
+        for (int j = 0; j < Z::C; ++j) {
+          const int k = i * kPer + 2 + 4 * j;
+          o[i][j].x += e * left<Z>(s, k, w.t), o[i][j].y += e * left<Z>(s, k + 1, w.t);
+          o[i][j].z += e * left<Z>(s, k + 2, w.t), o[i][j].w += e * left<Z>(s, k + 3, w.t);
+        }
+      }
+      m[i] = mn;
+    }
   }
 #pragma unroll
   for (int i = 0; i < Z::R; ++i) {
     const float inv = l[i] != 0.f ? 1.f / l[i] : 0.f;
 #pragma unroll
     for (int j = 0; j < Z::C; ++j) o[i][j].x *= inv, o[i][j].y *= inv, o[i][j].z *= inv, o[i][j].w *= inv;
-    const int q = q0 + ty + 16 * i;
-    if (tx == 0 && q < p.N)
+    const int q = q0 + w.ty + Z::RW * i;
+    if (w.tx == 0 && q < p.N)
       p.lse[((int64_t)b * p.N + q) * p.Hq + hq] = l[i] != 0.f ? m[i] + logf(l[i]) : -INFINITY;
   }
   const int64_t at = ((int64_t)b * p.N * p.Hq + hq) * p.Dv;
-  store_rows<T, TM, TN, DM>(static_cast<T*>(p.out) + at, (int64_t)p.Hq * p.Dv, q0, p.N, p.Dv, 1.f, o,
-                            p.out_low ? static_cast<T*>(p.out_low) + at : nullptr);
+  store_rows<T, Z>(static_cast<T*>(p.out) + at, (int64_t)p.Hq * p.Dv, q0, p.N, p.Dv, 1.f, w, o,
+                   p.out_low ? static_cast<T*>(p.out_low) + at : nullptr);
 }
 
 // P and dX of a score tile whose rows are queries (ROWS_Q) or keys.
@@ -409,177 +540,205 @@ __device__ __forceinline__ void grad_of(const CausalParams& p, const RowStat& r,
   *dx = see ? *pr * (dp - r.delta) * g : 0.f;
 }
 
-template <typename T, int TM, int TN, int DM>
+template <typename T, typename Z>
 __device__ __forceinline__ void dq_cores(const CausalParams& p, float* sm, int q0, int hq, int b) {
-  using Z = Tile<TM, TN, DM>;
+  constexpr int TM = Z::TM, TN = Z::TN, DM = Z::DM;
+  constexpr bool kAhead = Z::kFetch <= (Z::G == 1 ? 32 : 16);
+  const Place w = place<Z>();
+  float* groups = sm + Z::bwd_all();
   float* q_s = sm;
   float* g_s = q_s + TM * Z::RS;
-  float* k_s = g_s + TM * Z::RS;
+  float* k_s = groups + w.g * Z::bwd_group();
   float* v_s = k_s + TN * Z::RS;
   float* x_s = v_s + TN * Z::RS;
   const int hkv = hq / p.E;
-  const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
-  load_tile<T, TM, DM>(q_s, p.q, b * p.q_sb + hq * p.q_sh, p.q_sn, q0, p.N, p.Dk);
-  load_tile<T, TM, DM>(g_s, p.dout, ((int64_t)b * p.N * p.Hq + hq) * p.Dv, (int64_t)p.Hq * p.Dv, q0, p.N, p.Dv);
+  const int64_t gb = ((int64_t)b * p.N * p.Hq + hq) * p.Dv, gn = (int64_t)p.Hq * p.Dv;
+  load_tile<T, TM, DM, Z::NT>(q_s, p.q, b * p.q_sb + hq * p.q_sh, p.q_sn, q0, p.N, p.Dk, threadIdx.x, p.vec4);
+  load_tile<T, TM, DM, Z::NT>(g_s, p.dout, gb, gn, q0, p.N, p.Dv, threadIdx.x, p.vec4);
   RowStat st[Z::R];
   float4 acc[Z::R][Z::C];
 #pragma unroll
   for (int i = 0; i < Z::R; ++i) {
-    st[i] = row_stat(p, b, hq, q0 + ty + 16 * i);
+    st[i] = row_stat(p, b, hq, q0 + w.ty + Z::RW * i);
 #pragma unroll
     for (int j = 0; j < Z::C; ++j) acc[i][j] = make_float4(0.f, 0.f, 0.f, 0.f);
   }
-  const int end = min(q0 + TM, p.N), begin = first_key(p, b, q0) / 16 * 16;
+  const int end = min(q0 + TM, p.N), begin = first_key(p, b, q0) / 16 * 16 + w.g * TN, step = Z::G * TN;
   const int64_t kb = b * p.k_sb + hkv * p.k_sh, vb = b * p.v_sb + hkv * p.v_sh;
-  float kr[kFetch<TN, DM>], vr[kFetch<TN, DM>];
-  if (begin < end) {
-    fetch_tile<T, TN, DM>(kr, p.k, kb, p.k_sn, begin, p.N, p.Dk);
-    fetch_tile<T, TN, DM>(vr, p.v, vb, p.v_sn, begin, p.N, p.Dv);
+  float4 kr[kAhead ? Z::kFetch / 4 : 1], vr[kAhead ? Z::kFetch / 4 : 1];
+  if (kAhead && begin < end) {
+    fetch_tile<T, Z>(kr, p.k, kb, p.k_sn, begin, p.N, p.Dk, w.t, p.vec4);
+    fetch_tile<T, Z>(vr, p.v, vb, p.v_sn, begin, p.N, p.Dv, w.t, p.vec4);
   }
-  for (int k0 = begin; k0 < end; k0 += TN) {
-    __syncthreads();
-    put_tile<TN, DM>(k_s, kr);
-    put_tile<TN, DM>(v_s, vr);
-    __syncthreads();
-    if (k0 + TN < end) {
-      fetch_tile<T, TN, DM>(kr, p.k, kb, p.k_sn, k0 + TN, p.N, p.Dk);
-      fetch_tile<T, TN, DM>(vr, p.v, vb, p.v_sn, k0 + TN, p.N, p.Dv);
+  __syncthreads();
+  for (int k0 = begin; k0 < end; k0 += step) {
+    group_sync<Z>(w.g);
+    if constexpr (kAhead) {
+      put_tile<Z>(k_s, kr, w.t);
+      put_tile<Z>(v_s, vr, w.t);
+    } else {
+      load_tile<T, TN, DM, Z::GT>(k_s, p.k, kb, p.k_sn, k0, p.N, p.Dk, w.t, p.vec4);
+      load_tile<T, TN, DM, Z::GT>(v_s, p.v, vb, p.v_sn, k0, p.N, p.Dv, w.t, p.vec4);
+    }
+    group_sync<Z>(w.g);
+    if (kAhead && k0 + step < end) {
+      fetch_tile<T, Z>(kr, p.k, kb, p.k_sn, k0 + step, p.N, p.Dk, w.t, p.vec4);
+      fetch_tile<T, Z>(vr, p.v, vb, p.v_sn, k0 + step, p.N, p.Dv, w.t, p.vec4);
     }
     float s[Z::R][Z::S], d[Z::R][Z::S];
-    dot_tile<TM, TN, DM>(q_s, k_s, p.Dk, s);
-    dot_tile<TM, TN, DM>(g_s, v_s, p.Dv, d);
+    dot_tile<Z>(q_s, k_s, p.Dk, w, s);
+    dot_tile<Z>(g_s, v_s, p.Dv, w, d);
 #pragma unroll
     for (int i = 0; i < Z::R; ++i)
 #pragma unroll
       for (int j = 0; j < Z::S; ++j) {
         float pr, dx;
-        grad_of(p, st[i], k0 + tx + 16 * j, s[i][j], d[i][j], &pr, &dx);
-        x_s[(ty + 16 * i) * Z::PS + tx + 16 * j] = dx;
+        grad_of(p, st[i], k0 + w.tx + 16 * j, s[i][j], d[i][j], &pr, &dx);
+        x_s[(w.ty + Z::RW * i) * Z::PS + w.tx + 16 * j] = dx;
       }
-    __syncthreads();
-    mul_tile<TM, TN, DM>(x_s, k_s, acc);
+    group_sync<Z>(w.g);
+    mul_tile<Z>(x_s, k_s, w, acc);
   }
-  store_rows<T, TM, TN, DM>(static_cast<T*>(p.dq) + ((int64_t)b * p.N * p.Hq + hq) * p.Dk, (int64_t)p.Hq * p.Dk, q0, p.N,
-                        p.Dk, p.scale, acc);
+  group_sync<Z>(w.g);
+  if (!join_sums<Z, 0>(groups, Z::bwd_group(), w, acc, 0)) return;
+  store_rows<T, Z>(static_cast<T*>(p.dq) + ((int64_t)b * p.N * p.Hq + hq) * p.Dk, (int64_t)p.Hq * p.Dk, q0, p.N, p.Dk,
+                   p.scale, w, acc);
 }
 
 // dK, dV of TM keys of one key head: the queries that see them, head by head of
 // the group, in order (no atomics: the sum's order is fixed).
-template <typename T, int TM, int TN, int DM>
+template <typename T, typename Z>
 __device__ __forceinline__ void dkv_cores(const CausalParams& p, float* sm, int k0, int hkv, int b) {
-  using Z = Tile<TM, TN, DM>;
+  constexpr int TM = Z::TM, TN = Z::TN, DM = Z::DM;
+  constexpr bool kAhead = Z::kFetch <= (Z::G == 1 ? 32 : 16);
+  __shared__ RowStat st_all[Z::G][TN];
+  const Place w = place<Z>();
+  float* groups = sm + Z::bwd_all();
   float* k_s = sm;
   float* v_s = k_s + TM * Z::RS;
-  float* q_s = v_s + TM * Z::RS;
+  float* q_s = groups + w.g * Z::bwd_group();
   float* g_s = q_s + TN * Z::RS;
   float* p_s = g_s + TN * Z::RS;
   float* x_s = p_s + TM * Z::PS;
-  __shared__ RowStat st_s[TN];
-  const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
-  load_tile<T, TM, DM>(k_s, p.k, b * p.k_sb + hkv * p.k_sh, p.k_sn, k0, p.N, p.Dk);
-  load_tile<T, TM, DM>(v_s, p.v, b * p.v_sb + hkv * p.v_sh, p.v_sn, k0, p.N, p.Dv);
+  RowStat* st_s = st_all[w.g];
+  load_tile<T, TM, DM, Z::NT>(k_s, p.k, b * p.k_sb + hkv * p.k_sh, p.k_sn, k0, p.N, p.Dk, threadIdx.x, p.vec4);
+  load_tile<T, TM, DM, Z::NT>(v_s, p.v, b * p.v_sb + hkv * p.v_sh, p.v_sn, k0, p.N, p.Dv, threadIdx.x, p.vec4);
   float4 dk[Z::R][Z::C], dv[Z::R][Z::C];
 #pragma unroll
   for (int i = 0; i < Z::R; ++i)
 #pragma unroll
     for (int j = 0; j < Z::C; ++j) dk[i][j] = dv[i][j] = make_float4(0.f, 0.f, 0.f, 0.f);
-  const int end = query_end(p, b, min(k0 + TN, p.N) - 1);
-  float qr[kFetch<TN, DM>], gr[kFetch<TN, DM>];
-  auto fetch = [&](int hq, int q0) {
-    fetch_tile<T, TN, DM>(qr, p.q, b * p.q_sb + hq * p.q_sh, p.q_sn, q0, p.N, p.Dk);
-    fetch_tile<T, TN, DM>(gr, p.dout, ((int64_t)b * p.N * p.Hq + hq) * p.Dv, (int64_t)p.Hq * p.Dv, q0, p.N, p.Dv);
+  // tile i: queries k0 + i % steps TN of head i / steps
+  const int end = query_end(p, b, min(k0 + TM, p.N) - 1);
+  const int steps = max(0, (end - k0 + TN - 1) / TN), tiles = steps * p.E;
+  float4 qr[kAhead ? Z::kFetch / 4 : 1], gr[kAhead ? Z::kFetch / 4 : 1];
+  const int64_t qb = b * p.q_sb, gb = (int64_t)b * p.N * p.Hq * p.Dv, gn = (int64_t)p.Hq * p.Dv;
+  auto fetch = [&](int i) {
+    const int hq = hkv * p.E + i / steps, q0 = k0 + i % steps * TN;
+    fetch_tile<T, Z>(qr, p.q, qb + hq * p.q_sh, p.q_sn, q0, p.N, p.Dk, w.t, p.vec4);
+    fetch_tile<T, Z>(gr, p.dout, gb + hq * p.Dv, gn, q0, p.N, p.Dv, w.t, p.vec4);
   };
-  if (k0 < end) fetch(hkv * p.E, k0);
-  for (int e = 0; e < p.E; ++e) {
-    const int hq = hkv * p.E + e;
-    for (int q0 = k0; q0 < end; q0 += TN) {
-      __syncthreads();
-      put_tile<TN, DM>(q_s, qr);
-      put_tile<TN, DM>(g_s, gr);
-      if (threadIdx.x < TN) st_s[threadIdx.x] = row_stat(p, b, hq, q0 + threadIdx.x);
-      __syncthreads();
-      if (q0 + TN < end) fetch(hq, q0 + TN);
-      else if (e + 1 < p.E) fetch(hq + 1, k0);
-      float s[Z::R][Z::S], d[Z::R][Z::S];
-      dot_tile<TM, TN, DM>(k_s, q_s, p.Dk, s);
-      dot_tile<TM, TN, DM>(v_s, g_s, p.Dv, d);
-#pragma unroll
-      for (int i = 0; i < Z::R; ++i)
-#pragma unroll
-        for (int j = 0; j < Z::S; ++j) {
-          float pr, dx;
-          grad_of(p, st_s[tx + 16 * j], k0 + ty + 16 * i, s[i][j], d[i][j], &pr, &dx);
-          p_s[(ty + 16 * i) * Z::PS + tx + 16 * j] = pr;
-          x_s[(ty + 16 * i) * Z::PS + tx + 16 * j] = dx;
-        }
-      __syncthreads();
-      mul_tile<TM, TN, DM>(p_s, g_s, dv);
-      mul_tile<TM, TN, DM>(x_s, q_s, dk);
+  if (kAhead && w.g < tiles) fetch(w.g);
+  __syncthreads();
+  for (int i0 = w.g; i0 < tiles; i0 += Z::G) {
+    const int hq = hkv * p.E + i0 / steps, q0 = k0 + i0 % steps * TN;
+    group_sync<Z>(w.g);
+    if constexpr (kAhead) {
+      put_tile<Z>(q_s, qr, w.t);
+      put_tile<Z>(g_s, gr, w.t);
+    } else {
+      load_tile<T, TN, DM, Z::GT>(q_s, p.q, qb + hq * p.q_sh, p.q_sn, q0, p.N, p.Dk, w.t, p.vec4);
+      load_tile<T, TN, DM, Z::GT>(g_s, p.dout, gb + hq * p.Dv, gn, q0, p.N, p.Dv, w.t, p.vec4);
     }
+    if (w.t < TN) st_s[w.t] = row_stat(p, b, hq, q0 + w.t);
+    group_sync<Z>(w.g);
+    if (kAhead && i0 + Z::G < tiles) fetch(i0 + Z::G);
+    float s[Z::R][Z::S], d[Z::R][Z::S];
+    dot_tile<Z>(k_s, q_s, p.Dk, w, s);
+    dot_tile<Z>(v_s, g_s, p.Dv, w, d);
+#pragma unroll
+    for (int i = 0; i < Z::R; ++i)
+#pragma unroll
+      for (int j = 0; j < Z::S; ++j) {
+        float pr, dx;
+        grad_of(p, st_s[w.tx + 16 * j], k0 + w.ty + Z::RW * i, s[i][j], d[i][j], &pr, &dx);
+        p_s[(w.ty + Z::RW * i) * Z::PS + w.tx + 16 * j] = pr;
+        x_s[(w.ty + Z::RW * i) * Z::PS + w.tx + 16 * j] = dx;
+      }
+    group_sync<Z>(w.g);
+    mul_tile<Z>(p_s, g_s, w, dv);
+    mul_tile<Z>(x_s, q_s, w, dk);
   }
-  store_rows<T, TM, TN, DM>(static_cast<T*>(p.dk) + ((int64_t)b * p.N * p.Hkv + hkv) * p.Dk, (int64_t)p.Hkv * p.Dk, k0, p.N,
-                        p.Dk, p.scale, dk);
-  store_rows<T, TM, TN, DM>(static_cast<T*>(p.dv) + ((int64_t)b * p.N * p.Hkv + hkv) * p.Dv, (int64_t)p.Hkv * p.Dv, k0, p.N,
-                        p.Dv, 1.f, dv);
+  group_sync<Z>(w.g);
+  constexpr int kAt = Z::R * Z::C * 4;
+  const bool first = join_sums<Z, 0>(groups, Z::bwd_group(), w, dk, 0);
+  if (!join_sums<Z, 1>(groups, Z::bwd_group(), w, dv, kAt) || !first) return;
+  store_rows<T, Z>(static_cast<T*>(p.dk) + ((int64_t)b * p.N * p.Hkv + hkv) * p.Dk, (int64_t)p.Hkv * p.Dk, k0, p.N, p.Dk,
+                   p.scale, w, dk);
+  store_rows<T, Z>(static_cast<T*>(p.dv) + ((int64_t)b * p.N * p.Hkv + hkv) * p.Dv, (int64_t)p.Hkv * p.Dv, k0, p.N, p.Dv,
+                   1.f, w, dv);
 }
 
 // Both passes in one launch, the dK/dV blocks first (they do four products a tile
 // to the other's three), each from its longest: a small problem's blocks of both
 // share the SMs.
-template <typename T, int TM, int TN, int DM>
-__global__ void __launch_bounds__(NT, TM == 32 && DM <= 64 ? 2 : 1) bwd_cores(const __grid_constant__ CausalParams p) {
+template <typename T, typename Z>
+__global__ void __launch_bounds__(Z::NT) bwd_cores(const __grid_constant__ CausalParams p) {
   extern __shared__ __align__(16) float sm[];
-  const int tiles = (p.N + TM - 1) / TM, x = blockIdx.x, b = blockIdx.y;
+  const int tiles = (p.N + Z::TM - 1) / Z::TM, x = blockIdx.x, b = blockIdx.y;
   if (x < tiles * p.Hkv) {
-    dkv_cores<T, TM, TN, DM>(p, sm, x / p.Hkv * TM, x % p.Hkv, b);
+    dkv_cores<T, Z>(p, sm, x / p.Hkv * Z::TM, x % p.Hkv, b);
   } else {
     const int y = x - tiles * p.Hkv;
-    dq_cores<T, TM, TN, DM>(p, sm, (tiles - 1 - y / p.Hq) * TM, y % p.Hq, b);
+    dq_cores<T, Z>(p, sm, (tiles - 1 - y / p.Hq) * Z::TM, y % p.Hq, b);
   }
 }
 
 template <typename K>
-int launch_cores(K kernel, dim3 grid, size_t smem, const CausalParams& p, cudaStream_t st) {
+int launch_cores(K kernel, dim3 grid, int threads, size_t smem, const CausalParams& p, cudaStream_t st) {
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
     return TC_ERR_CUDA;
-  kernel<<<grid, NT, smem, st>>>(p);
+  kernel<<<grid, threads, smem, st>>>(p);
   return launch_status();
 }
 
-template <typename T, int TM, int TN, int DM>
+template <typename T, typename Z>
 int fwd_cores_launch(const CausalParams& p, cudaStream_t st) {
-  using Z = Tile<TM, TN, DM>;
-  const size_t smem = sizeof(float) * ((TM + TN) * Z::RS + TM * Z::PS);
-  return launch_cores(fwd_cores<T, TM, TN, DM>, dim3((p.N + TM - 1) / TM, p.Hq, p.B), smem, p, st);
+  constexpr size_t smem = sizeof(float) * (Z::fwd_all() + Z::G * Z::fwd_group());
+  static_assert(smem <= 227 * 1024, "forward shared memory exceeds the per-CTA limit");
+  return launch_cores(fwd_cores<T, Z>, dim3((p.N + Z::TM - 1) / Z::TM, p.Hq, p.B), Z::NT, smem, p, st);
 }
-template <typename T, int TM, int TN, int DM>
+template <typename T, typename Z>
 int bwd_cores_launch(const CausalParams& p, cudaStream_t st) {
-  using Z = Tile<TM, TN, DM>;
-  const size_t smem = sizeof(float) * (2 * (TM + TN) * Z::RS + 2 * TM * Z::PS);
-  const int64_t blocks = (int64_t)((p.N + TM - 1) / TM) * (p.Hq + p.Hkv);
+  constexpr size_t smem = sizeof(float) * (Z::bwd_all() + Z::G * Z::bwd_group());
+  static_assert(smem + Z::G * Z::TN * sizeof(RowStat) <= 227 * 1024, "backward shared memory exceeds the per-CTA limit");
+  const int64_t blocks = (int64_t)((p.N + Z::TM - 1) / Z::TM) * (p.Hq + p.Hkv);
   if (blocks > INT32_MAX) return TC_ERR_UNSUPPORTED;
-  return launch_cores(bwd_cores<T, TM, TN, DM>, dim3((unsigned)blocks, p.B), smem, p, st);
+  return launch_cores(bwd_cores<T, Z>, dim3((unsigned)blocks, p.B), Z::NT, smem, p, st);
 }
 
-// 64 rows to a block where the blocks give every SM two, else 32 (and 64 columns:
-// fewer, longer steps).  4 heads of 64 and 1024 tokens, both directions: 553 us in
-// blocks of 64 (64 of them walk up to 16 tiles each on 148 SMs), 363 us in 32 x 32,
-// 308 us in 32 x 64, 262 us with both backward passes in one launch.
+// Blocks of 32 rows whose four groups of 128 threads share the tiles (two groups in
+// the backward of D > 64, whose operands are wider; one of 256 threads above 128).
+// Against blocks of 64 rows with one group of 256, fp32: 4 heads of 64 and 1024
+// tokens 54 and 94 us forward and backward against 107 and 193, 4 key heads of 128
+// there 85 and 198 against 169 and 312 us; 32 heads of 4096 tokens the same forward
+// (2605 / 2580 us at 64, 4460 / 4516 at 128) and 8.5 against 9.1 ms backward at 64.
+// Only the backward of D > 64 is faster in blocks of 64 once they give every SM two:
+// 15.0 against 19.3 ms (its two groups are one block's threads on half the rows).
 template <typename T>
 int fwd_cores_any(const CausalParams& p, cudaStream_t st) {
   const int D = imax(p.Dk, p.Dv);
-  const bool wide = (int64_t)((p.N + 63) / 64) * p.Hq * p.B >= 2 * 148;
-  if (D <= 64) return wide ? fwd_cores_launch<T, 64, 64, 64>(p, st) : fwd_cores_launch<T, 32, 64, 64>(p, st);
-  if (D <= 128) return wide ? fwd_cores_launch<T, 64, 64, 128>(p, st) : fwd_cores_launch<T, 32, 64, 128>(p, st);
-  return fwd_cores_launch<T, 32, 32, 256>(p, st);
+  if (D <= 64) return fwd_cores_launch<T, Tile<32, 64, 64, 128, 4>>(p, st);
+  if (D <= 128) return fwd_cores_launch<T, Tile<32, 64, 128, 128, 4>>(p, st);
+  return fwd_cores_launch<T, Tile<32, 32, 256, 256, 1>>(p, st);
 }
 template <typename T>
 int bwd_cores_any(const CausalParams& p, cudaStream_t st) {
   const int D = imax(p.Dk, p.Dv);
+  if (D <= 64) return bwd_cores_launch<T, Tile<32, 64, 64, 128, 4>>(p, st);
+  if (D > 128) return bwd_cores_launch<T, Tile<32, 32, 256, 256, 1>>(p, st);
   const bool wide = (int64_t)((p.N + 63) / 64) * p.Hkv * p.B >= 2 * 148;
-  if (D <= 64) return wide ? bwd_cores_launch<T, 64, 64, 64>(p, st) : bwd_cores_launch<T, 32, 64, 64>(p, st);
-  if (D <= 128) return wide ? bwd_cores_launch<T, 64, 64, 128>(p, st) : bwd_cores_launch<T, 32, 64, 128>(p, st);
-  return bwd_cores_launch<T, 32, 32, 256>(p, st);
+  return wide ? bwd_cores_launch<T, Tile<64, 64, 128, 256, 1>>(p, st) : bwd_cores_launch<T, Tile<32, 64, 128, 128, 2>>(p, st);
 }
 
 int make_params(const tc_causal_args* a, CausalParams* p) {
@@ -600,6 +759,11 @@ int make_params(const tc_causal_args* a, CausalParams* p) {
   p->o = a->o, p->o_low = a->o_low, p->dout = a->dout, p->dlse = a->dlse, p->delta = a->delta;
   p->dq = a->dq, p->dk = a->dk, p->dv = a->dv;
   p->status = a->dev_status;
+  const int unit = a->dtype == TC_F32 ? 16 : 8;
+  const int64_t strides = a->q_stride_b | a->q_stride_n | a->q_stride_h | a->k_stride_b | a->k_stride_n | a->k_stride_h |
+                          a->v_stride_b | a->v_stride_n | a->v_stride_h | a->Dk | a->Dv;
+  const uintptr_t starts = (uintptr_t)a->q | (uintptr_t)a->k | (uintptr_t)a->v | (uintptr_t)a->dout;
+  p->vec4 = strides % 4 == 0 && starts % unit == 0;
   return TC_OK;
 }
 

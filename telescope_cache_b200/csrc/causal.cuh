@@ -27,6 +27,7 @@ struct CausalParams {
   void* dk;
   void* dv;
   int32_t* status;
+  bool vec4;  // rows of q, k, v, dout start on four elements, and their lengths are multiples
 };
 
 // First key that query n of row b sees (its last is n itself); n + 1 where it

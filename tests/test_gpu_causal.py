@@ -160,6 +160,23 @@ def test_gradients_against_differences():
         assert abs(float((got[i].double() * t).sum()) - want) <= 1e-4 * float(got[i].double().norm() * t.norm())
 
 
+@pytest.mark.parametrize("D", [72, 128])
+def test_gradients_of_many_blocks(D):
+    """fp32 with enough blocks of keys for every SM, and a tail of 6 tokens."""
+    from telescope_cache_b200 import causal_attention
+
+    dt, B, N, Hq, Hkv = torch.float32, 37, 70, 8, 4
+    q, k, v = (t.requires_grad_() for t in inputs(B, N, Hq, Hkv, D, D, dt, seed=6))
+    out, lse = causal_attention(q, k, v, scale=0.11)
+    gout, glse = torch.randn_like(out), torch.randn_like(lse)
+    got = torch.autograd.grad((out, lse), (q, k, v), (gout, glse))
+    x = [t.detach().double().requires_grad_() for t in (q, k, v)]
+    see = visible(None, B, N, "cuda")
+    o, l, _, _ = causal(*x, see, None, 0.11)
+    want = torch.autograd.grad((o * gout.double()).sum() + (l * glse.double()).sum(), x)
+    check_grads(got, want, gradient_terms(q, k, v, see, gout, glse, None, 0.11), dt)
+
+
 @pytest.mark.parametrize("dtype,D", [("bf16", 128), ("f16", 64), ("f32", 64)])
 def test_strided_views(dtype, D):
     """q, k, v as views of a fused projection, with heads before tokens, and with
