@@ -17,6 +17,7 @@
 #include <map>
 #include <stdexcept>
 #include <tuple>
+#include <vector>
 
 #include "../../../include/telescope_cache.h"
 
@@ -342,9 +343,12 @@ std::tuple<Tensor, Tensor> kv_read(const Tensor& ck, const Tensor& cv, const Ten
 
 // Workspace of the split attention: one per device and stream, since calls on one
 // stream run in order.  The arrival counts are zero between calls.  Never freed:
-// the process may end after the CUDA context.
+// the process may end after the CUDA context, and a captured graph goes on using
+// the workspace it was captured with, so one that was outgrown is kept too (each
+// is at least twice the one before).
 struct Work {
   Tensor scratch, counts;
+  std::vector<Tensor> outgrown;
 };
 Work& workspace(const Tensor& on, cudaStream_t stream, int64_t floats, int64_t counts) {
   static auto* all = new std::map<std::pair<int, cudaStream_t>, Work>;
@@ -353,8 +357,14 @@ Work& workspace(const Tensor& on, cudaStream_t stream, int64_t floats, int64_t c
   const bool more = !w.counts.defined() || w.counts.numel() < counts;
   CHECK_RUN(!(grow || more) || at::cuda::currentStreamCaptureStatusMayInitCtx() == at::cuda::CaptureStatus::None,
               "cached attention: run a call of this size on the stream before its capture (it allocates a workspace)");
-  if (grow) w.scratch = at::empty({floats}, on.options().dtype(at::kFloat));
-  if (more) w.counts = at::zeros({std::max<int64_t>(counts, 4096)}, on.options().dtype(at::kInt));
+  if (grow) {
+    if (w.scratch.defined()) w.outgrown.push_back(w.scratch);
+    w.scratch = at::empty({w.scratch.defined() ? std::max(floats, 2 * w.scratch.numel()) : floats}, on.options().dtype(at::kFloat));
+  }
+  if (more) {
+    if (w.counts.defined()) w.outgrown.push_back(w.counts);
+    w.counts = at::zeros({std::max<int64_t>(counts, w.counts.defined() ? 2 * w.counts.numel() : 4096)}, on.options().dtype(at::kInt));
+  }
   return w;
 }
 

@@ -741,7 +741,7 @@ __global__ void __launch_bounds__(kAtThreads, 3)
   const int hkv = hg / p.groups, e0 = (hg - hkv * p.groups) * 8;
   const int nE = min(8, p.E - e0);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int pos = p.lengths[b];
+  const int pos = max(p.lengths[b], 0);
   if (threadIdx.x == 0) {
     prefetch_tmap(&tmk);
     prefetch_tmap(&tmv);
@@ -1087,7 +1087,7 @@ __global__ void __launch_bounds__(kAnyThreads) attend_any(AttendParams p) {
   const int hkv = hg / p.groups, e0 = (hg - hkv * p.groups) * 8;
   const int nE = min(8, p.E - e0);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int pos = p.lengths[b];
+  const int pos = max(p.lengths[b], 0);
   const int ntok = (int)min((int64_t)(STEP ? pos + 1 : pos), p.cap);
   const int active = max(1, min(p.splits, (ntok + p.chunk - 1) / p.chunk));
   const int64_t slot0 = ((int64_t)b * p.Hkv * p.groups + hg) * p.splits;

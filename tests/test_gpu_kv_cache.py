@@ -295,3 +295,53 @@ def test_two_streams():
                 got.append(cached_attention(q, c)[0])
     torch.cuda.synchronize()
     assert all(torch.equal(g, want) for g in got)
+
+
+def test_a_negative_length_is_an_empty_row():
+    """Lengths set by hand: below zero reads nothing and the next token goes to slot 0."""
+    from telescope_cache_b200 import cached_attention, cached_attention_step, init_kv_cache
+
+    for D in (128, 40):
+        c = init_kv_cache(2, 100, 2, D)
+        c.lengths.copy_(torch.tensor([-7, -1]))
+        q, k, v = (rand(2, 1, 2, D, seed=i) for i in range(3))
+        out, lse = cached_attention(q, c)
+        assert bool((out == 0).all()) and bool((lse == -math.inf).all())
+        cached_attention_step(q, k, v, c)
+        assert c.lengths.tolist() == [1, 1]
+        assert bool((c.k_scale[:, :, 0] > 0).all()) and bool((c.k_scale[:, :, 1:] == 0).all())
+
+
+def test_replayed_steps_outlive_a_larger_call():
+    """A captured step goes on with its workspace after a larger call on its stream
+    took another one, and with lengths that pass those it was planned for."""
+    from telescope_cache_b200 import cached_attention, cached_attention_step, init_kv_cache, write_kv_cache
+
+    B, N, H, D = 2, 500, 2, 128
+    k, v = rand(B, N, H, D, seed=1), rand(B, N, H, D, seed=2)
+    caches = [init_kv_cache(B, 900, H, D) for _ in range(2)]
+    for c in caches:
+        write_kv_cache(c, k, v)
+    q, kt, vt = (rand(B, 1, h, D, dtype=torch.bfloat16, seed=5 + h) for h in (8, H, H))
+    s, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        cached_attention_step(q, kt, vt, caches[0], advance=False)
+    with torch.cuda.graph(graph, stream=s):
+        out, lse = cached_attention_step(q, kt, vt, caches[0])
+    big = init_kv_cache(8, 6000, 8, D)
+    write_kv_cache(big, rand(8, 6000, 8, D, seed=3), rand(8, 6000, 8, D, seed=4))
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        cached_attention(rand(8, 1, 64, D, dtype=torch.bfloat16, seed=9), big)
+    torch.cuda.synchronize()
+    junk = [torch.full((1 << i,), math.nan, device="cuda") for i in range(12, 22)]
+    for _ in range(300):
+        graph.replay()
+        want, wl = cached_attention_step(q, kt, vt, caches[1])
+    torch.cuda.synchronize()
+    assert len(junk) == 10 and caches[0].lengths.tolist() == caches[1].lengths.tolist() == [800, 800]
+    assert torch.equal(caches[0].k, caches[1].k) and torch.equal(caches[0].v_scale, caches[1].v_scale)
+    # other splits, the same formula: fp32 sums, then one rounding to bf16
+    assert float((out.float() - want.float()).abs().max()) <= 2.0 ** -7 * float(want.float().abs().max())
+    assert float((lse - wl).abs().max()) <= 1e-5 + 8e-6 * float(wl.abs().max())
