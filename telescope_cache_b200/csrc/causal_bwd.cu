@@ -33,6 +33,12 @@
 // during dX).  dQ pass, TMEM: S, two dP, dQ.  S of the next tile is issued as soon
 // as this one's is in registers and dP a tile ahead, so the compute warps wait
 // for no product that depends on them.
+//
+// Measured, 8 / 2 heads of 128, 16384 tokens, bf16: dQ 585 us (1410 TFLOP/s of its
+// three products), dK/dV 900-920 us (1200-1220 of its four and their extra step), the
+// tensor pipe busy 75 % of both.  Softcap, 2 x 4096, 16 heads, five examples: 166 and
+// 232 us.  The dK/dV pass with 8 compute warps of 64 columns: 1.00 ms for 0.96 with 16
+// of 32; lse and Delta from shared memory: 0.96 for 0.90.
 #include "causal_tc.cuh"
 
 namespace tc {

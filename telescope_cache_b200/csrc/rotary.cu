@@ -13,7 +13,9 @@
 // layout: the two chunks of eight pairs) for kHeads heads of one token, so that
 // the tables are loaded once for them and kHeads (half: 2 kHeads) loads are in
 // flight per thread.  q and k are read in place through their strides (views
-// of a fused projection need no copy) and written dense.
+// of a fused projection need no copy) and written dense.  Measured: 0.67 GB (4 x
+// 16384 tokens of 16 + 4 heads of 128, f16) in 109 us, 6.2 TB/s, 0.94 of a copy's
+// rate; one token of 64 sequences 2.5 us, of which nearly all is latency.
 #include "common.cuh"
 #include "rotary.cuh"
 
