@@ -223,14 +223,17 @@ __global__ void __launch_bounds__(256) advance_kernel(WriteParams p) {
   if (i < (int64_t)p.B * p.N) advance_row(p, (int)(i / p.N), (int)(i % p.N));
 }
 
-// LANES lanes per row, 16 bytes each; blockIdx.y: 0 keys, 1 values.  Bound by
-// HBM: the row is read once, its maximum goes round the lanes by shuffles, and
-// the codes leave as 8-byte (fp32: 4-byte) pieces of whole 32-byte sectors.  A
-// lane group takes kTok consecutive tokens of one head: lane j finds token j's
-// place, then kTok loads a lane are in flight (tokens without a place load
-// nothing).  4 x 16384 ragged tokens of 16 heads of 128, bf16 to int8: 154 us, 5.2
-// TB/s of values and codes, at 74 % of the issue slots (two tokens in flight and the
-// conversion instruction in place of the add in code(): 254 us).
+// LANES lanes per row, 16 bytes each; blockIdx.y: 0 keys, 1 values.  The row is read
+// once and the codes leave as 8-byte (fp32: 4-byte) pieces of whole 32-byte sectors.
+// A lane group takes kTok consecutive tokens of one head.  Their loads go out before
+// the places are known (a dependent read away), so tokens that go nowhere are read
+// too: 144 us for 161 without padding, 120 for 118 with one half padding.  The kTok
+// maxima are found together, half of the lanes going on with half of the tokens, and
+// each is divided by once.
+// Bound by HBM and issue alike: 4 x 16384 tokens of 16 heads of 128, bf16 to int8, 0.8
+// GB of values and codes in 144 us, 5.6 TB/s; one eighth of them padding: 138 us (maxima
+// one by one and a division a lane 171, the conversion instruction in place of the add
+// in code() and two tokens a group 254; eight tokens a group as four).
 constexpr int kTok = 4;
 template <typename T, int STORE, int LANES>
 __global__ void __launch_bounds__(256) write_vec(const __grid_constant__ WriteParams p) {
@@ -244,6 +247,13 @@ __global__ void __launch_bounds__(256) write_vec(const __grid_constant__ WritePa
   const uint32_t mask = LANES == 32 ? 0xffffffffu : ((1u << LANES) - 1u) << ((threadIdx.x & 31) / LANES * LANES);
   // lane j: row of codes of token n0 + j (rows of 64 or more bytes: 32 bits count
   // more of them than the memory holds)
+  const T* src = static_cast<const T*>(w.src) + b * w.sb + h * w.sh + lane * VE;
+  uint4 raw[kTok];
+#pragma unroll
+  for (int j = 0; j < kTok; ++j) {
+    raw[j] = make_uint4(0u, 0u, 0u, 0u);
+    if (n0 + j < p.N) raw[j] = *reinterpret_cast<const uint4*>(src + (int64_t)(n0 + j) * w.sn);
+  }
   uint32_t at = 0xffffffffu;
   if (lane < kTok && n0 + lane < p.N) {
     int row;
@@ -252,32 +262,39 @@ __global__ void __launch_bounds__(256) write_vec(const __grid_constant__ WritePa
     if (row >= 0) at = (uint32_t)(((int64_t)row * p.H + h) * p.cap + slot);
     if (p.fresh && keys && h == 0) advance_row(p, b, n0 + lane);
   }
-  const T* src = static_cast<const T*>(w.src) + b * w.sb + h * w.sh + lane * VE;
-  uint4 raw[kTok];
-  uint32_t to[kTok];
-  float mine = 0.f;  // lane j: token j's scale, so that they leave in one store
+  uint32_t to[kTok], m[kTok];
 #pragma unroll
   for (int j = 0; j < kTok; ++j) {
     to[j] = __shfl_sync(mask, at, j, LANES);
-    if (to[j] != 0xffffffffu) raw[j] = *reinterpret_cast<const uint4*>(src + (int64_t)(n0 + j) * w.sn);
   }
 #pragma unroll
-  for (int j = 0; j < kTok; ++j) {
-    if (to[j] == 0xffffffffu) continue;
-    uint32_t m = amax16<T>(raw[j]);
+  for (int j = 0; j < kTok; ++j) m[j] = amax16<T>(raw[j]);
+  int o = LANES / 2;
 #pragma unroll
-    for (int o = LANES / 2; o; o >>= 1) m = amax_join<T>(m, __shfl_xor_sync(mask, m, o));
-    float scale, inv, x[VE];
-    row_scale<STORE>(amax_float<T>(m), &scale, &inv);
+  for (int n = kTok / 2; n; n /= 2, o /= 2) {
+    const bool up = lane & o;
+#pragma unroll
+    for (int j = 0; j < n; ++j)
+      m[j] = amax_join<T>(up ? m[j + n] : m[j], __shfl_xor_sync(mask, up ? m[j] : m[j + n], o));
+  }
+#pragma unroll
+  for (; o; o /= 2) m[0] = amax_join<T>(m[0], __shfl_xor_sync(mask, m[0], o));
+  constexpr int kShare = LANES / kTok;  // lanes that hold one token's maximum
+  float scale, inv;
+  row_scale<STORE>(amax_float<T>(m[0]), &scale, &inv);
+#pragma unroll
+  for (int j = 0; j < kTok; ++j) {
+    const float by = __shfl_sync(mask, inv, j * kShare, LANES);
+    if (to[j] == 0xffffffffu) continue;
+    float x[VE];
     unpack16<T>(raw[j], x);
 #pragma unroll
-    for (int i = 0; i < VE; ++i) x[i] = __fmul_rn(x[i], inv);
+    for (int i = 0; i < VE; ++i) x[i] = __fmul_rn(x[i], by);
     uint8_t* dst = w.codes + (int64_t)to[j] * (LANES * VE) + lane * VE;
     if constexpr (VE == 8) *reinterpret_cast<uint2*>(dst) = make_uint2(Codec<STORE>::code4(x), Codec<STORE>::code4(x + 4));
     else *reinterpret_cast<uint32_t*>(dst) = Codec<STORE>::code4(x);
-    if (lane == j) mine = scale;
+    if (lane == j * kShare) w.scales[to[j]] = scale;
   }
-  if (at != 0xffffffffu) w.scales[at] = mine;
 }
 
 // Any head dim and strides: a warp per row, two passes over it.
