@@ -371,7 +371,8 @@ struct ReadParams {
 // A thread per V codes of one row (V = 16 / element size, or 1) and kReadTok
 // tokens; a CTA's threads run over the heads and dims of a token, so the output
 // is written in order.  Slots past a row's length are zeros and read nothing.  Bound
-// by HBM: the cache of the write's case in 128 us, 6.2 TB/s (one token a thread: 190).
+// by HBM: the cache of the write's case (0.77 GB of codes and values) in 128 us, 6.0
+// TB/s (one token a thread: 190).
 constexpr int kReadTok = 8;
 template <typename T, int STORE, int V>
 __global__ void __launch_bounds__(256) read_kernel(const __grid_constant__ ReadParams p) {
