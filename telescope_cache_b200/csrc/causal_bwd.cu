@@ -203,11 +203,11 @@ __global__ void __launch_bounds__(Shape<kDqCols>::kThreads, 1)
   uint64_t* s_full = v_empty + NV;
   uint64_t* s_free = s_full + 1;     // S in registers
   uint64_t* p_full = s_free + 1;     // [2] dP computed
-  uint64_t* x_full = p_full + 2;     // dX written
-  uint64_t* q_done = x_full + 1;
+  uint64_t* x_full = p_full + 2;     // [2] dX written
+  uint64_t* q_done = x_full + 2;
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(q_done + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
-  static_assert((2 + 2 * NK + 2 * NV + 6) * 8 + 8 <= 256, "barrier area");
+  static_assert((2 + 2 * NK + 2 * NV + 7) * 8 + 8 <= 256, "barrier area");
 
   const CausalParams& c = p.c;
   const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
@@ -233,7 +233,10 @@ __global__ void __launch_bounds__(Shape<kDqCols>::kThreads, 1)
     mbar_init(s_free, Shape<kDqCols>::kWarps);
     mbar_init(&p_full[0], 1);
     mbar_init(&p_full[1], 1);
-    mbar_init(x_full, Shape<kDqCols>::kWarps);
+    // one per dP buffer: a warp may be done with a tile's dX before another is with
+    // the last one's (not two tiles ahead: S of the next waits for s_free of all)
+    mbar_init(&x_full[0], Shape<kDqCols>::kWarps);
+    mbar_init(&x_full[1], Shape<kDqCols>::kWarps);
     mbar_init(q_done, 1);
     *abort_flag = 0;
     mbar_fence_init();
@@ -305,7 +308,7 @@ __global__ void __launch_bounds__(Shape<kDqCols>::kThreads, 1)
         // dP of i + 1 replaces dX of i - 1: behind the product that reads it
         if (!issue_s(i + 1) || !issue_p(i + 1)) break;
       }
-      if (!mbar_wait(x_full, i & 1, abort_flag, status)) break;
+      if (!mbar_wait(&x_full[i & 1], (i >> 1) & 1, abort_flag, status)) break;
       tc_fence_after();
       if (leader) {
         mma_tile_ts<Shape<kDqCols>::kSteps, kDqCols>(tm + kColQ, tm + kColP + (i & 1) * 128,
@@ -352,7 +355,7 @@ __global__ void __launch_bounds__(Shape<kDqCols>::kThreads, 1)
       else dx_columns<T, COLS, true, true>(x_addr, pg, nd2, jlo, jhi);
       tmem_wait_st();
       tc_fence_before();
-      warp_arrive(x_full, lane);
+      warp_arrive(&x_full[i & 1], lane);
     }
     if (alive && i > 0) alive = __all_sync(0xffffffffu, mbar_wait(q_done, 0, abort_flag, status));
     if (alive) {
