@@ -10,6 +10,7 @@ It has the same (out, lse) boundary, so ``apply_attention_sink`` and
 from typing import NamedTuple, Optional, Tuple, Union
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from .. import _lib
 from .attention import _impl_code
@@ -52,6 +53,7 @@ class _Causal(torch.autograd.Function):
         return out, lse
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dout, dlse):
         q, k, v, out, low, lse, starts, ends = ctx.saved_tensors
         if dout is None and dlse is None:

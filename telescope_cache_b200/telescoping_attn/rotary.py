@@ -78,8 +78,9 @@ class _Rotary(torch.autograd.Function):
     def backward(ctx, gq, gk):
         cos, sin, positions = ctx.saved_tensors
         layout, inverse, dtype = ctx.cfg
-        dq, dk = _lib.host(gq).rotary(gq.to(dtype), None if gk is None else gk.to(dtype), cos, sin, positions, layout,
-                                      not inverse)
+        # under create_graph the gradient is differentiated in its turn
+        turn = _Rotary.apply if torch.is_grad_enabled() else _lib.host(gq).rotary
+        dq, dk = turn(gq.to(dtype), None if gk is None else gk.to(dtype), cos, sin, positions, layout, not inverse)
         return dq, dk, None, None, None, None, None
 
 

@@ -313,3 +313,14 @@ def test_segment_bounds(N):
                 assert (int(seg.starts[b, n]), int(seg.ends[b, n])) == (s, e), (b, n)
     pos = seg.positions()
     assert bool((pos >= 0).all()) and torch.equal(pos[2].cpu(), torch.arange(N, dtype=torch.int32))
+
+
+def test_second_derivatives_are_refused():
+    """They are not built: an error, not zeros."""
+    from telescope_cache_b200 import causal_attention
+
+    q, k, v = (t.requires_grad_() for t in inputs(1, 20, 2, 1, 64, 64, torch.float32, seed=2))
+    out, _ = causal_attention(q, k, v)
+    (dq,) = torch.autograd.grad(out.square().sum(), (q,), create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        dq.square().sum().backward()

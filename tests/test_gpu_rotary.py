@@ -156,3 +156,16 @@ def test_agrees_with_apply_rope():
     got, _ = rotary(q, k, cos, sin)
     want = apply_rope(q, torch.arange(40, device="cuda")[None, :, None], cos, sin)
     assert float((got - want).abs().max()) <= 8 * 2.0 ** -24 * float(q.abs().max())
+
+
+def test_second_derivatives():
+    """y = Rx, g = R^T (2 Rx) = 2 x for tables of magnitude one: d(g^2)/dx = 8 x."""
+    from telescope_cache_b200 import rotary, rotary_tables
+
+    cos, sin = rotary_tables(9, 32, device="cuda")
+    q, k = (torch.randn(2, 9, h, 32, device="cuda", requires_grad=True) for h in (4, 2))
+    yq, yk = rotary(q, k, cos, sin)
+    g = torch.autograd.grad(yq.square().sum() + yk.square().sum(), (q, k), create_graph=True)
+    for x, dx in zip((q, k), torch.autograd.grad(sum(t.square().sum() for t in g), (q, k))):
+        # four rotations, each two products and a sum of at most sqrt(2) of the pair's size
+        assert float((dx - 8 * x).abs().max()) <= 4 * 6 * 2.0 ** -24 * 8 * float(x.abs().max()) + 8 * 4 * 2.0 ** -24
