@@ -21,11 +21,12 @@
 //
 // Both passes: warp 0 TMA producer, warp 1 MMA issuer, warps 4-11 compute: a
 // thread owns one TMEM lane (query, or key) and 64 of the tile's 128 columns.
-// P and dX leave as 16-bit pairs in the first 32 of the thread's own 64 columns
-// of S or dP and are the A operands of the accumulating products: they never
-// pass through shared memory.  The MMAs of one thread run in the order of their
-// issue, so the next tile's S (dP) is issued right behind the product that
-// reads P (dX) out of its columns.
+// P and dX leave as 16-bit pairs in tensor memory and are the A operands of the
+// accumulating products: they never pass through shared memory.  Where it is full
+// (dQ pass; dKV pass with HD 128) they take the first half of the thread's own
+// columns of S or dP.  MMAs are ordered only where they share an accumulator and a
+// shape, so there a next tile's S (dP) waits until the product that reads P (dX)
+// out of its columns has completed.
 //
 // dKV pass, TMEM: S^T, dP^T, dV, dK.  Per tile the compute warps work in two
 // halves, exp of S then dX of dP, and the tensor core does the other half's
@@ -95,15 +96,17 @@ __device__ __forceinline__ void p_pair(float2 s, float2 nl2, float kq, float kc,
 // Tile column base + i inside [jlo, jhi)?
 __device__ __forceinline__ bool inside(int i, int jlo, int jhi) { return i >= jlo && i < jhi; }
 
-// dX = pg (dP + nd), or pg dP unless DELTA, of a thread's COLS columns at x_addr, as 16-bit pairs over the
-// first half of them (each 32 are read before they are overwritten).
+// dX = pg (dP + nd), or pg dP unless DELTA, of a thread's COLS columns of dP at
+// d_addr, as 16-bit pairs at x_addr (which may be d_addr: each 32 are read before
+// they are overwritten).
 template <typename T, int COLS, bool MASK, bool DELTA>
-__device__ __forceinline__ void dx_columns(uint32_t x_addr, const float* pg, float2 nd, int jlo, int jhi) {
+__device__ __forceinline__ void dx_columns(uint32_t d_addr, uint32_t x_addr, const float* pg, float2 nd, int jlo,
+                                           int jhi) {
 #pragma unroll
   for (int h = 0; h < COLS / 32; ++h) {
     float dp[32];
     uint32_t w[16];
-    tmem_ld32(x_addr + 32 * h, dp);
+    tmem_ld32(d_addr + 32 * h, dp);
     tmem_wait_ld();
 #pragma unroll
     for (int k = 0; k < 32; k += 2) {
@@ -120,11 +123,11 @@ __device__ __forceinline__ void dx_columns(uint32_t x_addr, const float* pg, flo
   }
 }
 
-// P of a thread's COLS columns at s_addr (scores already in pg), as 16-bit pairs
-// over the first half of them; pg becomes P softcap'.  With the softcap nl holds
-// -lse2 per column; without it the scores come as s - lse / scale.
+// P of a thread's COLS columns (scores in pg), as 16-bit pairs at p_addr; pg
+// becomes P softcap'.  With the softcap nl holds -lse2 per column; without it the
+// scores come as s - lse / scale.
 template <typename T, int COLS, bool CAP, bool MASK>
-__device__ __forceinline__ void p_columns_t(uint32_t s_addr, float* pg, const float* nl, float kq, float kc, int jlo,
+__device__ __forceinline__ void p_columns_t(uint32_t p_addr, float* pg, const float* nl, float kq, float kc, int jlo,
                                             int jhi) {
 #pragma unroll
   for (int h = 0; h < COLS / 32; ++h) {
@@ -152,7 +155,7 @@ __device__ __forceinline__ void p_columns_t(uint32_t s_addr, float* pg, const fl
         x[1] = g.y;
       }
     }
-    tmem_st16u(s_addr + 16 * h, w);
+    tmem_st16u(p_addr + 16 * h, w);
   }
 }
 
@@ -305,8 +308,10 @@ __global__ void __launch_bounds__(Shape<kDqCols>::kThreads, 1)
     for (int i = 0; ok && i < n; ++i) {
       if (i + 1 < n) {
         if (!mbar_wait(s_free, i & 1, abort_flag, status)) break;
-        // dP of i + 1 replaces dX of i - 1: behind the product that reads it
-        if (!issue_s(i + 1) || !issue_p(i + 1)) break;
+        if (!issue_s(i + 1)) break;
+        // dP of i + 1 replaces dX of i - 1: the product that reads it has completed
+        if (i > 0 && !mbar_wait(&k_empty[(i - 1) % NK], ((i - 1) / NK) & 1, abort_flag, status)) break;
+        if (!issue_p(i + 1)) break;
       }
       if (!mbar_wait(&x_full[i & 1], (i >> 1) & 1, abort_flag, status)) break;
       tc_fence_after();
@@ -351,8 +356,10 @@ __global__ void __launch_bounds__(Shape<kDqCols>::kThreads, 1)
       alive = __all_sync(0xffffffffu, mbar_wait(&p_full[i & 1], (i >> 1) & 1, abort_flag, status));
       if (!alive) break;
       tc_fence_after();
-      if (__all_sync(0xffffffffu, jlo <= 0 && jhi >= COLS)) dx_columns<T, COLS, false, true>(x_addr, pg, nd2, jlo, jhi);
-      else dx_columns<T, COLS, true, true>(x_addr, pg, nd2, jlo, jhi);
+      if (__all_sync(0xffffffffu, jlo <= 0 && jhi >= COLS))
+        dx_columns<T, COLS, false, true>(x_addr, x_addr, pg, nd2, jlo, jhi);
+      else
+        dx_columns<T, COLS, true, true>(x_addr, x_addr, pg, nd2, jlo, jhi);
       tmem_wait_st();
       tc_fence_before();
       warp_arrive(&x_full[i & 1], lane);
@@ -384,7 +391,11 @@ __global__ void __launch_bounds__(Shape<kDkvCols>::kThreads, 1)
   using Z = BwdSmem<HD>;
   using Z2 = Shape<kDkvCols>;
   constexpr int TB = Z::kTile, NQ = Z::kNQ;
-  constexpr uint32_t kColP = 128, kColV = 256, kColK = 256 + HD;  // S^T, dP^T, dV, dK
+  constexpr uint32_t kColD = 128, kColV = 256, kColK = 256 + HD;  // S^T, dP^T, dV, dK
+  // P^T, dX^T: columns of their own, or the first halves of each thread's S^T, dP^T
+  constexpr bool kOwnP = HD == 64;
+  constexpr uint32_t kColP = kOwnP ? 256 + 2 * HD : 0, kColX = kOwnP ? kColP + 64 : kColD;
+  constexpr int kStepP = kOwnP ? kDkvCols / 2 : kDkvCols;  // from one part's pairs to the next's
   extern __shared__ uint8_t smem_raw[];
   uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* one_s = sm;                // [2] ones that pick -lse / scale (dims 0-2) and -Delta (3-5) out of aug_s
@@ -406,10 +417,11 @@ __global__ void __launch_bounds__(Shape<kDkvCols>::kThreads, 1)
   uint64_t* p_full = s_full + 1;    // P^T written
   uint64_t* d_full = p_full + 1;    // dP^T computed
   uint64_t* x_full = d_full + 1;    // dX^T written
-  uint64_t* done = x_full + 1;
+  uint64_t* v_done = x_full + 1;    // P^T read by its product
+  uint64_t* done = v_done + 1;
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(done + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
-  static_assert((2 + 5 * NQ + 5) * 8 + 8 <= 256, "barrier area");
+  static_assert((2 + 5 * NQ + 6) * 8 + 8 <= 256, "barrier area");
 
   const CausalParams& c = p.c;
   const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
@@ -436,6 +448,7 @@ __global__ void __launch_bounds__(Shape<kDkvCols>::kThreads, 1)
     mbar_init(p_full, Z2::kWarps);
     mbar_init(d_full, 1);
     mbar_init(x_full, Z2::kWarps);
+    mbar_init(v_done, 1);
     mbar_init(done, 1);
     *abort_flag = 0;
     mbar_fence_init();
@@ -499,8 +512,8 @@ __global__ void __launch_bounds__(Shape<kDkvCols>::kThreads, 1)
       if (!mbar_wait(&g_full[i % NQ], (i / NQ) & 1, abort_flag, status)) return false;
       tc_fence_after();
       if (leader) {
-        mma_tile_ss<HD>(tm + kColP, vd, gd0 + (((i % NQ) * TB) >> 4), kIdS);
-        mma_aug(tm + kColP, one0 + (kAugTile >> 4), aug0 + (((i % NQ) * kAugTile) >> 4));
+        mma_tile_ss<HD>(tm + kColD, vd, gd0 + (((i % NQ) * TB) >> 4), kIdS);
+        mma_aug(tm + kColD, one0 + (kAugTile >> 4), aug0 + (((i % NQ) * kAugTile) >> 4));
         mma_commit(d_full);
       }
       return true;
@@ -511,16 +524,21 @@ __global__ void __launch_bounds__(Shape<kDkvCols>::kThreads, 1)
       const int st = i % NQ;
       if (!mbar_wait(p_full, i & 1, abort_flag, status)) break;
       tc_fence_after();
-      if (leader) mma_tile_ts<Z2::kSteps, kDkvCols>(tm + kColV, tm, gt0 + ((st * TB) >> 4), kIdA, i > 0 ? 1u : 0u);
-      if (i + 1 < un && !issue_s(i + 1)) break;
+      if (leader) {
+        mma_tile_ts<Z2::kSteps, kStepP>(tm + kColV, tm + kColP, gt0 + ((st * TB) >> 4), kIdA, i > 0 ? 1u : 0u);
+        if constexpr (!kOwnP) mma_commit(v_done);
+      }
+      // HD 128: S of i + 1 replaces P of i
+      if (i + 1 < un && ((!kOwnP && !mbar_wait(v_done, i & 1, abort_flag, status)) || !issue_s(i + 1))) break;
       if (!mbar_wait(x_full, i & 1, abort_flag, status)) break;
       tc_fence_after();
       if (leader) {
-        mma_tile_ts<Z2::kSteps, kDkvCols>(tm + kColK, tm + kColP, qt0 + ((st * TB) >> 4), kIdA, i > 0 ? 1u : 0u);
+        mma_tile_ts<Z2::kSteps, kStepP>(tm + kColK, tm + kColX, qt0 + ((st * TB) >> 4), kIdA, i > 0 ? 1u : 0u);
         mma_commit(&q_empty[st]);
         if (i + 1 == un) mma_commit(done);
       }
-      if (i + 1 < un) ok = issue_d(i + 1);
+      // HD 128: dP of i + 1 replaces dX of i
+      if (i + 1 < un) ok = (kOwnP || mbar_wait(&q_empty[st], (i / NQ) & 1, abort_flag, status)) && issue_d(i + 1);
     }
   } else if (warp < 4) {
     // the tile's per-query numbers, two queries a thread
@@ -566,7 +584,8 @@ __global__ void __launch_bounds__(Shape<kDkvCols>::kThreads, 1)
     const int r = (threadIdx.x - 128) & 127, k = k0 + r;
     const bool row_ok = k < c.N;
     const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t s_addr = tmem + lane_base + part * COLS, x_addr = s_addr + kColP;
+    const uint32_t s_addr = tmem + lane_base + part * COLS, d_addr = s_addr + kColD;
+    const uint32_t p_addr = tmem + lane_base + kColP + part * kStepP, x_addr = tmem + lane_base + kColX + part * kStepP;
     const int qend = row_ok ? query_end(c, b, k) : 0;
     bool alive = true;
     int i = 0;
@@ -582,8 +601,8 @@ __global__ void __launch_bounds__(Shape<kDkvCols>::kThreads, 1)
       float pg[COLS];
       tmem_ld<COLS>(s_addr, pg);
       tmem_wait_ld();
-      if (interior) p_columns_t<T, COLS, CAP, false>(s_addr, pg, nl, p.kq, p.kc, jlo, jhi);
-      else p_columns_t<T, COLS, CAP, true>(s_addr, pg, nl, p.kq, p.kc, jlo, jhi);
+      if (interior) p_columns_t<T, COLS, CAP, false>(p_addr, pg, nl, p.kq, p.kc, jlo, jhi);
+      else p_columns_t<T, COLS, CAP, true>(p_addr, pg, nl, p.kq, p.kc, jlo, jhi);
       tmem_wait_st();
       tc_fence_before();
       if constexpr (CAP) warp_arrive(&i_empty[st], lane);
@@ -591,8 +610,8 @@ __global__ void __launch_bounds__(Shape<kDkvCols>::kThreads, 1)
       alive = __all_sync(0xffffffffu, mbar_wait(d_full, i & 1, abort_flag, status));
       if (!alive) break;
       tc_fence_after();
-      if (interior) dx_columns<T, COLS, false, false>(x_addr, pg, make_float2(0.f, 0.f), jlo, jhi);
-      else dx_columns<T, COLS, true, false>(x_addr, pg, make_float2(0.f, 0.f), jlo, jhi);
+      if (interior) dx_columns<T, COLS, false, false>(d_addr, x_addr, pg, make_float2(0.f, 0.f), jlo, jhi);
+      else dx_columns<T, COLS, true, false>(d_addr, x_addr, pg, make_float2(0.f, 0.f), jlo, jhi);
       tmem_wait_st();
       tc_fence_before();
       warp_arrive(x_full, lane);

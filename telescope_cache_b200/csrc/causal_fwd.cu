@@ -13,11 +13,11 @@
 //               and sum in fp32 (log2 units, O rescaled only when the maximum
 //               grew by more than 2^8), P rounded to the operand type for the
 //               second product, O / l, lse.
-// TMEM: S_A, S_B (128 columns each), O_A, O_B (HD each).  P_X takes the first 64
-// columns of S_X (16-bit pairs).  S_X of the next tile is issued right behind
-// PV_X: the MMAs of one thread run in the order of their issue, so it overwrites
-// P_X only after PV_X has read it, and its commit covers PV_X (O_X is current
-// when the softmax wakes).
+// TMEM: S_A, S_B (128 columns each), O_A, O_B (HD each), P_A, P_B (64: 16-bit pairs).
+// With HD 128 the first four fill it, and P_X takes the first half of S_X.  MMAs are
+// ordered only where they share an accumulator and a shape, so there the next S_X
+// waits for PV_X to complete before it overwrites P_X.  The commit of S_X covers the
+// PV_X before it: when the softmax wakes O_X is current and the last P_X read.
 //
 // A query tile's keys run from the first key of its first row (starts do not
 // descend) to the diagonal; tiles in between need no mask.  The heaviest blocks
@@ -141,6 +141,8 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
                       const __grid_constant__ CUtensorMap tmv, const __grid_constant__ FwdParams p) {
   using Z = FwdSmem<HD>;
   constexpr int TB = Z::kTile, NS = Z::kStages, BLK = 128 * 128;
+  constexpr bool kOwnP = HD == 64;  // columns of P: its own, or S's
+  constexpr uint32_t kColP = kOwnP ? 256 + 2 * HD : 0, kStepP = kOwnP ? 64 : 128;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* q_s = sm;             // [2] Q tiles
@@ -154,10 +156,11 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
   uint64_t* v_empty = v_full + NS;   // [NS]
   uint64_t* s_full = v_empty + NS;   // [2]
   uint64_t* p_full = s_full + 2;     // [2]
-  uint64_t* o_done = p_full + 2;     // [2]
+  uint64_t* pv_done = p_full + 2;    // [2] P read: the next S may overwrite it
+  uint64_t* o_done = pv_done + 2;    // [2]
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(o_done + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
-  static_assert((8 + 4 * NS) * 8 + 8 <= 256, "barrier area");
+  static_assert((10 + 4 * NS) * 8 + 8 <= 256, "barrier area");
 
   const CausalParams& c = p.c;
   const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
@@ -176,6 +179,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
       mbar_init(&q_full[i], 1);
       mbar_init(&s_full[i], 1);
       mbar_init(&p_full[i], 4);
+      mbar_init(&pv_done[i], 1);
       mbar_init(&o_done[i], 1);
     }
     for (int i = 0; i < NS; ++i) {
@@ -231,16 +235,24 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
               ub1 = uniform(has_b ? bhi : 0), u0 = uniform(j0), u1 = uniform(j1);
     const bool leader = elect_one();
     int np0 = 0, np1 = 0;
-    auto issue_s = [&](int x, int st) {
+    auto issue_s = [&](int x, int np, int st) -> bool {  // behind the tile's np products with V
+      if (!kOwnP && np > 0) {
+        if (!mbar_wait(&pv_done[x], (np - 1) & 1, abort_flag, status)) return false;
+        tc_fence_after();
+      }
       if (leader) {
         mma_tile_ss<HD>(tm + x * 128, qd0 + ((x * TB) >> 4), kd0 + ((st * TB) >> 4), kIdS);
         mma_commit(&s_full[x]);
       }
+      return true;
     };
     auto issue_pv = [&](int x, int& np, int st) -> bool {
       if (!mbar_wait(&p_full[x], np & 1, abort_flag, status)) return false;
       tc_fence_after();
-      if (leader) mma_tile_ts<8, 64>(tm + 256 + x * HD, tm + x * 128, vd0 + ((st * TB) >> 4), kIdO, np > 0 ? 1u : 0u);
+      if (leader) {
+        mma_tile_ts<8, 64>(tm + 256 + x * HD, tm + kColP + x * kStepP, vd0 + ((st * TB) >> 4), kIdO, np > 0 ? 1u : 0u);
+        if constexpr (!kOwnP) mma_commit(&pv_done[x]);
+      }
       ++np;
       return true;
     };
@@ -253,8 +265,8 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
     if (ok && ub0 < ub1) ok = mbar_wait(&q_full[1], 0, abort_flag, status);
     tc_fence_after();
     if (ok) {
-      if (u0 >= ua0 && u0 < ua1) issue_s(0, 0);
-      if (u0 >= ub0 && u0 < ub1) issue_s(1, 0);
+      if (u0 >= ua0 && u0 < ua1) issue_s(0, 0, 0);
+      if (u0 >= ub0 && u0 < ub1) issue_s(1, 0, 0);
       commit(&k_empty[0]);
     }
     for (int j = u0, i = 0; ok && j < u1; ++j, ++i) {
@@ -262,11 +274,11 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
       if (j + 1 < u1 && !mbar_wait(&k_full[st1], ((i + 1) / NS) & 1, abort_flag, status)) break;
       if (!mbar_wait(&v_full[st], (i / NS) & 1, abort_flag, status)) break;
       if (j >= ua0 && j < ua1 && !issue_pv(0, np0, st)) break;
-      if (j + 1 >= ua0 && j + 1 < ua1) issue_s(0, st1);
+      if (j + 1 >= ua0 && j + 1 < ua1 && !issue_s(0, np0, st1)) break;
       if (ua0 < ua1 && j + 1 == ua1) commit(&o_done[0]);
       if (j >= ub0 && j < ub1 && !issue_pv(1, np1, st)) break;
       commit(&v_empty[st]);
-      if (j + 1 >= ub0 && j + 1 < ub1) issue_s(1, st1);
+      if (j + 1 >= ub0 && j + 1 < ub1 && !issue_s(1, np1, st1)) break;
       if (ub0 < ub1 && j + 1 == ub1) commit(&o_done[1]);
       if (j + 1 < u1) commit(&k_empty[st1]);
     }
@@ -278,6 +290,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
     const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t s_addr = tmem + lane_base + x * 128;
     const uint32_t o_addr = tmem + lane_base + 256 + x * HD;
+    const uint32_t p_addr = tmem + lane_base + kColP + x * kStepP;
     const int first = row_ok ? first_key(c, b, q) : 1, end = row_ok ? q + 1 : 0;
     const int lo = x ? blo : alo, hi = x ? bhi : ahi;
     float m_used = -INFINITY, ell = 0.f;
@@ -372,8 +385,8 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
           else if (mode == kS9) ts += half_p<T, kS9>(interior, sv, c0, p, m_eff, jlo, jhi, pw);
           else ts += half_p<T, kTanh>(interior, sv, c0, p, m_eff, jlo, jhi, pw);
         }
-        tmem_st16u(s_addr + c0 / 2, pw);
-        tmem_st16u(s_addr + c0 / 2 + 16, pw + 16);
+        tmem_st16u(p_addr + c0 / 2, pw);
+        tmem_st16u(p_addr + c0 / 2 + 16, pw + 16);
       }
       ell += ts;
       tmem_wait_st();
