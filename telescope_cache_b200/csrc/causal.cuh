@@ -31,14 +31,15 @@ struct CausalParams {
 };
 
 // First key that query n of row b sees (its last is n itself); n + 1 where it
-// sees none.  Nondecreasing in n.
+// sees none.  Nondecreasing in n.  Bounds may come from the caller: kept inside
+// the row, where every tile that they lead to can be read.
 __device__ __forceinline__ int first_key(const CausalParams& p, int b, int n) {
-  return p.starts ? __ldg(p.starts + (int64_t)b * p.N + n) : 0;
+  return p.starts ? max(__ldg(p.starts + (int64_t)b * p.N + n), 0) : 0;
 }
 // End of the queries that see key n (the first is n itself); n where none do.
 // Nondecreasing in n.
 __device__ __forceinline__ int query_end(const CausalParams& p, int b, int n) {
-  return p.ends ? __ldg(p.ends + (int64_t)b * p.N + n) : p.N;
+  return p.ends ? min(__ldg(p.ends + (int64_t)b * p.N + n), p.N) : p.N;
 }
 
 bool causal_tc_supported(const CausalParams& p, int dtype);

@@ -172,7 +172,8 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
   key_tiles(c, b, q0, &alo, &ahi);
   key_tiles(c, b, q0 + 128, &blo, &bhi);
   const bool has_a = alo < ahi, has_b = blo < bhi;
-  const int j0 = has_a ? alo : blo, j1 = has_b ? bhi : ahi;  // starts do not descend: A's first tile is no later
+  // every tile that A or B waits for is issued, even if the caller's starts descend
+  const int j0 = has_a && has_b ? min(alo, blo) : has_a ? alo : blo, j1 = has_b ? bhi : ahi;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {

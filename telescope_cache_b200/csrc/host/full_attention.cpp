@@ -182,6 +182,7 @@ void causal_args(Causal& c, const Tensor& q, const Tensor& k, const Tensor& v, c
   CHECK_VALUE(q.scalar_type() == k.scalar_type() && q.scalar_type() == v.scalar_type(),
                     "q, k, v must share a dtype, got ", q.scalar_type(), ", ", k.scalar_type(), ", ", v.scalar_type());
   CHECK_VALUE(!softcap || *softcap > 0, "softcap must be positive, got ", softcap.value_or(0.));
+  CHECK_VALUE(starts.has_value() == ends.has_value(), "segment starts and ends go together");
   cuda(q);
   same_device(q, k);
   same_device(q, v);

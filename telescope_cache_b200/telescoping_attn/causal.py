@@ -18,7 +18,8 @@ from .attention import _impl_code
 
 class Segments(NamedTuple):
     """Bounds of the packed examples (segment_bounds): token n of row b sees
-    tokens starts[b, n] .. n and is seen by tokens n .. ends[b, n] - 1."""
+    tokens starts[b, n] .. n and is seen by tokens n .. ends[b, n] - 1.  Neither
+    descends along a row; what lies outside the row is cut off at its ends."""
 
     starts: torch.Tensor
     ends: torch.Tensor
