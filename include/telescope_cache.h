@@ -639,7 +639,7 @@ typedef struct tc_causal_args {
 /* Causal attention with grouped heads over packed examples: token n of a row
  * attends tokens [starts[n], n] of the row.  logit = c tanh(x / c),
  * x = scale q.k (x without softcap).  bf16 / f16 with Dk = Dv = 64 or 128 and
- * 16-byte aligned strides run on the tensor cores. */
+ * 16-byte aligned tensors and strides run on the tensor cores. */
 int tc_causal_fwd(const tc_causal_args* a, void* stream);
 /* Its gradients, the lse's among the incoming ones; deterministic. */
 int tc_causal_bwd(const tc_causal_args* a, void* stream);

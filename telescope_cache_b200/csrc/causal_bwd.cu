@@ -672,7 +672,8 @@ int dispatch_bwd(const CausalParams& a, int dtype, cudaStream_t st) {
 }  // namespace
 
 bool causal_bwd_tc_supported(const CausalParams& p, int dtype) {
-  return ctc::tc_shape(p, dtype) && (uintptr_t)p.dout % 16 == 0;
+  return ctc::tc_shape(p, dtype) &&
+         ((uintptr_t)p.dout | (uintptr_t)p.dq | (uintptr_t)p.dk | (uintptr_t)p.dv) % 16 == 0;
 }
 
 int causal_bwd_tc(const CausalParams& p, int dtype, cudaStream_t st) {

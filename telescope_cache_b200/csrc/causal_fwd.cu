@@ -472,7 +472,10 @@ int dispatch_fwd(const CausalParams& a, int dtype, cudaStream_t st) {
 
 }  // namespace
 
-bool causal_tc_supported(const CausalParams& p, int dtype) { return ctc::tc_shape(p, dtype); }
+// The results leave as 16-byte pieces (out_low may be null).
+bool causal_tc_supported(const CausalParams& p, int dtype) {
+  return ctc::tc_shape(p, dtype) && ((uintptr_t)p.out | (uintptr_t)p.out_low) % 16 == 0;
+}
 
 int causal_fwd_tc(const CausalParams& p, int dtype, cudaStream_t st) {
   return dtype == TC_BF16 ? dispatch_fwd<__nv_bfloat16>(p, dtype, st) : dispatch_fwd<__half>(p, dtype, st);

@@ -6,7 +6,8 @@ Tolerances are test_gpu_causal.py's, by check_forward and check_grads."""
 import pytest
 import torch
 
-from test_gpu_causal import DT, check_forward, ids_of, inputs
+from full_attention_reference import rel, visible
+from test_gpu_causal import DT, check_forward, grad_tol, ids_of, inputs
 
 pytestmark = pytest.mark.gpu
 
@@ -59,3 +60,40 @@ def test_starts_and_ends_go_together():
     for seg in (Segments(n, None), Segments(None, n)):
         with pytest.raises(ValueError, match="go together"):
             causal_attention(q, k, v, seq_idx=seg)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_c_entries_take_any_address(D):
+    """Results one element off a 16-byte boundary: the forward's out and what its
+    rounding left over, the backward's three gradients, one at a time."""
+    from telescope_cache_b200 import _lib
+
+    dt, B, N, Hq, Hkv = torch.bfloat16, 1, 200, 4, 2
+    q, k, v = inputs(B, N, Hq, Hkv, D, D, dt, seed=31)
+    lib, stream = _lib.lib(), torch.cuda.current_stream().cuda_stream
+    strides = {f"{n}_stride_{a}": t.stride(i) for n, t in (("q", q), ("k", k), ("v", v)) for i, a in enumerate("bnh")}
+    args = _lib.CausalArgs(B=B, N=N, Hq=Hq, Hkv=Hkv, Dk=D, Dv=D, dtype=_lib.dtype_code(dt), scale=D ** -0.5,
+                           q=q.data_ptr(), k=k.data_ptr(), v=v.data_ptr(), **strides)
+    gout = torch.randn_like(q)
+
+    def run(off):  # the named results start one element late
+        def room(name, *shape, dtype=dt):
+            n = torch.Size(shape).numel()
+            return torch.empty(n + 8, device="cuda", dtype=dtype)[int(name == off):][:n].view(shape)
+
+        r = {n: room(n, B, N, Hq, D) for n in ("out", "out_low", "dq")} | {n: room(n, B, N, Hkv, D) for n in ("dk", "dv")}
+        lse, delta = (torch.empty(B, N, Hq, device="cuda") for _ in range(2))
+        for n, t in r.items():
+            setattr(args, n, t.data_ptr())
+        args.lse, args.delta, args.o, args.o_low, args.dout = (t.data_ptr() for t in (lse, delta, r["out"], r["out_low"], gout))
+        assert lib.tc_causal_fwd(args, stream) == 0 and lib.tc_causal_bwd(args, stream) == 0
+        torch.cuda.synchronize()
+        return r, lse
+
+    base, base_lse = run(None)
+    check_forward(base["out"], base_lse, q, k, v, visible(None, B, N, "cuda"))
+    for off in base:
+        got, lse = run(off)
+        check_forward(got["out"], lse, q, k, v, visible(None, B, N, "cuda"))
+        for n in ("dq", "dk", "dv"):
+            assert rel(got[n], base[n].double()) <= 2 * grad_tol(dt)
