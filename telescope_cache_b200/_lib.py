@@ -237,6 +237,9 @@ def host(t):
         if _HOST is None:
             _load_host()
         require_cuda(t)
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("telescope_cache_b200: make a first call on the device before a capture "
+                               "(it allocates the device status word)")
         from .telescoping_attn.attention import device_status
 
         _HOST.set_status(device_status(t.device))

@@ -17,7 +17,6 @@
 #include <map>
 #include <stdexcept>
 #include <tuple>
-#include <vector>
 
 #include "../../../include/telescope_cache.h"
 
@@ -342,30 +341,28 @@ std::tuple<Tensor, Tensor> kv_read(const Tensor& ck, const Tensor& cv, const Ten
   return {k, v};
 }
 
-// Workspace of the split attention: one per device and stream, since calls on one
-// stream run in order.  The arrival counts are zero between calls.  Never freed:
-// the process may end after the CUDA context, and a captured graph goes on using
-// the workspace it was captured with, so one that was outgrown is kept too (each
-// is at least twice the one before).
+// Workspace of the split attention: scratch, and arrival counts that are zero
+// between calls.  One per device and stream, since calls on one stream run in
+// order; not freed, for the process may end after the CUDA context.  A captured call
+// replays on any stream, next to any other: it has a workspace of its own from the
+// graph's memory, whose counts the graph clears.
 struct Work {
   Tensor scratch, counts;
-  std::vector<Tensor> outgrown;
 };
-Work& workspace(const Tensor& on, cudaStream_t stream, int64_t floats, int64_t counts) {
+Work workspace(const Tensor& on, cudaStream_t stream, int64_t floats, int64_t counts) {
+  const auto f32 = on.options().dtype(at::kFloat), i32 = on.options().dtype(at::kInt);
+  if (at::cuda::currentStreamCaptureStatusMayInitCtx() != at::cuda::CaptureStatus::None) {
+    Work own{at::empty({floats}, f32), at::empty({counts}, i32)};
+    CHECK_RUN(cudaMemsetAsync(own.counts.data_ptr(), 0, counts * sizeof(int32_t), stream) == cudaSuccess,
+              "cached attention: clearing the arrival counts failed");
+    return own;
+  }
   static auto* all = new std::map<std::pair<int, cudaStream_t>, Work>;
   Work& w = (*all)[{on.device().index(), stream}];
-  const bool grow = floats > 0 && (!w.scratch.defined() || w.scratch.numel() < floats);
-  const bool more = !w.counts.defined() || w.counts.numel() < counts;
-  CHECK_RUN(!(grow || more) || at::cuda::currentStreamCaptureStatusMayInitCtx() == at::cuda::CaptureStatus::None,
-              "cached attention: run a call of this size on the stream before its capture (it allocates a workspace)");
-  if (grow) {
-    if (w.scratch.defined()) w.outgrown.push_back(w.scratch);
-    w.scratch = at::empty({w.scratch.defined() ? std::max(floats, 2 * w.scratch.numel()) : floats}, on.options().dtype(at::kFloat));
-  }
-  if (more) {
-    if (w.counts.defined()) w.outgrown.push_back(w.counts);
-    w.counts = at::zeros({std::max<int64_t>(counts, w.counts.defined() ? 2 * w.counts.numel() : 4096)}, on.options().dtype(at::kInt));
-  }
+  if (!w.scratch.defined() || w.scratch.numel() < floats)
+    w.scratch = at::empty({w.scratch.defined() ? std::max(floats, 2 * w.scratch.numel()) : floats}, f32);
+  if (!w.counts.defined() || w.counts.numel() < counts)
+    w.counts = at::zeros({std::max<int64_t>(counts, w.counts.defined() ? 2 * w.counts.numel() : 4096)}, i32);
   return w;
 }
 
@@ -435,9 +432,12 @@ std::tuple<Tensor, Tensor, OptTensor, OptTensor> kv_attend(const Tensor& ck, con
   }
   const int64_t floats = tc_kv_attend_scratch_floats(&c, a.B, a.Hq, a.max_tokens);
   const int64_t counts = B * (c.Hkv * ((Hq / c.Hkv + 7) / 8) + 1);
-  Work& w = workspace(q, call.stream, floats, counts);
-  if (floats > 0) a.scratch = w.scratch.data_ptr<float>(), a.scratch_floats = w.scratch.numel();
-  a.counters = w.counts.data_ptr<int32_t>(), a.num_counters = w.counts.numel();
+  Work w;
+  if (B > 0 && floats >= 0 && (floats > 0 || (step && advance))) {
+    w = workspace(q, call.stream, floats, counts);
+    a.scratch = w.scratch.data_ptr<float>(), a.scratch_floats = w.scratch.numel();
+    a.counters = w.counts.data_ptr<int32_t>(), a.num_counters = w.counts.numel();
+  }
   done(tc_kv_attend(&c, &a, call.stream), "tc_kv_attend");
   return {out, lse, stored && step ? OptTensor(k_new) : std::nullopt, stored && step ? OptTensor(v_new) : std::nullopt};
 }
