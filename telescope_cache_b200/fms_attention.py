@@ -276,6 +276,7 @@ class FullMultiHeadAttention(nn.Module):
         if use_gate:
             self.gate_proj = nn.Linear(emb_dim, nheads * emb_v, bias=False)
         self._rope: Tuple[int, Optional[torch.Tensor], Optional[torch.Tensor]] = (0, None, None)
+        self._outgrown = []
         self.reset_parameters()
 
     def reset_parameters(self):
@@ -288,10 +289,20 @@ class FullMultiHeadAttention(nn.Module):
             self.sinks.data.zero_()
 
     def _tables(self, n_pos, device):
+        """cos, sin of at least n_pos positions, for any later call: ordinary tensors
+        even under inference_mode, there for every stream, and never freed (a
+        captured step goes on reading the tables of its capture)."""
         have, cos, sin = self._rope
         if cos is None or have < n_pos or cos.device != device:
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError(f"rotary tables of {n_pos} positions have to be formed: make a call of this length "
+                                   "before a capture")
+            if cos is not None:
+                self._outgrown.append((cos, sin))
             have = max(n_pos, 2 * have)
-            cos, sin = rotary_tables(have, self.rope_dim, self.rope_base, device=device, **self.rope_scaling)
+            with torch.inference_mode(False):
+                cos, sin = rotary_tables(have, self.rope_dim, self.rope_base, device=device, **self.rope_scaling)
+            torch.cuda.current_stream(device).synchronize()
             self._rope = (have, cos, sin)
         return cos, sin
 
@@ -334,9 +345,10 @@ class FullMultiHeadAttention(nn.Module):
     @torch.no_grad()
     def decode(self, x_t: torch.Tensor, cache: KVCache) -> torch.Tensor:
         """One token of every sequence, x_t [B, 1, emb_dim] -> [B, 1, emb_dim]: its
-        key and value join the cache, at the end of each row."""
+        key and value join the cache, at the end of each row.  May be captured into
+        a CUDA graph after a first call with the cache."""
         q, k, v = self._qkv(x_t)
-        cos, sin = self._tables(cache.max_length + 1, x_t.device)
+        cos, sin = self._tables(cache.capacity, x_t.device)  # a replayed step may reach every slot
         out, lse = cached_attention_step(q, k, v, cache, rope_cos=cos, rope_sin=sin, layout=self.rope_layout,
                                          softcap=self.softcap)
         return self._finish(out, lse, x_t)
