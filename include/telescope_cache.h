@@ -562,7 +562,8 @@ typedef struct tc_kv_write_args {
                                 and was dropped                              */
 } tc_kv_write_args;
 
-/* Quantise keys and values into the cache and move the rows' lengths on. */
+/* Quantise keys and values into the cache and move the rows' lengths on.  fresh
+ * with N 0 and no seq_idx: rows 0 .. B - 1 become empty. */
 int tc_kv_write(const tc_kv_cache* c, const tc_kv_write_args* a, void* stream);
 
 /* The values that the first `length` slots of every row stand for, as

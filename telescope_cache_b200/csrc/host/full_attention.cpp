@@ -313,6 +313,7 @@ void kv_write(const Tensor& ck, const Tensor& cv, const Tensor& cks, const Tenso
     CHECK_VALUE(seq_idx->dim() == 2 && seq_idx->size(0) == B && seq_idx->size(1) == N && integral(*seq_idx),
                       "seq_idx must be an integer tensor [", B, ", ", N, "], got ", seq_idx->sizes(), " ", seq_idx->scalar_type());
     same_device(ck, *seq_idx);
+    if (B * N == 0) return;  // names no row
   }
   Call call(k0);
   if (seq_idx) {

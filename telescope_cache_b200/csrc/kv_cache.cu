@@ -1267,6 +1267,10 @@ void split_rule(int64_t most, int64_t heads, int B, int* chunk, int* splits) {
 
 extern "C" int tc_kv_write(const tc_kv_cache* c, const tc_kv_write_args* a, void* stream) {
   if (!cache_ok(c) || !a || a->B < 0 || a->N < 0) return TC_ERR_ARG;
+  if (a->N == 0 && a->B > 0 && a->fresh && !a->seq_idx) {  // B prompts of no tokens
+    if (a->B > c->rows) return TC_ERR_ARG;
+    return cudaMemsetAsync(c->lengths, 0, a->B * sizeof(int32_t), (cudaStream_t)stream) == cudaSuccess ? TC_OK : TC_ERR_CUDA;
+  }
   if ((int64_t)a->B * a->N == 0) return TC_OK;
   if (!a->k || !a->v || (a->seq_idx && !a->starts) || (!a->seq_idx && a->B > c->rows)) return TC_ERR_ARG;
   WriteParams p;
