@@ -1154,9 +1154,9 @@ __global__ void __launch_bounds__(kAnyThreads) attend_any(AttendParams p) {
       float xl = warp_sum(s) * p.ks[at] * p.qscale;
       if (p.has_cap) xl = p.softcap * tanhf(xl / p.softcap);
       xl *= kLog2e;
-      const float mn = fmaxf(m, xl);
+      const float mn = fmaxf(m, xl), ref = mn == -INFINITY ? 0.f : mn;
       const float cm = m == mn ? 1.f : exp2f(m - mn);
-      const float pr = exp2f(xl - mn);
+      const float pr = exp2f(xl - ref);  // a NaN logit: NaN, with the maximum as it was
       ell = ell * cm + pr;
       m = mn;
       const float w = pr * p.vs[at];
@@ -1173,16 +1173,14 @@ __global__ void __launch_bounds__(kAnyThreads) attend_any(AttendParams p) {
       l_s[warp] = ell;
     }
     __syncthreads();
-    float M = fmaxf(fmaxf(m_s[0], m_s[1]), fmaxf(m_s[2], m_s[3]));
+    const float M = fmaxf(fmaxf(m_s[0], m_s[1]), fmaxf(m_s[2], m_s[3])), ref = M == -INFINITY ? 0.f : M;
     for (int d = threadIdx.x; d < p.Dv; d += kAnyThreads) {
       float l = 0.f, ov = 0.f;
-      if (M > -INFINITY) {
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          const float c = exp2f(m_s[w] - M);
-          l += c * l_s[w];
-          ov += c * o_s[w][d];
-        }
+      for (int w = 0; w < 4; ++w) {  // no tokens: 0; NaN logits alone: NaN
+        const float c = exp2f(m_s[w] - ref);
+        l += c * l_s[w];
+        ov += c * o_s[w][d];
       }
       if (active == 1) {
         const int64_t hq = (int64_t)b * p.Hq + hkv * p.E + e0 + e;

@@ -33,3 +33,42 @@ def test_a_fresh_prompt_of_no_tokens_empties_its_rows():
     assert c.lengths.tolist() == [1, 1, 1, 1]
     held = quantise(v, "int8")[2]  # one token: the value as held
     assert float((out.cpu().double() - held).abs().max()) <= 2.0 ** -18 * float(held.abs().max())
+
+
+@pytest.mark.parametrize("dtype,D", [("bf16", 80), ("f32", 80), ("f16", 128), ("bf16", 64)])
+@pytest.mark.parametrize("N", [1, 30, 3000])
+def test_a_query_that_is_not_a_number(dtype, D, N):
+    """NaN logits make their own head's result NaN, not an empty row's, whatever
+    the number of splits; nothing else changes."""
+    from telescope_cache_b200 import cached_attention, init_kv_cache, write_kv_cache
+
+    dt = DT[dtype]
+    c = init_kv_cache(2, 3001, 2, D, dtype=dt)
+    write_kv_cache(c, rand(2, N, 2, D, dtype=dt, seed=1), rand(2, N, 2, D, dtype=dt, seed=2))
+    q = rand(2, 1, 6, D, dtype=dt, seed=3)
+    want, want_lse = cached_attention(q, c)
+    q[0, 0, 4, 7] = math.nan
+    out, lse = cached_attention(q, c)
+    bad = torch.zeros(2, 1, 6, dtype=torch.bool, device="cuda")
+    bad[0, 0, 4] = True
+    assert bool(out[bad].isnan().all()) and bool(lse[bad].isnan().all())
+    assert torch.equal(out[~bad], want[~bad]) and torch.equal(lse[~bad], want_lse[~bad])
+
+
+@pytest.mark.parametrize("D", [80, 128])
+@pytest.mark.parametrize("N", [20, 2000])
+def test_a_step_past_the_tables_is_nan(D, N):
+    """Lengths that moved on without the host's bound: the rotated query is NaN, and so
+    is the result; the other row's is not."""
+    from telescope_cache_b200 import cached_attention_step, init_kv_cache, write_kv_cache
+
+    c = init_kv_cache(2, N + 10, 2, D)
+    ids = torch.where(torch.arange(N) < torch.tensor([N, 5])[:, None], torch.arange(2)[:, None], -1)
+    write_kv_cache(c, rand(2, N, 2, D, seed=1), rand(2, N, 2, D, seed=2), seq_idx=ids.cuda())
+    c.max_length = 5
+    ang = torch.rand(8, 12, device="cuda")
+    q, k, v = (rand(2, 1, h, D, seed=h) for h in (4, 2, 2))
+    out, lse = cached_attention_step(q, k, v, c, rope_cos=ang.cos(), rope_sin=ang.sin())
+    assert bool(out[0].isnan().all()) and bool(lse[0].isnan().all())
+    assert bool(out[1].isfinite().all()) and bool(lse[1].isfinite().all())
+    assert c.lengths.tolist() == [N + 1, 6]
