@@ -147,8 +147,13 @@ inline bool strides_ok(const void* p, int64_t sb, int64_t sn, int64_t sh, int64_
          (N == 1 || (sn % 8 == 0 && sn > 0 && sn < most)) && (H == 1 || (sh % 8 == 0 && sh > 0 && sh < most));
 }
 
+// The kernels take a row's reference from its largest raw score and divide lse by
+// the scale: it is positive, and lse / scale and scale s stay in fp32's range.  Any
+// other scale takes the CUDA cores.
+inline bool logits_ok(const CausalParams& p) { return p.scale >= 1e-30f && p.scale <= 1e30f; }
+
 inline bool tc_shape(const CausalParams& p, int dtype) {
-  return (dtype == TC_BF16 || dtype == TC_F16) && p.Dk == p.Dv && (p.Dk == 64 || p.Dk == 128) &&
+  return logits_ok(p) && (dtype == TC_BF16 || dtype == TC_F16) && p.Dk == p.Dv && (p.Dk == 64 || p.Dk == 128) &&
          strides_ok(p.q, p.q_sb, p.q_sn, p.q_sh, p.B, p.N, p.Hq) &&
          strides_ok(p.k, p.k_sb, p.k_sn, p.k_sh, p.B, p.N, p.Hkv) &&
          strides_ok(p.v, p.v_sb, p.v_sn, p.v_sh, p.B, p.N, p.Hkv);

@@ -63,6 +63,12 @@ void done(int rc, const char* what) {
   CHECK_RUN(false, "telescope_cache_b200: ", what, " failed with status ", rc);
 }
 
+// The factor of q.k, 1 / sqrt(D) unless given.
+float scale_of(std::optional<double> scale, int64_t D) {
+  CHECK_VALUE(!scale || std::isfinite((float)*scale), "scale must be finite, got ", scale.value_or(0.));
+  return (float)scale.value_or(1.0 / std::sqrt((double)D));
+}
+
 int32_t i32(int64_t v, const char* what) {
   CHECK_VALUE(v >= 0 && v <= INT32_MAX, what, " of ", v, " does not fit 31 bits");
   return (int32_t)v;
@@ -203,7 +209,7 @@ void causal_args(Causal& c, const Tensor& q, const Tensor& k, const Tensor& v, c
   a.B = i32(B, "batch"), a.N = i32(N, "length"), a.Hq = i32(Hq, "heads"), a.Hkv = i32(Hkv, "heads");
   a.Dk = i32(Dk, "head dim"), a.Dv = i32(v.size(3), "head dim"), a.dtype = dtype_code(q.scalar_type());
   a.has_softcap = softcap.has_value(), a.softcap = (float)softcap.value_or(0.);
-  a.scale = (float)scale.value_or(1.0 / std::sqrt((double)Dk));
+  a.scale = scale_of(scale, Dk);
   a.q = c.q.data_ptr(), a.q_stride_b = c.q.stride(0), a.q_stride_n = c.q.stride(1), a.q_stride_h = c.q.stride(2);
   a.k = c.k.data_ptr(), a.k_stride_b = c.k.stride(0), a.k_stride_n = c.k.stride(1), a.k_stride_h = c.k.stride(2);
   a.v = c.v.data_ptr(), a.v_stride_b = c.v.stride(0), a.v_stride_n = c.v.stride(1), a.v_stride_h = c.v.stride(2);
@@ -413,7 +419,7 @@ std::tuple<Tensor, Tensor, OptTensor, OptTensor> kv_attend(const Tensor& ck, con
   a.max_tokens = (int32_t)std::min<int64_t>(max_length + (step ? 1 : 0), c.capacity);
   a.q = q.data_ptr(), a.q_stride_b = q.stride(0), a.q_stride_h = q.stride(2);
   a.has_softcap = softcap.has_value(), a.softcap = (float)softcap.value_or(1.);
-  a.scale = (float)scale.value_or(1.0 / std::sqrt((double)Dk));
+  a.scale = scale_of(scale, Dk);
   a.out = out.data_ptr(), a.lse = lse.data_ptr<float>(), a.dev_status = status_of(q);
   if (step) {
     k = dense_head(*k0), v = dense_head(*v0);

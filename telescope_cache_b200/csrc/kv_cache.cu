@@ -13,6 +13,7 @@
 #include <cuda_fp8.h>
 #include <float.h>
 
+#include <cmath>
 #include <type_traits>
 
 #include "rotary.cuh"
@@ -1317,6 +1318,7 @@ extern "C" int tc_kv_attend(const tc_kv_cache* c, const tc_kv_attend_args* a, vo
   if (int rc = attend_shape(c, a->B, a->Hq, a->max_tokens, &p.chunk, &p.splits)) return rc;
   if (a->B == 0) return TC_OK;
   if (a->B > c->rows || !a->q || !a->out || !a->lse || a->max_tokens > c->capacity) return TC_ERR_ARG;
+  if (!std::isfinite(a->scale)) return TC_ERR_ARG;
   if (c->Dk > 256 || c->Dv > 256 || a->B > 65535) return TC_ERR_UNSUPPORTED;
   const bool step = a->k_t != nullptr;
   if (step && !a->v_t) return TC_ERR_ARG;

@@ -6,8 +6,8 @@ Tolerances are test_gpu_causal.py's, by check_forward and check_grads."""
 import pytest
 import torch
 
-from full_attention_reference import rel, visible
-from test_gpu_causal import DT, check_forward, grad_tol, ids_of, inputs
+from full_attention_reference import causal, gradient_terms, rel, visible
+from test_gpu_causal import DT, check_forward, check_grads, grad_tol, ids_of, inputs
 
 pytestmark = pytest.mark.gpu
 
@@ -97,3 +97,43 @@ def test_c_entries_take_any_address(D):
         check_forward(got["out"], lse, q, k, v, visible(None, B, N, "cuda"))
         for n in ("dq", "dk", "dv"):
             assert rel(got[n], base[n].double()) <= 2 * grad_tol(dt)
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("softcap", [None, 15.0])
+@pytest.mark.parametrize("scale", [-0.11, 0.0, 1e-35])
+def test_any_finite_scale(dtype, D, softcap, scale):
+    from telescope_cache_b200 import causal_attention
+
+    dt, B, N, Hq, Hkv = DT[dtype], 1, 300, 4, 2
+    q, k, v = (t.requires_grad_() for t in inputs(B, N, Hq, Hkv, D, D, dt, seed=17))
+    see = visible(None, B, N, "cuda")
+    # softcap and negative scale: logits beyond the cap, where a series would leave tanh
+    q.data.mul_(8)
+    out, lse = causal_attention(q, k, v, softcap=softcap, scale=scale)
+    check_forward(out.detach(), lse.detach(), q.detach(), k.detach(), v.detach(), see, softcap, scale)
+    gout, glse = torch.randn_like(out), torch.randn_like(lse)
+    got = torch.autograd.grad((out, lse), (q, k, v), (gout, glse))
+    x = [t.detach().double().requires_grad_() for t in (q, k, v)]
+    o, l, _, _ = causal(*x, see, softcap, scale)
+    want = torch.autograd.grad((o * gout.double()).sum() + (l * glse.double()).sum(), x)
+    terms = gradient_terms(q, k, v, see, gout, glse, softcap, scale)
+    if dt == torch.float16 and scale == 1e-35:  # dq, dk are far below its smallest number
+        assert bool((got[0] == 0).all()) and bool((got[1] == 0).all())
+        got, want, terms = got[2:], want[2:], terms[2:]
+    check_grads(got, want, terms, dt)
+
+
+def test_scales_that_are_refused():
+    from telescope_cache_b200 import cached_attention, causal_attention, init_kv_cache
+
+    q, k, v = inputs(1, 20, 2, 1, 64, 64, torch.bfloat16)
+    c = init_kv_cache(1, 10, 1, 64)
+    for scale in (float("nan"), float("inf"), -float("inf"), 1e39):
+        with pytest.raises(ValueError, match="scale"):
+            causal_attention(q, k, v, scale=scale)
+        with pytest.raises(ValueError, match="scale"):
+            cached_attention(q[:, :1], c, scale=scale)
+    with pytest.raises(NotImplementedError):  # the tensor-core kernels need it positive
+        causal_attention(q, k, v, scale=-1.0, impl="tensor")
