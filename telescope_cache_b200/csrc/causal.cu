@@ -748,7 +748,8 @@ int make_params(const tc_causal_args* a, CausalParams* p) {
     return TC_ERR_ARG;
   if ((a->starts == nullptr) != (a->ends == nullptr)) return TC_ERR_ARG;
   if (a->dtype != TC_F32 && a->dtype != TC_BF16 && a->dtype != TC_F16) return TC_ERR_ARG;
-  if (a->impl < 0 || a->impl > 2 || !std::isfinite(a->scale) || (a->has_softcap && !(a->softcap > 0.f))) return TC_ERR_ARG;
+  if (a->impl < 0 || a->impl > 2 || !std::isfinite(a->scale)) return TC_ERR_ARG;
+  if (a->has_softcap && !(a->softcap > 0.f && std::isfinite(a->softcap))) return TC_ERR_ARG;
   if (a->B > 65535 || a->Hq > 65535) return TC_ERR_UNSUPPORTED;
   p->B = a->B, p->N = a->N, p->Hq = a->Hq, p->Hkv = a->Hkv, p->E = a->Hq / a->Hkv, p->Dk = a->Dk, p->Dv = a->Dv;
   p->scale = a->scale, p->cap = a->has_softcap ? a->softcap : 1.f, p->has_cap = a->has_softcap != 0;

@@ -36,6 +36,8 @@
 // maxima, gained 2 % without softcap and lost 12 % with it.
 //
 // Every mbarrier wait is bounded (tc_ptx.cuh).
+#include <cmath>
+
 #include "causal_tc.cuh"
 
 namespace tc {
@@ -60,6 +62,7 @@ struct FwdParams {
   GridOrder order;
   float kq, kc;              // logit2 = kq s, or kc tanh(kq s)
   float e1, e3, e5, e7, e9;  // its series in s
+  float top5, top9;          // largest |y| of each; below 0 where fp32 does not hold its terms
 };
 
 enum { kPlain = 0, kS5 = 1, kS9 = 2, kTanh = 3 };
@@ -340,7 +343,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
       int mode = kPlain;
       if constexpr (CAP) {
         const float ay = amax * p.kq;
-        mode = __all_sync(0xffffffffu, ay <= kPoly5) ? kS5 : __all_sync(0xffffffffu, ay <= kPoly9) ? kS9 : kTanh;
+        mode = __all_sync(0xffffffffu, ay <= p.top5) ? kS5 : __all_sync(0xffffffffu, ay <= p.top9) ? kS9 : kTanh;
       }
       float mx = -INFINITY;
       if (umax > -INFINITY) {
@@ -455,6 +458,8 @@ int launch_fwd(const CausalParams& a, int dtype, cudaStream_t st) {
   p.e5 = (float)(kc * kT5 * kq * kq * kq * kq * kq);
   p.e7 = (float)(kc * kT7 * kq * kq * kq * kq * kq * kq * kq);
   p.e9 = (float)(kc * kT9 * kq * kq * kq * kq * kq * kq * kq * kq * kq);
+  p.top5 = std::isnormal(p.e1) && std::isnormal(p.e3) && std::isnormal(p.e5) ? kPoly5 : -1.f;
+  p.top9 = p.top5 > 0.f && std::isnormal(p.e7) && std::isnormal(p.e9) ? kPoly9 : -1.f;
   auto k = causal_fwd_kernel<T, HD, CAP>;
   constexpr int smem = FwdSmem<HD>::kBytes;
   if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return TC_ERR_CUDA;

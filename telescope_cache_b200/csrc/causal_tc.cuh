@@ -148,9 +148,14 @@ inline bool strides_ok(const void* p, int64_t sb, int64_t sn, int64_t sh, int64_
 }
 
 // The kernels take a row's reference from its largest raw score and divide lse by
-// the scale: it is positive, and lse / scale and scale s stay in fp32's range.  Any
-// other scale takes the CUDA cores.
-inline bool logits_ok(const CausalParams& p) { return p.scale >= 1e-30f && p.scale <= 1e30f; }
+// the scale: it is positive, and lse / scale and scale s stay in fp32's range.  Their
+// tanh by 1 - 2 / (e^2y + 1) is off by 3e-7 at most, the logit by that times the
+// softcap: above 2048 (6e-4) it shows in the weights.  Any other scale or softcap
+// takes the CUDA cores.
+inline bool logits_ok(const CausalParams& p) {
+  const float kq = p.has_cap ? p.scale / p.cap : p.scale;
+  return p.scale >= 1e-30f && p.scale <= 1e30f && kq <= 1e30f && (!p.has_cap || p.cap <= 2048.f);
+}
 
 inline bool tc_shape(const CausalParams& p, int dtype) {
   return logits_ok(p) && (dtype == TC_BF16 || dtype == TC_F16) && p.Dk == p.Dv && (p.Dk == 64 || p.Dk == 128) &&

@@ -69,6 +69,11 @@ float scale_of(std::optional<double> scale, int64_t D) {
   return (float)scale.value_or(1.0 / std::sqrt((double)D));
 }
 
+void check_softcap(std::optional<double> softcap) {
+  CHECK_VALUE(!softcap || ((float)*softcap > 0.f && std::isfinite((float)*softcap)), "softcap must be positive and finite, got ",
+              softcap.value_or(0.));
+}
+
 int32_t i32(int64_t v, const char* what) {
   CHECK_VALUE(v >= 0 && v <= INT32_MAX, what, " of ", v, " does not fit 31 bits");
   return (int32_t)v;
@@ -186,7 +191,7 @@ void causal_args(Causal& c, const Tensor& q, const Tensor& k, const Tensor& v, c
   CHECK_VALUE(Hkv != 0 && Hq % Hkv == 0, "Hq=", Hq, " must be divisible by Hkv=", Hkv, ".");
   CHECK_VALUE(q.scalar_type() == k.scalar_type() && q.scalar_type() == v.scalar_type(),
                     "q, k, v must share a dtype, got ", q.scalar_type(), ", ", k.scalar_type(), ", ", v.scalar_type());
-  CHECK_VALUE(!softcap || *softcap > 0, "softcap must be positive, got ", softcap.value_or(0.));
+  check_softcap(softcap);
   CHECK_VALUE(starts.has_value() == ends.has_value(), "segment starts and ends go together");
   cuda(q);
   same_device(q, k);
@@ -386,7 +391,7 @@ std::tuple<Tensor, Tensor, OptTensor, OptTensor> kv_attend(const Tensor& ck, con
   CHECK_VALUE(Dk == c.Dk && B <= c.rows, "q_t ", q0.sizes(), " incompatible with the cache's ", c.rows, " rows, ", c.Hkv,
                     " heads of ", c.Dk);
   CHECK_VALUE(Hq % c.Hkv == 0 && Hq > 0, "Hq=", Hq, " must be divisible by Hkv=", c.Hkv, ".");
-  CHECK_VALUE(!softcap || *softcap > 0, "softcap must be positive, got ", softcap.value_or(0.));
+  check_softcap(softcap);
   same_device(ck, q0);
   tc_kv_attend_args a{};
   const bool step = k0.has_value();

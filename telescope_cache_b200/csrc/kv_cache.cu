@@ -1230,7 +1230,7 @@ int launch_attend(const AttendParams& p, int64_t rows, cudaStream_t st) {
   const dim3 grid(p.splits, p.Hkv * p.groups, p.B);
   const int64_t heads = rows * p.Hkv;
   const bool mma = p.Dk == p.Dv && (p.Dk == 64 || p.Dk == 128) && (uintptr_t)p.k % 16 == 0 && (uintptr_t)p.v % 16 == 0 &&
-                   heads <= INT32_MAX && p.cap * p.Dk < (int64_t(1) << 40);
+                   heads <= INT32_MAX && p.cap * p.Dk < (int64_t(1) << 40) && !(p.has_cap && p.softcap < 1e-30f);
   if (mma && p.Dk == 128)
     return p.has_cap ? launch_mma<TQ, STORE, 128, true, STEP>(p, heads, grid, st)
                      : launch_mma<TQ, STORE, 128, false, STEP>(p, heads, grid, st);
@@ -1318,7 +1318,7 @@ extern "C" int tc_kv_attend(const tc_kv_cache* c, const tc_kv_attend_args* a, vo
   if (int rc = attend_shape(c, a->B, a->Hq, a->max_tokens, &p.chunk, &p.splits)) return rc;
   if (a->B == 0) return TC_OK;
   if (a->B > c->rows || !a->q || !a->out || !a->lse || a->max_tokens > c->capacity) return TC_ERR_ARG;
-  if (!std::isfinite(a->scale)) return TC_ERR_ARG;
+  if (!std::isfinite(a->scale) || (a->has_softcap && !(a->softcap > 0.f && std::isfinite(a->softcap)))) return TC_ERR_ARG;
   if (c->Dk > 256 || c->Dv > 256 || a->B > 65535) return TC_ERR_UNSUPPORTED;
   const bool step = a->k_t != nullptr;
   if (step && !a->v_t) return TC_ERR_ARG;

@@ -71,8 +71,8 @@ def causal_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *,
     reads key head h // (Hq / Hkv).
 
     S = c tanh(X / c) (X without softcap), X = scale q.k, scale 1 / sqrt(Dk) by
-    default (any finite one; one that is not positive, or outside 1e-30 .. 1e30, runs
-    on the CUDA cores).  seq_idx [B, N]: ids of the row's packed examples, one run each: a
+    default (any finite one; one that is not positive, or outside 1e-30 .. 1e30, and a
+    softcap above 2048 run on the CUDA cores).  seq_idx [B, N]: ids of the row's packed examples, one run each: a
     token attends its own example only; a token with a negative id is padding
     (out 0, lse -inf, zero gradients).  The bounds of segment_bounds may be
     given in its place, so that the layers of a model form them once.

@@ -137,3 +137,42 @@ def test_scales_that_are_refused():
             cached_attention(q[:, :1], c, scale=scale)
     with pytest.raises(NotImplementedError):  # the tensor-core kernels need it positive
         causal_attention(q, k, v, scale=-1.0, impl="tensor")
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("softcap", [1e-7, 1e-3, 1500.0, 1e5, 1e7])
+def test_any_softcap(dtype, D, softcap):
+    """Caps far below and above the logits.  One query is large: its logits pass the
+    larger caps while those of its neighbours stay small beside them."""
+    from telescope_cache_b200 import causal_attention
+
+    dt, B, N, Hq, Hkv = DT[dtype], 1, 300, 4, 2
+    q, k, v = inputs(B, N, Hq, Hkv, D, D, dt, seed=18)
+    if softcap < 1e-5 and dtype != "f16":  # logits around the cap (f16 has no numbers so small)
+        q.mul_(1e-8)
+    elif softcap > 1000:
+        q[:, 7] *= softcap / 30 if dtype != "f16" else min(softcap / 30, 8000.0)
+    see = visible(None, B, N, "cuda")
+    q, k, v = (t.requires_grad_() for t in (q, k, v))
+    out, lse = causal_attention(q, k, v, softcap=softcap)
+    check_forward(out.detach(), lse.detach(), q.detach(), k.detach(), v.detach(), see, softcap)
+    gout, glse = torch.randn_like(out), torch.randn_like(lse)
+    gout[:, 7], glse[:, 7] = 0, 0  # the neighbours' gradients are what is looked at
+    got = torch.autograd.grad((out, lse), (q, k, v), (gout, glse))
+    x = [t.detach().double().requires_grad_() for t in (q, k, v)]
+    o, l, _, _ = causal(*x, see, softcap)
+    want = torch.autograd.grad((o * gout.double()).sum() + (l * glse.double()).sum(), x)
+    check_grads(got, want, gradient_terms(q, k, v, see, gout, glse, softcap), dt)
+
+
+def test_softcaps_that_are_refused():
+    from telescope_cache_b200 import cached_attention, causal_attention, init_kv_cache
+
+    q, k, v = inputs(1, 20, 2, 1, 64, 64, torch.bfloat16)
+    c = init_kv_cache(1, 10, 1, 64)
+    for softcap in (float("nan"), float("inf"), 0.0, -2.0, 1e-50, 1e39):
+        with pytest.raises(ValueError, match="softcap"):
+            causal_attention(q, k, v, softcap=softcap)
+        with pytest.raises(ValueError, match="softcap"):
+            cached_attention(q[:, :1], c, softcap=softcap)
