@@ -533,6 +533,7 @@ int tc_rotary(const tc_rotary_args* a, void* stream);
  * [B, N] lies in (int32 [B, N] each, token indices of its row).  Tokens with a
  * negative id belong to no run: start = n + 1, end = n. */
 int tc_segment_bounds(int32_t B, int32_t N, const int32_t* seq_idx, int32_t* starts, int32_t* ends, void* stream);
+int tc_segment_bounds_i64(int32_t B, int32_t N, const int64_t* seq_idx, int32_t* starts, int32_t* ends, void* stream);
 
 #define TC_KV_INT8 0  /* code = round(x 127 / amax) + 128 in a byte          */
 #define TC_KV_FP8 1   /* code = e4m3 float of x 448 / amax                   */

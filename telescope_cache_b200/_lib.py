@@ -178,6 +178,7 @@ SIGNATURES = {
     "tc_decode_init": [ctypes.POINTER(DecodeInitArgs), _c_vp],
     "tc_rotary": [ctypes.POINTER(RotaryArgs), _c_vp],
     "tc_segment_bounds": [_c_i32, _c_i32, _c_vp, _c_vp, _c_vp, _c_vp],
+    "tc_segment_bounds_i64": [_c_i32, _c_i32, _c_vp, _c_vp, _c_vp, _c_vp],
     "tc_kv_write": [ctypes.POINTER(KVCacheArgs), ctypes.POINTER(KVWriteArgs), _c_vp],
     "tc_kv_read": [ctypes.POINTER(KVCacheArgs), _c_i32, _c_i32, _c_vp, _c_vp, _c_vp],
     "tc_kv_attend_scratch_floats": [ctypes.POINTER(KVCacheArgs), _c_i32, _c_i32, _c_i32],

@@ -24,10 +24,10 @@ namespace {
 constexpr int kBoundThreads = 512, kBoundTok = 4 * kBoundThreads, kReach = 16;
 // Largest (FORWARD: smallest) run start over [lo, hi), -1 (N) where there is none;
 // the same for every thread.
-template <bool FORWARD>
-__device__ int edge(const int32_t* id, int lo, int hi, int N, int* box) {
+template <bool FORWARD, typename Id>
+__device__ int edge(const Id* id, int lo, int hi, int N, int* box) {
   int best = FORWARD ? N : -1;
-  int v[kReach], w[kReach];
+  Id v[kReach], w[kReach];
 #pragma unroll
   for (int k = 0; k < kReach; ++k) {
     const int n = lo + threadIdx.x + k * kBoundThreads;
@@ -51,14 +51,15 @@ __device__ int edge(const int32_t* id, int lo, int hi, int N, int* box) {
   return *box;
 }
 
-__global__ void __launch_bounds__(kBoundThreads) bounds_kernel(int N, const int32_t* seq, int32_t* starts, int32_t* ends) {
+template <typename Id>
+__global__ void __launch_bounds__(kBoundThreads) bounds_kernel(int N, const Id* seq, int32_t* starts, int32_t* ends) {
   __shared__ int last_w[kBoundThreads / 32], first_w[kBoundThreads / 32], box;
   const int64_t row = (int64_t)blockIdx.y * N;
-  const int32_t* id = seq + row;
+  const Id* id = seq + row;
   const int c0 = blockIdx.x * kBoundTok, c1 = min(N, c0 + kBoundTok);
   const int n0 = c0 + 4 * threadIdx.x;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int v[5];  // id[n0 - 1 .. n0 + 3]
+  Id v[5];  // id[n0 - 1 .. n0 + 3]
 #pragma unroll
   for (int k = 0; k < 5; ++k) {
     const int n = n0 - 1 + k;
@@ -121,6 +122,16 @@ __global__ void __launch_bounds__(kBoundThreads) bounds_kernel(int N, const int3
     ends[row + n] = v[k + 1] < 0 ? n : end;
     if (n == 0 || v[k + 1] != v[k]) end = n;
   }
+}
+
+template <typename Id>
+int launch_bounds(int32_t B, int32_t N, const Id* seq_idx, int32_t* starts, int32_t* ends, cudaStream_t st) {
+  if (B < 0 || N < 0) return TC_ERR_ARG;
+  if ((int64_t)B * N == 0) return TC_OK;
+  if (!seq_idx || !starts || !ends) return TC_ERR_ARG;
+  if (B > 65535) return TC_ERR_UNSUPPORTED;
+  bounds_kernel<<<dim3((N + kBoundTok - 1) / kBoundTok, B), kBoundThreads, 0, st>>>(N, seq_idx, starts, ends);
+  return launch_status();
 }
 
 // ---------------------------------------------------------------------------
@@ -780,12 +791,12 @@ int causal_delta(const CausalParams& p, int dtype, cudaStream_t st) {
 
 extern "C" int tc_segment_bounds(int32_t B, int32_t N, const int32_t* seq_idx, int32_t* starts, int32_t* ends,
                                  void* stream) {
-  if (B < 0 || N < 0) return TC_ERR_ARG;
-  if ((int64_t)B * N == 0) return TC_OK;
-  if (!seq_idx || !starts || !ends) return TC_ERR_ARG;
-  if (B > 65535) return TC_ERR_UNSUPPORTED;
-  bounds_kernel<<<dim3((N + kBoundTok - 1) / kBoundTok, B), kBoundThreads, 0, (cudaStream_t)stream>>>(N, seq_idx, starts, ends);
-  return launch_status();
+  return launch_bounds(B, N, seq_idx, starts, ends, (cudaStream_t)stream);
+}
+
+extern "C" int tc_segment_bounds_i64(int32_t B, int32_t N, const int64_t* seq_idx, int32_t* starts, int32_t* ends,
+                                     void* stream) {
+  return launch_bounds(B, N, seq_idx, starts, ends, (cudaStream_t)stream);
 }
 
 extern "C" int tc_causal_fwd(const tc_causal_args* a, void* stream) {

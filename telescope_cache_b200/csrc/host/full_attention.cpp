@@ -83,10 +83,15 @@ Tensor dense_head(const Tensor& t) { return t.stride(-1) == 1 || t.size(-1) == 1
 Tensor table(const Tensor& t) {
   return t.scalar_type() == at::kFloat && t.is_contiguous() ? t : t.to(at::kFloat).contiguous();
 }
-Tensor ints(const Tensor& t) {
-  return t.scalar_type() == at::kInt && t.is_contiguous() ? t : t.to(at::kInt).contiguous();
+bool integral(const Tensor& t) {
+  const auto k = t.scalar_type();
+  return k == at::kInt || k == at::kLong || k == at::kShort || k == at::kChar || k == at::kByte;
 }
-bool integral(const Tensor& t) { return c10::isIntegralType(t.scalar_type(), false); }
+// Indices (positions, cache rows) as int32: one of 64 bits that does not fit goes to
+// the nearest that is no index.
+Tensor indices(const Tensor& t) {
+  return (t.scalar_type() == at::kLong ? t.clamp(-1, INT32_MAX) : t).to(at::kInt).contiguous();
+}
 
 // The device status word: one int32 per device, shared with the Python layer.
 std::map<int, Tensor>& status_words() {
@@ -133,7 +138,7 @@ std::tuple<Tensor, OptTensor> rotary(const Tensor& q0, const OptTensor& k0, cons
                       "positions must be integers [", N, "] or [", B, ", ", N, "], got ", positions->sizes(), " ",
                       positions->scalar_type());
     same_device(q0, *positions);
-    pos = ints(*positions);
+    pos = indices(*positions);
   } else {
     CHECK_VALUE(cos0.size(0) >= N, "rotary tables cover ", cos0.size(0), " positions, q has ", N);
   }
@@ -166,11 +171,14 @@ std::tuple<Tensor, Tensor> segment_bounds(const Tensor& seq_idx) {
                     seq_idx.sizes(), " ", seq_idx.scalar_type());
   cuda(seq_idx);
   Call call(seq_idx);
-  const Tensor ids = ints(seq_idx);
-  Tensor both = at::empty({2, ids.size(0), ids.size(1)}, ids.options());
+  const bool wide = seq_idx.scalar_type() == at::kLong;  // ids of 64 bits are compared as they are
+  const Tensor ids = (wide ? seq_idx : seq_idx.to(at::kInt)).contiguous();
+  Tensor both = at::empty({2, ids.size(0), ids.size(1)}, ids.options().dtype(at::kInt));
   Tensor starts = both.select(0, 0), ends = both.select(0, 1);
-  done(tc_segment_bounds(i32(ids.size(0), "batch"), i32(ids.size(1), "length"), ids.data_ptr<int32_t>(),
-                         starts.data_ptr<int32_t>(), ends.data_ptr<int32_t>(), call.stream),
+  const int32_t B = i32(ids.size(0), "batch"), N = i32(ids.size(1), "length");
+  int32_t *s = starts.data_ptr<int32_t>(), *e = ends.data_ptr<int32_t>();
+  done(wide ? tc_segment_bounds_i64(B, N, ids.data_ptr<int64_t>(), s, e, call.stream)
+            : tc_segment_bounds(B, N, ids.data_ptr<int32_t>(), s, e, call.stream),
        "tc_segment_bounds");
   return {starts, ends};
 }
@@ -328,7 +336,7 @@ void kv_write(const Tensor& ck, const Tensor& cv, const Tensor& cks, const Tenso
   }
   Call call(k0);
   if (seq_idx) {
-    ids = ints(*seq_idx);
+    ids = indices(*seq_idx);
     std::tie(starts, ends) = segment_bounds(ids);
   }
   const Tensor k = dense_head(k0), v = dense_head(v0);

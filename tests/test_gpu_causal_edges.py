@@ -176,3 +176,50 @@ def test_softcaps_that_are_refused():
             causal_attention(q, k, v, softcap=softcap)
         with pytest.raises(ValueError, match="softcap"):
             cached_attention(q[:, :1], c, softcap=softcap)
+
+
+@pytest.mark.parametrize("N", [5, 300, 2500])
+def test_ids_of_64_bits(N):
+    """Ids that agree in their low 32 bits, or whose low 32 bits are negative, are
+    what they are in 64."""
+    from telescope_cache_b200 import causal_attention, segment_bounds
+
+    ids = ids_of([N // 3, -(N // 5), N // 4], N)[None].long()
+    want = segment_bounds(ids.int())
+    for wide in (ids * 2 ** 32 + 7, ids * 2 ** 40 + 2 ** 31, 2 ** 62 - ids):
+        wide = torch.where(ids < 0, -(2 ** 33), wide)
+        for t in (wide, wide.expand(3, N), wide.repeat_interleave(2, 1)[:, ::2]):
+            got = segment_bounds(t)
+            for a, b in zip(got, want):
+                assert a.dtype == torch.int32 and torch.equal(a, b.expand(t.shape[0], N))
+    for small in (torch.int8, torch.uint8, torch.int16):
+        t = ids.to(small) if small != torch.uint8 else ids.clamp(min=0).to(small)
+        got, ref = segment_bounds(t), segment_bounds(t.int())
+        assert torch.equal(got.starts, ref.starts) and torch.equal(got.ends, ref.ends)
+    q, k, v = inputs(1, N, 2, 1, 64, 64, torch.bfloat16, seed=2)
+    wide = torch.where(ids < 0, -1, ids * 2 ** 32 + 2 ** 31)
+    assert torch.equal(causal_attention(q, k, v, seq_idx=wide)[0], causal_attention(q, k, v, seq_idx=want)[0])
+
+
+def test_positions_of_64_bits():
+    from telescope_cache_b200 import rotary
+
+    q, k, _ = inputs(1, 5, 2, 1, 64, 64, torch.float32)
+    ang = torch.rand(8, 32, device="cuda")
+    pos = torch.tensor([0, 2 ** 32 + 1, -(2 ** 32) + 2, 2 ** 33, 7], device="cuda")
+    y, _ = rotary(q, k, ang.cos(), ang.sin(), positions=pos)
+    want, _ = rotary(q, k, ang.cos(), ang.sin(), positions=torch.tensor([0, -1, -1, -1, 7], device="cuda"))
+    assert bool(y[:, 1:4].isnan().all()) and torch.equal(y[:, [0, 4]], want[:, [0, 4]]) and bool(y[:, [0, 4]].isfinite().all())
+
+
+def test_cache_rows_of_64_bits():
+    from telescope_cache_b200 import init_kv_cache, write_kv_cache
+    from telescope_cache_b200.telescoping_attn.attention import read_device_status
+
+    read_device_status("cuda:0")
+    c = init_kv_cache(2, 8, 1, 64)
+    k = torch.randn(1, 6, 1, 64, device="cuda")
+    ids = torch.tensor([[0, 0, 2 ** 32, 2 ** 32 + 1, -(2 ** 32) + 1, 1]], device="cuda")
+    write_kv_cache(c, k, k, seq_idx=ids)
+    assert read_device_status("cuda:0") & 2  # rows that do not exist
+    assert c.lengths.tolist() == [2, 1]
