@@ -89,11 +89,12 @@ template <> struct Codec<TC_KV_FP8> {
   }
 };
 
-// scale and top / amax of a row from its amax (NaN and infinity kept).
+// scale and top / amax of a row from its amax; the scale of a row with an infinity
+// is NaN as that of one with a NaN is, so that all of it reads back as NaN.
 template <int STORE>
 __device__ __forceinline__ void row_scale(float amax, float* scale, float* inv) {
   const bool tiny = amax < kTiny;
-  *scale = tiny ? 0.f : __fdiv_rn(amax, Codec<STORE>::kTop);
+  *scale = tiny ? 0.f : amax <= FLT_MAX ? __fdiv_rn(amax, Codec<STORE>::kTop) : NAN;
   *inv = tiny ? 0.f : __fdiv_rn(Codec<STORE>::kTop, amax);
 }
 
@@ -150,7 +151,7 @@ __device__ __forceinline__ float amax_float(uint32_t a) {
 // |x| as bits: ordered as the floats are, with every NaN above infinity.
 __device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 
-// The value of a code: infinite or NaN only where the scale is (127 times a
+// The value of a code: NaN only where the scale is, never infinite (127 times a
 // scale that was rounded up may pass the largest float).
 __device__ __forceinline__ float held(float v, float scale) {
   v *= scale;

@@ -72,3 +72,26 @@ def test_a_step_past_the_tables_is_nan(D, N):
     assert bool(out[0].isnan().all()) and bool(lse[0].isnan().all())
     assert bool(out[1].isfinite().all()) and bool(lse[1].isfinite().all())
     assert c.lengths.tolist() == [N + 1, 6]
+
+
+@pytest.mark.parametrize("store", ["int8", "fp8"])
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("D", [64, 40])
+def test_an_infinity_makes_its_row_nan(store, dtype, D):
+    """Every element of the row, of either sign, written as a prompt or as a step."""
+    from telescope_cache_b200 import cached_attention_step, init_kv_cache, read_kv_cache, write_kv_cache
+
+    dt = DT[dtype]
+    c = init_kv_cache(2, 8, 2, D, store=store, dtype=dt)
+    k, v = rand(2, 4, 2, D, dtype=dt, seed=1), rand(2, 4, 2, D, dtype=dt, seed=2)
+    k[0, 1, 0, 3], v[0, 2, 1, 9] = math.inf, -math.inf
+    write_kv_cache(c, k, v)
+    q, kt, vt = (rand(2, 1, 2, D, dtype=dt, seed=i) for i in (3, 4, 5))
+    kt[1, 0, 1, 0], vt[1, 0, 0, 5] = -math.inf, math.inf
+    _, _, kn, vn = cached_attention_step(q, kt, vt, c, return_stored=True)
+    rk, rv = read_kv_cache(c)
+    bk, bv = (torch.zeros(2, 5, 2, dtype=torch.bool, device="cuda") for _ in range(2))
+    bk[0, 1, 0] = bv[0, 2, 1] = bk[1, 4, 1] = bv[1, 4, 0] = True
+    for r, bad, last in ((rk, bk, kn), (rv, bv, vn)):
+        assert bool(r[bad].isnan().all()) and bool(r[~bad].isfinite().all())
+        assert torch.equal(last[:, 0].isnan(), r[:, 4].isnan())
