@@ -33,7 +33,8 @@ def device_status(device) -> torch.Tensor:
     key = torch.device(device).index
     t = _STATUS.get(key)
     if t is None:
-        t = torch.zeros(1, dtype=torch.int32, device=device)
+        with torch.inference_mode(False):  # read_device_status writes to it later on
+            t = torch.zeros(1, dtype=torch.int32, device=device)
         _STATUS[key] = t
     return t
 
