@@ -321,11 +321,14 @@ class FullMultiHeadAttention(nn.Module):
             out = apply_output_gate(out, x, self.gate_proj.weight)
         return MultiHeadAttention._linear(out.reshape(x.shape[0], x.shape[1], -1), self.dense)
 
-    def forward(self, x: torch.Tensor, seq_idx: Optional[torch.Tensor] = None, *, cache: Optional[KVCache] = None):
+    def forward(self, x: torch.Tensor, seq_idx: Optional[torch.Tensor] = None, *, cache: Optional[KVCache] = None,
+                max_tokens: Optional[int] = None):
         """x [B, N, emb_dim] -> [B, N, emb_dim].  seq_idx [B, N]: ids of packed
         examples (negative: padding); positions restart with each.  With a cache
         (new_cache), its rows start anew with these prompts: batch row b in cache
-        row b, or the example with id i in cache row i."""
+        row b, or the example with id i in cache row i; max_tokens is then the
+        longest prompt's length (by default N: packed prompts are shorter, and the
+        cache need not hold them end to end)."""
         B, N, _ = x.shape
         q, k, v = self._qkv(x)
         cos, sin = self._tables(N, x.device)
@@ -334,7 +337,7 @@ class FullMultiHeadAttention(nn.Module):
         out, lse = causal_attention(q, k, v, seq_idx=seg, softcap=self.softcap)
         if cache is not None:
             with torch.no_grad():
-                write_kv_cache(cache, k.detach(), v.detach(), seq_idx=seq_idx, fresh=True)
+                write_kv_cache(cache, k.detach(), v.detach(), seq_idx=seq_idx, fresh=True, max_tokens=max_tokens)
         return self._finish(out, lse, x)
 
     def new_cache(self, rows: int, capacity: int, dtype: torch.dtype = torch.bfloat16, device=None) -> KVCache:

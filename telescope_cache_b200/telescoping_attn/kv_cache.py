@@ -43,6 +43,12 @@ class KVCache:
     def capacity(self) -> int:
         return self.k.shape[2]
 
+    def clear(self) -> None:
+        """Forget every row's tokens, and the bound with them: the cache for another batch."""
+        with torch.inference_mode():  # the cache may have been made under it
+            self.lengths.zero_()
+        self.max_length = 0
+
 
 def init_kv_cache(rows: int, capacity: int, kvheads: int, k_dim: int, v_dim: Optional[int] = None, *,
                   store: str = "int8", dtype: torch.dtype = torch.bfloat16, device=None) -> KVCache:
@@ -79,9 +85,9 @@ def write_kv_cache(cache: KVCache, k: torch.Tensor, v: torch.Tensor, *,
     Without seq_idx, batch row b goes to cache row b.  With seq_idx [B, N]
     integers, token (b, n) goes to cache row seq_idx[b, n] (negative: nowhere):
     packed prompts and padded batches alike; a cache row's tokens are one run,
-    in order, and rows that no token names keep what they hold.  max_tokens:
-    the most tokens that any row gets (by default N).  Raises when a row may not
-    fit; a token whose row or slot does not exist all the same is dropped and
+    in order, and rows that no token names keep what they hold (cache.clear()
+    empties them all).  max_tokens: the most tokens that any row gets (by default N;
+    for packed prompts, the longest).  Raises when a row may not fit; a token whose row or slot does not exist all the same is dropped and
     flagged in the device status word."""
     most = k.shape[1] if max_tokens is None else int(max_tokens)
     end = (0 if fresh else cache.max_length) + most

@@ -110,3 +110,13 @@ def test_layer_parameters():
         args.update(kw)
         with pytest.raises(ValueError):
             FullMultiHeadAttention(**args)
+
+
+def test_a_cleared_cache_is_empty():
+    for mode in (torch.no_grad, torch.inference_mode):
+        with mode():
+            c = init_kv_cache(3, 4, 1, 8, device="cpu")
+            c.lengths.fill_(2)
+        c.max_length = 2
+        c.clear()
+        assert c.lengths.tolist() == [0, 0, 0] and c.max_length == 0

@@ -105,3 +105,29 @@ def test_tables_are_there_for_any_stream():
                 y = m(x)
             torch.cuda.synchronize()
             assert torch.equal(y, m(x))
+
+
+@pytest.mark.parametrize("store", ["int8", "fp8"])
+def test_packed_prompts_longer_than_the_cache_together(store):
+    """Eight prompts in a row of 520 tokens, a cache of 100 slots: each example has to
+    fit, the row need not.  Then tokens, then the same cache for another batch."""
+    from test_gpu_full_attention import layer as make
+
+    m = make(64, torch.float32, cache_store=store)
+    cache = m.new_cache(8, 100, torch.float32, "cuda")
+    for lens in ([65] * 8, [95, 1, 40, 7, 95, 95, 95, 92]):
+        cache.clear()
+        assert cache.lengths.tolist() == [0] * 8 and cache.max_length == 0
+        xs = [torch.randn(1, n + 3, 96, device="cuda") for n in lens]
+        packed = torch.cat([x[:, :n] for x, n in zip(xs, lens)], 1)
+        ids = torch.cat([torch.full((n,), i, device="cuda") for i, n in enumerate(lens)])[None]
+        with torch.no_grad():
+            m(packed, seq_idx=ids, cache=cache, max_tokens=max(lens))
+            assert cache.lengths.tolist() == lens and cache.max_length == max(lens)
+            full = [m(x) for x in xs]
+            for s in range(3):
+                out = m.decode(torch.cat([x[:, n + s: n + s + 1] for x, n in zip(xs, lens)]), cache)
+                for i, n in enumerate(lens):  # as in test_layer_prompt_then_tokens
+                    assert rel(out[i, 0], full[i][0, n + s]) <= (0.03 if store == "int8" else 0.08)
+    with pytest.raises(ValueError, match="capacity"):
+        m(packed, seq_idx=ids, cache=cache)  # the default bound is the row
