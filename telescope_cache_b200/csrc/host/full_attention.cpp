@@ -16,6 +16,7 @@
 #include <cmath>
 #include <map>
 #include <stdexcept>
+#include <string>
 #include <tuple>
 
 #include "../../../include/telescope_cache.h"
@@ -53,14 +54,21 @@ void same_device(const Tensor& a, const Tensor& b) {
   CHECK_VALUE(a.device() == b.device(), "tensors on ", a.device(), " and ", b.device());
 }
 
+[[noreturn]] void not_implemented(const std::string& what) {
+  PyErr_SetString(PyExc_NotImplementedError, what.c_str());
+  throw py::error_already_set();
+}
 void done(int rc, const char* what) {
   if (rc == TC_OK) return;
-  if (rc == TC_ERR_ARG || rc == TC_ERR_SCHEDULE) CHECK_VALUE(false, "telescope_cache_b200: ", what, " failed with status ", rc);
-  if (rc == TC_ERR_UNSUPPORTED) {
-    PyErr_SetString(PyExc_NotImplementedError, c10::str("telescope_cache_b200: ", what, " failed with status ", rc).c_str());
-    throw py::error_already_set();
-  }
-  CHECK_RUN(false, "telescope_cache_b200: ", what, " failed with status ", rc);
+  const std::string text = c10::str("telescope_cache_b200: ", what, " failed with status ", rc);
+  if (rc == TC_ERR_ARG || rc == TC_ERR_SCHEDULE) CHECK_VALUE(false, text);
+  if (rc == TC_ERR_UNSUPPORTED) not_implemented(text);
+  CHECK_RUN(false, text);
+}
+
+// A tangent would be dropped without a word.
+void no_tangent(const Tensor& t) {
+  if (t._fw_grad(0).defined()) not_implemented("telescope_cache_b200: forward-mode derivatives are not supported");
 }
 
 // The factor of q.k, 1 / sqrt(D) unless given.
@@ -131,6 +139,8 @@ std::tuple<Tensor, OptTensor> rotary(const Tensor& q0, const OptTensor& k0, cons
   if (k0) same_device(q0, *k0);
   same_device(q0, cos0);
   same_device(q0, sin0);
+  for (const Tensor* t : {&q0, &cos0, &sin0}) no_tangent(*t);
+  if (k0) no_tangent(*k0);
   Tensor pos;
   if (positions) {
     const bool shared = positions->dim() == 1 && positions->size(0) == N;
@@ -237,6 +247,7 @@ std::tuple<Tensor, Tensor, OptTensor> causal_forward(const Tensor& q, const Tens
                                           std::optional<double> scale, int impl, bool keep_low) {
   Causal c;
   causal_args(c, q, k, v, seq, starts, ends, softcap, scale, impl);
+  for (const Tensor* t : {&q, &k, &v}) no_tangent(*t);
   Call call(q);
   Tensor out = at::empty({q.size(0), q.size(1), q.size(2), v.size(3)}, q.options());
   Tensor lse = at::empty({q.size(0), q.size(1), q.size(2)}, q.options().dtype(at::kFloat));
@@ -401,6 +412,7 @@ std::tuple<Tensor, Tensor, OptTensor, OptTensor> kv_attend(const Tensor& ck, con
   CHECK_VALUE(Hq % c.Hkv == 0 && Hq > 0, "Hq=", Hq, " must be divisible by Hkv=", c.Hkv, ".");
   check_softcap(softcap);
   same_device(ck, q0);
+  no_tangent(q0);
   tc_kv_attend_args a{};
   const bool step = k0.has_value();
   if (step) {
@@ -423,6 +435,8 @@ std::tuple<Tensor, Tensor, OptTensor, OptTensor> kv_attend(const Tensor& ck, con
     CHECK_VALUE(max_length < c.capacity, "a row may be full: max_length ", max_length, ", capacity ", c.capacity);
     same_device(ck, *k0);
     same_device(ck, *v0);
+    no_tangent(*k0);
+    no_tangent(*v0);
   }
   Call call(q0);
   const Tensor q = dense_head(q0);

@@ -111,7 +111,8 @@ def cached_attention(q_t: torch.Tensor, cache: KVCache, *, softcap: Optional[flo
                      scale: Optional[float] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """(out [B, 1, Hq, Dv], lse [B, 1, Hq] fp32) of one query per sequence,
     q_t [B, 1, Hq, Dk] (already rotated), over the tokens that rows 0 .. B - 1 of
-    the cache hold; an empty row gives out 0 and lse -inf."""
+    the cache hold; an empty row gives out 0 and lse -inf.  For serving: the results
+    have no gradients."""
     out, lse, _, _ = _lib.host(q_t).kv_attend(*_parts(cache), cache.dtype, cache.max_length, q_t, None, None, None, None,
                                               False, softcap, scale, False, False)
     return out, lse
@@ -128,7 +129,8 @@ def cached_attention_step(q_t: torch.Tensor, k_t: torch.Tensor, v_t: torch.Tenso
     tried at its place and the next call writes there again).
 
     Returns (out [B, 1, Hq, Dv], lse [B, 1, Hq] fp32), and with return_stored
-    the key and value that the written codes stand for, [B, 1, Hkv, D]."""
+    the key and value that the written codes stand for, [B, 1, Hkv, D].  The results
+    have no gradients."""
     if layout not in LAYOUTS:
         raise ValueError(f"layout must be one of {LAYOUTS}, got {layout!r}")
     if k_t is None or v_t is None:

@@ -223,3 +223,26 @@ def test_cache_rows_of_64_bits():
     write_kv_cache(c, k, k, seq_idx=ids)
     assert read_device_status("cuda:0") & 2  # rows that do not exist
     assert c.lengths.tolist() == [2, 1]
+
+
+def test_tangents_are_refused():
+    """Forward-mode derivatives are not built: an error, not a result without one."""
+    import torch.autograd.forward_ad as fwd
+    from telescope_cache_b200 import cached_attention, causal_attention, init_kv_cache, rotary
+
+    q, k, v = inputs(1, 20, 2, 1, 64, 64, torch.float32)
+    ang = torch.rand(20, 32, device="cuda")
+    c = init_kv_cache(1, 10, 1, 64)
+    with fwd.dual_level():
+        for i in range(3):
+            x = [q, k, v]
+            x[i] = fwd.make_dual(x[i], torch.ones_like(x[i]))
+            with pytest.raises((NotImplementedError, RuntimeError), match="forward-mode|forward AD|jvp"):
+                causal_attention(*x)
+            if i < 2:
+                with pytest.raises((NotImplementedError, RuntimeError), match="forward-mode|forward AD|jvp"):
+                    rotary(*x[:2], ang.cos(), ang.sin())
+        with pytest.raises((NotImplementedError, RuntimeError), match="forward-mode|forward AD|jvp"):
+            cached_attention(fwd.make_dual(q[:, :1], torch.ones_like(q[:, :1])), c)
+        out, _ = causal_attention(q, k, v)  # none of them dual: as ever
+    assert bool(out.isfinite().all())
