@@ -208,6 +208,9 @@ template <int TM_, int TN_, int DM_, int GT_, int G_> struct Tile {
   static constexpr int C = DM / 64;     // float4 output columns per thread
   static constexpr int NT = GT * G;
   static constexpr int kFetch = TN * DM / GT;  // elements of an operand tile per thread
+  // backward: a lone group's next loads run under its own products (of several groups,
+  // one loads under another's)
+  static constexpr bool kAhead = G == 1;
   // floats of shared memory: of the CTA, and of each group
   static constexpr int fwd_all() { return TM * RS; }
   static constexpr int fwd_group() { return TN * RS + TM * PS; }
@@ -250,8 +253,8 @@ __device__ __forceinline__ float4 load4(const T* x, int d, int D, bool there, bo
 }
 
 // Rows [r0, r0 + ROWS) of a head, zeros outside [0, N) x [0, D), by THREADS threads.
-// fetch_tile and put_tile: into registers, so that the loads run under products, and
-// from there into shared memory.
+// fetch_tile and put_tile (backward of one group): into registers, so that the loads
+// run under products, and from there into shared memory.
 template <typename T, typename Z>
 __device__ __forceinline__ void fetch_tile(float4* r, const void* x, int64_t base, int64_t sn, int r0, int N, int D, int t,
                                            bool vec) {
@@ -393,7 +396,6 @@ __device__ __forceinline__ void store_rows(T* out, int64_t row_stride, int r0, i
 template <typename T, typename Z>
 __global__ void __launch_bounds__(Z::NT) fwd_cores(CausalParams p) {
   constexpr int TM = Z::TM, TN = Z::TN, DM = Z::DM;
-  constexpr bool kAhead = Z::kFetch <= 16;  // the next tile's loads under this one's products
   extern __shared__ __align__(16) float sm[];
   const Place w = place<Z>();
   float* groups = sm + Z::fwd_all();
@@ -416,18 +418,11 @@ __global__ void __launch_bounds__(Z::NT) fwd_cores(CausalParams p) {
   }
   const int end = min(q0 + TM, p.N), begin = first_key(p, b, q0) / 16 * 16 + w.g * TN, step = Z::G * TN;
   const int64_t kb = b * p.k_sb + hkv * p.k_sh, vb = b * p.v_sb + hkv * p.v_sh;
-  float4 kr[kAhead ? Z::kFetch / 4 : 1], vr[kAhead ? Z::kFetch / 4 : 1];
-  if (kAhead && begin < end) {
-    fetch_tile<T, Z>(kr, p.k, kb, p.k_sn, begin, p.N, p.Dk, w.t, p.vec4);
-    fetch_tile<T, Z>(vr, p.v, vb, p.v_sn, begin, p.N, p.Dv, w.t, p.vec4);
-  }
   __syncthreads();
   for (int k0 = begin; k0 < end; k0 += step) {
     group_sync<Z>(w.g);
-    if constexpr (kAhead) put_tile<Z>(kv_s, kr, w.t);
-    else load_tile<T, TN, DM, Z::GT>(kv_s, p.k, kb, p.k_sn, k0, p.N, p.Dk, w.t, p.vec4);
+    load_tile<T, TN, DM, Z::GT>(kv_s, p.k, kb, p.k_sn, k0, p.N, p.Dk, w.t, p.vec4);
     group_sync<Z>(w.g);
-    if (kAhead && k0 + step < end) fetch_tile<T, Z>(kr, p.k, kb, p.k_sn, k0 + step, p.N, p.Dk, w.t, p.vec4);
     float s[Z::R][Z::S];
     dot_tile<Z>(q_s, kv_s, p.Dk, w, s);
 #pragma unroll
@@ -462,10 +457,8 @@ __global__ void __launch_bounds__(Z::NT) fwd_cores(CausalParams p) {
       for (int j = 0; j < Z::C; ++j) o[i][j].x *= c, o[i][j].y *= c, o[i][j].z *= c, o[i][j].w *= c;
     }
     group_sync<Z>(w.g);
-    if constexpr (kAhead) put_tile<Z>(kv_s, vr, w.t);
-    else load_tile<T, TN, DM, Z::GT>(kv_s, p.v, vb, p.v_sn, k0, p.N, p.Dv, w.t, p.vec4);
+    load_tile<T, TN, DM, Z::GT>(kv_s, p.v, vb, p.v_sn, k0, p.N, p.Dv, w.t, p.vec4);
     group_sync<Z>(w.g);
-    if (kAhead && k0 + step < end) fetch_tile<T, Z>(vr, p.v, vb, p.v_sn, k0 + step, p.N, p.Dv, w.t, p.vec4);
     mul_tile<Z>(p_s, kv_s, w, o);
   }
   if constexpr (Z::G > 1) {
@@ -556,7 +549,7 @@ __device__ __forceinline__ void grad_of(const CausalParams& p, const RowStat& r,
 template <typename T, typename Z>
 __device__ __forceinline__ void dq_cores(const CausalParams& p, float* sm, int q0, int hq, int b) {
   constexpr int TM = Z::TM, TN = Z::TN, DM = Z::DM;
-  constexpr bool kAhead = Z::kFetch <= (Z::G == 1 ? 32 : 16);
+  constexpr bool kAhead = Z::kAhead;
   const Place w = place<Z>();
   float* groups = sm + Z::bwd_all();
   float* q_s = sm;
@@ -623,7 +616,7 @@ __device__ __forceinline__ void dq_cores(const CausalParams& p, float* sm, int q
 template <typename T, typename Z>
 __device__ __forceinline__ void dkv_cores(const CausalParams& p, float* sm, int k0, int hkv, int b) {
   constexpr int TM = Z::TM, TN = Z::TN, DM = Z::DM;
-  constexpr bool kAhead = Z::kFetch <= (Z::G == 1 ? 32 : 16);
+  constexpr bool kAhead = Z::kAhead;
   __shared__ RowStat st_all[Z::G][TN];
   const Place w = place<Z>();
   float* groups = sm + Z::bwd_all();

@@ -110,7 +110,6 @@ int32_t* status_of(const Tensor& t) {
   auto it = status_words().find(t.device().index());
   return it == status_words().end() ? nullptr : it->second.data_ptr<int32_t>();
 }
-bool has_status(const Tensor& t) { return status_words().count(t.device().index()) != 0; }
 void set_status(const Tensor& word) { status_words()[word.device().index()] = word; }
 
 struct Call {  // device and stream of a call
@@ -479,7 +478,6 @@ std::tuple<Tensor, Tensor, OptTensor, OptTensor> kv_attend(const Tensor& ck, con
 }  // namespace
 
 PYBIND11_MODULE(_full_attention, m) {
-  m.def("has_status", &has_status);
   m.def("set_status", &set_status);
   m.def("rotary", &rotary);
   m.def("segment_bounds", &segment_bounds);
