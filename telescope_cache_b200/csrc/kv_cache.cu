@@ -709,9 +709,9 @@ __device__ __forceinline__ float tanh_rel(float y) {
 //     q and rows 8-15 what the roundings left over, so S = row h + row h + 8
 //     has q to 22 bits; B = codes, exact in f16.
 //   O[head, dim] += P V:     A = P, split in two the same way, with the value
-//     rows' scales folded into it (relative to their largest so far, times 2^9,
-//     so that a weight of 2^5 and a scale of 2 fit: the f16 leftovers of a weight
-//     2^-k keep 22 - max(0, k - 12) bits).
+//     rows' scales folded into it, relative to the head's largest such product so
+//     far, times 2^9 (2^6 of growth fit): the f16 leftovers of one that is 2^-k of
+//     the largest keep 22 - max(0, k - 12) bits.
 // A dot product does not care about the order of its terms, so a lane reads 16
 // consecutive codes of a token and the A operand follows that order; likewise
 // output dims follow the value reads.  P leaves S's accumulator layout as the A
@@ -720,11 +720,13 @@ __device__ __forceinline__ float tanh_rel(float y) {
 // memory phase then meet eight different bank groups, for keys and for values.
 //
 // Bound by HBM where it is long: 2 (D + 4) bytes a token and key head.  64 sequences
-// of up to 32768 tokens, 16 / 4 heads of 128, int8: 213 us, 5.4 TB/s; 131072 tokens
-// of one sequence, 32 / 8 heads, e4m3, softcap: 52 us of reads and 13 for the start
-// and the join; 1024 tokens: 10 us, latency alone.
+// of up to 32768 tokens, 16 / 4 heads of 128, int8: 210 us, 5.4 TB/s; 131072 tokens
+// of one sequence, 32 / 8 heads, e4m3, softcap: 59 us, of which 42 are its reads at a
+// copy's rate and the rest the start and the join; 1024 tokens: 10 us, latency alone.
+// (With the values' scales relative to the largest scale, and the maxima joined in
+// every unit: 211 and 65 us, and a value row 2^24 of the others' cost them their bits.)
 constexpr int kAtThreads = 32 * kAtWarps;
-constexpr float kUp = 512.f, kLazy = 5.f;
+constexpr float kUp = 512.f, kLazy = 4.f, kGrow = 64.f;
 constexpr int kUnit = 32;  // tokens per stage
 
 template <int D> struct AtSmem {
@@ -899,7 +901,7 @@ __global__ void __launch_bounds__(kAtThreads, 3)
     float o[ND][4];
 #pragma unroll
     for (int i = 0; i < ND; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-    float m = -INFINITY, ell = 0.f, vref = kTiny;
+    float m = -INFINITY, ell = 0.f, winv = 0.f;  // winv: kUp / the reference of weight times scale
     // a lane holds the key and value scale of token `lane` of the warp's unit
     const float* ksb = p.ks + head * p.cap + c0 + warp * kUnit + lane;
     const float* vsb = p.vs + head * p.cap + c0 + warp * kUnit + lane;
@@ -959,48 +961,50 @@ __global__ void __launch_bounds__(kAtThreads, 3)
       }
       if (i + 1 < mine) load_scales(i + 1);
 
-      float mx = x[0], vx = vsc[0];
+      // m moves only where a weight would pass 2^4, winv only then or where a product of
+      // weight and scale would pass 2^6 of its reference: most units after the first
+      // leave the accumulators alone, and the four lanes of a head join their maxima
+      // in the others only
+      float mx = x[0], cm = 1.f;
 #pragma unroll
-      for (int j = 1; j < 8; ++j) {
-        mx = fmaxf(mx, x[j]);
-        vx = fmaxf(vx, vsc[j]);
-      }
+      for (int j = 1; j < 8; ++j) mx = fmaxf(mx, x[j]);
+      const bool moved = __any_sync(0xffffffffu, mx > m + kLazy);
+      if (moved) {
 #pragma unroll
-      for (int d = 1; d <= 2; d <<= 1) {
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
-        vx = fmaxf(vx, __shfl_xor_sync(0xffffffffu, vx, d));
-      }
-      // m and vref move only where a weight could pass 2^5 of them (vref 2): most
-      // units after the first leave the accumulators alone
-      if (__any_sync(0xffffffffu, mx > m + kLazy || vx > 2.f * vref)) {
-        const float mn = fmaxf(m, mx), vn = fmaxf(vref, vx);
-        const float cm = m == mn ? 1.f : ex2(m - mn);  // m -inf: 0
-        const float co = cm * (vref / vn);
+        for (int d = 1; d <= 2; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+        const float mn = fmaxf(m, mx);
+        cm = m == mn ? 1.f : ex2(m - mn);  // m -inf: 0
         ell *= cm;
+        m = mn;
+      }
+      const float me = m == -INFINITY ? 0.f : m;
+      float wx = 0.f;  // vsc becomes weight times scale
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float e = ex2(x[j] - me);
+        ell += e;
+        vsc[j] *= e;
+        wx = fmaxf(wx, vsc[j]);
+      }
+      if (moved || __any_sync(0xffffffffu, wx * winv > kGrow * kUp)) {
+#pragma unroll
+        for (int d = 1; d <= 2; d <<= 1) wx = fmaxf(wx, __shfl_xor_sync(0xffffffffu, wx, d));
+        const float wr = winv > 0.f ? __fdividef(kUp, winv) * cm : 0.f, wn = fmaxf(fmaxf(wr, wx), kTiny), co = wr / wn;
 #pragma unroll
         for (int d = 0; d < ND; ++d) o[d][0] *= co, o[d][1] *= co, o[d][2] *= co, o[d][3] *= co;
-        m = mn;
-        vref = vn;
+        winv = __fdividef(kUp, wn);
       }
-      const float vinv = __fdividef(kUp, vref);
-      const float me = m == -INFINITY ? 0.f : m;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {  // sixteen tokens: one k step of the second product
         uint32_t pa[4];
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          float pr[2];
-#pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            const int j = 4 * h + 2 * c + k;
-            const float e = ex2(x[j] - me);
-            ell += e;
-            pr[k] = e * (vsc[j] * vinv);
-          }
-          const uint32_t hi = pack_h2(pr[0], pr[1]);
+          const int j = 4 * h + 2 * c;
+          const float p0 = vsc[j] * winv, p1 = vsc[j + 1] * winv;
+          const uint32_t hi = pack_h2(p0, p1);
           const float2 h2 = unpack_h2(hi);
           pa[2 * c] = hi;
-          pa[2 * c + 1] = pack_h2(pr[0] - h2.x, pr[1] - h2.y);
+          pa[2 * c + 1] = pack_h2(p0 - h2.x, p1 - h2.y);
         }
         uint32_t vw[4][VB / 4];
 #pragma unroll
@@ -1052,7 +1056,7 @@ __global__ void __launch_bounds__(kAtThreads, 3)
       l_s[warp][g] = ell;
     }
     float* ow = o_s + (warp * 8 + g) * OS;
-    const float vout = vref / kUp;
+    const float vout = winv > 0.f ? 1.f / winv : 0.f;
 #pragma unroll
     for (int c = 0; c < 2; ++c)
 #pragma unroll

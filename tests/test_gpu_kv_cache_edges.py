@@ -6,8 +6,8 @@ import math
 import pytest
 import torch
 
-from full_attention_reference import quantise
-from test_gpu_kv_cache import DT, check, rand, slots
+from full_attention_reference import UNIT, quantise
+from test_gpu_kv_cache import DT, formula, rand
 
 pytestmark = pytest.mark.gpu
 
@@ -95,3 +95,32 @@ def test_an_infinity_makes_its_row_nan(store, dtype, D):
     for r, bad, last in ((rk, bk, kn), (rv, bv, vn)):
         assert bool(r[bad].isnan().all()) and bool(r[~bad].isfinite().all())
         assert torch.equal(last[:, 0].isnan(), r[:, 4].isnan())
+
+
+@pytest.mark.parametrize("store", ["int8", "fp8"])
+@pytest.mark.parametrize("dtype,D,Hq", [("f32", 128, 5), ("f32", 64, 8), ("bf16", 128, 2), ("f32", 80, 3)])
+@pytest.mark.parametrize("power", [12, 24, 36, 90])
+def test_values_of_very_different_sizes(store, dtype, D, Hq, power):
+    """A token with values 2^power times the others' that hardly any head weighs:
+    the others' weights keep their bits.  (One head's logits fall towards it, so
+    that its weight counts there.)"""
+    from telescope_cache_b200 import cached_attention, init_kv_cache, write_kv_cache
+
+    dt, N = DT[dtype], 900
+    k, v = rand(1, N, 1, D, dtype=dt, seed=1), rand(1, N, 1, D, dtype=dt, seed=2)
+    q = rand(1, 1, Hq, D, dtype=dt, seed=3)
+    q[..., 0] = 8.0
+    q[:, :, Hq - 1, 0] = -8.0 * power / 90
+    k[:, :, :, 0] = 0
+    for at in (1, 400, 899):
+        k[:, at, :, 0] = -15.0 * D ** 0.5
+        v[:, at] *= 2.0 ** power
+    c = init_kv_cache(1, N, 1, D, store=store, dtype=dt)
+    write_kv_cache(c, k, v)
+    out, lse = cached_attention(q, c)
+    held = [quantise(t, store)[2][0] for t in (k, v)]
+    o, l, size, top = formula(q[0, 0].double().cpu(), *held, None, D ** -0.5)
+    # as check(), and the fp32 error of logits of size top in the weights
+    err = (out[0, 0].double().cpu() - o).abs()
+    assert bool((err <= UNIT[dt] * o.abs() + (2.0 ** -18 + 4 * top * 2.0 ** -23) * size).all()), float((err / size).max())
+    assert float((lse[0, 0].double().cpu() - l).abs().max()) <= 1e-5 + 4e-6 * top
