@@ -137,8 +137,9 @@ int launch_bounds(int32_t B, int32_t N, const Id* seq_idx, int32_t* starts, int3
 // ---------------------------------------------------------------------------
 // Delta = rowsum(dO * out) - dlse, with out to twice its bits where its rounding's
 // leftovers were kept: the rounding of out alone puts an error of 2^-9 of a row's
-// |dO| |out| into every dX of the row (bf16, normal data: dQ off by 2.5e-3 of its
-// norm without, 2.3e-3 with, of which 1.7e-3 are its own rounding and as much dX's)
+// |dO| |out| into every dX of the row (bf16, 1000 tokens: dQ off by 2.4e-3 of its norm
+// with and without for normal data, by 2.4e-3 and 1.5e-2 for values of mean 8; 1.7e-3
+// are its own rounding and as much dX's)
 // ---------------------------------------------------------------------------
 // LANES lanes per row, 16 bytes of dO and out each (LANES 0: a warp per row of
 // any length).  Bound by HBM.

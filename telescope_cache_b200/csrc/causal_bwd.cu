@@ -11,6 +11,11 @@
 // Seven products instead of the five of a single pass, and nothing is summed by
 // atomics: the results do not depend on the order in which CTAs run.
 //
+// Delta comes from the forward's out, whose weights were rounded: its error is that of
+// one more rounding of dX where few keys share a row.  Where a query tile has one key
+// tile only, the dQ pass forms it from P and dP instead, before dX, and leaves it for
+// the dKV pass (rows of 2 to 128 keys: dK 1.40 of its own rounding's error for 1.46).
+//
 // -lse and -Delta: in the dQ pass a row's two numbers sit in its thread.  In the
 // dKV pass they belong to columns, and reading them from shared memory for every
 // element took half of the compute warps' time (128 words a warp and tile);
@@ -35,11 +40,11 @@
 // as this one's is in registers and dP a tile ahead, so the compute warps wait
 // for no product that depends on them.
 //
-// Measured, 8 / 2 heads of 128, 16384 tokens, bf16: dQ 585 us (1410 TFLOP/s of its
-// three products), dK/dV 900-920 us (1200-1220 of its four and their extra step), the
-// tensor pipe busy 75 % of both.  Softcap, 2 x 4096, 16 heads, five examples: 166 and
-// 232 us.  The dK/dV pass with 8 compute warps of 64 columns: 1.00 ms for 0.96 with 16
-// of 32; lse and Delta from shared memory: 0.96 for 0.90.
+// Measured, 8 / 2 heads of 128, 16384 tokens, bf16: dQ 598 us (1380 TFLOP/s of its
+// three products), dK/dV 980 us (1120 of its four and their extra step).  The dK/dV
+// pass with the products in the order dV, dK, S, dP: 5 % slower.  Before its waits for
+// the reading products it took 900-920 us; with 8 compute warps of 64 columns then
+// 1.00 ms for 0.96 with 16 of 32, with lse and Delta from shared memory 0.96 for 0.90.
 #include "causal_tc.cuh"
 
 namespace tc {
@@ -67,7 +72,7 @@ template <int HD> struct BwdSmem {
   static constexpr int kTile = 128 * HD * 2;
   static constexpr int kNK = 3, kNV = 2, kNQ = 2;
   static constexpr int kAug = (2 + kNQ) * kAugTile;
-  static constexpr int kDq = (2 + kNK + kNV) * kTile + 256 + 1024;
+  static constexpr int kDq = (2 + kNK + kNV) * kTile + 2 * 128 * 4 + 256 + 1024;
   static constexpr int kDkv = (2 + 2 * kNQ) * kTile + kAug + kNQ * 128 * 4 + 256 + 1024;
   static_assert(kDq <= 227 * 1024 && kDkv <= 227 * 1024, "backward shared memory exceeds the per-CTA limit");
 };
@@ -121,6 +126,30 @@ __device__ __forceinline__ void dx_columns(uint32_t d_addr, uint32_t x_addr, con
     }
     tmem_st16u(x_addr + 16 * h, w);
   }
+}
+
+// Sum of P dP over a thread's COLS columns inside [jlo, jhi), dP at d_addr and scores
+// in pg, which become P softcap'.
+template <int COLS, bool CAP>
+__device__ __forceinline__ float p_sum(uint32_t d_addr, float* pg, float2 nl2, float kq, float kc, int jlo, int jhi) {
+  float sum = 0.f;
+#pragma unroll
+  for (int h = 0; h < COLS / 32; ++h) {
+    float dp[32];
+    tmem_ld32(d_addr + 32 * h, dp);
+    tmem_wait_ld();
+#pragma unroll
+    for (int k = 0; k < 32; k += 2) {
+      float* x = pg + 32 * h + k;
+      float2 pr, g;
+      p_pair<CAP>(make_float2(x[0], x[1]), nl2, kq, kc, &pr, &g);
+      if (inside(32 * h + k, jlo, jhi)) sum += pr.x * dp[k];
+      if (inside(32 * h + k + 1, jlo, jhi)) sum += pr.y * dp[k + 1];
+      x[0] = g.x;
+      x[1] = g.y;
+    }
+  }
+  return sum;
 }
 
 // P of a thread's COLS columns (scores in pg), as 16-bit pairs at p_addr; pg
@@ -196,7 +225,8 @@ __global__ void __launch_bounds__(Shape<kDqCols>::kThreads, 1)
   uint8_t* g_s = q_s + TB;
   uint8_t* k_s = g_s + TB;
   uint8_t* v_s = k_s + NK * TB;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(v_s + NV * TB);
+  float* sum_s = reinterpret_cast<float*>(v_s + NV * TB);  // [2][128] sums of P dP of the rows' halves
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sum_s + 2 * 128);
   uint64_t* q_full = bars;           // Q
   uint64_t* g_full = bars + 1;       // dO
   uint64_t* k_full = g_full + 1;     // [NK]
@@ -335,7 +365,29 @@ __global__ void __launch_bounds__(Shape<kDqCols>::kThreads, 1)
     const uint32_t s_addr = tmem + lane_base + part * COLS;
     bool alive = true;
     int i = 0;
-    for (int j = j0; j < j1; ++j, ++i) {
+    if (j1 - j0 == 1) {  // the rows' only tile: Delta from it, for this pass and the next
+      const int jlo = first - j0 * 128 - part * COLS, jhi = end - j0 * 128 - part * COLS;
+      const uint32_t x_addr = s_addr + kColP;
+      alive = __all_sync(0xffffffffu, mbar_wait(s_full, 0, abort_flag, status) && mbar_wait(&p_full[0], 0, abort_flag, status));
+      float pg[COLS];
+      if (alive) {
+        tc_fence_after();
+        tmem_ld<COLS>(s_addr, pg);
+        tmem_wait_ld();
+        sum_s[part * 128 + r] = p_sum<COLS, CAP>(x_addr, pg, nl2, p.kq, p.kc, jlo, jhi);
+      }
+      named_bar(1, 32 * Shape<COLS>::kWarps);
+      if (alive) {
+        const float delta = sum_s[r] + sum_s[128 + r] - (row_ok && c.dlse ? c.dlse[row] : 0.f);
+        if (row_ok && part == 0) c.delta[row] = delta;
+        dx_columns<T, COLS, true, true>(x_addr, x_addr, pg, make_float2(-delta, -delta), jlo, jhi);
+        tmem_wait_st();
+        tc_fence_before();
+        warp_arrive(&x_full[0], lane);
+        i = 1;
+      }
+    }
+    for (int j = j0 + i; alive && j < j1; ++j, ++i) {
       alive = __all_sync(0xffffffffu, mbar_wait(s_full, i & 1, abort_flag, status));
       if (!alive) break;
       tc_fence_after();

@@ -10,9 +10,15 @@
 //               from TMEM
 //   warps 4-7   softmax of tile A, warps 8-11 of tile B: a thread owns a query
 //               row and all 128 keys of a tile: mask, softcap, running maximum
-//               and sum in fp32 (log2 units, O rescaled only when the maximum
+//               and sums in fp32 (log2 units, O rescaled only when the maximum
 //               grew by more than 2^8), P rounded to the operand type for the
-//               second product, O / l, lse.
+//               second product, O over the sum of the rounded weights, lse from
+//               that of the others.
+// P in 16 bits leaves out 1.8e-3 to 2.0e-3 of its norm off (bf16; its own rounding
+// alone: 1.6e-3); a second product for what the rounding left over would cost half of
+// a tile's products again.  Weights that sum to one as they are used matter to the
+// backward: Delta = sum w dP then errs by roundings of dX, not of P dP (values of mean
+// 8, sharp rows: dQ 2.5e-3 off for 1.3e-2).  The second sum costs 5 %: 495 -> 522 us.
 // TMEM: S_A, S_B (128 columns each), O_A, O_B (HD each), P_A, P_B (64: 16-bit pairs).
 // With HD 128 the first four fill it, and P_X takes the first half of S_X.  MMAs are
 // ordered only where they share an accumulator and a shape, so there the next S_X
@@ -37,6 +43,7 @@
 //
 // Every mbarrier wait is bounded (tc_ptx.cuh).
 #include <cmath>
+#include <type_traits>
 
 #include "causal_tc.cuh"
 
@@ -78,13 +85,20 @@ __device__ __forceinline__ float logit2(float s, const FwdParams& p) {
   return p.kc * (1.f - __fdividef(2.f, exp2_fast(s * p.kq * (2.f * kLog2e)) + 1.f));
 }
 
+// The two values of a packed pair.
+template <typename T> __device__ __forceinline__ float2 unpack2(uint32_t w) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value)
+    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+  else
+    return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+
 // exp2(logit - m) of 32 scores as packed pairs, columns outside [jlo, jhi) zero;
-// returns their sum.
+// adds them up as they are (sum) and as the pairs hold them (held).
 template <typename T, int MODE, bool MASK>
-__device__ __forceinline__ float chunk_p(const float* sv, int c0, const FwdParams& p, float m, int jlo, int jhi,
-                                         uint32_t* pw) {
+__device__ __forceinline__ void chunk_p(const float* sv, int c0, const FwdParams& p, float m, int jlo, int jhi,
+                                        uint32_t* pw, float2* sum, float2* held) {
   const float2 negm = f2(-m);
-  float2 s0 = f2(0.f), s1 = f2(0.f);
 #pragma unroll
   for (int c = 0; c < 32; c += 2) {
     const float2 u = make_float2(sv[c], sv[c + 1]);
@@ -110,22 +124,22 @@ __device__ __forceinline__ float chunk_p(const float* sv, int c0, const FwdParam
       a.y = (c0 + c + 1 >= jlo && c0 + c + 1 < jhi) ? a.y : -INFINITY;
     }
     const float2 e = make_float2(exp2_fast(a.x), exp2_fast(a.y));
-    if ((c >> 1) & 1) s1 = fadd2(s1, e);
-    else s0 = fadd2(s0, e);
+    *sum = fadd2(*sum, e);
     pw[c >> 1] = Pack2<T>::pack(e.x, e.y);
+    *held = fadd2(*held, unpack2<T>(pw[c >> 1]));
   }
-  const float2 s = fadd2(s0, s1);
-  return s.x + s.y;
 }
 
 template <typename T, int MODE>
-__device__ __forceinline__ float half_p(bool interior, const float* sv, int c0, const FwdParams& p, float m, int jlo,
-                                        int jhi, uint32_t* pw) {
-  if (interior)
-    return chunk_p<T, MODE, false>(sv, c0, p, m, jlo, jhi, pw) +
-           chunk_p<T, MODE, false>(sv + 32, c0 + 32, p, m, jlo, jhi, pw + 16);
-  return chunk_p<T, MODE, true>(sv, c0, p, m, jlo, jhi, pw) +
-         chunk_p<T, MODE, true>(sv + 32, c0 + 32, p, m, jlo, jhi, pw + 16);
+__device__ __forceinline__ void half_p(bool interior, const float* sv, int c0, const FwdParams& p, float m, int jlo,
+                                       int jhi, uint32_t* pw, float2* sum, float2* held) {
+  if (interior) {
+    chunk_p<T, MODE, false>(sv, c0, p, m, jlo, jhi, pw, sum, held);
+    chunk_p<T, MODE, false>(sv + 32, c0 + 32, p, m, jlo, jhi, pw + 16, sum, held);
+  } else {
+    chunk_p<T, MODE, true>(sv, c0, p, m, jlo, jhi, pw, sum, held);
+    chunk_p<T, MODE, true>(sv + 32, c0 + 32, p, m, jlo, jhi, pw + 16, sum, held);
+  }
 }
 
 // The key tiles [lo, hi) of a 128-query tile that starts at q0 (none: 0, 0).
@@ -297,7 +311,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
     const uint32_t p_addr = tmem + lane_base + kColP + x * kStepP;
     const int first = row_ok ? first_key(c, b, q) : 1, end = row_ok ? q + 1 : 0;
     const int lo = x ? blo : alo, hi = x ? bhi : ahi;
-    float m_used = -INFINITY, ell = 0.f;
+    float m_used = -INFINITY, ell = 0.f, kept = 0.f;  // sums of the weights, and of the rounded ones
     bool alive = true;
     int n = 0;
     for (int j = lo; j < hi; ++j, ++n) {
@@ -363,6 +377,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
       }
       if (__any_sync(0xffffffffu, rescale)) {
         ell *= alpha;
+        kept *= alpha;
 #pragma unroll 1
         for (int d = 0; d < HD; d += 32) {
           float ov[32];
@@ -374,7 +389,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
         }
       }
       const float m_eff = m_used > -INFINITY ? m_used : 0.f;
-      float ts = 0.f;
+      float2 sum = f2(0.f), held = f2(0.f);
 #pragma unroll 1
       for (int c0 = 0; c0 < KT; c0 += 64) {
         float sv[64];
@@ -383,16 +398,17 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
         tmem_ld32(s_addr + c0 + 32, sv + 32);
         tmem_wait_ld();
         if constexpr (!CAP) {
-          ts += half_p<T, kPlain>(interior, sv, c0, p, m_eff, jlo, jhi, pw);
+          half_p<T, kPlain>(interior, sv, c0, p, m_eff, jlo, jhi, pw, &sum, &held);
         } else {
-          if (mode == kS5) ts += half_p<T, kS5>(interior, sv, c0, p, m_eff, jlo, jhi, pw);
-          else if (mode == kS9) ts += half_p<T, kS9>(interior, sv, c0, p, m_eff, jlo, jhi, pw);
-          else ts += half_p<T, kTanh>(interior, sv, c0, p, m_eff, jlo, jhi, pw);
+          if (mode == kS5) half_p<T, kS5>(interior, sv, c0, p, m_eff, jlo, jhi, pw, &sum, &held);
+          else if (mode == kS9) half_p<T, kS9>(interior, sv, c0, p, m_eff, jlo, jhi, pw, &sum, &held);
+          else half_p<T, kTanh>(interior, sv, c0, p, m_eff, jlo, jhi, pw, &sum, &held);
         }
         tmem_st16u(p_addr + c0 / 2, pw);
         tmem_st16u(p_addr + c0 / 2 + 16, pw + 16);
       }
-      ell += ts;
+      ell += sum.x + sum.y;
+      kept += held.x + held.y;
       tmem_wait_st();
       tc_fence_before();
       warp_arrive(&p_full[x], lane);
@@ -400,7 +416,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
     if (alive && n > 0) alive = __all_sync(0xffffffffu, mbar_wait(&o_done[x], 0, abort_flag, status));
     if (alive) {
       tc_fence_after();
-      const float inv = ell != 0.f ? 1.f / ell : 0.f;
+      const float inv = kept != 0.f ? 1.f / kept : 0.f;
       const int64_t at = (((int64_t)b * c.N + q) * c.Hq + hq) * HD;
       T* out = static_cast<T*>(c.out) + at;
       T* low = c.out_low ? static_cast<T*>(c.out_low) + at : nullptr;

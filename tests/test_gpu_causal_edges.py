@@ -246,3 +246,43 @@ def test_tangents_are_refused():
             cached_attention(fwd.make_dual(q[:, :1], torch.ones_like(q[:, :1])), c)
         out, _ = causal_attention(q, k, v)  # none of them dual: as ever
     assert bool(out.isfinite().all())
+
+
+def rounded_gradients(q, k, v, gout, glse, see, scale, dt):
+    """dq, dk in 64 bits, and as they are with dX rounded to dt before its products and
+    the results after them: what a kernel with 16-bit operands cannot avoid."""
+    E = q.shape[2] // k.shape[2]
+    p = causal(q, k, v, see, None, scale)[3]
+    dp = torch.einsum("bnhd,bmhd->bhnm", gout, v.repeat_interleave(E, 2))
+    dx = p * (dp - (p * dp).sum(-1, keepdim=True) + glse.permute(0, 2, 1)[..., None])
+    out = []
+    for x, r in ((dx, lambda t: t), (dx.float().to(dt).double(), lambda t: t.float().to(dt).double())):
+        dq = r(torch.einsum("bhnm,bmhd->bnhd", x, k.repeat_interleave(E, 2)) * scale)
+        dk = r(torch.einsum("bhnm,bnhd->bmhd", x, q).unflatten(2, (-1, E)).sum(3) * scale)
+        out.append((dq, dk))
+    return out
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("N,mean,sharp,example", [(40, 8.0, 1, 40), (128, 8.0, 1, 5), (128, 0.0, 1, 3), (700, 8.0, 1, 700),
+                                                  (700, 8.0, 4, 700), (700, 2.0, 4, 90), (700, 0.0, 4, 700)])
+def test_gradients_of_values_that_share_a_mean(dtype, D, N, mean, sharp, example):
+    """dP - Delta is small beside its terms there.  Delta comes from the forward's
+    rounded weights: normalised by their own sum, each adds a rounding of its share
+    of dX, at most as much again as the rounding of dX itself: with it and the
+    result's, three for two, sqrt(3 / 2) = 1.22 of what rounded_gradients leaves."""
+    from telescope_cache_b200 import causal_attention
+
+    dt, Hq, Hkv, scale = DT[dtype], 4, 2, D ** -0.5
+    q, k, v = inputs(1, N, Hq, Hkv, D, D, dt, seed=23)
+    q, v = (q.float() * sharp).to(dt), (v.float() + mean).to(dt)
+    ids = (torch.arange(N, device="cuda") // example)[None]
+    see = visible(ids, 1, N, "cuda")
+    q, k, v = (t.detach().requires_grad_() for t in (q, k, v))
+    out, lse = causal_attention(q, k, v, seq_idx=ids)
+    gout, glse = torch.randn_like(out), torch.randn_like(lse)
+    got = torch.autograd.grad((out, lse), (q, k), (gout, glse))
+    want, near = rounded_gradients(*(t.detach().double() for t in (q, k, v, gout, glse)), see, scale, dt)
+    for a, w, n in zip(got, want, near):
+        assert rel(a, w) <= 1.25 * rel(n, w), (rel(a, w), rel(n, w))
