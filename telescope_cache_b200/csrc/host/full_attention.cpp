@@ -9,7 +9,6 @@
 // TypeError on other element types.
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
-#include <ATen/cuda/CUDAGraphsUtils.cuh>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/utils/pybind.h>
 
@@ -374,21 +373,32 @@ std::tuple<Tensor, Tensor> kv_read(const Tensor& ck, const Tensor& cv, const Ten
 // Workspace of the split attention: scratch, and arrival counts that are zero
 // between calls.  One per device and stream, since calls on one stream run in
 // order; not freed, for the process may end after the CUDA context.  A captured call
-// replays on any stream, next to any other: it has a workspace of its own from the
-// graph's memory, whose counts the graph clears.
+// replays on any stream, next to any other, so it takes both from the graph's memory:
+// scratch of its own, and counts for the calls of its capture on its stream, which
+// the graph clears where the first of them was recorded.
 struct Work {
   Tensor scratch, counts;
+  unsigned long long capture;  // counts: of this capture
 };
 Work workspace(const Tensor& on, cudaStream_t stream, int64_t floats, int64_t counts) {
+  static auto* eager = new std::map<std::pair<int, cudaStream_t>, Work>;
+  static auto* captured = new std::map<std::pair<int, cudaStream_t>, Work>;
   const auto f32 = on.options().dtype(at::kFloat), i32 = on.options().dtype(at::kInt);
-  if (at::cuda::currentStreamCaptureStatusMayInitCtx() != at::cuda::CaptureStatus::None) {
-    Work own{at::empty({floats}, f32), at::empty({counts}, i32)};
-    CHECK_RUN(cudaMemsetAsync(own.counts.data_ptr(), 0, counts * sizeof(int32_t), stream) == cudaSuccess,
-              "cached attention: clearing the arrival counts failed");
-    return own;
+  const std::pair<int, cudaStream_t> key{on.device().index(), stream};
+  cudaStreamCaptureStatus status;
+  unsigned long long id = 0;
+  CHECK_RUN(cudaStreamGetCaptureInfo(stream, &status, &id) == cudaSuccess, "cached attention: the stream's state is not known");
+  if (status != cudaStreamCaptureStatusNone) {
+    Work& w = (*captured)[key];
+    if (!w.counts.defined() || w.capture != id || w.counts.numel() < counts) {
+      w.counts = at::empty({std::max<int64_t>(counts, 4096)}, i32);
+      w.capture = id;
+      CHECK_RUN(cudaMemsetAsync(w.counts.data_ptr(), 0, w.counts.nbytes(), stream) == cudaSuccess,
+                "cached attention: clearing the arrival counts failed");
+    }
+    return {at::empty({floats}, f32), w.counts, id};
   }
-  static auto* all = new std::map<std::pair<int, cudaStream_t>, Work>;
-  Work& w = (*all)[{on.device().index(), stream}];
+  Work& w = (*eager)[key];
   if (!w.scratch.defined() || w.scratch.numel() < floats)
     w.scratch = at::empty({w.scratch.defined() ? std::max(floats, 2 * w.scratch.numel()) : floats}, f32);
   if (!w.counts.defined() || w.counts.numel() < counts)

@@ -107,3 +107,30 @@ def test_nothing_to_attend_in_a_capture():
     g.replay()
     torch.cuda.synchronize()
     assert out.shape == (0, 1, 2, 64) and lse.shape == (0, 1, 2) and c.lengths.tolist() == [0, 0]
+
+
+def test_calls_of_a_graph_that_need_more_and_more():
+    """Counts that grow inside a capture, and branches of a capture side by side."""
+    from telescope_cache_b200 import cached_attention, init_kv_cache, write_kv_cache
+
+    caches = []
+    for B, H, N in ((1, 4, 300), (700, 8, 130), (2, 2, 700)):
+        c = init_kv_cache(B, N, H, 64)
+        write_kv_cache(c, rand(B, N, H, 64, seed=B), rand(B, N, H, 64, seed=B + 1))
+        caches.append((c, rand(B, 1, 2 * H, 64, dtype=torch.bfloat16, seed=B + 2)))
+    want = [cached_attention(q, c) for c, q in caches]
+    g, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(g):
+        got = [cached_attention(q, c) for c, q in caches]
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            branch = [cached_attention(q, c) for c, q in reversed(caches)]
+        again = [cached_attention(q, c) for c, q in caches]
+        torch.cuda.current_stream().wait_stream(side)
+    for _ in range(20):
+        g.replay()
+    torch.cuda.synchronize()
+    for r in (got, branch[::-1], again):
+        for (a, b), (o, l) in zip(r, want):
+            assert torch.equal(a, o) and torch.equal(b, l)
