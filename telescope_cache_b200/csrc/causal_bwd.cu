@@ -40,11 +40,15 @@
 // as this one's is in registers and dP a tile ahead, so the compute warps wait
 // for no product that depends on them.
 //
-// Measured, 8 / 2 heads of 128, 16384 tokens, bf16: dQ 598 us (1380 TFLOP/s of its
-// three products), dK/dV 980 us (1120 of its four and their extra step).  The dK/dV
-// pass with the products in the order dV, dK, S, dP: 5 % slower.  Before its waits for
-// the reading products it took 900-920 us; with 8 compute warps of 64 columns then
-// 1.00 ms for 0.96 with 16 of 32, with lse and Delta from shared memory 0.96 for 0.90.
+// Measured, 8 / 2 heads of 128, 16384 tokens, bf16: dQ 573-598 us (1380-1440 TFLOP/s of
+// its three products), dK/dV 925-980 us (1120-1190 of its four and their extra step),
+// the tensor pipe busy 71 and 68 %.  Softcap, 2 x 4096, 16 heads, five examples: 156 and
+// 222 us, bound by the exp2 unit: exp2 and a quotient for the tanh and exp2 for P are
+// three results an element, 16 a clock, twice (the softcap dK/dV kernels also spill 44
+// to 68 bytes).  The dK/dV pass with the products in the order dV, dK, S, dP: 5 %
+// slower; without its waits for the reading products it took 900-920 us, with 8 compute
+// warps of 64 columns then 1.00 ms for 0.96 with 16 of 32, and with lse and Delta from
+// shared memory 0.96 for 0.90.
 #include "causal_tc.cuh"
 
 namespace tc {

@@ -18,7 +18,8 @@
 // alone: 1.6e-3); a second product for what the rounding left over would cost half of
 // a tile's products again.  Weights that sum to one as they are used matter to the
 // backward: Delta = sum w dP then errs by roundings of dX, not of P dP (values of mean
-// 8, sharp rows: dQ 2.5e-3 off for 1.3e-2).  The second sum costs 5 %: 495 -> 522 us.
+// 8, sharp rows: dQ 2.5e-3 off for 1.3e-2).  The second sum costs 4 %: 491 -> 511 us
+// (pairs unpacked and added two at a time: 522).
 // TMEM: S_A, S_B (128 columns each), O_A, O_B (HD each), P_A, P_B (64: 16-bit pairs).
 // With HD 128 the first four fill it, and P_X takes the first half of S_X.  MMAs are
 // ordered only where they share an accumulator and a shape, so there the next S_X
@@ -33,13 +34,14 @@
 // tanh comes from its odd Maclaurin series (through y^5 below 0.15, y^9 below
 // 0.5: 1e-6 and 1e-5 of the value), else as 1 - 2 / (e^2y + 1).
 //
-// Measured, 8 / 2 heads of 128, 16384 tokens, bf16: 520-544 us, 1010-1060 TFLOP/s of
-// visible entries, 0.62-0.65 of a large GEMM's burst rate, tensor pipe 53 %.  Bound by
-// each tile's chain (scores, maximum, exp2, product): of a warp's 3600 clocks a tile
-// 1750 go to exp2 and rounding, which both tiles' warps share, 360 to the maximum.
-// Packed prompts (2 x 8192, 16 / 4 heads, seven examples): 235 us; with softcap (2 x
-// 4096, 16 heads, five examples): 120 us.  Two threads a row, with a swap of their
-// maxima, gained 2 % without softcap and lost 12 % with it.
+// Measured, 8 / 2 heads of 128, 16384 tokens, bf16: 511-555 us (from box to box and
+// with q, k, v as views of one projection), 990-1070 TFLOP/s of visible entries,
+// 0.61-0.66 of a large GEMM's burst rate, tensor pipe 50 %.  Bound by each tile's chain
+// (scores, maximum, exp2, product): of a warp's 3600 clocks a tile 1750 went to exp2 and
+// rounding, which both tiles' warps share, 360 to the maximum.  Packed prompts (2 x
+// 8192, 16 / 4 heads, seven examples): 230 us; with softcap (2 x 4096, 16 heads, five
+// examples): 128 us.  Two threads a row, with a swap of their maxima, gained 2 % without
+// softcap and lost 12 % with it.
 //
 // Every mbarrier wait is bounded (tc_ptx.cuh).
 #include <cmath>
@@ -85,12 +87,18 @@ __device__ __forceinline__ float logit2(float s, const FwdParams& p) {
   return p.kc * (1.f - __fdividef(2.f, exp2_fast(s * p.kq * (2.f * kLog2e)) + 1.f));
 }
 
-// The two values of a packed pair.
-template <typename T> __device__ __forceinline__ float2 unpack2(uint32_t w) {
+// s += the two values of a packed pair (sums of a 16-bit and a 32-bit float).
+template <typename T> __device__ __forceinline__ void add_pair(float2* s, uint32_t w) {
   if constexpr (std::is_same<T, __nv_bfloat16>::value)
-    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\t"
+        "add.f32.bf16 %0, l, %0;\n\tadd.f32.bf16 %1, h, %1;\n\t}"
+        : "+f"(s->x), "+f"(s->y)
+        : "r"(w));
   else
-    return __half22float2(*reinterpret_cast<const __half2*>(&w));
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\t"
+        "add.f32.f16 %0, l, %0;\n\tadd.f32.f16 %1, h, %1;\n\t}"
+        : "+f"(s->x), "+f"(s->y)
+        : "r"(w));
 }
 
 // exp2(logit - m) of 32 scores as packed pairs, columns outside [jlo, jhi) zero;
@@ -126,7 +134,7 @@ __device__ __forceinline__ void chunk_p(const float* sv, int c0, const FwdParams
     const float2 e = make_float2(exp2_fast(a.x), exp2_fast(a.y));
     *sum = fadd2(*sum, e);
     pw[c >> 1] = Pack2<T>::pack(e.x, e.y);
-    *held = fadd2(*held, unpack2<T>(pw[c >> 1]));
+    add_pair<T>(held, pw[c >> 1]);
   }
 }
 
