@@ -71,20 +71,26 @@ def causal_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *,
     reads key head h // (Hq / Hkv).
 
     S = c tanh(X / c) (X without softcap), X = scale q.k, scale 1 / sqrt(Dk) by
-    default (any finite one; one that is not positive, or outside 1e-30 .. 1e30, and a
-    softcap above 2048 run on the CUDA cores).  seq_idx [B, N]: ids of the row's packed examples, one run each: a
+    default.  seq_idx [B, N]: ids of the row's packed examples, one run each: a
     token attends its own example only; a token with a negative id is padding
     (out 0, lse -inf, zero gradients).  The bounds of segment_bounds may be
     given in its place, so that the layers of a model form them once.
 
-    Differentiable in q, k, v through both results (for 16-bit types the graph also
-    keeps what the rounding of out left over, a tensor of its size).  bf16 / f16 with Dk = Dv of
-    64 or 128 run on the tensor cores (strided q, k, v in place where strides
-    and addresses are multiples of 16 bytes), other types and head dims up to
-    256 on the CUDA cores.  Products with tokens outside a row's view are formed
-    and masked: a NaN or infinity in one example's values reaches the rows of
-    its neighbours in the same 128 tokens.  ``impl`` ('simt' | 'tensor' | None)
-    pins a kernel family for testing."""
+    Differentiable in q, k, v through both results, once and in reverse mode (for
+    16-bit types the graph also keeps what the rounding of out left over, a tensor
+    of its size).
+
+    bf16 / f16 with Dk = Dv of 64 or 128 run on the tensor cores: strided q, k, v in
+    place where strides and addresses are multiples of 16 bytes and no stride is
+    zero, with a scale of 1e-30 to 1e30 and a softcap of at most 2048.  Everything
+    else, head dims up to 256, runs on the CUDA cores, up to 30 times slower: copy
+    16-bit views that do not qualify.  The tensor cores take weights and gradients of
+    logits in the type of q: in f16 the latter, up to twice |dout| |v| of a token,
+    have to stay below 65504 and well above 6e-8 (a loss scale that fits the other
+    f16 gradients does).  Products with tokens outside a row's view are formed and
+    masked: a NaN or infinity in one example's values reaches the rows of its
+    neighbours in the same 128 tokens.  ``impl`` ('simt' | 'tensor' | None) pins a
+    kernel family for testing."""
     code = _impl_code(impl)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         if seq_idx is not None and not isinstance(seq_idx, Segments):
